@@ -1,0 +1,449 @@
+// Kernels that move rows of the paged cache: the commit of confirmed drafted tokens, and eviction by accumulated attention weight.
+// Both work on all layers of a group of planes at once: keys and values [layers, slots, kv heads, head size].
+#include "common.cuh"
+
+namespace {
+
+// The cache row of a place of a request, or -1 for a page that is none of the cache's: such a place is neither read nor written.
+__device__ __forceinline__ int slot_of(const int* table, int page_size, int num_slots, int place) {
+    const int page = table[place / page_size];
+    const long long slot = (long long)page * page_size + place % page_size;
+    return page >= 0 && slot < num_slots ? (int)slot : -1;
+}
+
+// ---- the confirmed drafted tokens --------------------------------------------------------------------------------------------
+// A request's nodes are its rows: node 0 is the newest confirmed token, every other node continues its parent (of a lower number)
+// with a drafted token.  What the model chooses behind a node confirms the first of the node's children with that token:
+//     path[0] = 0,   path[d + 1] = the lowest c with parents[c] = path[d] and tokens[c] = targets[path[d]]
+// The keys and values of node path[d] lie at place pos + path[d] and belong to pos + d.  path rises strictly, so path[d] >= d: a row
+// never moves onto one that is still to be read when the rows move in the path's order, and a thread that moves the same 16 bytes of
+// every row needs no meeting with others; it reads eight rows ahead.
+// Every block works out the path for itself (a warp looks at 32 nodes at a time), which is less than a second launch would take.
+constexpr int COMMIT_THREADS = 128;
+constexpr int COMMIT_MAX_PATH = 1024;
+constexpr int COMMIT_AHEAD = 8;
+struct CommitParams {
+    const int* tokens;
+    const int* parents;
+    const int* targets;
+    const int* span_row;
+    const int* span_len;
+    const int* span_pos;
+    const int* table;
+    char* k;
+    char* v;
+    int* path;
+    int* count;
+    int* next;
+    int S, T, L, max_pages, page_size, num_slots, width;
+    int row_units;               // of one slot's row of K (or V), in units of the copies
+    int layers_a_block;
+};
+
+template <typename U>
+__global__ void __launch_bounds__(COMMIT_THREADS) tree_commit_kernel(const CommitParams p) {
+    __shared__ int path_s[COMMIT_MAX_PATH];
+    __shared__ int slot_s[2][COMMIT_MAX_PATH];
+    __shared__ int count_s;
+    llb_after_previous();
+    const int s = blockIdx.x, lane = threadIdx.x & 31;
+    const int row = p.span_row[s], pos = max(p.span_pos[s], 0);
+    int n = min(min(p.span_len[s], p.T - row), p.max_pages * p.page_size - pos);
+    if (row < 0 || n < 0) n = 0;
+    if (threadIdx.x < 32) {
+        int count = 0, cur = 0;
+        if (n > 0) {
+            if (lane == 0) path_s[0] = 0;
+            count = 1;
+            while (count < p.width) {
+                const int want = p.targets[row + cur];
+                int child = -1;
+                for (int c0 = cur + 1; c0 < n; c0 += 32) {
+                    const int c = c0 + lane;
+                    const unsigned fits = __ballot_sync(0xffffffffu, c < n && p.parents[row + c] == cur && p.tokens[row + c] == want);
+                    if (fits) {
+                        child = c0 + __ffs(fits) - 1;
+                        break;
+                    }
+                }
+                if (child < 0) break;
+                cur = child;
+                if (lane == 0) path_s[count] = cur;
+                ++count;
+            }
+        }
+        if (lane == 0) count_s = count;
+        if (blockIdx.y == 0) {
+            __syncwarp();
+            for (int d = lane; d < p.width; d += 32) p.path[(size_t)s * p.width + d] = d < count ? path_s[d] : -1;
+            if (lane == 0) {
+                p.count[s] = count;
+                p.next[s] = count > 0 ? p.targets[row + cur] : -1;
+            }
+        }
+    }
+    __syncthreads();
+    const int count = count_s;
+    const int* table = p.table + (size_t)s * p.max_pages;
+    for (int d = threadIdx.x; d < count; d += COMMIT_THREADS) {
+        slot_s[0][d] = path_s[d] == d ? -1 : slot_of(table, p.page_size, p.num_slots, pos + path_s[d]);
+        slot_s[1][d] = path_s[d] == d ? -1 : slot_of(table, p.page_size, p.num_slots, pos + d);
+    }
+    __syncthreads();
+    const int units = 2 * p.row_units;
+    for (int i = threadIdx.x; i < p.layers_a_block * units; i += COMMIT_THREADS) {
+        const int layer = blockIdx.y * p.layers_a_block + i / units;
+        if (layer >= p.L) break;
+        const int u = i % units;
+        U* base = (U*)(u < p.row_units ? p.k : p.v) + (size_t)layer * p.num_slots * p.row_units + (u < p.row_units ? u : u - p.row_units);
+        for (int d0 = 1; d0 < count; d0 += COMMIT_AHEAD) {
+            U x[COMMIT_AHEAD];
+#pragma unroll
+            for (int e = 0; e < COMMIT_AHEAD; ++e)
+                if (d0 + e < count && slot_s[0][d0 + e] >= 0) x[e] = base[(size_t)slot_s[0][d0 + e] * p.row_units];
+#pragma unroll
+            for (int e = 0; e < COMMIT_AHEAD; ++e)
+                if (d0 + e < count && slot_s[0][d0 + e] >= 0 && slot_s[1][d0 + e] >= 0) base[(size_t)slot_s[1][d0 + e] * p.row_units] = x[e];
+        }
+    }
+}
+
+// ---- eviction ------------------------------------------------------------------------------------------------------------------
+// For every layer, request and kv head: of the n places that are held the `budget` that are worth most stay, a place's worth being
+// the weight that its key has received, above everything else the places of the first and of the latest positions, and of equal
+// ones the lowest place.  What stays lies in the places below the budget afterwards: the dropped ones among them (holes, in rising
+// order) take the keys, values, weights and positions of those that stay beyond it (in rising order).  Attention does not ask for
+// the order of its keys (they carry their rotation), so nothing else moves: as many rows as there are holes instead of nearly all.
+//
+// A block takes one (layer, request, kv head).  The worth of all places as whole numbers in the floats' order is kept in shared
+// memory (or read again where there are too many); the budget's threshold is found digit by digit from the top, 11, 11 and 10 bits,
+// by counting, the dropping of a single place by one search for the least.  The places that stay become a bit each, which
+// gives holes and fillers their numbers by counting bits; the moves are then dealt evenly to all threads, 16 bytes at a time.
+constexpr int EV_THREADS = 512;
+constexpr int EV_WARPS = EV_THREADS / 32;
+constexpr int EV_BINS = 2048;
+constexpr int EV_LIST = 2048;             // moves that are listed at a time
+constexpr int EV_MAX_PLACES = 1 << 20;
+struct EvictParams {
+    char* k;
+    char* v;
+    const float* mass;                    // [L, Hkv, num_slots]
+    const int* positions;
+    float* mass_out;
+    int* positions_out;
+    const int* lengths;                   // [S] places that are held
+    const int* ends;                      // [S] position of the request's next token
+    const int* table;
+    int S, max_pages, page_size, num_slots, Hkv, budget, first, latest;
+    int head_units;                       // of one head's row of K (or V), in units of the copies
+    int cache_places;                     // as many worths as shared memory holds
+};
+
+__device__ __forceinline__ unsigned order_of(float f) {
+    if (f != f) return 0xfffffffeu;                      // NaN: above infinity
+    const unsigned u = __float_as_uint(f + 0.0f);        // (-0 becomes +0)
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+template <typename U>
+__global__ void __launch_bounds__(EV_THREADS) cache_evict_kernel(const EvictParams p) {
+    extern __shared__ unsigned ev_sm[];
+    __shared__ unsigned hist[EV_BINS];
+    __shared__ unsigned list_s[2][EV_LIST];
+    __shared__ unsigned warp_s[EV_WARPS][2];
+    __shared__ unsigned long long least_s[EV_WARPS];
+    __shared__ unsigned found_s[2];
+    llb_after_previous();
+    const int s = blockIdx.x / p.Hkv, h = blockIdx.x - s * p.Hkv, layer = blockIdx.y;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int n = max(0, min(p.lengths[s], p.max_pages * p.page_size)), budget = p.budget;
+    const int* table = p.table + (size_t)s * p.max_pages;
+    const size_t plane = ((size_t)layer * p.Hkv + h) * p.num_slots;
+    const bool apart = p.mass_out != p.mass;
+    unsigned* bits = ev_sm;                              // [words] places that stay
+    const int words = (n + 31) / 32;
+    unsigned* worth_s = ev_sm + (p.max_pages * p.page_size + 31) / 32;
+    if (n <= budget) {
+        if (apart)
+            for (int i = tid; i < n; i += EV_THREADS) {
+                const int slot = slot_of(table, p.page_size, p.num_slots, i);
+                if (slot < 0) continue;
+                p.mass_out[plane + slot] = p.mass[plane + slot];
+                p.positions_out[plane + slot] = p.positions[plane + slot];
+            }
+        return;
+    }
+    const int from = p.ends[s] - p.latest;
+    auto compute = [&](int i) -> unsigned {
+        const int slot = slot_of(table, p.page_size, p.num_slots, i);
+        if (slot < 0) return 0u;
+        const int pos = p.positions[plane + slot];
+        if (pos < p.first || pos >= from) return 0xffffffffu;
+        return order_of(p.mass[plane + slot]);
+    };
+    const bool cached = n <= p.cache_places;
+    auto worth = [&](int i) -> unsigned { return cached ? worth_s[i] : compute(i); };
+
+    if (n == budget + 1) {
+        // one place goes: the least worth, of equal ones the highest place
+        unsigned long long least = ~0ull;
+        for (int i = tid; i < n; i += EV_THREADS) {
+            const unsigned long long x = ((unsigned long long)compute(i) << 32) | (unsigned)(n - 1 - i);
+            least = x < least ? x : least;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const unsigned long long x = __shfl_xor_sync(0xffffffffu, least, o);
+            least = x < least ? x : least;
+        }
+        if (lane == 0) least_s[warp] = least;
+        __syncthreads();
+        least = least_s[0];
+#pragma unroll
+        for (int w = 1; w < EV_WARPS; ++w) least = least_s[w] < least ? least_s[w] : least;
+        const int hole = n - 1 - (int)(unsigned)least;
+        if (apart)
+            for (int i = tid; i < budget; i += EV_THREADS) {
+                const int slot = slot_of(table, p.page_size, p.num_slots, i);
+                if (slot < 0 || i == hole) continue;
+                p.mass_out[plane + slot] = p.mass[plane + slot];
+                p.positions_out[plane + slot] = p.positions[plane + slot];
+            }
+        if (hole == n - 1) return;
+        const int dst = slot_of(table, p.page_size, p.num_slots, hole), src = slot_of(table, p.page_size, p.num_slots, n - 1);
+        if (dst < 0 || src < 0) return;
+        for (int u = tid; u < 2 * p.head_units; u += EV_THREADS) {
+            const int e = u < p.head_units ? u : u - p.head_units;
+            U* base = (U*)(u < p.head_units ? p.k : p.v) + ((size_t)layer * p.num_slots * p.Hkv + h) * p.head_units + e;
+            base[(size_t)dst * p.Hkv * p.head_units] = base[(size_t)src * p.Hkv * p.head_units];
+        }
+        if (tid == 0) {
+            p.mass_out[plane + dst] = p.mass[plane + src];
+            p.positions_out[plane + dst] = p.positions[plane + src];
+        }
+        return;
+    }
+
+    // the threshold: the budget-th largest worth, and how many of its equals stay
+    unsigned prefix = 0, wanted = budget;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
+        for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += EV_THREADS) {
+            const unsigned x = pass == 0 ? compute(i) : worth(i);
+            if (pass == 0 && cached) worth_s[i] = x;
+            // (64 bits: a shift by 32 would be none)
+            if (((unsigned long long)(x ^ prefix) >> (shift + width)) == 0) atomicAdd(&hist[(x >> shift) & ((1u << width) - 1u)], 1u);
+        }
+        __syncthreads();
+        // how many lie above each thread's four bins, counted from the top
+        constexpr int PER = EV_BINS / EV_THREADS;
+        unsigned mine = 0;
+        const int top = EV_BINS - 1 - tid * PER;
+#pragma unroll
+        for (int b = 0; b < PER; ++b) mine += hist[top - b];
+        unsigned sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        if (lane == 31) warp_s[warp][0] = sum;
+        __syncthreads();
+        unsigned above = sum - mine;
+        for (int w = 0; w < warp; ++w) above += warp_s[w][0];
+        if (above < wanted && above + mine >= wanted) {
+#pragma unroll
+            for (int b = 0; b < PER; ++b) {
+                const unsigned c = hist[top - b];
+                if (above < wanted && above + c >= wanted) {
+                    found_s[0] = prefix | ((unsigned)(top - b) << shift);
+                    found_s[1] = wanted - above;
+                }
+                above += c;
+            }
+        }
+        __syncthreads();
+        prefix = found_s[0];
+        wanted = found_s[1];
+    }
+    // a bit for every place that stays: a warp takes words in a row, so that equals are counted in the places' order
+    const int per_warp = (words + EV_WARPS - 1) / EV_WARPS;
+    const int w0 = min(words, warp * per_warp), w1 = min(words, w0 + per_warp);
+    unsigned equals = 0;
+    for (int w = w0; w < w1; ++w) {
+        const int i = w * 32 + lane;
+        equals += __popc(__ballot_sync(0xffffffffu, i < n && worth(i) == prefix));
+    }
+    if (lane == 0) warp_s[warp][1] = equals;
+    __syncthreads();
+    unsigned before = 0;
+    for (int w = 0; w < warp; ++w) before += warp_s[w][1];
+    for (int w = w0; w < w1; ++w) {
+        const int i = w * 32 + lane;
+        const unsigned x = i < n ? worth(i) : 0u;
+        const unsigned same = __ballot_sync(0xffffffffu, i < n && x == prefix);
+        const bool stays = i < n && (x > prefix || (x == prefix && before + __popc(same & ((1u << lane) - 1u)) < wanted));
+        const unsigned word = __ballot_sync(0xffffffffu, stays);
+        if (lane == 0) bits[w] = word;
+        before += __popc(same);
+    }
+    __syncthreads();
+    // numbers of the holes and of those that fill them
+    const int per = (words + EV_THREADS - 1) / EV_THREADS;
+    const int a0 = min(words, tid * per), a1 = min(words, a0 + per);
+    auto below = [&](int w) -> unsigned {                // the word's places below the budget
+        const int m = budget - w * 32;
+        return m <= 0 ? 0u : m >= 32 ? 0xffffffffu : (1u << m) - 1u;
+    };
+    unsigned holes = 0, fillers = 0;
+    for (int w = a0; w < a1; ++w) {
+        holes += __popc(~bits[w] & below(w));
+        fillers += __popc(bits[w] & ~below(w));
+    }
+    unsigned hs = holes, fs = fillers;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, hs, o), y = __shfl_up_sync(0xffffffffu, fs, o);
+        if (lane >= o) {
+            hs += x;
+            fs += y;
+        }
+    }
+    if (lane == 31) {
+        warp_s[warp][0] = hs;
+        warp_s[warp][1] = fs;
+    }
+    __syncthreads();
+    hs -= holes;
+    fs -= fillers;
+    unsigned moves = 0;
+    for (int w = 0; w < EV_WARPS; ++w) {
+        if (w < warp) {
+            hs += warp_s[w][0];
+            fs += warp_s[w][1];
+        }
+        moves += warp_s[w][0];
+    }
+    if (apart)
+        for (int i = tid; i < budget; i += EV_THREADS) {
+            if (!((bits[i >> 5] >> (i & 31)) & 1u)) continue;
+            const int slot = slot_of(table, p.page_size, p.num_slots, i);
+            if (slot < 0) continue;
+            p.mass_out[plane + slot] = p.mass[plane + slot];
+            p.positions_out[plane + slot] = p.positions[plane + slot];
+        }
+    for (unsigned m0 = 0; m0 < moves; m0 += EV_LIST) {
+        const unsigned count = min((unsigned)EV_LIST, moves - m0);
+        unsigned hr = hs, fr = fs;
+        for (int w = a0; w < a1; ++w) {
+            for (unsigned x = ~bits[w] & below(w); x; x &= x - 1, ++hr)
+                if (hr - m0 < count) list_s[0][hr - m0] = slot_of(table, p.page_size, p.num_slots, w * 32 + __ffs(x) - 1);
+            for (unsigned x = bits[w] & ~below(w); x; x &= x - 1, ++fr)
+                if (fr - m0 < count) list_s[1][fr - m0] = slot_of(table, p.page_size, p.num_slots, w * 32 + __ffs(x) - 1);
+        }
+        __syncthreads();
+        const unsigned units = 2 * p.head_units, total = count * units;
+        const size_t stride = (size_t)p.Hkv * p.head_units, base = (size_t)layer * p.num_slots * stride + (size_t)h * p.head_units;
+        constexpr int AHEAD = 4;
+        for (unsigned i0 = tid; i0 < total; i0 += EV_THREADS * AHEAD) {
+            U x[AHEAD];
+#pragma unroll
+            for (int e = 0; e < AHEAD; ++e) {
+                const unsigned i = i0 + e * EV_THREADS;
+                if (i >= total) continue;
+                const unsigned m = i / units, u = i - m * units;
+                const int src = (int)list_s[1][m];
+                const U* from_row = (const U*)(u < (unsigned)p.head_units ? p.k : p.v) + base + (u < (unsigned)p.head_units ? u : u - p.head_units);
+                if (src >= 0) x[e] = from_row[(size_t)src * stride];
+            }
+#pragma unroll
+            for (int e = 0; e < AHEAD; ++e) {
+                const unsigned i = i0 + e * EV_THREADS;
+                if (i >= total) continue;
+                const unsigned m = i / units, u = i - m * units;
+                const int src = (int)list_s[1][m], dst = (int)list_s[0][m];
+                U* to_row = (U*)(u < (unsigned)p.head_units ? p.k : p.v) + base + (u < (unsigned)p.head_units ? u : u - p.head_units);
+                if (src >= 0 && dst >= 0) to_row[(size_t)dst * stride] = x[e];
+            }
+        }
+        for (unsigned m = tid; m < count; m += EV_THREADS) {
+            const int src = (int)list_s[1][m], dst = (int)list_s[0][m];
+            if (src < 0 || dst < 0) continue;
+            p.mass_out[plane + dst] = p.mass[plane + src];
+            p.positions_out[plane + dst] = p.positions[plane + src];
+        }
+        __syncthreads();
+    }
+}
+
+// The widest unit that divides a row's bytes and every address that rows begin at.
+int unit_bytes(const void* k, const void* v, long long row_bytes) {
+    const uintptr_t all = (uintptr_t)k | (uintptr_t)v | (uintptr_t)row_bytes;
+    return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
+}
+
+template <typename U> int launch_commit(const CommitParams& p, cudaStream_t stream) {
+    llb_launch(tree_commit_kernel<U>, dim3(p.S, llb_ceil_div(p.L, p.layers_a_block)), dim3(COMMIT_THREADS), 0, stream, p);
+    return llb_check_launch("tree_commit");
+}
+template <typename U> int launch_evict(EvictParams p, int L, cudaStream_t stream) {
+    const int places = p.max_pages * p.page_size, bit_words = (places + 31) / 32;
+    // two blocks an SM have room for 20,000 worths each; places beyond that are read again in every pass
+    p.cache_places = places < 20000 ? places : 20000;
+    if (bit_words > 8192) p.cache_places = 8192;
+    const size_t smem = sizeof(unsigned) * ((size_t)bit_words + p.cache_places);
+    cudaError_t e = cudaFuncSetAttribute(cache_evict_kernel<U>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return llb_fail("cache_evict: cannot opt in to %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    llb_launch(cache_evict_kernel<U>, dim3(p.S * p.Hkv, L), dim3(EV_THREADS), smem, stream, p);
+    return llb_check_launch("cache_evict");
+}
+
+}  // namespace
+
+// tokens, parents, targets int [T]; caches [L, num_slots, row_bytes]; path [S, width], count [S], next [S].
+LLB_EXPORT int llb_tree_commit(const int* tokens, const int* parents, const int* targets, void* k, void* v, const int* span_row,
+                               const int* span_len, const int* span_pos, const int* table, int S, int T, int L, int max_pages,
+                               int page_size, int num_slots, int row_bytes, int* path, int width, int* count, int* next,
+                               cudaStream_t stream) {
+    if (S == 0) return 0;
+    LLB_REQUIRE(S > 0 && T >= 0 && L > 0 && L <= 65535 && max_pages >= 0 && page_size > 0 && num_slots > 0 && row_bytes > 0 && row_bytes % 2 == 0 &&
+                (long long)max_pages * page_size <= 0x7fffffff, "tree_commit: bad sizes");
+    LLB_REQUIRE(width > 0 && width <= COMMIT_MAX_PATH, "tree_commit: path has room for %d nodes, 1 to %d are possible", width, COMMIT_MAX_PATH);
+    CommitParams p;
+    p.tokens = tokens; p.parents = parents; p.targets = targets; p.k = (char*)k; p.v = (char*)v; p.span_row = span_row;
+    p.span_len = span_len; p.span_pos = span_pos; p.table = table; p.S = S; p.T = T; p.L = L; p.max_pages = max_pages;
+    p.page_size = page_size; p.num_slots = num_slots; p.path = path; p.width = width; p.count = count; p.next = next;
+    const int unit = unit_bytes(k, v, row_bytes);
+    p.row_units = row_bytes / unit;
+    p.layers_a_block = COMMIT_THREADS / (2 * p.row_units) > 1 ? COMMIT_THREADS / (2 * p.row_units) : 1;
+    if (unit == 16) return launch_commit<uint4>(p, stream);
+    if (unit == 8) return launch_commit<uint2>(p, stream);
+    if (unit == 4) return launch_commit<unsigned>(p, stream);
+    return launch_commit<unsigned short>(p, stream);
+}
+
+// caches [L, num_slots, Hkv, head_bytes]; mass, positions and their outputs [L, Hkv, num_slots] (the outputs may be the inputs).
+LLB_EXPORT int llb_cache_evict(void* k, void* v, const float* mass, const int* positions, float* mass_out, int* positions_out,
+                               const int* lengths, const int* ends, const int* table, int S, int L, int Hkv, int max_pages, int page_size,
+                               int num_slots, int head_bytes, int budget, int first, int latest, cudaStream_t stream) {
+    if (S == 0) return 0;
+    LLB_REQUIRE(S > 0 && L > 0 && L <= 65535 && Hkv > 0 && (long long)S * Hkv < (1ll << 31) && page_size > 0 && max_pages >= 0 && num_slots > 0 &&
+                head_bytes > 0 && head_bytes % 2 == 0, "cache_evict: bad sizes");
+    LLB_REQUIRE((long long)max_pages * page_size <= EV_MAX_PLACES, "cache_evict: a block table of %d pages of %d names more than %d places", max_pages,
+                page_size, EV_MAX_PLACES);
+    LLB_REQUIRE(budget > 0 && first >= 0 && latest >= 0 && (long long)first + latest <= budget,
+                "cache_evict: a budget of %d places does not hold the first %d and the latest %d", budget, first, latest);
+    EvictParams p;
+    p.k = (char*)k; p.v = (char*)v; p.mass = mass; p.positions = positions; p.mass_out = mass_out; p.positions_out = positions_out;
+    p.lengths = lengths; p.ends = ends; p.table = table; p.S = S; p.max_pages = max_pages; p.page_size = page_size; p.num_slots = num_slots;
+    p.Hkv = Hkv; p.budget = budget; p.first = first; p.latest = latest; p.cache_places = 0;
+    const int unit = unit_bytes(k, v, head_bytes);
+    p.head_units = head_bytes / unit;
+    if (unit == 16) return launch_evict<uint4>(p, L, stream);
+    if (unit == 8) return launch_evict<uint2>(p, L, stream);
+    if (unit == 4) return launch_evict<unsigned>(p, L, stream);
+    return launch_evict<unsigned short>(p, L, stream);
+}

@@ -17,7 +17,7 @@ from . import build as _build
 
 F32, BF16 = 0, 1
 EPI_STORE, EPI_STORE_F32, EPI_RESIDUAL, EPI_SWIGLU = 0, 1, 2, 3
-ABI_VERSION = 26
+ABI_VERSION = 27
 
 _lib: Optional[ctypes.CDLL] = None
 
@@ -1341,6 +1341,211 @@ def paged_decode_mma(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         max_pages, page_size, num_heads, num_kv_heads, head_dim, window, ctypes.c_float(scale),
         ctypes.c_float(softcap or 0.0), nsplit,
         _ptr(scratch), _ptr(sinks), cross, 1 if out.dtype == torch.float32 else 0, keep, _ptr(slopes), fresh, _stream()))
+
+
+# ---- a cache that is drafted into and thinned out (csrc/span_attention.cu, csrc/cache_rows.cu) ---------------------------
+def _check_here(what: str, *tensors) -> None:
+    """Every tensor contiguous and on the current device, which the launch goes to."""
+    first = tensors[0].get_device()
+    device = torch.cuda.current_device() if first >= 0 else 0
+    for t in tensors:
+        if t is not None and (t.get_device() != device or not t.is_contiguous()):
+            raise KernelError(f"{what}: a tensor of shape {tuple(t.shape)} on {t.device} must be contiguous and on cuda:{device}, "
+                              "the current device; there is no CPU path")
+
+
+def _check_spans(what: str, span_row, span_len, span_pos, block_table, page_size: int):
+    """(requests, pages a request) of a call over whole requests: the index arrays are int32 of one length."""
+    S = span_len.shape[0]
+    for t, shape in ((span_row, (S,)), (span_len, (S,)), (span_pos, (S,))):
+        if t is not None and (t.dtype != torch.int32 or t.shape != shape):
+            raise KernelError(f"{what}: the index arrays are int32 [{S}], got {t.dtype} {tuple(t.shape)}")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != S:
+        raise KernelError(f"{what}: block_table must be int32 [{S}, pages], got {block_table.dtype} {tuple(block_table.shape)}")
+    if page_size <= 0:
+        raise KernelError(f"{what}: page size {page_size}")
+    return S, block_table.shape[1]
+
+
+def _check_span_attention(what, q, k_cache, v_cache, out, num_heads, num_kv_heads, head_dim) -> int:
+    """The dtype code of an attention over whole requests, after the checks of its operands."""
+    T = q.shape[0]
+    if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
+        raise KernelError(f"{what}: {num_heads} query heads are not a multiple of {num_kv_heads} kv heads")
+    if q.numel() != T * num_heads * head_dim or out.shape != q.shape or out.dtype != q.dtype:
+        raise KernelError(f"{what}: q and out are [T, {num_heads * head_dim}] of one dtype, got {tuple(q.shape)} {q.dtype}, "
+                          f"{tuple(out.shape)} {out.dtype}")
+    shape = (k_cache.shape[0], num_kv_heads, head_dim)
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype or k_cache.shape != shape or v_cache.shape != shape:
+        raise KernelError(f"{what}: the caches are {q.dtype} [slots, {num_kv_heads}, {head_dim}], got {k_cache.dtype} "
+                          f"{tuple(k_cache.shape)}, {v_cache.dtype} {tuple(v_cache.shape)}")
+    return _dt(q)
+
+
+_span_scratch = {}
+
+
+def _span_scratch_floats(dt: int, T: int, S: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, num_slots: int,
+                         mass: int) -> int:
+    key = (dt, T, S, num_heads, num_kv_heads, head_dim, page_size, num_slots, mass, torch.cuda.current_device())
+    n = _span_scratch.get(key)
+    if n is None:
+        if len(_span_scratch) > 4096:
+            _span_scratch.clear()
+        n = _span_scratch[key] = int(lib().llb_span_scratch_floats(*key[:-1]))
+    return n
+
+
+def tree_mask(parents) -> torch.Tensor:
+    """The masks of drafted trees for :func:`tree_attention`, int64 [nodes, words] on the CPU: ``parents`` holds a sequence of
+    parents for every request, node 0 its root (-1), a parent always before its children.  A node sees itself and its ancestors."""
+    words = max([1] + [-(-len(p) // 64) for p in parents])
+    rows = []
+    for tree in parents:
+        seen = []
+        for i, up in enumerate(tree):
+            if (up != -1) if i == 0 else not 0 <= up < i:
+                raise ValueError(f"tree_mask: node {i} has the parent {up}; the root is node 0 (-1), other nodes follow their parent")
+            seen.append((1 << i) | (seen[up] if i else 0))
+        # words are unsigned; as signed numbers the upper half wraps around
+        rows += [[(((bits >> 64 * w) + (1 << 63)) & ((1 << 64) - 1)) - (1 << 63) for w in range(words)] for bits in seen]
+    return torch.tensor(rows, dtype=torch.int64).reshape(-1, words)
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, mask: torch.Tensor,
+                   span_row: torch.Tensor, span_len: torch.Tensor, span_pos: torch.Tensor, block_table: torch.Tensor,
+                   page_size: int, num_heads: int, num_kv_heads: int, head_dim: int, scale: float) -> None:
+    """Attention of the nodes of every request's tree of drafted tokens, one step that verifies all of them.
+
+    Request s brings the rows ``span_row[s] .. + span_len[s]`` of ``q`` (a row a node) behind ``span_pos[s]`` keys that it holds;
+    the keys and values of node i are in the cache at place ``span_pos[s] + i`` (:func:`rope_kv_write` puts them there, each with the
+    position of its depth).  A row sees the keys that its request holds and the nodes that ``mask`` names: bit ``j % 64`` of
+    ``mask[row, j // 64]`` stands for node j of the row's own request (:func:`tree_mask` makes ancestors' masks; a row's own bit
+    counts like any other; bits from ``span_len[s]`` on are ignored).  A row that sees nothing gets zeros.
+
+    q, out [T, heads * head_dim], caches [slots, kv heads, head_dim], all float32 or all bfloat16; mask int64 [T, words]; span arrays
+    int32 [requests], block_table int32 [requests, pages].  Nothing is read on the host: a captured graph serves other trees,
+    lengths and tables of the same sizes.  Rows of no request are left as they were."""
+    S, pages = _check_spans("tree_attention", span_row, span_len, span_pos, block_table, page_size)
+    dt = _check_span_attention("tree_attention", q, k_cache, v_cache, out, num_heads, num_kv_heads, head_dim)
+    T, slots = q.shape[0], k_cache.shape[0]
+    if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != T or mask.shape[1] == 0:
+        raise KernelError(f"tree_attention: mask must be int64 [{T}, words], got {mask.dtype} {tuple(mask.shape)}")
+    _check_here("tree_attention", q, k_cache, v_cache, out, mask, span_row, span_len, span_pos, block_table)
+    scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, slots, 0), dtype=torch.float32, device=q.device)
+    _check(lib().llb_tree_attention(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), dt, mask.data_ptr(), mask.shape[1], span_row.data_ptr(),
+        span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, pages, page_size, slots, num_heads, num_kv_heads,
+        head_dim, scale, scratch.data_ptr(), _stream()))
+
+
+def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, mass: torch.Tensor,
+                         span_row: torch.Tensor, span_len: torch.Tensor, span_pos: torch.Tensor, block_table: torch.Tensor,
+                         page_size: int, num_heads: int, num_kv_heads: int, head_dim: int, scale: float, max_len: int,
+                         mass_in: Optional[torch.Tensor] = None) -> None:
+    """Causal attention of every request's newest rows over all its keys that also counts the weight which every key receives:
+
+        mass[h, slot of key j] = (mass_in[h, slot of key j] if j < span_pos[s] else 0) + the sum of the softmax weights of key j over
+                                 the request's rows and kv head h's query heads
+
+    for every key of the requests that bring rows (:func:`cache_evict` goes by these sums).  ``mass_in`` may be ``mass`` itself
+    (sums go on from step to step; a new key starts from zero whatever an earlier owner left in its slot) or ``None`` (all start
+    from zero).  ``mass`` float32 [kv heads, slots].  ``max_len``: the most rows that a request brings (longer ones
+    are cut to it); 1 takes the form for single tokens, which reads every key once.  The other arguments as
+    :func:`tree_attention`.  Sums are made in one order: equal calls give equal bits."""
+    S, pages = _check_spans("paged_attention_mass", span_row, span_len, span_pos, block_table, page_size)
+    dt = _check_span_attention("paged_attention_mass", q, k_cache, v_cache, out, num_heads, num_kv_heads, head_dim)
+    T, slots = q.shape[0], k_cache.shape[0]
+    for t in (mass, mass_in):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (num_kv_heads, slots)):
+            raise KernelError(f"paged_attention_mass: weights are float32 [{num_kv_heads}, {slots}], got {t.dtype} {tuple(t.shape)}")
+    if max_len <= 0:
+        raise KernelError(f"paged_attention_mass: max_len is {max_len}")
+    _check_here("paged_attention_mass", q, k_cache, v_cache, out, mass, mass_in, span_row, span_len, span_pos, block_table)
+    scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, slots, 2 if max_len == 1 else 1),
+                          dtype=torch.float32, device=q.device)
+    _check(lib().llb_paged_attention_mass(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), dt, None if mass_in is None else mass_in.data_ptr(),
+        mass.data_ptr(), span_row.data_ptr(), span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, max_len, pages,
+        page_size, slots, num_heads, num_kv_heads, head_dim, scale, scratch.data_ptr(), _stream()))
+
+
+def _check_planes(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor):
+    """(layers, slots, kv heads, head size) of planes [slots, kv heads, head_dim] or [layers, slots, kv heads, head_dim]."""
+    if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype or k_cache.dim() not in (3, 4) or k_cache.numel() == 0:
+        raise KernelError(f"{what}: keys and values are [slots, kv heads, head_dim] or [layers, ...] of one shape and dtype, got "
+                          f"{tuple(k_cache.shape)} {k_cache.dtype}, {tuple(v_cache.shape)} {v_cache.dtype}")
+    _dt(k_cache)
+    if k_cache.data_ptr() == v_cache.data_ptr():
+        raise KernelError(f"{what}: keys and values must be planes of their own")
+    return (1, *k_cache.shape) if k_cache.dim() == 3 else tuple(k_cache.shape)
+
+
+def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, targets: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                span_row: torch.Tensor, span_len: torch.Tensor, span_pos: torch.Tensor, block_table: torch.Tensor, page_size: int,
+                path: torch.Tensor, count: torch.Tensor, next_token: torch.Tensor) -> None:
+    """Which drafted tokens the model confirms, and their keys and values moved to where the sequence goes on.
+
+    Node 0 of a request is its newest confirmed token; ``parents[row]`` is a node's parent (its number in the request, lower than
+    the node's own), ``tokens[row]`` the drafted token, ``targets[row]`` what the model chooses behind the node (:func:`argmax` of its logits).
+    From the root on, the first child whose token its parent's target names is confirmed:
+
+        path[s] = the confirmed nodes (0 first), -1 behind them;  count[s] = how many;  next_token[s] = the last one's target
+
+    (count 0 and next_token -1 where a request brings no rows; a path ends at its width).  The row of node ``path[s, d]`` moves from place
+    ``span_pos[s] + path[s, d]`` to ``span_pos[s] + d`` in every layer: the request then holds ``span_pos[s] + count[s]`` keys, what lies
+    behind them is left over.  tokens, parents, targets int32 [T]; caches [slots, kv heads, head_dim] or [layers, ...]; path int32
+    [requests, width], width up to 1,024; count, next_token int32 [requests]."""
+    S, pages = _check_spans("tree_commit", span_row, span_len, span_pos, block_table, page_size)
+    L, slots, heads, hd = _check_planes("tree_commit", k_cache, v_cache)
+    T = tokens.shape[0]
+    for t, shape in ((tokens, (T,)), (parents, (T,)), (targets, (T,)), (count, (S,)), (next_token, (S,))):
+        if t.dtype != torch.int32 or t.shape != shape:
+            raise KernelError(f"tree_commit: tokens, parents, targets are int32 [{T}], count and next_token int32 [{S}], got {t.dtype} {tuple(t.shape)}")
+    if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != S:
+        raise KernelError(f"tree_commit: path must be int32 [{S}, width], got {path.dtype} {tuple(path.shape)}")
+    _check_here("tree_commit", tokens, parents, targets, k_cache, v_cache, span_row, span_len, span_pos, block_table, path, count, next_token)
+    _check(lib().llb_tree_commit(
+        tokens.data_ptr(), parents.data_ptr(), targets.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), span_row.data_ptr(),
+        span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, L, pages, page_size, slots,
+        heads * hd * k_cache.element_size(), path.data_ptr(), path.shape[1], count.data_ptr(), next_token.data_ptr(), _stream()))
+
+
+def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor,
+                ends: torch.Tensor, block_table: torch.Tensor, page_size: int, budget: int, first: int, latest: int,
+                mass_out: Optional[torch.Tensor] = None, positions_out: Optional[torch.Tensor] = None) -> None:
+    """Every layer, request and kv head keeps the ``budget`` keys that are worth most, in the request's first ``budget`` places.
+
+    ``lengths[s]`` places are held; ``mass`` is the weight that each place's key has received (:func:`paged_attention_mass`),
+    ``positions`` its position in the sequence, ``ends[s]`` the position of the request's next token.  Places of the first ``first``
+    positions and of the ``latest`` latest ones stay in any case (``first + latest <= budget``), then those of the largest mass, of
+    equal ones the lowest place (NaN counts as the largest).  The i-th place below the budget that does not stay takes the key, value, mass and
+    position of the i-th place beyond it that does; all others stay where they are.  So the order of the places says nothing of the
+    keys' positions afterwards: for attention that does not go by it (no window, no bias by distance).  A request then holds
+    ``min(lengths[s], budget)`` places; one of no more than the budget is left as it is.
+
+    Caches [slots, kv heads, head_dim] or [layers, ...]; mass float32 and positions int32 [kv heads, slots] or [layers, ...];
+    lengths, ends int32 [requests].  ``mass_out`` and ``positions_out`` (both or neither): planes that receive the mass and position
+    of every place that is held afterwards, in the place of the planes that are read; nothing else in them is written."""
+    S, pages = _check_spans("cache_evict", ends, lengths, None, block_table, page_size)
+    L, slots, heads, hd = _check_planes("cache_evict", k_cache, v_cache)
+    shape = (heads, slots) if k_cache.dim() == 3 else (L, heads, slots)
+    if (mass_out is None) != (positions_out is None):
+        raise KernelError("cache_evict: mass_out and positions_out are given both or neither")
+    if mass_out is None:
+        mass_out, positions_out = mass, positions
+    elif (mass_out.data_ptr() == mass.data_ptr()) != (positions_out.data_ptr() == positions.data_ptr()):
+        raise KernelError("cache_evict: mass_out and positions_out are both the planes that are read, or neither is")
+    for t, dtype in ((mass, torch.float32), (mass_out, torch.float32), (positions, torch.int32), (positions_out, torch.int32)):
+        if t.dtype != dtype or t.shape != shape:
+            raise KernelError(f"cache_evict: mass is float32 and positions int32 {shape}, got {t.dtype} {tuple(t.shape)}")
+    if budget <= 0 or first < 0 or latest < 0 or first + latest > budget:
+        raise KernelError(f"cache_evict: a budget of {budget} places does not hold the first {first} and the latest {latest}")
+    _check_here("cache_evict", k_cache, v_cache, mass, positions, lengths, ends, block_table, mass_out, positions_out)
+    _check(lib().llb_cache_evict(
+        k_cache.data_ptr(), v_cache.data_ptr(), mass.data_ptr(), positions.data_ptr(), mass_out.data_ptr(), positions_out.data_ptr(),
+        lengths.data_ptr(), ends.data_ptr(), block_table.data_ptr(), S, L, heads, pages, page_size, slots, hd * k_cache.element_size(),
+        budget, first, latest, _stream()))
 
 
 # Where the blocks that share a long row of logits meet (a 64-bit slot and a counter per row), per device.

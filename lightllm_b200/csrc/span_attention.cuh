@@ -1,0 +1,150 @@
+// What the attention kernels over whole requests share (span_attention.cu, span_attention_tcgen05.cu): which rows see which keys,
+// how the work is cut among the blocks, and where partial results meet.
+//
+// A request (a span) brings `len` rows behind `pos` keys that it holds already; all of their keys and values are in the cache, at
+// the places 0 .. pos + len - 1 of its block table.  A row sees the `pos` keys and, of the keys of the rows it comes with,
+//   tree     those that its mask names (bit j of its words: the key of row j of its request), or
+//   causal   those up to its own.
+// The G query heads of a kv head read the same keys, so the rows of a job are (row, head of the group) pairs, G to a row: a job is
+// so many rows of one request and one kv head, over all key tiles that they see.  All jobs' tiles, one job after the other, make one
+// line that is cut into equal lengths, one a block, whatever the lengths of the requests are: no block waits for a longer one.
+// A job that a cut falls into leaves partial results (O, m, l), which a second kernel joins in the order of the blocks, so the
+// result does not depend on which block is first.  Everything is worked out on the device: a captured graph serves other lengths.
+#pragma once
+#include "common.cuh"
+
+struct LlbSpanArgs {
+    const int* span_row;             // [S]
+    const int* span_len;
+    const int* span_pos;
+    const int* table;                // [S, max_pages]
+    int S, T, max_pages, page_size, max_len, num_slots;
+    int Hq, Hkv, hd, group;
+    const unsigned long long* mask;  // tree: [T, words]; null: causal
+    int words;
+    float scale_log2e;               // scores are kept in base-2 units
+    void* out;                       // [T, Hq, hd]
+    float* lse;                      // [T, Hq] or null: log2 of the sum of 2^score; +infinity in a row that sees nothing
+    float* scores;                   // [Hq, num_slots] or null: the scores of requests of one row, by slot
+    float* part_o;                   // [2 * blocks, rows, hd]: what a block has of a job that began before it (0) and goes on after it (1)
+    float* part_ml;                  // [2 * blocks, rows, 2]
+    int* open;                       // [blocks, 4]: the job that begins in a block and goes on after it: request, first row, kv head, last block
+    int nodes;                       // rows of a request that a job holds at most
+    int rows;                        // nodes * group, rounded up: (row, head) pairs of a job in the partial results
+};
+
+struct LlbSpan {
+    int row, len, pos;
+};
+// What request s brings, held to what its arguments and the block table have room for.
+__device__ __forceinline__ LlbSpan llb_span(const LlbSpanArgs& a, int s) {
+    LlbSpan z;
+    z.row = a.span_row[s];
+    z.pos = max(a.span_pos[s], 0);
+    z.len = min(min(a.span_len[s], a.max_len), min(a.T - z.row, a.max_pages * a.page_size - z.pos));
+    if (z.row < 0 || z.len < 0) z.len = 0;
+    return z;
+}
+// How many keys the rows up to `upto` (of the request) see between them.
+__device__ __forceinline__ int llb_span_keys(const LlbSpanArgs& a, const LlbSpan& z, int upto) {
+    return z.pos + (a.mask ? z.len : min(z.len, upto));
+}
+// The cache row of a key, or -1 for a page that is none of the cache's: such a key reads as zeros.
+__device__ __forceinline__ int llb_span_slot(const LlbSpanArgs& a, int s, int key) {
+    const int page = a.table[(size_t)s * a.max_pages + key / a.page_size];
+    const long long slot = (long long)page * a.page_size + key % a.page_size;
+    return page >= 0 && slot < a.num_slots ? (int)slot : -1;
+}
+
+// A job and its tiles' place in the line of all tiles.
+struct LlbJob {
+    LlbSpan z;
+    int s, first, kvh;       // first: its first row in its request
+    int keys, tiles, begin;  // begin: of its first tile in the line
+    __device__ __forceinline__ void measure(const LlbSpanArgs& a, int tile) {
+        keys = llb_span_keys(a, z, first + a.nodes);
+        tiles = (keys + tile - 1) / tile;
+    }
+    __device__ __forceinline__ int count(const LlbSpanArgs& a) const { return min(a.nodes, z.len - first); }
+    // the next job of the line (there is one)
+    __device__ __forceinline__ void next(const LlbSpanArgs& a, int tile) {
+        begin += tiles;
+        if (++kvh < a.Hkv) return;
+        kvh = 0;
+        first += a.nodes;
+        while (first >= z.len) {
+            ++s;
+            z = llb_span(a, s);
+            first = 0;
+        }
+        measure(a, tile);
+    }
+};
+// A block's piece of the line: tiles [t0, t1), the job that t0 lies in; `blocks` of the grid have a piece.
+struct LlbPiece {
+    int t0, t1, total, blocks;
+    LlbJob job;
+};
+__device__ __forceinline__ int llb_span_tiles(const LlbSpanArgs& a, const LlbSpan& z, int tile) {
+    int n = 0;
+    if (z.len > 0 && a.mask) n = (z.len + a.nodes - 1) / a.nodes * ((z.pos + z.len + tile - 1) / tile);
+    else
+        for (int c = 0; c < z.len; c += a.nodes) n += (llb_span_keys(a, z, c + a.nodes) + tile - 1) / tile;
+    return n * a.Hkv;
+}
+// By one whole warp; every lane gets the answer.  A block has `least` tiles or more where there are enough.
+__device__ __forceinline__ LlbPiece llb_piece(const LlbSpanArgs& a, int tile, int block, int grid, int least, int lane) {
+    LlbPiece p;
+    int mine = 0;
+    p.total = 0;
+    for (int base = 0; base < a.S; base += 32) {
+        mine = base + lane < a.S ? llb_span_tiles(a, llb_span(a, base + lane), tile) : 0;
+        p.total += __reduce_add_sync(0xffffffffu, mine);
+    }
+    p.blocks = min(grid, (p.total + least - 1) / least);
+    p.t0 = p.t1 = 0;
+    if (block >= p.blocks) return p;
+    p.t0 = (int)((long long)p.total * block / p.blocks);
+    p.t1 = (int)((long long)p.total * (block + 1) / p.blocks);
+    int before = 0;
+    for (int base = 0; base < a.S; base += 32) {
+        if (a.S > 32) mine = base + lane < a.S ? llb_span_tiles(a, llb_span(a, base + lane), tile) : 0;
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, before + sum > p.t0);
+        if (past) {
+            const int at = __ffs(past) - 1;
+            p.job.s = base + at;
+            p.job.begin = before + __shfl_sync(0xffffffffu, sum - mine, at);
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    p.job.z = llb_span(a, p.job.s);
+    p.job.first = 0;
+    for (;;) {
+        p.job.measure(a, tile);
+        if (p.t0 < p.job.begin + p.job.tiles * a.Hkv) break;
+        p.job.begin += p.job.tiles * a.Hkv;
+        p.job.first += a.nodes;
+    }
+    p.job.kvh = (p.t0 - p.job.begin) / p.job.tiles;
+    p.job.begin += p.job.kvh * p.job.tiles;
+    return p;
+}
+// Which block has tile t of the line.
+__device__ __forceinline__ int llb_piece_owner(const LlbPiece& p, int t) {
+    return (int)(((long long)(t + 1) * p.blocks + p.total - 1) / p.total) - 1;
+}
+// Where a job's partial result goes when the block [t0, t1) has not all of it: 0 or 1, or -1 when it has.
+__device__ __forceinline__ int llb_part_of(const LlbPiece& p, const LlbJob& j) {
+    if (j.begin < p.t0) return 0;
+    return j.begin + j.tiles > p.t1 ? 1 : -1;
+}
+
+// Joins the partial results of cut jobs and writes their rows (and lse); `blocks` is the grid of the attention kernel.
+int llb_span_merge(const LlbSpanArgs& a, int dtype, int blocks, cudaStream_t stream);

@@ -1,0 +1,562 @@
+"""Attention of drafted trees, their commit, attention that counts keys' weights and eviction, against plain forms in 64 bits."""
+import math
+import random
+
+import pytest
+import torch
+
+from tests.plain import draft_cache_plain as P
+
+pytestmark = pytest.mark.gpu
+HEADS = [(14, 2, 64), (12, 2, 128), (28, 4, 128), (4, 2, 16), (3, 1, 32), (8, 8, 64), (16, 1, 128), (5, 1, 20), (2, 1, 256), (64, 1, 64)]
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from lightllm_b200.csrc import ops as o
+    o.lib()
+    return o
+
+
+def dev():
+    return torch.device("cuda:0")
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=dev())
+
+
+class Requests:
+    """Requests of ``held`` keys and ``rows`` new rows each in shuffled pages; what no request owns is NaN, and rows of no request lie
+    between the requests' rows."""
+
+    def __init__(self, held, rows, heads, dtype, page, seed, gap=1):
+        self.held, self.rows, self.page, self.dtype = held, rows, page, dtype
+        self.hq, self.hkv, self.hd = heads
+        g = torch.Generator().manual_seed(seed)
+        S = len(held)
+        need = [-(-(h + n) // page) for h, n in zip(held, rows)]
+        pages = sum(need) + 3
+        order = torch.randperm(pages, generator=g).tolist()
+        width = max(need + [1]) + 1
+        table, at = [], 0
+        for n in need:
+            table.append(order[at:at + n] + [-1] * (width - n))
+            at += n
+        self.table = table
+        self.slots = [[table[s][j // page] * page + j % page for j in range(held[s] + rows[s])] for s in range(S)]
+        self.num_slots = pages * page
+        self.k, self.v = (torch.full((self.num_slots, self.hkv, self.hd), math.nan) for _ in range(2))
+        for s in range(S):
+            for c in (self.k, self.v):
+                c[self.slots[s]] = torch.randn((len(self.slots[s]), self.hkv, self.hd), generator=g)
+        self.first = [sum(rows[:s]) + gap * (s + 1) for s in range(S)]
+        self.T = sum(rows) + gap * (S + 1)
+        self.q = torch.randn((self.T, self.hq, self.hd), generator=g)
+        self.k, self.v, self.q = (x.to(dtype) for x in (self.k, self.v, self.q))
+        self.scale = self.hd ** -0.5
+
+    def spans(self):
+        return i32(self.first), i32(self.rows), i32(self.held), i32(self.table).reshape(len(self.held), -1)
+
+    def args(self):
+        return (*self.spans(), self.page, self.hq, self.hkv, self.hd, self.scale)
+
+    def of(self, s):
+        return self.q[self.first[s]:self.first[s] + self.rows[s]], self.k[self.slots[s]], self.v[self.slots[s]]
+
+    def tolerance(self, s, want):
+        """Scores are off by score_error, and so (twice: in the weight and in the sum) are weights in proportion; sums of so many weights
+        by half a step of 32 bits a term at most; with bf16 every weight is rounded for the product with the values, and the result."""
+        q, k, v = self.of(s)
+        rel = 2 * P.score_error(q, k, self.scale) + (len(self.slots[s]) + 8) * 2.0 ** -24 + 2.0 ** -21
+        top = float(v.double().abs().nan_to_num(0.0, 0.0, 0.0).max()) if v.numel() else 0.0
+        if self.dtype == torch.bfloat16:
+            return (rel + 2.0 ** -8) * top + 2.0 ** -8 * want.abs()
+        return rel * top + 2.0 ** -24 * want.abs()
+
+
+def trees(rng, rows):
+    return [[-1] + [rng.randrange(max(0, i - 5), i) for i in range(1, n)] if n else [] for n in rows]
+
+
+def run_tree(ops, r, mask):
+    out = torch.full((r.T, r.hq * r.hd), 7.0, dtype=r.dtype, device=dev())
+    ops.tree_attention(r.q.reshape(r.T, -1).to(dev()), r.k.to(dev()), r.v.to(dev()), out, mask.to(dev()), *r.args())
+    ops.check_async_errors(dev())
+    return out.cpu().reshape(r.T, r.hq, r.hd)
+
+
+def check_rows(r, got, sees):
+    """All rows of all requests, and that rows of no request were left alone."""
+    mine = torch.zeros(r.T, dtype=torch.bool)
+    for s, n in enumerate(r.rows):
+        if not n:
+            continue
+        q, k, v = r.of(s)
+        want, _ = P.attention(q, k, v, sees[s], r.scale)
+        rows = got[r.first[s]:r.first[s] + n].double()
+        mine[r.first[s]:r.first[s] + n] = True
+        assert torch.equal(rows.isfinite(), want.isfinite())
+        off = (rows - want).abs() - r.tolerance(s, want)
+        off = off[want.isfinite()]
+        assert not off.numel() or float(off.max()) <= 0, (s, float(off.max()))
+    assert bool((got[~mine] == 7.0).all())
+
+
+def tree_sees(r, mask):
+    sees = []
+    for s, n in enumerate(r.rows):
+        bits = torch.ones((n, r.held[s] + n), dtype=torch.bool)
+        for i in range(n):
+            for j in range(n):
+                bits[i, r.held[s] + j] = j // 64 < mask.shape[1] and bool((int(mask[r.first[s] + i, j // 64]) >> (j % 64)) & 1)
+        sees.append(bits)
+    return sees
+
+
+def spread_mask(ops, r, parents):
+    m = ops.tree_mask(parents)
+    mask = torch.full((r.T, m.shape[1]), -1, dtype=torch.int64)
+    at = 0
+    for s, n in enumerate(r.rows):
+        mask[r.first[s]:r.first[s] + n] = m[at:at + n]
+        at += n
+    return mask
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("page", [8, 16])
+def test_trees_of_many_sizes(ops, dtype, heads, page):
+    """Requests of no keys and of many, trees of one node to more than a mask's word, a request without rows among them."""
+    rng = random.Random(3)
+    held = [0, 1, 63, 64, 65, 127, 128, 300, 17, 1000]
+    rows = [5, 1, 19, 37, 2, 9, 64, 0, 70, 3]
+    r = Requests(held, rows, heads, dtype, page, 11)
+    mask = spread_mask(ops, r, trees(rng, rows))
+    check_rows(r, run_tree(ops, r, mask), tree_sees(r, mask))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (12, 2, 128), (3, 1, 32)], ids=str)
+@pytest.mark.parametrize("held", [1, 127, 129, 2000, 5003])
+@pytest.mark.parametrize("n", [1, 8, 21, 64])
+def test_one_request(ops, dtype, heads, held, n):
+    """A single request's keys are shared by all blocks."""
+    r = Requests([held], [n], heads, dtype, 16, 12, gap=0)
+    mask = spread_mask(ops, r, trees(random.Random(held + n), [n]))
+    check_rows(r, run_tree(ops, r, mask), tree_sees(r, mask))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (12, 2, 128), (3, 1, 32)], ids=str)
+def test_any_mask(ops, dtype, heads):
+    """Masks that are no trees: random bits (those beyond the request's nodes among them), rows that see no drafted node and, in
+    requests that hold no keys, nothing at all: zeros."""
+    g = torch.Generator().manual_seed(5)
+    held, rows = [0, 0, 40, 130], [3, 66, 30, 90]
+    r = Requests(held, rows, heads, dtype, 16, 13)
+    mask = torch.randint(-2 ** 63, 2 ** 63 - 1, (r.T, 3), generator=g)
+    mask[::3] = 0
+    got, sees = run_tree(ops, r, mask), tree_sees(r, mask)
+    check_rows(r, got, sees)
+    empty = [r.first[s] + i for s in (0, 1) for i in range(rows[s]) if not sees[s][i].any()]
+    assert empty and bool((got[empty] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (12, 2, 128), (3, 1, 32)], ids=str)
+@pytest.mark.parametrize("held", [0, 50, 1000])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_what_is_masked_is_nothing(ops, dtype, heads, held, bad):
+    """A node's keys or values that are no finite numbers show in the rows that see it and in no others."""
+    r = Requests([held, 9], [40, 6], heads, dtype, 16, 14)
+    parents = trees(random.Random(8), r.rows)
+    mask = spread_mask(ops, r, parents)
+    r.v[r.slots[0][held + 7], 0, 3] = bad
+    r.v[r.slots[0][held + 31], :, :] = bad
+    if bad != math.inf:
+        r.k[r.slots[0][held + 22], 0, :] = math.nan
+    got, sees = run_tree(ops, r, mask), tree_sees(r, mask)
+    assert not sees[0][:, held + 7].all() and not sees[0][:, held + 22].all()
+    check_rows(r, got, sees)
+
+
+def test_keys_whose_scores_stand_out(ops):
+    """The running maximum rises late and by much, in the last tile and among the drafted nodes."""
+    for dtype in DTYPES:
+        for heads in ((14, 2, 64), (12, 2, 128)):
+            r = Requests([700, 1500], [20, 3], heads, dtype, 16, 15)
+            for s in range(2):
+                for j, x in ((100, 4.0), (650, 9.0), (r.held[s], 14.0)):
+                    r.k[r.slots[s][j]] = x * torch.sign(r.q[r.first[s], 0]).to(dtype)
+            mask = spread_mask(ops, r, trees(random.Random(9), r.rows))
+            check_rows(r, run_tree(ops, r, mask), tree_sees(r, mask))
+
+
+def run_mass(ops, r, mass_in, max_len=None, in_place=False):
+    out = torch.full((r.T, r.hq * r.hd), 7.0, dtype=r.dtype, device=dev())
+    mass = mass_in.to(dev()) if in_place else torch.full((r.hkv, r.num_slots), -5.0, device=dev())
+    given = mass if in_place else None if mass_in is None else mass_in.to(dev())
+    ops.paged_attention_mass(r.q.reshape(r.T, -1).to(dev()), r.k.to(dev()), r.v.to(dev()), out, mass, *r.args(),
+                             max(r.rows) if max_len is None else max_len, mass_in=given)
+    ops.check_async_errors(dev())
+    return out.cpu().reshape(r.T, r.hq, r.hd), mass.cpu()
+
+
+def check_mass(r, got, mass, mass_in, left):
+    sees = [torch.cat([torch.ones((n, h), dtype=torch.bool), torch.ones((n, n), dtype=torch.bool).tril()], 1) for h, n in zip(r.held, r.rows)]
+    check_rows(r, got, sees)
+    touched = torch.zeros(r.num_slots, dtype=torch.bool)
+    for s, n in enumerate(r.rows):
+        if not n:
+            continue
+        q, k, v = r.of(s)
+        _, w = P.attention(q, k, v, sees[s], r.scale)
+        sums = w.reshape(r.hkv, -1, w.shape[-1]).sum(1)
+        before = torch.zeros_like(sums)
+        if mass_in is not None:
+            before[:, :r.held[s]] = mass_in[:, r.slots[s][:r.held[s]]].double()
+        have = mass[:, r.slots[s]].double()
+        # a weight's score and its row's sum are off by score_error each; the exponential, the logarithm and so many additions by half
+        # a step or a few of 32 bits
+        rel = 2 * P.score_error(q, k, r.scale) + (n * r.hq // r.hkv + len(r.slots[s]) + 16) * 2.0 ** -24 + 2.0 ** -20
+        assert bool(((have - before - sums).abs() <= rel * sums + 2.0 ** -23 * before.abs()).all()), (s, float((have - before - sums).abs().max()))
+        touched[r.slots[s]] = True
+    assert torch.equal(mass[:, ~touched], left[:, ~touched])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("rows", ["single", "portions"])
+def test_mass(ops, dtype, heads, rows):
+    """One token of every request, and portions of several lengths beside single tokens, onto sums of before."""
+    held = [0, 1, 15, 63, 64, 127, 128, 333, 1500]
+    n = [1] * len(held) if rows == "single" else [7, 1, 130, 20, 64, 1, 3, 0, 40]
+    r = Requests(held, n, heads, dtype, 16, 21)
+    mass_in = torch.rand((r.hkv, r.num_slots), generator=torch.Generator().manual_seed(22))
+    left = torch.full_like(mass_in, -5.0)
+    got, mass = run_mass(ops, r, mass_in)
+    check_mass(r, got, mass, mass_in, left)
+    again, mass2 = run_mass(ops, r, mass_in.clone(), in_place=True)
+    check_mass(r, again, mass2, mass_in, mass_in)
+    assert torch.equal(got, again)
+    got, mass = run_mass(ops, r, None)
+    check_mass(r, got, mass, None, left)
+    # a longer most than any request has is no other result
+    got2, mass3 = run_mass(ops, r, None, max_len=max(n) + 70)
+    check_mass(r, got2, mass3, None, left)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (12, 2, 128), (3, 1, 32)], ids=str)
+@pytest.mark.parametrize("held,n", [(0, 1), (5000, 1), (0, 300), (250, 257), (3000, 2)])
+def test_mass_of_one_request(ops, dtype, heads, held, n):
+    r = Requests([held], [n], heads, dtype, 8, 23, gap=0)
+    mass_in = torch.rand((r.hkv, r.num_slots), generator=torch.Generator().manual_seed(24))
+    got, mass = run_mass(ops, r, mass_in)
+    check_mass(r, got, mass, mass_in, torch.full_like(mass_in, -5.0))
+
+
+def test_mass_sums_to_the_rows(ops):
+    """Every row's weights add up to one: all keys' together to rows times the group."""
+    r = Requests([100, 2000], [77, 1], (14, 2, 64), torch.bfloat16, 16, 25)
+    _, mass = run_mass(ops, r, None)
+    for s, n in enumerate(r.rows):
+        assert torch.allclose(mass[:, r.slots[s]].double().sum(1), torch.full((2,), 7.0 * n, dtype=torch.float64), rtol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (4, 2, 16), (3, 1, 5), (28, 4, 128)], ids=str)
+@pytest.mark.parametrize("layers", [0, 1, 5])
+def test_commit(ops, dtype, heads, layers):
+    """Paths of all lengths, several children with the right token (the first goes on), requests without rows, a width that cuts."""
+    rng = random.Random(31)
+    held = [0, 5, 16, 31, 100, 7, 64]
+    rows = [1, 9, 40, 0, 70, 26, 3]
+    r = Requests(held, rows, heads, dtype, 16, 32)
+    parents = trees(rng, rows)
+    for width in (1, 4, 70):
+        tokens = [[rng.randrange(4) for _ in t] for t in parents]
+        targets = [[rng.randrange(4) for _ in t] for t in parents]
+        for t, k, g in zip(parents, tokens, targets):          # most nodes go on
+            for i in range(1, len(t)):
+                if rng.random() < 0.5:
+                    g[t[i]] = k[i]
+        flat = [torch.full((r.T,), 99, dtype=torch.int32) for _ in range(3)]
+        for x, lists in zip(flat, (tokens, parents, targets)):
+            for s, v in enumerate(lists):
+                x[r.first[s]:r.first[s] + rows[s]] = torch.tensor(v, dtype=torch.int32)
+        shape = ((layers,) if layers else ()) + tuple(r.k.shape)
+        g = torch.Generator().manual_seed(33)
+        k, v = (torch.randn(shape, generator=g).to(dtype) for _ in range(2))
+        kd, vd = k.to(dev()), v.to(dev())
+        path = torch.full((len(held), width), 5, dtype=torch.int32, device=dev())
+        count, nxt = i32([9] * len(held)), i32([9] * len(held))
+        ops.tree_commit(*(x.to(dev()) for x in flat), kd, vd, *r.spans(), r.page, path, count, nxt)
+        for s in range(len(held)):
+            want, last = P.commit(tokens[s], parents[s], targets[s], width)
+            assert path[s].tolist() == want + [-1] * (width - len(want))
+            assert int(count[s]) == len(want) and int(nxt[s]) == last
+            src = [r.slots[s][held[s] + a] for a in want]
+            dst = [r.slots[s][held[s] + d] for d in range(len(want))]
+            for c in (k, v):
+                c[..., dst, :, :] = c[..., src, :, :].clone()
+        assert torch.equal(kd.cpu(), k) and torch.equal(vd.cpu(), v)
+
+
+def evict_case(held, heads, dtype, page, layers, seed, ties=False):
+    g = torch.Generator().manual_seed(seed)
+    r = Requests(held, [0] * len(held), heads, torch.float32, page, seed)
+    L = max(1, layers)
+    k, v = (torch.randn((L, r.num_slots, r.hkv, r.hd), generator=g).to(dtype) for _ in range(2))
+    mass = torch.exp(2.0 * torch.randn((L, r.hkv, r.num_slots), generator=g))
+    if ties:
+        mass = torch.randint(0, 5, mass.shape, generator=g).float() * torch.where(torch.rand(mass.shape, generator=g) < 0.1, -1.0, 1.0)
+        mass[torch.rand(mass.shape, generator=g) < 0.02] = math.nan
+        mass[torch.rand(mass.shape, generator=g) < 0.02] = math.inf
+        mass[torch.rand(mass.shape, generator=g) < 0.02] = -math.inf
+    pos = torch.zeros((L, r.hkv, r.num_slots), dtype=torch.int32)
+    for s, n in enumerate(held):
+        for l in range(L):
+            for h in range(r.hkv):
+                pos[l, h, r.slots[s]] = torch.randperm(n + 20, generator=g)[:n].to(torch.int32)
+    return r, k, v, mass, pos, [n + 20 for n in held]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (4, 2, 16), (3, 1, 5)], ids=str)
+@pytest.mark.parametrize("held,budget,first,latest", [
+    ([33, 5, 200, 1, 0, 64], 32, 4, 8), ([129, 128, 127, 130], 128, 0, 0), ([1, 2, 3], 1, 0, 1), ([3000, 77, 2500], 1000, 4, 128),
+    ([500], 499, 0, 0), ([700, 20], 10, 3, 7), ([4097], 2048, 100, 100)])
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("ties", [False, True])
+def test_evict(ops, dtype, heads, held, budget, first, latest, apart, ties):
+    """One place and many, equal worths, budgets that are all first and latest places, in place and into other planes."""
+    layers = 2 if len(held) > 1 else 0
+    r, k, v, mass, pos, ends = evict_case(held, heads, dtype, 16, layers, 41, ties)
+    pick = (lambda x: x) if layers else (lambda x: x[0])
+    kd, vd, md, pd = (pick(x).contiguous().to(dev()) for x in (k, v, mass, pos))
+    mo, po = (torch.full_like(md, -3.0), torch.full_like(pd, -3)) if apart else (None, None)
+    ops.cache_evict(kd, vd, md, pd, i32(held), i32(ends), r.spans()[3], r.page, budget, first, latest, mass_out=mo, positions_out=po)
+    want_m, want_p = (torch.full_like(mass, -3.0), torch.full_like(pos, -3)) if apart else (mass.clone(), pos.clone())
+    before_m, before_p = mass.clone(), pos.clone()
+    for l in range(mass.shape[0]):
+        for h in range(r.hkv):
+            for s, n in enumerate(held):
+                at = r.slots[s]
+                moves = P.evict(before_m[l, h, at].tolist(), before_p[l, h, at].tolist(), ends[s], budget, first, latest)
+                stay = at[:min(n, budget)]
+                want_m[l, h, stay], want_p[l, h, stay] = before_m[l, h, stay], before_p[l, h, stay]
+                for hole, filler in moves:
+                    a, b = at[hole], at[filler]
+                    k[l, a, h], v[l, a, h] = k[l, b, h].clone(), v[l, b, h].clone()
+                    want_m[l, h, a], want_p[l, h, a] = before_m[l, h, b], before_p[l, h, b]
+    assert torch.equal(kd.cpu(), pick(k)) and torch.equal(vd.cpu(), pick(v))
+    for got, want in (((mo if apart else md).cpu(), pick(want_m)), ((po if apart else pd).cpu(), pick(want_p))):
+        assert torch.equal(got.nan_to_num(1e30, 2e30, -2e30) if got.is_floating_point() else got,
+                           want.nan_to_num(1e30, 2e30, -2e30) if want.is_floating_point() else want)
+    if apart:
+        assert torch.equal(pd.cpu(), pick(pos))
+
+
+def test_evict_more_places_than_shared_memory_holds(ops):
+    held = [30000, 20001]
+    r, k, v, mass, pos, ends = evict_case(held, (2, 1, 4), torch.float32, 16, 1, 42)
+    kd, vd, md, pd = (x.to(dev()) for x in (k, v, mass, pos))
+    ops.cache_evict(kd, vd, md, pd, i32(held), i32(ends), r.spans()[3], r.page, 9000, 4, 500)
+    for s in range(2):
+        at = r.slots[s]
+        for hole, filler in P.evict(mass[0, 0, at].tolist(), pos[0, 0, at].tolist(), ends[s], 9000, 4, 500):
+            for c in (k, v):
+                c[0, at[hole]] = c[0, at[filler]].clone()
+            mass[0, 0, at[hole]], pos[0, 0, at[hole]] = mass[0, 0, at[filler]].clone(), pos[0, 0, at[filler]].clone()
+    for got, want in ((kd, k), (vd, v), (md, mass), (pd, pos)):
+        assert torch.equal(got.cpu(), want)
+
+
+def test_pages_outside_the_cache(ops):
+    """A table that names no page of the cache inside a request: its keys read as zeros, its rows are not moved and not written."""
+    for dtype in DTYPES:
+        r = Requests([100], [9], (4, 2, 64), dtype, 16, 51)
+        r.k[r.slots[0][32:48]], r.v[r.slots[0][32:48]] = 0, 0
+        for page in (-1, 10 ** 6, 2 ** 31 - 1):
+            r.table[0][2] = page
+            mask = spread_mask(ops, r, trees(random.Random(1), r.rows))
+            check_rows(r, run_tree(ops, r, mask), tree_sees(r, mask))
+            got, mass = run_mass(ops, r, None)
+            assert bool((mass[:, r.slots[0][32:48]] == -5.0).all())
+            kd, vd = r.k.to(dev()), r.v.to(dev())
+            md, pd = torch.rand((2, r.num_slots), device=dev()), torch.zeros((2, r.num_slots), dtype=torch.int32, device=dev())
+            keep = kd[r.slots[0][32:48]].clone()
+            ops.cache_evict(kd, vd, md, pd, i32([100]), i32([200]), r.spans()[3], 16, 40, 0, 0)
+            assert torch.equal(kd[r.slots[0][32:48]], keep)
+
+
+def test_captured(ops):
+    """One graph of all four, replayed for other trees, lengths and tables of the same sizes, on a stream of its own; eager calls of the
+    same operators run between the replays."""
+    heads, page, dtype = (14, 2, 64), 16, torch.bfloat16
+    rng = random.Random(61)
+    cases = []
+    for seed in range(3):
+        rows = [rng.randrange(1, 9) for _ in range(3)]
+        rows.append(20 - sum(rows) if 0 < 20 - sum(rows) < 9 else 1)
+        held = [rng.randrange(0, 300) for _ in rows]
+        cases.append((held, rows))
+    T, slots, width = 40, 100 * page, 24
+    z = lambda *s, d=torch.int32: torch.zeros(s, dtype=d, device=dev())  # noqa: E731
+    q, k, v = (torch.randn(s, device=dev()).to(dtype) for s in ((T, 14 * 64), (slots, 2, 64), (slots, 2, 64)))
+    row, length, held_d, table, mask = z(4), z(4), z(4), z(4, width), z(T, 1, d=torch.int64)
+    tokens, parents, targets, path, count, nxt = z(T), z(T), z(T), z(4, 9), z(4), z(4)
+    out, out2, mass, pos, ends = torch.zeros_like(q), torch.zeros_like(q), z(2, slots, d=torch.float32), z(2, slots), z(4)
+    k2, v2, mass2, pos2 = (torch.empty_like(x) for x in (k, v, mass, pos))
+
+    def step():
+        ops.tree_attention(q, k, v, out, mask, row, length, held_d, table, page, *heads, 0.125)
+        ops.paged_attention_mass(q, k, v, out2, mass, row, length, held_d, table, page, *heads, 0.125, 9)
+        k2.copy_(k), v2.copy_(v)
+        ops.tree_commit(tokens, parents, targets, k2, v2, row, length, held_d, table, page, path, count, nxt)
+        ops.cache_evict(k2, v2, mass, pos, held_d, ends, table, page, 64, 2, 16, mass_out=mass2, positions_out=pos2)
+
+    def load(case, seed):
+        held, rows = case
+        g = torch.Generator().manual_seed(seed)
+        order = torch.randperm(100, generator=g).tolist()
+        t, at = [], 0
+        for h, n in zip(held, rows):
+            need = -(-(h + n) // page)
+            t.append(order[at:at + need] + [-1] * (width - need))
+            at += need
+        row.copy_(i32([sum(rows[:s]) for s in range(4)])), length.copy_(i32(rows)), held_d.copy_(i32(held)), table.copy_(i32(t))
+        parent = trees(random.Random(seed), rows)
+        m = ops.tree_mask(parent)
+        mask[:m.shape[0]] = m.to(dev())
+        flat = [p for t in parent for p in t]
+        parents[:len(flat)] = i32(flat)
+        tokens.copy_(torch.randint(0, 2, (T,), generator=g)), targets.copy_(torch.randint(0, 2, (T,), generator=g))
+        pos.copy_(torch.randint(0, 400, pos.shape, generator=g)), ends.copy_(i32([h + 30 for h in held]))
+
+    def results():
+        torch.cuda.synchronize()
+        return [x.clone() for x in (out, out2, mass, k2, v2, path, count, nxt)]
+
+    def clear():
+        for x in (out, out2, mass, k2, v2, path, count, nxt, mass2, pos2):
+            x.zero_()
+
+    load(cases[0], 70)
+    step()
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for i, case in enumerate(cases * 2):
+        load(case, 71 + i)
+        clear()
+        step()
+        want = results()
+        clear()
+        graph.replay()
+        got = results()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    ops.check_async_errors(dev())
+
+
+def test_a_run_of_them(ops):
+    """Requests as they would be served, one layer: a prompt with its keys' weights, then steps that draft a tree, attend to it, confirm a
+    path, and thin the cache to a budget; the plain forms go the same way beside it."""
+    hq, hkv, hd, page, dtype, budget = 14, 2, 64, 16, torch.float32, 96
+    g, rng = torch.Generator().manual_seed(81), random.Random(81)
+    S, width, slots = 3, 12, 40 * page
+    order = torch.randperm(36, generator=g).tolist()
+    table = [order[s * width:(s + 1) * width] for s in range(S)]
+    slot = lambda s, j: table[s][j // page] * page + j % page  # noqa: E731
+    kc, vc = (torch.full((slots, hkv, hd), math.nan, device=dev()) for _ in range(2))
+    mass, pos = torch.full((hkv, slots), math.nan, device=dev()), torch.zeros((hkv, slots), dtype=torch.int32, device=dev())
+    rn = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    lens = [140, 40, 97]
+    # what each request holds, in its places' order, for the plain side: lists per kv head of (key, value, mass, position)
+    plain = [[[] for _ in range(hkv)] for _ in range(S)]
+    held, ends = [0] * S, [0] * S
+
+    def bring(rows):
+        q, k, v = (rn(sum(rows), h, hd) for h in (hq, hkv, hkv))
+        first = [sum(rows[:s]) for s in range(S)]
+        for s in range(S):
+            for i in range(rows[s]):
+                kc[slot(s, held[s] + i)], vc[slot(s, held[s] + i)] = k[first[s] + i].to(dev()), v[first[s] + i].to(dev())
+        return q, k, v, first
+
+    def plain_rows(s, q, k, v, sees):
+        out, weights = [], []
+        for h in range(hkv):
+            pk = torch.stack([e[0] for e in plain[s][h]] + list(k[:, h])) if plain[s][h] else k[:, h]
+            pv = torch.stack([e[1] for e in plain[s][h]] + list(v[:, h])) if plain[s][h] else v[:, h]
+            o, w = P.attention(q[:, h * 7:(h + 1) * 7], pk[:, None], pv[:, None], sees, hd ** -0.5)
+            out.append(o)
+            weights.append(w.sum((0, 1)))
+        return torch.cat(out, 1), weights
+
+    rows = lens
+    for step in range(5):
+        q, k, v, first = bring(rows)
+        out = torch.zeros((sum(rows), hq * hd), device=dev())
+        spans = (i32(first), i32(rows), i32(held), i32(table))
+        if step % 2 == 0:          # a portion, or one token each
+            ops.paged_attention_mass(q.reshape(-1, hq * hd).to(dev()), kc, vc, out, mass, *spans, page, hq, hkv, hd, hd ** -0.5, max(rows), mass_in=mass)
+            for s, n in enumerate(rows):
+                sees = torch.cat([torch.ones((n, held[s]), dtype=torch.bool), torch.ones((n, n), dtype=torch.bool).tril()], 1)
+                a = slice(first[s], first[s] + n)
+                want, w = plain_rows(s, q[a], k[a], v[a], sees)
+                assert torch.allclose(out[a].cpu().double().reshape(n, hq, hd), want, atol=2e-5)
+                for h in range(hkv):
+                    for j, e in enumerate(plain[s][h]):
+                        e[2] += float(w[h][j])
+                    for i in range(n):
+                        plain[s][h].append([k[first[s] + i, h], v[first[s] + i, h], float(w[h][held[s] + i]), ends[s] + i])
+                for i in range(n):
+                    pos[:, slot(s, held[s] + i)] = ends[s] + i
+            held, ends = [h + n for h, n in zip(held, rows)], [e + n for e, n in zip(ends, rows)]
+            for s in range(S):
+                have = mass[:, [slot(s, j) for j in range(held[s])]].cpu().double()
+                want = torch.tensor([[e[2] for e in plain[s][h]] for h in range(hkv)], dtype=torch.float64)
+                assert torch.allclose(have, want, rtol=1e-4, atol=1e-6)
+            ops.cache_evict(kc, vc, mass, pos, i32(held), i32(ends), i32(table), page, budget, 4, 16)
+            for s in range(S):
+                for h in range(hkv):
+                    at = [slot(s, j) for j in range(held[s])]
+                    # (the plain side's own sums: equal choices need sums further apart than the rounding, which random ones are)
+                    for a, b in P.evict([e[2] for e in plain[s][h]], [e[3] for e in plain[s][h]], ends[s], budget, 4, 16):
+                        plain[s][h][a] = list(plain[s][h][b])
+                    del plain[s][h][budget:]
+                    n = min(held[s], budget)
+                    assert pos[h, at[:n]].tolist() == [e[3] for e in plain[s][h]]
+                    assert torch.equal(kc[at[:n], h].cpu(), torch.stack([e[0] for e in plain[s][h]]))
+            held = [min(h, budget) for h in held]
+            rows = [9, 5, 12]
+        else:
+            parents = trees(rng, rows)
+            tokens = [[rng.randrange(3) for _ in t] for t in parents]
+            targets = [[rng.randrange(3) for _ in t] for t in parents]
+            ops.tree_attention(q.reshape(-1, hq * hd).to(dev()), kc, vc, out, ops.tree_mask(parents).to(dev()), *spans, page, hq, hkv, hd, hd ** -0.5)
+            path, count, nxt = i32([[0] * 12] * S), i32([0] * S), i32([0] * S)
+            flat = [i32([x for t in lists for x in t]) for lists in (tokens, parents, targets)]
+            ops.tree_commit(*flat, kc, vc, *spans, page, path, count, nxt)
+            for s, n in enumerate(rows):
+                a = slice(first[s], first[s] + n)
+                sees = torch.cat([torch.ones((n, held[s]), dtype=torch.bool), P.ancestors(parents[s])], 1)
+                want, _ = plain_rows(s, q[a], k[a], v[a], sees)
+                assert torch.allclose(out[a].cpu().double().reshape(n, hq, hd), want, atol=2e-5)
+                took, last = P.commit(tokens[s], parents[s], targets[s], 12)
+                assert path[s].tolist()[:len(took)] == took and int(count[s]) == len(took) and int(nxt[s]) == last
+                for d, node in enumerate(took):
+                    for h in range(hkv):
+                        plain[s][h].append([k[first[s] + node, h], v[first[s] + node, h], 0.0, ends[s] + d])
+                    mass[:, slot(s, held[s] + d)] = 0.0
+                    pos[:, slot(s, held[s] + d)] = ends[s] + d
+                held[s], ends[s] = held[s] + len(took), ends[s] + len(took)
+            rows = [1, 1, 1]
