@@ -1436,7 +1436,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _check(lib().llb_tree_attention(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), dt, mask.data_ptr(), mask.shape[1], span_row.data_ptr(),
         span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, pages, page_size, slots, num_heads, num_kv_heads,
-        head_dim, scale, scratch.data_ptr(), _stream()))
+        head_dim, scale, scratch.data_ptr(), async_error_flag(q.device).data_ptr(), _stream()))
 
 
 def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, mass: torch.Tensor,
@@ -1467,7 +1467,7 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     _check(lib().llb_paged_attention_mass(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), dt, None if mass_in is None else mass_in.data_ptr(),
         mass.data_ptr(), span_row.data_ptr(), span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, max_len, pages,
-        page_size, slots, num_heads, num_kv_heads, head_dim, scale, scratch.data_ptr(), _stream()))
+        page_size, slots, num_heads, num_kv_heads, head_dim, scale, scratch.data_ptr(), async_error_flag(q.device).data_ptr(), _stream()))
 
 
 def _check_planes(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor):

@@ -470,25 +470,31 @@ int check(const LlbSpanArgs& a, int dtype) {
     return 0;
 }
 
-// Scratch: the partial results, the blocks' open jobs, lse, scores.
+// Whether the tensor-core kernels take these sizes (they may still pass a call on, see llb_span_tc_takes).
+bool tc_sizes(int dtype, int hd, int page_size) {
+    return dtype == LLB_BF16 && (hd == 64 || hd == 128) && page_size % 8 == 0 && page_size <= 128 && 128 % page_size == 0;
+}
+// Scratch: the partial results, the blocks' open jobs, the partial sums of the weights, lse, scores.
 struct Layout {
-    long long part_o, part_ml, open, lse, scores, floats;
+    long long part_o, part_ml, open, part_mass, lse, scores, floats;
 };
 Layout layout(int T, int Hq, int hd, int num_slots, int rows, int blocks, int mass) {
     Layout l;
     l.part_o = 0;
     l.part_ml = l.part_o + 2ll * blocks * rows * hd;
     l.open = l.part_ml + 2ll * blocks * rows * 2;
-    l.lse = l.open + 4ll * blocks;
+    l.part_mass = l.open + 4ll * blocks;
+    l.lse = l.part_mass + (mass == 1 ? 2ll * blocks * 128 : 0);
     l.scores = l.lse + (mass > 0 ? (long long)T * Hq : 0);
     l.floats = l.scores + (mass == 2 ? (long long)Hq * num_slots : 0);
     return l;
 }
 
-// mass as llb_span_scratch_floats.
-int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtype, float* scratch, int mass, cudaStream_t stream) {
-    const int rows = simt_rows(a.T, a.S, a.group);
-    const int blocks = simt_blocks();
+// mass as llb_span_scratch_floats; tc: on the tensor cores.
+int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtype, float* scratch, int mass, bool tc, float** part_mass,
+           int* error_flag, cudaStream_t stream) {
+    const int rows = tc ? 2 * llb_span_tc_pairs(a.group) * a.group : simt_rows(a.T, a.S, a.group);
+    const int blocks = tc ? min(llb_device_sms(), MERGE_PARTS) : simt_blocks();
     const Layout l = layout(a.T, a.Hq, a.hd, a.num_slots, rows, blocks, mass);
     a.rows = rows;
     a.nodes = rows / a.group;
@@ -497,11 +503,16 @@ int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtyp
     a.open = (int*)(scratch + l.open);
     a.lse = mass > 0 ? scratch + l.lse : nullptr;
     a.scores = mass == 2 ? scratch + l.scores : nullptr;
-    SimtParams p;
-    p.a = a; p.q = q; p.k = k; p.v = v;
+    *part_mass = scratch + l.part_mass;
     int rc;
-    if (dtype == LLB_F32) rc = rows == 16 ? launch_attention_hd<float, 16>(p, blocks, stream) : launch_attention_hd<float, 64>(p, blocks, stream);
-    else rc = rows == 16 ? launch_attention_hd<__nv_bfloat16, 16>(p, blocks, stream) : launch_attention_hd<__nv_bfloat16, 64>(p, blocks, stream);
+    if (tc) {
+        rc = llb_span_attention_tc(a, q, k, v, blocks, error_flag, stream);
+    } else {
+        SimtParams p;
+        p.a = a; p.q = q; p.k = k; p.v = v;
+        if (dtype == LLB_F32) rc = rows == 16 ? launch_attention_hd<float, 16>(p, blocks, stream) : launch_attention_hd<float, 64>(p, blocks, stream);
+        else rc = rows == 16 ? launch_attention_hd<__nv_bfloat16, 16>(p, blocks, stream) : launch_attention_hd<__nv_bfloat16, 64>(p, blocks, stream);
+    }
     if (rc) return rc;
     return llb_span_merge(a, dtype, blocks, stream);
 }
@@ -521,14 +532,19 @@ LlbSpanArgs span_args(const void* out, const int* span_row, const int* span_len,
 LLB_EXPORT long long llb_span_scratch_floats(int dtype, int T, int S, int Hq, int Hkv, int hd, int page_size, int num_slots, int mass) {
     if (Hkv <= 0 || Hq < Hkv || S <= 0) return 1;
     const int group = Hq / Hkv;
-    return layout(T, Hq, hd, num_slots, simt_rows(T, S, group), simt_blocks(), mass).floats;
+    long long n = layout(T, Hq, hd, num_slots, simt_rows(T, S, group), simt_blocks(), mass).floats;
+    if (tc_sizes(dtype, hd, page_size) && group <= 128) {
+        const long long tc = layout(T, Hq, hd, num_slots, 2 * llb_span_tc_pairs(group) * group, min(llb_device_sms(), MERGE_PARTS), mass).floats;
+        n = tc > n ? tc : n;
+    }
+    return n;
 }
 
 // q, out [T, Hq, hd]; caches [num_slots, Hkv, hd]; span arrays [S]; table [S, max_pages]; mask [T, words] 64-bit words.
 LLB_EXPORT int llb_tree_attention(const void* q, const void* k, const void* v, void* out, int dtype, const unsigned long long* mask,
                                   int words, const int* span_row, const int* span_len, const int* span_pos, const int* table, int S, int T,
                                   int max_pages, int page_size, int num_slots, int Hq, int Hkv, int hd, float scale, float* scratch,
-                                  cudaStream_t stream) {
+                                  int* error_flag, cudaStream_t stream) {
     LlbSpanArgs a = span_args(out, span_row, span_len, span_pos, table, S, T, max_pages, page_size, num_slots, Hq, Hkv, hd, scale, 0);
     if (int rc = check(a, dtype)) return rc;
     LLB_REQUIRE(words > 0 && words <= (1 << 20) && mask && scratch, "tree_attention: no mask or no scratch");
@@ -536,21 +552,25 @@ LLB_EXPORT int llb_tree_attention(const void* q, const void* k, const void* v, v
     a.mask = mask;
     a.words = words;
     a.max_len = words * 64;
-    return attend(a, q, k, v, dtype, scratch, 0, stream);
+    float* unused;
+    return attend(a, q, k, v, dtype, scratch, 0, tc_sizes(dtype, hd, page_size) && llb_span_tc_takes(a, q, k, v, out), &unused, error_flag, stream);
 }
 
 // Causal; mass_in (may be null) and mass [Hkv, num_slots] float, may be the same.
 LLB_EXPORT int llb_paged_attention_mass(const void* q, const void* k, const void* v, void* out, int dtype, const float* mass_in, float* mass,
                                         const int* span_row, const int* span_len, const int* span_pos, const int* table, int S, int T,
                                         int max_len, int max_pages, int page_size, int num_slots, int Hq, int Hkv, int hd, float scale,
-                                        float* scratch, cudaStream_t stream) {
+                                        float* scratch, int* error_flag, cudaStream_t stream) {
     LlbSpanArgs a = span_args(out, span_row, span_len, span_pos, table, S, T, max_pages, page_size, num_slots, Hq, Hkv, hd, scale, max_len);
     if (int rc = check(a, dtype)) return rc;
     LLB_REQUIRE(max_len > 0 && mass && scratch, "paged_attention_mass: no weights, no scratch or rows");
     LLB_REQUIRE((long long)S * Hkv < (1ll << 31), "paged_attention_mass: too many requests");
     if (S == 0 || T == 0) return 0;
     const bool single = max_len == 1;
-    if (int rc = attend(a, q, k, v, dtype, scratch, single ? 2 : 1, stream)) return rc;
+    const bool tc = tc_sizes(dtype, hd, page_size) && llb_span_tc_takes(a, q, k, v, out);
+    float* part_mass;
+    if (int rc = attend(a, q, k, v, dtype, scratch, single ? 2 : 1, tc, &part_mass, error_flag, stream)) return rc;
+    if (tc && !single) return llb_span_mass_tc(a, q, k, mass_in, mass, part_mass, min(llb_device_sms(), MERGE_PARTS), error_flag, stream);
     const int sms = llb_device_sms();
     if (single) {
         MassParams p;

@@ -148,3 +148,11 @@ __device__ __forceinline__ int llb_part_of(const LlbPiece& p, const LlbJob& j) {
 
 // Joins the partial results of cut jobs and writes their rows (and lse); `blocks` is the grid of the attention kernel.
 int llb_span_merge(const LlbSpanArgs& a, int dtype, int blocks, cudaStream_t stream);
+
+// The tensor-core kernels (span_attention_tcgen05.cu): whether they take a call, how many rows of a request fill 128 pairs, the attention
+// (a.nodes twice that many, a.rows 2 x 128), and the weights of keys (part: 2 * blocks * 128 floats).
+bool llb_span_tc_takes(const LlbSpanArgs& a, const void* q, const void* k, const void* v, const void* out);
+int llb_span_tc_pairs(int group);
+int llb_span_attention_tc(const LlbSpanArgs& a, const void* q, const void* k, const void* v, int blocks, int* error_flag, cudaStream_t stream);
+int llb_span_mass_tc(const LlbSpanArgs& a, const void* q, const void* k, const float* mass_in, float* mass, float* part, int blocks,
+                     int* error_flag, cudaStream_t stream);

@@ -1,0 +1,957 @@
+// Attention over whole requests on the 5th-generation tensor cores (sm_100a, bf16, heads of 64 and 128): rows with a tree mask or causal
+// ones, and the sums of the weights that keys receive.  Which rows see which keys, jobs and their cut: span_attention.cuh.
+//
+// 128 (row, head of the group) pairs are the 128 lanes of tensor memory, so all query heads that read the same keys read them at
+// once: a few drafted nodes fill the lanes that their heads' keys pay for anyway.  A block has two softmax groups of 128 threads (a
+// thread a lane) and one line of key tiles that are loaded once:
+//     more than 128 pairs     each group has 128 pairs of its own, both see every tile
+//     up to 128 pairs         both have the same pairs, the first sees the even tiles and the second the odd ones; they are joined at
+//                             the end through tensor memory (the same pair has the same lane in both)
+// While one group works on its scores the tensor cores work for the other.  For every tile of 128 keys of a group:
+//     S = Q K^T               tcgen05.mma, 128 columns of tensor memory
+//     m, p = 2^(S - m), l     a thread reads its lane's 128 scores once, keeps them in registers; p goes back to tensor memory as bf16
+//                             (over S) and is the A operand of the next product without a way through shared memory
+//     O += P V                in tensor memory; it is scaled only when a lane's maximum has grown by more than 2^8 since its last
+//                             scaling (any reference works for a softmax, and 2^8 leaves floats and bf16 their accuracy)
+// K and V tiles go through a ring of half tiles (128 keys of K, or of V) that TMA fills page by page, several ahead, across jobs.
+#include <cuda.h>
+
+#include "span_attention.cuh"
+#include "tcgen05_common.cuh"
+#include "warp_mma.cuh"
+
+namespace {
+
+using namespace t5;
+using wm::fast_exp2;
+
+constexpr int BQ = 128, BK = 128;
+constexpr int NUM_THREADS = 384;               // two softmax groups of 128; a third with the warp that issues products and the loader warp
+constexpr int MMA_WARP = 8, LOAD_WARP = 9;
+constexpr uint32_t TILE_BYTES = 128 * 128;     // [128 rows][64 elements]
+constexpr float RESCALE = 8.0f;                // how far (powers of two) a lane's maximum may pass its reference
+constexpr int BAR_PAIR = 1;                    // both softmax groups
+
+template <int HD> struct Shape {
+    static constexpr int KB = HD / 64;
+    static constexpr uint32_t HALF = KB * TILE_BYTES;           // 128 rows of Q, K or V
+    static constexpr int RING = HD == 64 ? 10 : 5;
+    static constexpr size_t SMEM = (size_t)(2 + RING) * HALF + 1024;
+};
+
+struct TcParams {
+    LlbSpanArgs a;
+    const __nv_bfloat16* v;
+    int pairs_nodes;            // rows of a request whose pairs fill 128 lanes
+    int* error_flag;
+};
+
+// A block is launched with 3 x 168 registers a thread of its three groups; the third one needs few, the softmax groups hold a row
+// of 128 scores: 88 + 2 x 208 = 504.
+__device__ __forceinline__ void registers_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
+__device__ __forceinline__ void registers_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
+__device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
+}
+// D[128 x N] += A B with A in tensor memory (bf16, two to a column).
+__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&u)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]),
+          "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]),
+          "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]),
+          "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 bits of a row's mask from node j0 on (which may be negative), those of nodes from len on cleared.
+__device__ __forceinline__ uint32_t mask_bits(const unsigned long long* row, int words, int j0, int len) {
+    if (j0 <= -32 || j0 >= len) return 0u;
+    uint32_t bits;
+    if (j0 < 0) bits = (uint32_t)row[0] << -j0;
+    else {
+        const int w = j0 >> 6, sh = j0 & 63;
+        unsigned long long x = row[w] >> sh;
+        if (sh > 32 && w + 1 < words) x |= row[w + 1] << (64 - sh);
+        bits = (uint32_t)x;
+    }
+    return len - j0 < 32 ? bits & ((1u << (len - j0)) - 1u) : bits;
+}
+__device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+__device__ __forceinline__ bool bf16_odd(uint32_t pair) { return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u; }
+
+// Four bytes a page: the cache row that a page of a tile begins at, or num_slots (TMA reads zeros there) for one that holds no key of
+// the job or is none of the cache's.
+__device__ __forceinline__ int page_row(const LlbSpanArgs& a, int s, int page_of, int keys) {
+    if (page_of >= a.max_pages || page_of * a.page_size >= keys) return a.num_slots;
+    const int page = a.table[(size_t)s * a.max_pages + page_of];
+    return page >= 0 && (long long)page * a.page_size < a.num_slots ? page * a.page_size : a.num_slots;
+}
+
+// What the roles share of a block's walk through its jobs.
+struct Segment {
+    int k0, k1;              // tiles of the job
+    bool two;                // the groups have pairs of their own
+    int part;
+};
+__device__ __forceinline__ Segment segment_of(const TcParams& p, const LlbPiece& pc, const LlbJob& job, int t) {
+    Segment g;
+    g.k0 = t - job.begin;
+    g.k1 = min(job.tiles, pc.t1 - job.begin);
+    g.two = job.count(p.a) > p.pairs_nodes;
+    g.part = llb_part_of(pc, job);
+    return g;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                         const __grid_constant__ CUtensorMap map_v, const TcParams p) {
+    constexpr int KB = Shape<HD>::KB, RING = Shape<HD>::RING;
+    constexpr uint32_t HALF = Shape<HD>::HALF;
+    constexpr uint32_t TMEM_COLS = 512;              // S (and P) of the groups: 0.., 128..; O: 256.., 384..
+    __shared__ __align__(8) uint64_t bar_q_full[2], bar_q_free[2], bar_kv_full[RING], bar_kv_free[RING], bar_s[2], bar_p[2], bar_o[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_s, odd_s;
+    __shared__ LlbPiece piece_s;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* q_s = smem;                             // two buffers
+    uint8_t* ring = smem + 2 * HALF;
+    volatile int* abort_flag = &abort_s;
+    const LlbSpanArgs& a = p.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar_q_full[i], 1);
+            mbar_init(&bar_q_free[i], 1);
+            mbar_init(&bar_s[i], 1);
+            mbar_init(&bar_p[i], 4);
+            mbar_init(&bar_o[i], 1);
+        }
+        for (int i = 0; i < RING; ++i) {
+            mbar_init(&bar_kv_full[i], 1);
+            mbar_init(&bar_kv_free[i], 2);
+        }
+        abort_s = 0;
+        odd_s = 0;
+        mbar_init_fence();
+    }
+    if (warp == MMA_WARP) tmem_alloc(&tmem_slot, TMEM_COLS);
+    griddep_wait();
+    griddep_launch_dependents();
+    if (warp == 0) {
+        const LlbPiece pc = llb_piece(a, BK, blockIdx.x, gridDim.x, 2, lane);
+        if (lane == 0) {
+            piece_s = pc;
+            a.open[blockIdx.x * 4] = -1;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_slot;
+    const LlbPiece pc = piece_s;
+    LlbJob job = pc.job;
+    constexpr uint32_t IDESC_S = idesc_bf16(BQ, BK, 0), IDESC_PV = idesc_bf16(BQ, HD, 1);
+    // Q buffers: jobs of two pair tiles take both, others one after the other
+    uint32_t q_uses[2] = {0, 0};
+    int q_next = 0;
+    uint32_t tiles_before = 0;                       // tiles of the block's jobs before this one
+
+    if (warp >= MMA_WARP) {
+    registers_give();
+    if (warp == LOAD_WARP) {
+        bool ok = true;
+        const uint32_t q_bytes = (uint32_t)p.pairs_nodes * a.group * 128 * KB;
+        const int ppt = BK / a.page_size;
+        uint32_t loaded = 0;
+        for (int t = pc.t0; t < pc.t1;) {
+            const Segment g = segment_of(p, pc, job, t);
+            for (int x = 0; x < (g.two ? 2 : 1); ++x) {
+                const int b = g.two ? x : q_next;
+                if (q_uses[b] > 0) ok = mbar_wait(&bar_q_free[b], (q_uses[b] - 1) & 1, abort_flag) && ok;
+                if (lane == 0 && ok) {
+                    mbar_expect_tx(&bar_q_full[b], q_bytes);
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb)
+                        tma_load_3d(q_s + b * HALF + kb * TILE_BYTES, &map_q, kb * 64, job.kvh * a.group,
+                                    job.z.row + job.first + x * p.pairs_nodes, &bar_q_full[b]);
+                }
+                ++q_uses[b];
+            }
+            if (!g.two) q_next ^= 1;
+            for (int k = g.k0; k < g.k1; ++k) {
+                const int row = lane < ppt ? page_row(a, job.s, k * ppt + lane, job.keys) : a.num_slots;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t slot = loaded % RING;
+                    if (loaded >= RING) ok = mbar_wait(&bar_kv_free[slot], (loaded / RING - 1) & 1, abort_flag) && ok;
+                    if (ok) {
+                        if (lane == 0) mbar_expect_tx(&bar_kv_full[slot], HALF);
+                        __syncwarp();
+                        if (lane < ppt) {
+                            uint8_t* dst = ring + slot * HALF + (uint32_t)lane * a.page_size * 128;
+#pragma unroll
+                            for (int kb = 0; kb < KB; ++kb)
+                                tma_load_2d(dst + kb * TILE_BYTES, half ? &map_v : &map_k, job.kvh * HD + kb * 64, row, &bar_kv_full[slot]);
+                        }
+                        ++loaded;
+                    }
+                    __syncwarp();
+                }
+            }
+            t = job.begin + g.k1;
+            if (t < pc.t1) job.next(a, BK);
+        }
+        // after a wait has run out: what was asked for arrives before the block ends
+        if (!ok) {
+            for (uint32_t i = loaded > RING ? loaded - RING : 0; i < loaded; ++i) {
+                const long long since = clock64();
+                while (!mbar_try_wait(&bar_kv_full[i % RING], (i / RING) & 1) && clock64() - since < WAIT_LIMIT_CYCLES / 64) {
+                }
+            }
+        }
+    } else if (warp == MMA_WARP) {
+        bool ok = true;
+        uint32_t n_p[2] = {0, 0};
+        auto full = [&](uint32_t half) {             // half tile number `half` of the block has arrived
+            ok = mbar_wait(&bar_kv_full[half % RING], (half / RING) & 1, abort_flag) && ok;
+            tc_fence_after();
+        };
+        auto issue_s = [&](int x, int b, uint32_t half) {
+            if (lane == 0 && ok) {
+                const uint32_t qa = smem_u32(q_s + b * HALF), ka = smem_u32(ring + half % RING * HALF);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_bf16(tmem_base + x * 128, desc_kmajor(qa + kb * TILE_BYTES + k * 32), desc_kmajor(ka + kb * TILE_BYTES + k * 32),
+                                  IDESC_S, (kb > 0 || k > 0) ? 1u : 0u);
+            }
+            __syncwarp();
+        };
+        for (int t = pc.t0; t < pc.t1;) {
+            const Segment g = segment_of(p, pc, job, t);
+            const int n = g.k1 - g.k0, step = g.two ? 1 : 2;
+            int buf[2];
+            for (int x = 0; x < 2; ++x) {
+                const int b = g.two ? x : q_next;
+                buf[x] = b;
+                if (g.two || x == 0) ok = mbar_wait(&bar_q_full[b], q_uses[b]++ & 1, abort_flag) && ok;
+                const int first = g.two ? 0 : x;
+                if (first >= n) continue;
+                full(2 * (tiles_before + first));
+                issue_s(x, b, 2 * (tiles_before + first));
+                if (lane == 0 && ok) umma_commit(&bar_s[x]);
+                __syncwarp();
+            }
+            if (!g.two) q_next ^= 1;
+            for (int j0 = 0; j0 < n; j0 += step) {
+                for (int x = 0; x < 2; ++x) {
+                    const int j = g.two ? j0 : j0 + x;
+                    if (j >= n) continue;
+                    full(2 * (tiles_before + j) + 1);
+                    ok = mbar_wait(&bar_p[x], n_p[x]++ & 1, abort_flag) && ok;
+                    tc_fence_after();
+                    if (lane == 0 && ok) {
+                        const uint32_t va = smem_u32(ring + (2 * (tiles_before + j) + 1) % RING * HALF);
+#pragma unroll
+                        for (int k = 0; k < BK / 16; ++k)
+                            umma_bf16_ts(tmem_base + 256 + x * 128, tmem_base + x * 128 + k * 8, desc_mnmajor(va + k * 16 * 128, TILE_BYTES),
+                                         IDESC_PV, (j0 > 0 || k > 0) ? 1u : 0u);
+                    }
+                    __syncwarp();
+                    if (j + step < n) {
+                        full(2 * (tiles_before + j + step));
+                        issue_s(x, buf[x], 2 * (tiles_before + j + step));
+                        if (lane == 0 && ok) umma_commit(&bar_s[x]);       // this P V and the next S
+                    } else if (lane == 0 && ok) {
+                        umma_commit(&bar_o[x]);
+                    }
+                    __syncwarp();
+                }
+            }
+            tiles_before += n;
+            t = job.begin + g.k1;
+            if (t < pc.t1) job.next(a, BK);
+        }
+    }
+    } else {
+        registers_take();
+        const int x = warp >> 2, r = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tmem_s = tmem_base + x * 128 + lanes, tmem_o = tmem_base + 256 + lanes;
+        bool ok = true;
+        uint32_t n_s = 0, n_o = 0;
+        for (int t = pc.t0; t < pc.t1;) {
+            const Segment g = segment_of(p, pc, job, t);
+            const int n = g.k1 - g.k0, step = g.two ? 1 : 2;
+            const int node0 = g.two ? x * p.pairs_nodes : 0;
+            const int pairs = min(p.pairs_nodes, job.count(a) - node0) * a.group;
+            const bool mine = r < pairs;
+            const int node = job.first + node0 + (mine ? r / a.group : 0);
+            const LlbSpan z = job.z;
+            const unsigned long long* mask = a.mask ? a.mask + (size_t)(z.row + node) * a.words : nullptr;
+            const int all = a.mask ? z.pos : z.pos + job.first + 1;         // keys that every row of the job sees
+            const int own = a.mask ? z.pos : z.pos + node + 1;              // first keys that this row sees
+            const bool scores = a.scores && z.len == 1 && mine;
+            const bool busy = (warp & 3) * 32 < pairs;                      // any pair in this warp's lanes
+            float m_ref = -INFINITY, l_run = 0.0f;
+            for (int j = g.two ? 0 : x; j < n; j += step) {
+                const int key0 = (g.k0 + j) * BK;
+                const uint32_t half = 2 * (tiles_before + j);
+                ok = mbar_wait(&bar_s[x], n_s++ & 1, abort_flag) && ok;
+                tc_fence_after();
+                if (r == 0) {
+                    // S has read K, and the product before it V
+                    mbar_arrive_n(&bar_kv_free[half % RING], g.two ? 1 : 2);
+                    if (j >= step) mbar_arrive_n(&bar_kv_free[(half + 1 - 2 * step) % RING], g.two ? 1 : 2);
+                }
+                const bool interior = key0 + BK <= all;
+                if (!interior) {
+                    // Values that no row or not every row sees: what earlier owners left behind the last key, and numbers that are
+                    // none in rows that see them, would reach the other rows as 0 * inf.  They become zeros here; rows that see the
+                    // latter get them back at the end.
+                    ok = mbar_wait(&bar_kv_full[(half + 1) % RING], ((half + 1) / RING) & 1, abort_flag) && ok;
+                    const int key = key0 + r;
+                    if (key >= all && ok) {
+                        uint8_t* row = ring + (half + 1) % RING * HALF + (uint32_t)r * 128;
+#pragma unroll
+                        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) {
+                                uint4* at = reinterpret_cast<uint4*>(row + kb * TILE_BYTES + c * 16);
+                                if (key >= job.keys) {
+                                    *at = make_uint4(0u, 0u, 0u, 0u);
+                                    continue;
+                                }
+                                uint4 w = *at;
+                                if (bf16_odd(w.x) || bf16_odd(w.y) || bf16_odd(w.z) || bf16_odd(w.w)) {
+                                    odd_s = 1;
+                                    __threadfence_block();
+                                    uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        if ((u[e] & 0x7f80u) == 0x7f80u) u[e] &= 0xffff0000u;
+                                        if ((u[e] & 0x7f800000u) == 0x7f800000u) u[e] &= 0xffffu;
+                                    }
+                                    *at = w;
+                                }
+                            }
+                    }
+                    fence_async_smem();
+                }
+                if (busy) {
+                    float s[128];
+                    tmem_ld32_nowait(tmem_s, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+                    tmem_ld32_nowait(tmem_s + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+                    tmem_ld32_nowait(tmem_s + 64, *reinterpret_cast<uint32_t(*)[32]>(&s[64]));
+                    tmem_ld32_nowait(tmem_s + 96, *reinterpret_cast<uint32_t(*)[32]>(&s[96]));
+                    tmem_wait_ld();
+                    if (!interior) {
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            uint32_t bits = first_bits(own - key0 - 32 * w);
+                            if (mask && mine) bits |= mask_bits(mask, a.words, key0 + 32 * w - z.pos, z.len);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) s[32 * w + i] = (bits >> i) & 1u ? s[32 * w + i] : -INFINITY;
+                        }
+                    }
+                    if (scores) {
+                        float* to = a.scores + (size_t)(job.kvh * a.group + r) * a.num_slots;
+#pragma unroll
+                        for (int c = 0; c < 128; c += 8) {
+                            const int key = key0 + c;         // (pages are multiples of 8 keys)
+                            const int slot = key < job.keys ? llb_span_slot(a, job.s, key) : -1;
+                            if (slot < 0) continue;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (slot + i < a.num_slots) to[slot + i] = s[c + i] * a.scale_log2e;
+                        }
+                    }
+                    float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
+#pragma unroll
+                    for (int i = 4; i < 128; i += 4) {
+                        t0 = fmaxf(t0, s[i]);
+                        t1 = fmaxf(t1, s[i + 1]);
+                        t2 = fmaxf(t2, s[i + 2]);
+                        t3 = fmaxf(t3, s[i + 3]);
+                    }
+                    const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * a.scale_log2e;
+                    __syncwarp();
+                    if (j < step) m_ref = top;              // (no O yet)
+                    else if (__any_sync(0xffffffffu, top > m_ref + RESCALE)) {
+                        float corr = 1.0f;
+                        if (top > m_ref + RESCALE) {
+                            corr = m_ref == -INFINITY ? 0.0f : fast_exp2(m_ref - top);
+                            m_ref = top;
+                        }
+                        l_run *= corr;
+#pragma unroll
+                        for (int c = 0; c < HD; c += 32) {
+                            float o[32];
+                            tmem_ld32(tmem_o + x * 128 + c, o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] *= corr;
+                            tmem_st32(tmem_o + x * 128 + c, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+                        }
+                    }
+                    __syncwarp();
+                    const float shift = m_ref == -INFINITY ? 0.0f : -m_ref;
+                    float l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < 128; c += 64) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float p0 = fast_exp2(fmaf(s[c + 2 * i], a.scale_log2e, shift));
+                            const float p1 = fast_exp2(fmaf(s[c + 2 * i + 1], a.scale_log2e, shift));
+                            const float p2 = fast_exp2(fmaf(s[c + 2 * i + 2], a.scale_log2e, shift));
+                            const float p3 = fast_exp2(fmaf(s[c + 2 * i + 3], a.scale_log2e, shift));
+                            l0 += p0;
+                            l1 += p1;
+                            l2 += p2;
+                            l3 += p3;
+                            w[i] = wm::pack_bf16(p0, p1);
+                            w[i + 1] = wm::pack_bf16(p2, p3);
+                        }
+                        tmem_st32(tmem_s + c / 2, w);
+                    }
+                    l_run += (l0 + l1) + (l2 + l3);
+                    tmem_wait_st();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_p[x]);
+            }
+            const bool any = g.two || x < n;
+            if (any) {
+                ok = mbar_wait(&bar_o[x], n_o++ & 1, abort_flag) && ok;
+                tc_fence_after();
+                if (r == 0) {
+                    const int last = g.two ? n - 1 : x + (n - 1 - x) / 2 * 2;
+                    mbar_arrive_n(&bar_kv_free[(2 * (tiles_before + last) + 1) % RING], g.two ? 1 : 2);
+                }
+            }
+            const int buf = g.two ? x : q_next;
+            float w_own = 1.0f, w_other = 0.0f;
+            if (!g.two) {
+                // the groups' maxima and sums meet in the job's Q buffer, which nothing reads any more once both have passed
+                float2* meet = reinterpret_cast<float2*>(q_s + buf * HALF);
+                named_barrier(BAR_PAIR, 256);
+                meet[x * 128 + r] = make_float2(m_ref, l_run);
+                named_barrier(BAR_PAIR, 256);
+                const float2 other = meet[(x ^ 1) * 128 + r];
+                const float M = fmaxf(m_ref, other.x);
+                w_own = m_ref == -INFINITY ? (l_run == 0.0f ? 0.0f : 1.0f) : fast_exp2(m_ref - M);
+                w_other = other.x == -INFINITY ? (other.y == 0.0f ? 0.0f : 1.0f) : fast_exp2(other.x - M);
+                l_run = l_run * w_own + other.y * w_other;
+                m_ref = M;
+                q_next ^= 1;
+            }
+            const int head = job.kvh * a.group + (mine ? r % a.group : 0), row = z.row + node;
+            const int d0 = g.two ? 0 : x * (HD / 2), d1 = g.two ? HD : d0 + HD / 2;
+            const float inv = l_run > 0.0f || m_ref != -INFINITY || z.pos > 0 ? 1.0f / l_run : 0.0f;
+            const bool both = !g.two && n > 1;
+            const bool odd = *(volatile int*)&odd_s != 0;
+            if (busy) {
+#pragma unroll
+                for (int c = 0; c < HD; c += 32) {
+                    if (c < d0 || c >= d1) continue;
+                    float o[32];
+                    __syncwarp();
+                    if (g.two) {
+                        tmem_ld32(tmem_o + x * 128 + c, o);
+                    } else {
+                        // (group 0 has tiles in any case)
+                        tmem_ld32(tmem_o + c, o);
+                        const float w0 = x == 0 ? w_own : w_other, w1 = x == 0 ? w_other : w_own;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] *= w0;
+                        if (both) {
+                            float o1[32];
+                            tmem_ld32(tmem_o + 128 + c, o1);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = fmaf(o1[i], w1, o[i]);
+                        }
+                    }
+                    if (odd && mine) {
+                        for (int key = max(all, g.k0 * BK); key < min(job.keys, g.k1 * BK); ++key) {
+                            const int jn = key - z.pos;
+                            const bool sees = mask ? (mask[jn >> 6] >> (jn & 63)) & 1ull : jn <= node;
+                            const int slot = sees ? llb_span_slot(a, job.s, key) : -1;
+                            if (slot < 0) continue;
+                            const __nv_bfloat16* vr = p.v + ((size_t)slot * a.Hkv + job.kvh) * HD + c;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const float f = __bfloat162float(vr[i]);
+                                if (!(fabsf(f) < INFINITY)) o[i] += f;
+                            }
+                        }
+                    }
+                    if (!mine || !ok) {
+                    } else if (g.part >= 0) {
+                        float* po = a.part_o + ((size_t)(blockIdx.x * 2 + g.part) * a.rows + node0 * a.group + r) * HD + c;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(po + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    } else {
+                        __nv_bfloat16* dst = (__nv_bfloat16*)a.out + ((size_t)row * a.Hq + head) * HD + c;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8)
+                            *reinterpret_cast<uint4*>(dst + i) =
+                                make_uint4(wm::pack_bf16(o[i] * inv, o[i + 1] * inv), wm::pack_bf16(o[i + 2] * inv, o[i + 3] * inv),
+                                           wm::pack_bf16(o[i + 4] * inv, o[i + 5] * inv), wm::pack_bf16(o[i + 6] * inv, o[i + 7] * inv));
+                    }
+                }
+            }
+            if (mine && ok && (g.two || x == 0)) {
+                if (g.part >= 0) {
+                    float* ml = a.part_ml + ((size_t)(blockIdx.x * 2 + g.part) * a.rows + node0 * a.group + r) * 2;
+                    ml[0] = m_ref;
+                    ml[1] = l_run;
+                } else if (a.lse) {
+                    a.lse[(size_t)row * a.Hq + head] = l_run == 0.0f ? INFINITY : m_ref + log2f(l_run);
+                }
+            }
+            if (g.part == 1 && threadIdx.x == 0) {
+                int* d = a.open + blockIdx.x * 4;
+                d[0] = job.s; d[1] = job.first; d[2] = job.kvh; d[3] = llb_piece_owner(pc, job.begin + job.tiles - 1);
+            }
+            // O and Q are free for the next job (the groups have read each other's O)
+            tc_fence_before();
+            fence_async_smem();
+            if (!g.two) named_barrier(BAR_PAIR, 256);
+            else named_barrier(BAR_PAIR + 1 + x, 128);
+            if (r == 0 && (g.two || x == 0)) mbar_arrive(&bar_q_free[buf]);
+            tiles_before += n;
+            t = job.begin + g.k1;
+            if (t < pc.t1) job.next(a, BK);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag && threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 4);
+    if (warp == MMA_WARP) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, TMEM_COLS);
+    }
+}
+
+// ---- the weights that keys receive -----------------------------------------------------------------------------------------------
+// mass_j = sum over rows i and heads of 2^(x_ij - lse_i), the scores made once more with keys and queries in each other's place:
+//     S^T = K Q^T             128 keys are the lanes, 128 (row, head) pairs the columns
+// so that a key's sum is a sum in one thread's register, made in one order, with no meeting of threads and no atomics.  What bounds it
+// is the exponential of every score (16 a cycle and SM).  A job is a tile of 128 keys of one request and kv head; the tiles of rows
+// that see any of its keys make the line that is cut among the blocks, as above; K stays in shared memory for the job, the tiles of Q
+// go through the ring, every other one to one of two groups of 128 threads, each with two score tiles in tensor memory so that
+// the next is made while one is read.
+struct MassArgs {
+    TcParams p;
+    const float* mass_in;
+    float* mass;
+    float* part;                // [2 * blocks, 128]
+};
+struct MassJob {
+    LlbSpan z;
+    int s, tile, kvh;
+    int from, units, begin;     // first tile of rows that sees the keys, how many do, the job's place in the line
+    __device__ __forceinline__ void measure(int pairs_nodes) {
+        from = max(0, tile * BK - z.pos) / pairs_nodes;
+        units = (z.len + pairs_nodes - 1) / pairs_nodes - from;
+    }
+    __device__ __forceinline__ int tiles() const { return z.len > 0 ? (z.pos + z.len + BK - 1) / BK : 0; }
+    __device__ __forceinline__ void next(const LlbSpanArgs& a, int pairs_nodes) {
+        begin += units;
+        if (++kvh < a.Hkv) return;
+        kvh = 0;
+        ++tile;
+        while (tile >= tiles()) {
+            z = llb_span(a, ++s);
+            tile = 0;
+        }
+        measure(pairs_nodes);
+    }
+};
+struct MassPiece {
+    int t0, t1, total, blocks;
+    MassJob job;
+};
+__device__ __forceinline__ int mass_units(const LlbSpanArgs& a, const LlbSpan& z, int pairs_nodes) {
+    if (z.len == 0) return 0;
+    const int rows = (z.len + pairs_nodes - 1) / pairs_nodes, whole = z.pos / BK + 1, tiles = (z.pos + z.len + BK - 1) / BK;
+    int n = whole * rows;          // (whole <= tiles: the first row sees key pos)
+    for (int i = whole; i < tiles; ++i) n += rows - (i * BK - z.pos) / pairs_nodes;
+    return n * a.Hkv;
+}
+__device__ __forceinline__ MassPiece mass_piece(const LlbSpanArgs& a, int pairs_nodes, int block, int grid, int lane) {
+    MassPiece p;
+    int mine = 0;
+    p.total = 0;
+    for (int base = 0; base < a.S; base += 32) {
+        mine = base + lane < a.S ? mass_units(a, llb_span(a, base + lane), pairs_nodes) : 0;
+        p.total += __reduce_add_sync(0xffffffffu, mine);
+    }
+    p.blocks = min(grid, (p.total + 1) / 2);
+    p.t0 = p.t1 = 0;
+    if (block >= p.blocks) return p;
+    p.t0 = (int)((long long)p.total * block / p.blocks);
+    p.t1 = (int)((long long)p.total * (block + 1) / p.blocks);
+    int before = 0;
+    for (int base = 0; base < a.S; base += 32) {
+        if (a.S > 32) mine = base + lane < a.S ? mass_units(a, llb_span(a, base + lane), pairs_nodes) : 0;
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, before + sum > p.t0);
+        if (past) {
+            const int at = __ffs(past) - 1;
+            p.job.s = base + at;
+            p.job.begin = before + __shfl_sync(0xffffffffu, sum - mine, at);
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    p.job.z = llb_span(a, p.job.s);
+    p.job.tile = 0;
+    for (;;) {
+        p.job.measure(pairs_nodes);
+        if (p.t0 < p.job.begin + p.job.units * a.Hkv) break;
+        p.job.begin += p.job.units * a.Hkv;
+        ++p.job.tile;
+    }
+    p.job.kvh = (p.t0 - p.job.begin) / p.job.units;
+    p.job.begin += p.job.kvh * p.job.units;
+    return p;
+}
+__device__ __forceinline__ void add_mass(const LlbSpanArgs& a, const float* mass_in, float* mass, const LlbSpan& z, int s, int key, int kvh, float sum) {
+    const int slot = key < z.pos + z.len ? llb_span_slot(a, s, key) : -1;
+    if (slot < 0) return;
+    const size_t at = (size_t)kvh * a.num_slots + slot;
+    mass[at] = key < z.pos && mass_in ? mass_in[at] + sum : sum;
+}
+
+template <int HD> struct MassShape {
+    static constexpr int RING = HD == 64 ? 8 : 4;
+    static constexpr size_t SMEM = (size_t)(2 + RING) * Shape<HD>::HALF + 1024;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const MassArgs m) {
+    constexpr int KB = Shape<HD>::KB, RING = MassShape<HD>::RING;
+    constexpr uint32_t HALF = Shape<HD>::HALF;
+    constexpr uint32_t TMEM_COLS = 512;              // two score tiles of each group
+    __shared__ __align__(8) uint64_t bar_k_full[2], bar_k_free[2], bar_q_full[RING], bar_q_free[RING], bar_s[4], bar_free[4];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_s;
+    __shared__ MassPiece piece_s;
+    __shared__ __align__(16) float lse_s[2][2][128];
+    __shared__ float sum_s[128];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* k_s = smem;                             // two buffers: this job's and the next one's
+    uint8_t* ring = smem + 2 * HALF;
+    volatile int* abort_flag = &abort_s;
+    const LlbSpanArgs& a = m.p.a;
+    const int pairs_nodes = m.p.pairs_nodes, pairs_tile = pairs_nodes * a.group;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar_k_full[i], 1);
+            mbar_init(&bar_k_free[i], 1);
+        }
+        for (int i = 0; i < RING; ++i) {
+            mbar_init(&bar_q_full[i], 1);
+            mbar_init(&bar_q_free[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&bar_s[i], 1);
+            mbar_init(&bar_free[i], 4);
+        }
+        abort_s = 0;
+        mbar_init_fence();
+    }
+    if (warp == MMA_WARP) tmem_alloc(&tmem_slot, TMEM_COLS);
+    // columns that no pair has (128 is no multiple of the group) stay zero
+    for (int i = threadIdx.x; i < RING * KB * (128 - pairs_tile) * 8; i += NUM_THREADS) {
+        const int tile = i / ((128 - pairs_tile) * 8), rest = i - tile * ((128 - pairs_tile) * 8);
+        *reinterpret_cast<uint4*>(ring + (size_t)tile * TILE_BYTES + (pairs_tile + rest / 8) * 128 + rest % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_async_smem();
+    griddep_wait();
+    griddep_launch_dependents();
+    if (warp == 0) {
+        const MassPiece pc = mass_piece(a, pairs_nodes, blockIdx.x, gridDim.x, lane);
+        if (lane == 0) {
+            piece_s = pc;
+            a.open[blockIdx.x * 4] = -1;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_slot;
+    const MassPiece pc = piece_s;
+    MassJob job = pc.job;
+    uint32_t jobs = 0, units_before = 0;
+    constexpr uint32_t IDESC = idesc_bf16(BK, BQ, 0);
+
+    if (warp == LOAD_WARP) {
+        bool ok = true;
+        const uint32_t q_bytes = (uint32_t)pairs_tile * 128 * KB;
+        const int ppt = BK / a.page_size;
+        uint32_t loaded = 0;
+        for (int t = pc.t0; t < pc.t1;) {
+            const int u0 = t - job.begin, u1 = min(job.units, pc.t1 - job.begin), b = jobs & 1;
+            const int row = lane < ppt ? page_row(a, job.s, job.tile * ppt + lane, job.z.pos + job.z.len) : a.num_slots;
+            if (jobs >= 2) ok = mbar_wait(&bar_k_free[b], (jobs / 2 - 1) & 1, abort_flag) && ok;
+            if (ok) {
+                if (lane == 0) mbar_expect_tx(&bar_k_full[b], HALF);
+                __syncwarp();
+                if (lane < ppt) {
+                    uint8_t* dst = k_s + b * HALF + (uint32_t)lane * a.page_size * 128;
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb) tma_load_2d(dst + kb * TILE_BYTES, &map_k, job.kvh * HD + kb * 64, row, &bar_k_full[b]);
+                }
+            }
+            __syncwarp();
+            for (int u = u0; u < u1; ++u) {
+                const uint32_t slot = loaded % RING;
+                if (loaded >= RING) ok = mbar_wait(&bar_q_free[slot], (loaded / RING - 1) & 1, abort_flag) && ok;
+                if (ok) {
+                    if (lane == 0) {
+                        mbar_expect_tx(&bar_q_full[slot], q_bytes);
+#pragma unroll
+                        for (int kb = 0; kb < KB; ++kb)
+                            tma_load_3d(ring + slot * HALF + kb * TILE_BYTES, &map_q, kb * 64, job.kvh * a.group,
+                                        job.z.row + (job.from + u) * pairs_nodes, &bar_q_full[slot]);
+                    }
+                    ++loaded;
+                }
+                __syncwarp();
+            }
+            ++jobs;
+            t = job.begin + u1;
+            if (t < pc.t1) job.next(a, pairs_nodes);
+        }
+        if (!ok) {
+            for (uint32_t i = loaded > RING ? loaded - RING : 0; i < loaded; ++i) {
+                const long long since = clock64();
+                while (!mbar_try_wait(&bar_q_full[i % RING], (i / RING) & 1) && clock64() - since < WAIT_LIMIT_CYCLES / 64) {
+                }
+            }
+        }
+    } else if (warp == MMA_WARP) {
+        bool ok = true;
+        for (int t = pc.t0; t < pc.t1;) {
+            const int u0 = t - job.begin, u1 = min(job.units, pc.t1 - job.begin), b = jobs & 1;
+            ok = mbar_wait(&bar_k_full[b], (jobs >> 1) & 1, abort_flag) && ok;
+            for (int u = u0; u < u1; ++u) {
+                const uint32_t at = units_before + (u - u0);          // the block's tiles of rows go to four score tiles in turn
+                const uint32_t slot = at % RING, place = at & 3;
+                ok = mbar_wait(&bar_q_full[slot], (at / RING) & 1, abort_flag) && ok;
+                if (at >= 4) ok = mbar_wait(&bar_free[place], ((at >> 2) - 1) & 1, abort_flag) && ok;
+                tc_fence_after();
+                if (lane == 0 && ok) {
+                    const uint32_t ka = smem_u32(k_s + b * HALF), qa = smem_u32(ring + slot * HALF);
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            umma_bf16(tmem_base + place * 128, desc_kmajor(ka + kb * TILE_BYTES + k * 32), desc_kmajor(qa + kb * TILE_BYTES + k * 32),
+                                      IDESC, (kb > 0 || k > 0) ? 1u : 0u);
+                    umma_commit(&bar_s[place]);
+                }
+                __syncwarp();
+            }
+            units_before += u1 - u0;
+            ++jobs;
+            t = job.begin + u1;
+            if (t < pc.t1) job.next(a, pairs_nodes);
+        }
+    } else if (warp < MMA_WARP) {
+        const int x = warp >> 2, r = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        bool ok = true;
+        for (int t = pc.t0; t < pc.t1;) {
+            const int u0 = t - job.begin, u1 = min(job.units, pc.t1 - job.begin), n = u1 - u0;
+            const LlbSpan z = job.z;
+            const int key = job.tile * BK + r;
+            float sum0 = 0.0f, sum1 = 0.0f, sum2 = 0.0f, sum3 = 0.0f;
+            // the lse of a tile's pair r, +infinity where there is none
+            auto lse_of = [&](int j) -> float {
+                const int node = (job.from + u0 + j) * pairs_nodes + r / a.group;
+                return j < n && r < pairs_tile && node < z.len ? a.lse[(size_t)(z.row + node) * a.Hq + job.kvh * a.group + r % a.group] : INFINITY;
+            };
+            const int first = (int)((x - units_before) & 1);          // the group's first tile of the job
+            float lse = lse_of(first);
+            for (int j = first; j < n; j += 2) {
+                const uint32_t at = units_before + j, place = at & 3;
+                float* lse_t = lse_s[x][place >> 1];
+                lse_t[r] = lse;
+                lse = lse_of(j + 2);
+                named_barrier(BAR_PAIR + 1 + x, 128);
+                ok = mbar_wait(&bar_s[place], (at >> 2) & 1, abort_flag) && ok;
+                tc_fence_after();
+                if (r == 0) mbar_arrive(&bar_q_free[at % RING]);
+                // pairs below `least` belong to rows before the key
+                const int node0 = (job.from + u0 + j) * pairs_nodes;
+                const int least = (key - z.pos - node0) * a.group;
+                const int upto = min(pairs_tile, (z.len - node0) * a.group);
+                const bool interior = job.tile * BK + BK - 1 - z.pos - node0 <= 0 && upto == pairs_tile;
+                const uint32_t tmem = tmem_base + place * 128 + lanes;
+#pragma unroll
+                for (int c = 0; c < 128; c += 64) {
+                    float s[64];
+                    tmem_ld32_nowait(tmem + c, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+                    tmem_ld32_nowait(tmem + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+                    tmem_wait_ld();
+                    if (!interior) {
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) s[i] = c + i >= least && c + i < upto ? s[i] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 64; i += 4) {
+                        const float4 e = *reinterpret_cast<const float4*>(lse_t + c + i);
+                        sum0 += fast_exp2(fmaf(s[i], a.scale_log2e, -e.x));
+                        sum1 += fast_exp2(fmaf(s[i + 1], a.scale_log2e, -e.y));
+                        sum2 += fast_exp2(fmaf(s[i + 2], a.scale_log2e, -e.z));
+                        sum3 += fast_exp2(fmaf(s[i + 3], a.scale_log2e, -e.w));
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_free[place]);
+            }
+            float sum = (sum0 + sum1) + (sum2 + sum3);
+            if (x == 1) sum_s[r] = sum;
+            named_barrier(BAR_PAIR, 256);
+            if (x == 0 && ok) {
+                sum += sum_s[r];
+                const int part = job.begin < pc.t0 ? 0 : job.begin + job.units > pc.t1 ? 1 : -1;
+                if (part >= 0) m.part[(size_t)(blockIdx.x * 2 + part) * 128 + r] = sum;
+                else add_mass(a, m.mass_in, m.mass, z, job.s, key, job.kvh, sum);
+                if (part == 1 && r == 0) {
+                    int* d = a.open + blockIdx.x * 4;
+                    d[0] = job.s; d[1] = job.tile; d[2] = job.kvh;
+                    d[3] = (int)(((long long)(job.begin + job.units) * pc.blocks + pc.total - 1) / pc.total) - 1;
+                }
+            }
+            named_barrier(BAR_PAIR, 256);
+            if (threadIdx.x == 0) mbar_arrive(&bar_k_free[jobs & 1]);          // both groups have had all scores of the job
+            units_before += n;
+            ++jobs;
+            t = job.begin + u1;
+            if (t < pc.t1) job.next(a, pairs_nodes);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag && threadIdx.x == 0 && m.p.error_flag) atomicExch(m.p.error_flag, 5);
+    if (warp == MMA_WARP) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, TMEM_COLS);
+    }
+}
+
+// The sums of keys whose rows several blocks had, in the blocks' order.
+__global__ void __launch_bounds__(128) span_mass_merge_kernel(const MassArgs m) {
+    llb_after_previous();
+    const LlbSpanArgs& a = m.p.a;
+    const int* d = a.open + blockIdx.x * 4;
+    if (d[0] < 0) return;
+    float sum = m.part[(size_t)(blockIdx.x * 2 + 1) * 128 + threadIdx.x];
+    for (int b = blockIdx.x + 1; b <= d[3]; ++b) sum += m.part[(size_t)b * 2 * 128 + threadIdx.x];
+    add_mass(a, m.mass_in, m.mass, llb_span(a, d[0]), d[0], d[1] * BK + threadIdx.x, d[2], sum);
+}
+
+// q [T, Hq, hd] in boxes of the group's heads of `nodes` rows.
+int make_map_q(const void* q, int T, int Hq, int hd, int group, int nodes, CUtensorMap* out) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return llb_fail("cuTensorMapEncodeTiled is not available from the driver");
+    cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)Hq, (cuuint64_t)T};
+    cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)Hq * hd * 2};
+    cuuint32_t box[3] = {64u, (cuuint32_t)group, (cuuint32_t)nodes};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult rc = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return llb_fail("cuTensorMapEncodeTiled failed with code %d", (int)rc);
+    return 0;
+}
+
+// The softmax groups' registers come out of what the block was launched with: a build that gives a thread fewer is refused.
+template <int HD> bool registers_suffice() {
+    cudaFuncAttributes at;
+    return cudaFuncGetAttributes(&at, span_attention_tc_kernel<HD>) == cudaSuccess && at.numRegs * 3 >= 88 + 2 * 208;
+}
+template <int HD>
+int launch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& p, int blocks, cudaStream_t stream) {
+    static const bool suffice = registers_suffice<HD>();
+    LLB_REQUIRE(suffice, "span_attention_tcgen05: the kernel was built with too few registers a thread");
+    cudaError_t e = cudaFuncSetAttribute(span_attention_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<HD>::SMEM);
+    if (e == cudaSuccess) e = launch_pdl(span_attention_tc_kernel<HD>, dim3(blocks), dim3(NUM_THREADS), Shape<HD>::SMEM, stream, mq, mk, mv, p);
+    if (e != cudaSuccess) return llb_fail("span_attention_tcgen05: launch failed: %s", cudaGetErrorString(e));
+    return llb_check_launch("span_attention_tcgen05");
+}
+template <int HD> int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const MassArgs& m, int blocks, cudaStream_t stream) {
+    cudaError_t e = cudaFuncSetAttribute(span_mass_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MassShape<HD>::SMEM);
+    if (e == cudaSuccess) e = launch_pdl(span_mass_tc_kernel<HD>, dim3(blocks), dim3(NUM_THREADS), MassShape<HD>::SMEM, stream, mq, mk, m);
+    if (e != cudaSuccess) return llb_fail("span_mass_tcgen05: launch failed: %s", cudaGetErrorString(e));
+    return llb_check_launch("span_mass_tcgen05");
+}
+
+}  // namespace
+
+bool llb_span_tc_takes(const LlbSpanArgs& a, const void* q, const void* k, const void* v, const void* out) {
+    return (a.hd == 64 || a.hd == 128) && a.group <= 128 && a.page_size % 8 == 0 && a.page_size <= 128 && 128 % a.page_size == 0 &&
+           (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0 && a.scale_log2e > 0.0f;
+}
+int llb_span_tc_pairs(int group) { return 128 / group; }
+
+int llb_span_attention_tc(const LlbSpanArgs& a, const void* q, const void* k, const void* v, int blocks, int* error_flag, cudaStream_t stream) {
+    TcParams p;
+    p.a = a; p.v = (const __nv_bfloat16*)v; p.pairs_nodes = llb_span_tc_pairs(a.group); p.error_flag = error_flag;
+    CUtensorMap mq, mk, mv;
+    int rc;
+    if ((rc = make_map_q(q, a.T, a.Hq, a.hd, a.group, p.pairs_nodes, &mq))) return rc;
+    if ((rc = make_map_bf16(k, a.num_slots, (long long)a.Hkv * a.hd, a.page_size, &mk))) return rc;
+    if ((rc = make_map_bf16(v, a.num_slots, (long long)a.Hkv * a.hd, a.page_size, &mv))) return rc;
+    return a.hd == 64 ? launch_tc<64>(mq, mk, mv, p, blocks, stream) : launch_tc<128>(mq, mk, mv, p, blocks, stream);
+}
+
+int llb_span_mass_tc(const LlbSpanArgs& a, const void* q, const void* k, const float* mass_in, float* mass, float* part, int blocks, int* error_flag,
+                     cudaStream_t stream) {
+    MassArgs m;
+    m.p.a = a; m.p.v = nullptr; m.p.pairs_nodes = llb_span_tc_pairs(a.group); m.p.error_flag = error_flag;
+    m.mass_in = mass_in; m.mass = mass; m.part = part;
+    CUtensorMap mq, mk;
+    int rc;
+    if ((rc = make_map_q(q, a.T, a.Hq, a.hd, a.group, m.p.pairs_nodes, &mq))) return rc;
+    if ((rc = make_map_bf16(k, a.num_slots, (long long)a.Hkv * a.hd, a.page_size, &mk))) return rc;
+    if ((rc = a.hd == 64 ? launch_mass_tc<64>(mq, mk, m, blocks, stream) : launch_mass_tc<128>(mq, mk, m, blocks, stream))) return rc;
+    llb_launch(span_mass_merge_kernel, dim3(blocks), dim3(128), 0, stream, m);
+    return llb_check_launch("span_mass_merge");
+}
