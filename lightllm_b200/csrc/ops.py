@@ -1344,14 +1344,21 @@ def paged_decode_mma(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
 
 # ---- a cache that is drafted into and thinned out (csrc/span_attention.cu, csrc/cache_rows.cu) ---------------------------
-def _check_here(what: str, *tensors) -> None:
-    """Every tensor contiguous and on the current device, which the launch goes to."""
-    first = tensors[0].get_device()
-    device = torch.cuda.current_device() if first >= 0 else 0
+def _check_here(what: str, *tensors) -> int:
+    """The current device, which the launch goes to: every tensor is there, and contiguous."""
+    device = tensors[0].get_device()
     for t in tensors:
-        if t is not None and (t.get_device() != device or not t.is_contiguous()):
-            raise KernelError(f"{what}: a tensor of shape {tuple(t.shape)} on {t.device} must be contiguous and on cuda:{device}, "
-                              "the current device; there is no CPU path")
+        if t is not None and (t.get_device() != device or device < 0 or not t.is_contiguous()):
+            raise KernelError(f"{what}: a tensor of shape {tuple(t.shape)} on {t.device} must be contiguous and on the device of "
+                              "the others, a CUDA device; there is no CPU path")
+    if device != torch.cuda.current_device():
+        raise KernelError(f"{what}: the tensors are on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
+    return device
+
+
+def _stream_on(device: int) -> int:
+    """The stream of a launch (see :func:`_stream`), asked for by the device's number: no stream object is made."""
+    return _scoped_stream if _scoped_stream is not None else torch._C._cuda_getCurrentRawStream(device)
 
 
 def _check_spans(what: str, span_row, span_len, span_pos, block_table, page_size: int):
@@ -1386,14 +1393,30 @@ _span_scratch = {}
 
 
 def _span_scratch_floats(dt: int, T: int, S: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, num_slots: int,
-                         mass: int) -> int:
-    key = (dt, T, S, num_heads, num_kv_heads, head_dim, page_size, num_slots, mass, torch.cuda.current_device())
+                         mass: int, device: int) -> int:
+    key = (dt, T, S, num_heads, num_kv_heads, head_dim, page_size, num_slots, mass, device)
     n = _span_scratch.get(key)
     if n is None:
         if len(_span_scratch) > 4096:
             _span_scratch.clear()
         n = _span_scratch[key] = int(lib().llb_span_scratch_floats(*key[:-1]))
     return n
+
+
+_span_counters = {}
+
+
+def _counters_of_spans(device: int, stream: int) -> torch.Tensor:
+    """The counters by which the blocks of an attention over whole requests find each other, zero before and after every launch.  Calls
+    on one stream follow one another and share them; a graph gets its own, since it may be replayed beside anything."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(lib().llb_span_counters(), dtype=torch.int32, device=f"cuda:{device}")
+    counters = _span_counters.get((device, stream))
+    if counters is None:
+        counters = torch.zeros(lib().llb_span_counters(), dtype=torch.int32, device=f"cuda:{device}")
+        _span_counters[(device, stream)] = counters
+        _reset_on_error.append(counters)
+    return counters
 
 
 def tree_mask(parents) -> torch.Tensor:
@@ -1431,12 +1454,15 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     T, slots = q.shape[0], k_cache.shape[0]
     if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != T or mask.shape[1] == 0:
         raise KernelError(f"tree_attention: mask must be int64 [{T}, words], got {mask.dtype} {tuple(mask.shape)}")
-    _check_here("tree_attention", q, k_cache, v_cache, out, mask, span_row, span_len, span_pos, block_table)
-    scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, slots, 0), dtype=torch.float32, device=q.device)
+    device = _check_here("tree_attention", q, k_cache, v_cache, out, mask, span_row, span_len, span_pos, block_table)
+    stream = _stream_on(device)
+    scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, slots, 0, device),
+                          dtype=torch.float32, device=q.device)
     _check(lib().llb_tree_attention(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), dt, mask.data_ptr(), mask.shape[1], span_row.data_ptr(),
         span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, pages, page_size, slots, num_heads, num_kv_heads,
-        head_dim, scale, scratch.data_ptr(), async_error_flag(q.device).data_ptr(), _stream()))
+        head_dim, scale, scratch.data_ptr(), _counters_of_spans(device, stream).data_ptr(),
+        async_error_flag(q.device).data_ptr(), stream))
 
 
 def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, mass: torch.Tensor,
@@ -1461,13 +1487,15 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
             raise KernelError(f"paged_attention_mass: weights are float32 [{num_kv_heads}, {slots}], got {t.dtype} {tuple(t.shape)}")
     if max_len <= 0:
         raise KernelError(f"paged_attention_mass: max_len is {max_len}")
-    _check_here("paged_attention_mass", q, k_cache, v_cache, out, mass, mass_in, span_row, span_len, span_pos, block_table)
-    scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, slots, 2 if max_len == 1 else 1),
+    device = _check_here("paged_attention_mass", q, k_cache, v_cache, out, mass, mass_in, span_row, span_len, span_pos, block_table)
+    stream = _stream_on(device)
+    scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, slots, 2 if max_len == 1 else 1, device),
                           dtype=torch.float32, device=q.device)
     _check(lib().llb_paged_attention_mass(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), dt, None if mass_in is None else mass_in.data_ptr(),
         mass.data_ptr(), span_row.data_ptr(), span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, max_len, pages,
-        page_size, slots, num_heads, num_kv_heads, head_dim, scale, scratch.data_ptr(), async_error_flag(q.device).data_ptr(), _stream()))
+        page_size, slots, num_heads, num_kv_heads, head_dim, scale, scratch.data_ptr(), _counters_of_spans(device, stream).data_ptr(),
+        async_error_flag(q.device).data_ptr(), stream))
 
 
 def _check_planes(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor):
@@ -1504,11 +1532,12 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, targets: torch.Tens
             raise KernelError(f"tree_commit: tokens, parents, targets are int32 [{T}], count and next_token int32 [{S}], got {t.dtype} {tuple(t.shape)}")
     if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != S:
         raise KernelError(f"tree_commit: path must be int32 [{S}, width], got {path.dtype} {tuple(path.shape)}")
-    _check_here("tree_commit", tokens, parents, targets, k_cache, v_cache, span_row, span_len, span_pos, block_table, path, count, next_token)
+    device = _check_here("tree_commit", tokens, parents, targets, k_cache, v_cache, span_row, span_len, span_pos, block_table, path, count, next_token)
     _check(lib().llb_tree_commit(
         tokens.data_ptr(), parents.data_ptr(), targets.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), span_row.data_ptr(),
         span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, L, pages, page_size, slots,
-        heads * hd * k_cache.element_size(), path.data_ptr(), path.shape[1], count.data_ptr(), next_token.data_ptr(), _stream()))
+        heads * hd * k_cache.element_size(), path.data_ptr(), path.shape[1], count.data_ptr(), next_token.data_ptr(),
+        _stream_on(device)))
 
 
 def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor,
@@ -1541,11 +1570,11 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor
             raise KernelError(f"cache_evict: mass is float32 and positions int32 {shape}, got {t.dtype} {tuple(t.shape)}")
     if budget <= 0 or first < 0 or latest < 0 or first + latest > budget:
         raise KernelError(f"cache_evict: a budget of {budget} places does not hold the first {first} and the latest {latest}")
-    _check_here("cache_evict", k_cache, v_cache, mass, positions, lengths, ends, block_table, mass_out, positions_out)
+    device = _check_here("cache_evict", k_cache, v_cache, mass, positions, lengths, ends, block_table, mass_out, positions_out)
     _check(lib().llb_cache_evict(
         k_cache.data_ptr(), v_cache.data_ptr(), mass.data_ptr(), positions.data_ptr(), mass_out.data_ptr(), positions_out.data_ptr(),
         lengths.data_ptr(), ends.data_ptr(), block_table.data_ptr(), S, L, heads, pages, page_size, slots, hd * k_cache.element_size(),
-        budget, first, latest, _stream()))
+        budget, first, latest, _stream_on(device)))
 
 
 # Where the blocks that share a long row of logits meet (a 64-bit slot and a counter per row), per device.

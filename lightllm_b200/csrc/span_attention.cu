@@ -1,6 +1,5 @@
 // Attention over whole requests on CUDA cores, in 32-bit floats: rows with a tree mask or causal ones (see span_attention.cuh), any
-// head size up to 256, group and page size, float or bf16 inputs; the joining of cut jobs for this kernel and the tensor-core one;
-// and the sums of the weights that keys receive.
+// head size up to 256, group and page size, float or bf16 inputs; and the sums of the weights that keys receive.
 //
 //     x_ij = scale * q_i . k_j,   m_i = max_j x_ij,   l_i = sum_j 2^(x_ij - m_i),   out_i = sum_j 2^(x_ij - m_i) v_j / l_i
 //
@@ -66,7 +65,7 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
     float* v_s = k_s + KT * kp;                        // [KT][64 * NI]
     float* s_s = v_s + KT * 64 * NI;                   // [RB][SP]
     __shared__ float m_s[RB], l_s[RB], c_s[RB];
-    __shared__ int odd_s;
+    __shared__ int odd_s, flag_s;
     __shared__ LlbPiece piece_s;
     const int tid = threadIdx.x, ty = tid / CT, tx = tid % CT;
     llb_after_previous();
@@ -77,7 +76,6 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
     __syncthreads();
     const LlbPiece pc = piece_s;
     LlbJob job = pc.job;
-    if (tid == 0) a.open[blockIdx.x * 4] = -1;
     for (int t = pc.t0; t < pc.t1;) {
         const int rows = job.count(a) * a.group;
         const int k0 = t - job.begin, k1 = min(job.tiles, pc.t1 - job.begin);
@@ -157,11 +155,8 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
                 for (int j = c; j < KT; j += TPR) top = fmaxf(top, row[j]);
 #pragma unroll
                 for (int w = TPR / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-                if (a.scores && job.z.len == 1 && r < rows)
-                    for (int j = c; j < KT; j += TPR) {
-                        const int slot = key0 + j < job.keys ? llb_span_slot(a, job.s, key0 + j) : -1;
-                        if (slot >= 0) a.scores[(size_t)(job.kvh * a.group + r) * a.num_slots + slot] = row[j];
-                    }
+                if (a.scores && job.z.len == 1 && r < rows && job.begin + kt < a.score_tiles)
+                    for (int j = c; j < KT; j += TPR) a.scores[((size_t)(job.begin + kt) * a.group + r) * KT + j] = row[j];
                 const float m_old = m_s[r], m_new = fmaxf(m_old, top), use = m_new == -INFINITY ? 0.0f : m_new;
                 float sum = 0.0f;
                 for (int j = c; j < KT; j += TPR) {
@@ -218,6 +213,7 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
             }
         }
         const int part = llb_part_of(pc, job);
+        __syncthreads();                               // the scores have been read: their place serves the job's end
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = ty * 4 + i;
@@ -225,8 +221,7 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
             const float l = l_s[r], m = m_s[r];
             const int node = job.first + r / a.group, row = job.z.row + node, head = job.kvh * a.group + r % a.group;
             float* po = a.part_o + ((size_t)(blockIdx.x * 2 + max(part, 0)) * a.rows + r) * hd;
-            // a row that sees nothing has no sum and gets zeros; one whose visible scores are all minus infinity has none either: NaN
-            const float inv = l > 0.0f || m != -INFINITY || job.z.pos > 0 ? 1.0f / l : 0.0f;
+            const float inv = llb_inverse(m, l, job.z.pos);
             T* dst = (T*)a.out + ((size_t)row * a.Hq + head) * hd;
 #pragma unroll
             for (int d = 0; d < DPT; ++d) {
@@ -240,89 +235,42 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
                     float* ml = a.part_ml + ((size_t)(blockIdx.x * 2 + part) * a.rows + r) * 2;
                     ml[0] = m;
                     ml[1] = l;
-                } else if (a.lse) {
-                    a.lse[(size_t)row * a.Hq + head] = l == 0.0f ? INFINITY : m + log2f(l);
+                } else {
+                    if (a.lse) a.lse[(size_t)row * a.Hq + head] = llb_lse(m, l);
+                    s_s[2 * r] = m;
+                    s_s[2 * r + 1] = l;
                 }
             }
         }
-        if (tid == 0 && part == 1) {
-            int* d = a.open + blockIdx.x * 4;
-            d[0] = job.s; d[1] = job.first; d[2] = job.kvh; d[3] = llb_piece_owner(pc, job.begin + job.tiles - 1);
-        }
+        llb_finish_job<T, KT, NI == 1 ? 16 : 32>(a, pc, job, part, s_s, RB * SP, &flag_s, tid, [] { __syncthreads(); });
+        __syncthreads();                               // the next job's Q, maxima and sums take the places of this one's
         t = job.begin + k1;
         if (t < pc.t1) job.next(a, KT);
     }
 }
 
-// out = sum_b 2^(m_b - M) O_b / sum_b 2^(m_b - M) l_b over the blocks that hold parts of a job, in their order.  A block takes four
-// rows at a time; the parts' factors are worked out once a row.
-constexpr int MERGE_ROWS = 4, MERGE_PARTS = 512;
-template <typename T>
-__global__ void __launch_bounds__(THREADS) span_merge_kernel(const LlbSpanArgs a) {
-    __shared__ float w_s[MERGE_ROWS][MERGE_PARTS];
-    __shared__ float inv_s[MERGE_ROWS];
-    llb_after_previous();
-    const int* open = a.open + blockIdx.x * 4;
-    const int s = open[0];
-    if (s < 0) return;
-    const int first = open[1], kvh = open[2], count = open[3] - blockIdx.x + 1;
-    const LlbSpan z = llb_span(a, s);
-    const int rows = min(a.nodes, z.len - first) * a.group;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    auto part = [&](int b) { return (size_t)(blockIdx.x + b) * 2 + (b == 0 ? 1 : 0); };
-    for (int r0 = blockIdx.y * MERGE_ROWS; r0 < rows; r0 += gridDim.y * MERGE_ROWS) {
-        __syncthreads();
-        if (warp < MERGE_ROWS && r0 + warp < rows) {
-            const int r = r0 + warp;
-            float M = -INFINITY;
-            for (int b = lane; b < count; b += 32) M = fmaxf(M, a.part_ml[(part(b) * a.rows + r) * 2]);
-            M = llb_warp_max(M);
-            float L = 0.0f;
-            for (int b = lane; b < count; b += 32) {
-                const float m = a.part_ml[(part(b) * a.rows + r) * 2], l = a.part_ml[(part(b) * a.rows + r) * 2 + 1];
-                const float w = m == -INFINITY ? 0.0f : exp2f(m - M);
-                w_s[warp][b] = w;
-                // (0 * l: a part without visible keys has l = 0; a NaN of another part stays)
-                L += w * l;
-            }
-            L = llb_warp_sum(L);
-            if (lane == 0) {
-                inv_s[warp] = L > 0.0f || M != -INFINITY || z.pos > 0 ? 1.0f / L : 0.0f;
-                if (a.lse) a.lse[(size_t)(z.row + first + r / a.group) * a.Hq + kvh * a.group + r % a.group] = L == 0.0f ? INFINITY : M + log2f(L);
-            }
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < MERGE_ROWS * a.hd; i += THREADS) {
-            const int w = i / a.hd, d = i - w * a.hd, r = r0 + w;
-            if (r >= rows) break;
-            float acc = 0.0f;
-            for (int b = 0; b < count; ++b) acc = fmaf(w_s[w][b], a.part_o[(part(b) * a.rows + r) * a.hd + d], acc);
-            T* dst = (T*)a.out + ((size_t)(z.row + first + r / a.group) * a.Hq + kvh * a.group + r % a.group) * a.hd;
-            dst[d] = llb_from_float<T>(acc * inv_s[w]);
-        }
-    }
-}
-
-// What every key of requests of one row received: the sum of 2^(score - lse) over its kv head's query heads.
-struct MassParams {
-    LlbSpanArgs a;
-    const float* mass_in;       // [Hkv, num_slots] or null: zeros
-    float* mass;                // [Hkv, num_slots]; may be mass_in
-};
-__global__ void __launch_bounds__(THREADS) span_mass_of_scores_kernel(const MassParams p) {
-    const LlbSpanArgs& a = p.a;
+// What every key of requests of one row received: the sum of 2^(score - lse) over its kv head's query heads.  For requests of so many keys
+// that one block a kv head (llb_finish_job) would be slow at it.
+template <int TILE> __global__ void __launch_bounds__(THREADS) span_mass_of_scores_kernel(const LlbSpanArgs a) {
+    __shared__ int before_s;
     llb_after_previous();
     const int s = blockIdx.x / a.Hkv, kvh = blockIdx.x - s * a.Hkv;
     const LlbSpan z = llb_span(a, s);
     if (z.len != 1) return;
+    if (threadIdx.x < 32) {          // tiles of the requests before
+        int n = 0;
+        for (int i = threadIdx.x; i < s; i += 32) n += llb_span_tiles(a, llb_span(a, i), TILE);
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (threadIdx.x == 0) before_s = n + kvh * ((z.pos + TILE) / TILE);
+    }
+    __syncthreads();
     const float* lse = a.lse + (size_t)z.row * a.Hq + kvh * a.group;
     for (int key = blockIdx.y * THREADS + threadIdx.x; key <= z.pos; key += gridDim.y * THREADS) {
-        const int slot = llb_span_slot(a, s, key);
-        if (slot < 0) continue;
+        const int tile = before_s + key / TILE;
         float sum = 0.0f;
-        for (int g = 0; g < a.group; ++g) sum += exp2f(a.scores[(size_t)(kvh * a.group + g) * a.num_slots + slot] - lse[g]);
-        const size_t at = (size_t)kvh * a.num_slots + slot;
-        p.mass[at] = key < z.pos && p.mass_in ? p.mass_in[at] + sum : sum;
+        if (tile < a.score_tiles)
+            for (int g = 0; g < a.group; ++g) sum += exp2f(a.scores[((size_t)tile * a.group + g) * TILE + key % TILE] - lse[g]);
+        llb_add_mass(a, z, s, key, kvh, sum);
     }
 }
 
@@ -333,9 +281,6 @@ struct ColumnParams {
     LlbSpanArgs a;
     const void* q;
     const void* k;
-    const float* mass_in;
-    float* mass;
-    int blocks_x;
 };
 template <typename T>
 __global__ void __launch_bounds__(THREADS) span_mass_kernel(const ColumnParams p) {
@@ -415,11 +360,7 @@ __global__ void __launch_bounds__(THREADS) span_mass_kernel(const ColumnParams p
                 float total = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) total += sum_s[i][tid];
-                const int key = key0 + tid, slot = llb_span_slot(a, s, key);
-                if (slot >= 0) {
-                    const size_t at = (size_t)kvh * a.num_slots + slot;
-                    p.mass[at] = key < z.pos && p.mass_in ? p.mass_in[at] + total : total;
-                }
+                llb_add_mass(a, z, s, key0 + tid, kvh, total);
             }
         }
         tile -= tiles;
@@ -445,19 +386,15 @@ int launch_attention_hd(const SimtParams& p, int blocks, cudaStream_t stream) {
 
 }  // namespace
 
-int llb_span_merge(const LlbSpanArgs& a, int dtype, int blocks, cudaStream_t stream) {
-    LLB_REQUIRE(blocks <= MERGE_PARTS, "span_merge: %d blocks", blocks);
-    const int y = min(llb_ceil_div(a.rows, MERGE_ROWS), 16);
-    if (dtype == LLB_F32) llb_launch(span_merge_kernel<float>, dim3(blocks, y), dim3(THREADS), 0, stream, a);
-    else llb_launch(span_merge_kernel<__nv_bfloat16>, dim3(blocks, y), dim3(THREADS), 0, stream, a);
-    return llb_check_launch("span_merge");
-}
-
 namespace {
 
 // (row, head) pairs a job of the CUDA-core kernel holds: 16 where requests bring about that many or fewer on average.
 int simt_rows(int T, int S, int group) { return group <= 16 && (long long)T * group <= 16ll * S ? 16 : 64; }
-int simt_blocks() { return min(2 * llb_device_sms(), MERGE_PARTS); }
+int simt_blocks() { return min(2 * llb_device_sms(), LLB_SPAN_BLOCKS); }
+int tc_blocks() { return min(llb_device_sms(), LLB_SPAN_BLOCKS); }
+// Up to so many keys a request (by its block table) the block that joins a job adds up the weights as well: 8,192 keys of six heads are
+// about 3 us of one block, a launch of its own costs the call as much.
+constexpr long long JOINED_MASS_KEYS = 8192;
 
 int check(const LlbSpanArgs& a, int dtype) {
     LLB_REQUIRE(dtype == LLB_F32 || dtype == LLB_BF16, "span_attention: unknown dtype %d", dtype);
@@ -474,47 +411,43 @@ int check(const LlbSpanArgs& a, int dtype) {
 bool tc_sizes(int dtype, int hd, int page_size) {
     return dtype == LLB_BF16 && (hd == 64 || hd == 128) && page_size % 8 == 0 && page_size <= 128 && 128 % page_size == 0;
 }
-// Scratch: the partial results, the blocks' open jobs, the partial sums of the weights, lse, scores.
+// Scratch: the partial results, the partial sums of the weights, lse, scores.  (Requests share no pages, so that all tiles of one-row
+// requests hold no more keys than there are slots, and a piece of a tile each.)
 struct Layout {
-    long long part_o, part_ml, open, part_mass, lse, scores, floats;
+    long long part_o, part_ml, part_mass, lse, scores, score_tiles, floats;
 };
-Layout layout(int T, int Hq, int hd, int num_slots, int rows, int blocks, int mass) {
+Layout layout(int T, int S, int Hq, int group, int hd, int num_slots, int rows, int blocks, int tile, int mass) {
     Layout l;
     l.part_o = 0;
     l.part_ml = l.part_o + 2ll * blocks * rows * hd;
-    l.open = l.part_ml + 2ll * blocks * rows * 2;
-    l.part_mass = l.open + 4ll * blocks;
+    l.part_mass = l.part_ml + 2ll * blocks * rows * 2;
     l.lse = l.part_mass + (mass == 1 ? 2ll * blocks * 128 : 0);
-    l.scores = l.lse + (mass > 0 ? (long long)T * Hq : 0);
-    l.floats = l.scores + (mass == 2 ? (long long)Hq * num_slots : 0);
+    l.scores = (l.lse + (mass > 0 ? (long long)T * Hq : 0) + 3) & ~3ll;
+    l.score_tiles = mass == 2 ? ((long long)num_slots / tile + S) * (Hq / group) : 0;
+    l.floats = l.scores + l.score_tiles * group * tile;
     return l;
 }
 
 // mass as llb_span_scratch_floats; tc: on the tensor cores.
-int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtype, float* scratch, int mass, bool tc, float** part_mass,
-           int* error_flag, cudaStream_t stream) {
+int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtype, float* scratch, unsigned* counters, int mass, bool tc,
+           float** part_mass, int* error_flag, cudaStream_t stream) {
     const int rows = tc ? 2 * llb_span_tc_pairs(a.group) * a.group : simt_rows(a.T, a.S, a.group);
-    const int blocks = tc ? min(llb_device_sms(), MERGE_PARTS) : simt_blocks();
-    const Layout l = layout(a.T, a.Hq, a.hd, a.num_slots, rows, blocks, mass);
+    const int blocks = tc ? tc_blocks() : simt_blocks();
+    const Layout l = layout(a.T, a.S, a.Hq, a.group, a.hd, a.num_slots, rows, blocks, tc ? 128 : KT, mass);
     a.rows = rows;
     a.nodes = rows / a.group;
     a.part_o = scratch + l.part_o;
     a.part_ml = scratch + l.part_ml;
-    a.open = (int*)(scratch + l.open);
+    a.arrived = counters;
     a.lse = mass > 0 ? scratch + l.lse : nullptr;
     a.scores = mass == 2 ? scratch + l.scores : nullptr;
+    a.score_tiles = (int)min(l.score_tiles, 0x7fffffffll);
     *part_mass = scratch + l.part_mass;
-    int rc;
-    if (tc) {
-        rc = llb_span_attention_tc(a, q, k, v, blocks, error_flag, stream);
-    } else {
-        SimtParams p;
-        p.a = a; p.q = q; p.k = k; p.v = v;
-        if (dtype == LLB_F32) rc = rows == 16 ? launch_attention_hd<float, 16>(p, blocks, stream) : launch_attention_hd<float, 64>(p, blocks, stream);
-        else rc = rows == 16 ? launch_attention_hd<__nv_bfloat16, 16>(p, blocks, stream) : launch_attention_hd<__nv_bfloat16, 64>(p, blocks, stream);
-    }
-    if (rc) return rc;
-    return llb_span_merge(a, dtype, blocks, stream);
+    if (tc) return llb_span_attention_tc(a, q, k, v, blocks, error_flag, stream);
+    SimtParams p;
+    p.a = a; p.q = q; p.k = k; p.v = v;
+    if (dtype == LLB_F32) return rows == 16 ? launch_attention_hd<float, 16>(p, blocks, stream) : launch_attention_hd<float, 64>(p, blocks, stream);
+    return rows == 16 ? launch_attention_hd<__nv_bfloat16, 16>(p, blocks, stream) : launch_attention_hd<__nv_bfloat16, 64>(p, blocks, stream);
 }
 
 LlbSpanArgs span_args(const void* out, const int* span_row, const int* span_len, const int* span_pos, const int* table, int S, int T,
@@ -528,13 +461,16 @@ LlbSpanArgs span_args(const void* out, const int* span_row, const int* span_len,
 
 }  // namespace
 
+// Counters that the calls below take, zero before and after each: calls that may run at the same time have their own.
+LLB_EXPORT int llb_span_counters() { return 2 * LLB_SPAN_BLOCKS; }
+
 // Floats of scratch that the calls below take; `mass` 0: a tree, 1: with the keys' weights, 2: the same where max_len is 1.
 LLB_EXPORT long long llb_span_scratch_floats(int dtype, int T, int S, int Hq, int Hkv, int hd, int page_size, int num_slots, int mass) {
     if (Hkv <= 0 || Hq < Hkv || S <= 0) return 1;
     const int group = Hq / Hkv;
-    long long n = layout(T, Hq, hd, num_slots, simt_rows(T, S, group), simt_blocks(), mass).floats;
+    long long n = layout(T, S, Hq, group, hd, num_slots, simt_rows(T, S, group), simt_blocks(), KT, mass).floats;
     if (tc_sizes(dtype, hd, page_size) && group <= 128) {
-        const long long tc = layout(T, Hq, hd, num_slots, 2 * llb_span_tc_pairs(group) * group, min(llb_device_sms(), MERGE_PARTS), mass).floats;
+        const long long tc = layout(T, S, Hq, group, hd, num_slots, 2 * llb_span_tc_pairs(group) * group, tc_blocks(), 128, mass).floats;
         n = tc > n ? tc : n;
     }
     return n;
@@ -544,49 +480,53 @@ LLB_EXPORT long long llb_span_scratch_floats(int dtype, int T, int S, int Hq, in
 LLB_EXPORT int llb_tree_attention(const void* q, const void* k, const void* v, void* out, int dtype, const unsigned long long* mask,
                                   int words, const int* span_row, const int* span_len, const int* span_pos, const int* table, int S, int T,
                                   int max_pages, int page_size, int num_slots, int Hq, int Hkv, int hd, float scale, float* scratch,
-                                  int* error_flag, cudaStream_t stream) {
+                                  unsigned* counters, int* error_flag, cudaStream_t stream) {
     LlbSpanArgs a = span_args(out, span_row, span_len, span_pos, table, S, T, max_pages, page_size, num_slots, Hq, Hkv, hd, scale, 0);
     if (int rc = check(a, dtype)) return rc;
-    LLB_REQUIRE(words > 0 && words <= (1 << 20) && mask && scratch, "tree_attention: no mask or no scratch");
+    LLB_REQUIRE(words > 0 && words <= (1 << 20) && mask && scratch && counters, "tree_attention: no mask or no scratch");
     if (S == 0 || T == 0) return 0;
     a.mask = mask;
     a.words = words;
     a.max_len = words * 64;
     float* unused;
-    return attend(a, q, k, v, dtype, scratch, 0, tc_sizes(dtype, hd, page_size) && llb_span_tc_takes(a, q, k, v, out), &unused, error_flag, stream);
+    return attend(a, q, k, v, dtype, scratch, counters, 0, tc_sizes(dtype, hd, page_size) && llb_span_tc_takes(a, q, k, v, out), &unused, error_flag, stream);
 }
 
 // Causal; mass_in (may be null) and mass [Hkv, num_slots] float, may be the same.
 LLB_EXPORT int llb_paged_attention_mass(const void* q, const void* k, const void* v, void* out, int dtype, const float* mass_in, float* mass,
                                         const int* span_row, const int* span_len, const int* span_pos, const int* table, int S, int T,
                                         int max_len, int max_pages, int page_size, int num_slots, int Hq, int Hkv, int hd, float scale,
-                                        float* scratch, int* error_flag, cudaStream_t stream) {
+                                        float* scratch, unsigned* counters, int* error_flag, cudaStream_t stream) {
     LlbSpanArgs a = span_args(out, span_row, span_len, span_pos, table, S, T, max_pages, page_size, num_slots, Hq, Hkv, hd, scale, max_len);
     if (int rc = check(a, dtype)) return rc;
-    LLB_REQUIRE(max_len > 0 && mass && scratch, "paged_attention_mass: no weights, no scratch or rows");
+    LLB_REQUIRE(max_len > 0 && mass && scratch && counters, "paged_attention_mass: no weights, no scratch or rows");
     LLB_REQUIRE((long long)S * Hkv < (1ll << 31), "paged_attention_mass: too many requests");
     if (S == 0 || T == 0) return 0;
     const bool single = max_len == 1;
     const bool tc = tc_sizes(dtype, hd, page_size) && llb_span_tc_takes(a, q, k, v, out);
+    const bool joined = (long long)max_pages * page_size <= JOINED_MASS_KEYS;
     float* part_mass;
-    if (int rc = attend(a, q, k, v, dtype, scratch, single ? 2 : 1, tc, &part_mass, error_flag, stream)) return rc;
-    if (tc && !single) return llb_span_mass_tc(a, q, k, mass_in, mass, part_mass, min(llb_device_sms(), MERGE_PARTS), error_flag, stream);
+    a.mass_in = mass_in;
+    a.mass = single && !joined ? nullptr : mass;
+    if (int rc = attend(a, q, k, v, dtype, scratch, counters, single ? 2 : 1, tc, &part_mass, error_flag, stream)) return rc;
+    if (single && joined) return 0;
+    a.mass = mass;
     const int sms = llb_device_sms();
     if (single) {
-        MassParams p;
-        p.a = a; p.mass_in = mass_in; p.mass = mass;
         const long long keys = (long long)max_pages * page_size;
         const int y = (int)max(1ll, min((keys + THREADS - 1) / THREADS, (long long)llb_ceil_div(8 * sms, S * Hkv)));
-        llb_launch(span_mass_of_scores_kernel, dim3(S * Hkv, y), dim3(THREADS), 0, stream, p);
+        llb_launch(tc ? span_mass_of_scores_kernel<128> : span_mass_of_scores_kernel<KT>, dim3(S * Hkv, y), dim3(THREADS), 0, stream, a);
         return llb_check_launch("span_mass_of_scores");
     }
+    a.arrived = counters + LLB_SPAN_BLOCKS;
+    if (tc) return llb_span_mass_tc(a, q, k, part_mass, tc_blocks(), error_flag, stream);
     ColumnParams p;
-    p.a = a; p.q = q; p.k = k; p.mass_in = mass_in; p.mass = mass; p.blocks_x = 2 * sms;
+    p.a = a; p.q = q; p.k = k;
     const int hd4 = (hd + 3) & ~3;
     const size_t smem = sizeof(float) * ((size_t)64 * hd4 + KT * (hd4 + 4));
     auto kernel = dtype == LLB_F32 ? span_mass_kernel<float> : span_mass_kernel<__nv_bfloat16>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return llb_fail("span_mass: cannot opt in to %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
-    llb_launch(kernel, dim3(p.blocks_x), dim3(THREADS), smem, stream, p);
+    llb_launch(kernel, dim3(2 * sms), dim3(THREADS), smem, stream, p);
     return llb_check_launch("span_mass");
 }

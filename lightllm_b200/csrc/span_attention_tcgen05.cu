@@ -130,7 +130,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     constexpr uint32_t TMEM_COLS = 512;              // S (and P) of the groups: 0.., 128..; O: 256.., 384..
     __shared__ __align__(8) uint64_t bar_q_full[2], bar_q_free[2], bar_kv_full[RING], bar_kv_free[RING], bar_s[2], bar_p[2], bar_o[2];
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_s, odd_s;
+    __shared__ int abort_s, odd_s, join_s;
     __shared__ LlbPiece piece_s;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -161,10 +161,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     griddep_launch_dependents();
     if (warp == 0) {
         const LlbPiece pc = llb_piece(a, BK, blockIdx.x, gridDim.x, 2, lane);
-        if (lane == 0) {
-            piece_s = pc;
-            a.open[blockIdx.x * 4] = -1;
-        }
+        if (lane == 0) piece_s = pc;
     }
     tc_fence_before();
     __syncthreads();
@@ -314,7 +311,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const unsigned long long* mask = a.mask ? a.mask + (size_t)(z.row + node) * a.words : nullptr;
             const int all = a.mask ? z.pos : z.pos + job.first + 1;         // keys that every row of the job sees
             const int own = a.mask ? z.pos : z.pos + node + 1;              // first keys that this row sees
-            const bool scores = a.scores && z.len == 1 && mine;
+            const bool scores_of = a.scores && z.len == 1, scores = scores_of && mine;
             const bool busy = (warp & 3) * 32 < pairs;                      // any pair in this warp's lanes
             float m_ref = -INFINITY, l_run = 0.0f;
             for (int j = g.two ? 0 : x; j < n; j += step) {
@@ -340,7 +337,8 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                             for (int c = 0; c < 8; ++c) {
-                                uint4* at = reinterpret_cast<uint4*>(row + kb * TILE_BYTES + c * 16);
+                                // (neighbouring threads begin at other chunks: their rows lie in the same banks)
+                                uint4* at = reinterpret_cast<uint4*>(row + kb * TILE_BYTES + ((c ^ r) & 7) * 16);
                                 if (key >= job.keys) {
                                     *at = make_uint4(0u, 0u, 0u, 0u);
                                     continue;
@@ -377,17 +375,12 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             for (int i = 0; i < 32; ++i) s[32 * w + i] = (bits >> i) & 1u ? s[32 * w + i] : -INFINITY;
                         }
                     }
-                    if (scores) {
-                        float* to = a.scores + (size_t)(job.kvh * a.group + r) * a.num_slots;
+                    if (scores && job.begin + g.k0 + j < a.score_tiles) {
+                        float* to = a.scores + ((size_t)(job.begin + g.k0 + j) * a.group + r) * BK;
 #pragma unroll
-                        for (int c = 0; c < 128; c += 8) {
-                            const int key = key0 + c;         // (pages are multiples of 8 keys)
-                            const int slot = key < job.keys ? llb_span_slot(a, job.s, key) : -1;
-                            if (slot < 0) continue;
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if (slot + i < a.num_slots) to[slot + i] = s[c + i] * a.scale_log2e;
-                        }
+                        for (int c = 0; c < 128; c += 4)
+                            *reinterpret_cast<float4*>(to + c) = make_float4(s[c] * a.scale_log2e, s[c + 1] * a.scale_log2e,
+                                                                             s[c + 2] * a.scale_log2e, s[c + 3] * a.scale_log2e);
                     }
                     float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
 #pragma unroll
@@ -471,7 +464,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
             const int head = job.kvh * a.group + (mine ? r % a.group : 0), row = z.row + node;
             const int d0 = g.two ? 0 : x * (HD / 2), d1 = g.two ? HD : d0 + HD / 2;
-            const float inv = l_run > 0.0f || m_ref != -INFINITY || z.pos > 0 ? 1.0f / l_run : 0.0f;
+            const float inv = llb_inverse(m_ref, l_run, z.pos);
             const bool both = !g.two && n > 1;
             const bool odd = *(volatile int*)&odd_s != 0;
             if (busy) {
@@ -524,23 +517,30 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     }
                 }
             }
+            float* room = reinterpret_cast<float*>(q_s + buf * HALF);
             if (mine && ok && (g.two || x == 0)) {
                 if (g.part >= 0) {
                     float* ml = a.part_ml + ((size_t)(blockIdx.x * 2 + g.part) * a.rows + node0 * a.group + r) * 2;
                     ml[0] = m_ref;
                     ml[1] = l_run;
                 } else if (a.lse) {
-                    a.lse[(size_t)row * a.Hq + head] = l_run == 0.0f ? INFINITY : m_ref + log2f(l_run);
+                    a.lse[(size_t)row * a.Hq + head] = llb_lse(m_ref, l_run);
                 }
             }
-            if (g.part == 1 && threadIdx.x == 0) {
-                int* d = a.open + blockIdx.x * 4;
-                d[0] = job.s; d[1] = job.first; d[2] = job.kvh; d[3] = llb_piece_owner(pc, job.begin + job.tiles - 1);
+            if (g.part >= 0 || scores_of) {
+                // (what the groups exchanged in the buffer has been read, and of a job of two tiles of pairs the first one's Q)
+                if (g.two) room = reinterpret_cast<float*>(q_s);
+                named_barrier(BAR_PAIR, 256);
+                if (g.part < 0 && mine && x == 0) {
+                    room[2 * r] = m_ref;
+                    room[2 * r + 1] = l_run;
+                }
+                llb_finish_job<__nv_bfloat16, BK, HD / 4>(a, pc, job, g.part, room, HALF / 4, &join_s, threadIdx.x, [] { named_barrier(BAR_PAIR, 256); });
             }
             // O and Q are free for the next job (the groups have read each other's O)
             tc_fence_before();
             fence_async_smem();
-            if (!g.two) named_barrier(BAR_PAIR, 256);
+            if (!g.two || g.part >= 0) named_barrier(BAR_PAIR, 256);
             else named_barrier(BAR_PAIR + 1 + x, 128);
             if (r == 0 && (g.two || x == 0)) mbar_arrive(&bar_q_free[buf]);
             tiles_before += n;
@@ -567,8 +567,6 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 // the next is made while one is read.
 struct MassArgs {
     TcParams p;
-    const float* mass_in;
-    float* mass;
     float* part;                // [2 * blocks, 128]
 };
 struct MassJob {
@@ -646,13 +644,6 @@ __device__ __forceinline__ MassPiece mass_piece(const LlbSpanArgs& a, int pairs_
     p.job.begin += p.job.kvh * p.job.units;
     return p;
 }
-__device__ __forceinline__ void add_mass(const LlbSpanArgs& a, const float* mass_in, float* mass, const LlbSpan& z, int s, int key, int kvh, float sum) {
-    const int slot = key < z.pos + z.len ? llb_span_slot(a, s, key) : -1;
-    if (slot < 0) return;
-    const size_t at = (size_t)kvh * a.num_slots + slot;
-    mass[at] = key < z.pos && mass_in ? mass_in[at] + sum : sum;
-}
-
 template <int HD> struct MassShape {
     static constexpr int RING = HD == 64 ? 8 : 4;
     static constexpr size_t SMEM = (size_t)(2 + RING) * Shape<HD>::HALF + 1024;
@@ -666,7 +657,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     constexpr uint32_t TMEM_COLS = 512;              // two score tiles of each group
     __shared__ __align__(8) uint64_t bar_k_full[2], bar_k_free[2], bar_q_full[RING], bar_q_free[RING], bar_s[4], bar_free[4];
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_s;
+    __shared__ int abort_s, join_s;
     __shared__ MassPiece piece_s;
     __shared__ __align__(16) float lse_s[2][2][128];
     __shared__ float sum_s[128];
@@ -705,10 +696,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     griddep_launch_dependents();
     if (warp == 0) {
         const MassPiece pc = mass_piece(a, pairs_nodes, blockIdx.x, gridDim.x, lane);
-        if (lane == 0) {
-            piece_s = pc;
-            a.open[blockIdx.x * 4] = -1;
-        }
+        if (lane == 0) piece_s = pc;
     }
     tc_fence_before();
     __syncthreads();
@@ -849,16 +837,28 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             float sum = (sum0 + sum1) + (sum2 + sum3);
             if (x == 1) sum_s[r] = sum;
             named_barrier(BAR_PAIR, 256);
-            if (x == 0 && ok) {
+            if (x == 0) {
                 sum += sum_s[r];
                 const int part = job.begin < pc.t0 ? 0 : job.begin + job.units > pc.t1 ? 1 : -1;
-                if (part >= 0) m.part[(size_t)(blockIdx.x * 2 + part) * 128 + r] = sum;
-                else add_mass(a, m.mass_in, m.mass, z, job.s, key, job.kvh, sum);
-                if (part == 1 && r == 0) {
-                    int* d = a.open + blockIdx.x * 4;
-                    d[0] = job.s; d[1] = job.tile; d[2] = job.kvh;
-                    d[3] = (int)(((long long)(job.begin + job.units) * pc.blocks + pc.total - 1) / pc.total) - 1;
+                auto owner = [&](int at) { return (int)(((long long)(at + 1) * pc.blocks + pc.total - 1) / pc.total) - 1; };
+                bool joined = true;
+                if (part >= 0) {
+                    // the last block that leaves a part of the sums adds them up, in the blocks' order
+                    const int from = owner(job.begin), parts = owner(job.begin + job.units - 1) - from + 1;
+                    m.part[(size_t)(blockIdx.x * 2 + part) * 128 + r] = sum;
+                    __threadfence();
+                    named_barrier(BAR_PAIR + 1, 128);
+                    if (r == 0) join_s = atomicInc(a.arrived + from, parts - 1) == (unsigned)parts - 1;
+                    named_barrier(BAR_PAIR + 1, 128);
+                    joined = join_s;
+                    if (joined) {
+                        __threadfence();
+                        sum = 0.0f;
+#pragma unroll 4
+                        for (int i = 0; i < parts; ++i) sum += __ldcg(m.part + (size_t)((from + i) * 2 + (i == 0 ? 1 : 0)) * 128 + r);
+                    }
                 }
+                if (joined && ok) llb_add_mass(a, z, job.s, key, job.kvh, sum);
             }
             named_barrier(BAR_PAIR, 256);
             if (threadIdx.x == 0) mbar_arrive(&bar_k_free[jobs & 1]);          // both groups have had all scores of the job
@@ -875,17 +875,6 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         tc_fence_after();
         tmem_dealloc(tmem_base, TMEM_COLS);
     }
-}
-
-// The sums of keys whose rows several blocks had, in the blocks' order.
-__global__ void __launch_bounds__(128) span_mass_merge_kernel(const MassArgs m) {
-    llb_after_previous();
-    const LlbSpanArgs& a = m.p.a;
-    const int* d = a.open + blockIdx.x * 4;
-    if (d[0] < 0) return;
-    float sum = m.part[(size_t)(blockIdx.x * 2 + 1) * 128 + threadIdx.x];
-    for (int b = blockIdx.x + 1; b <= d[3]; ++b) sum += m.part[(size_t)b * 2 * 128 + threadIdx.x];
-    add_mass(a, m.mass_in, m.mass, llb_span(a, d[0]), d[0], d[1] * BK + threadIdx.x, d[2], sum);
 }
 
 // q [T, Hq, hd] in boxes of the group's heads of `nodes` rows.
@@ -942,16 +931,13 @@ int llb_span_attention_tc(const LlbSpanArgs& a, const void* q, const void* k, co
     return a.hd == 64 ? launch_tc<64>(mq, mk, mv, p, blocks, stream) : launch_tc<128>(mq, mk, mv, p, blocks, stream);
 }
 
-int llb_span_mass_tc(const LlbSpanArgs& a, const void* q, const void* k, const float* mass_in, float* mass, float* part, int blocks, int* error_flag,
-                     cudaStream_t stream) {
+int llb_span_mass_tc(const LlbSpanArgs& a, const void* q, const void* k, float* part, int blocks, int* error_flag, cudaStream_t stream) {
     MassArgs m;
     m.p.a = a; m.p.v = nullptr; m.p.pairs_nodes = llb_span_tc_pairs(a.group); m.p.error_flag = error_flag;
-    m.mass_in = mass_in; m.mass = mass; m.part = part;
+    m.part = part;
     CUtensorMap mq, mk;
     int rc;
     if ((rc = make_map_q(q, a.T, a.Hq, a.hd, a.group, m.p.pairs_nodes, &mq))) return rc;
     if ((rc = make_map_bf16(k, a.num_slots, (long long)a.Hkv * a.hd, a.page_size, &mk))) return rc;
-    if ((rc = a.hd == 64 ? launch_mass_tc<64>(mq, mk, m, blocks, stream) : launch_mass_tc<128>(mq, mk, m, blocks, stream))) return rc;
-    llb_launch(span_mass_merge_kernel, dim3(blocks), dim3(128), 0, stream, m);
-    return llb_check_launch("span_mass_merge");
+    return a.hd == 64 ? launch_mass_tc<64>(mq, mk, m, blocks, stream) : launch_mass_tc<128>(mq, mk, m, blocks, stream);
 }
