@@ -1403,22 +1403,6 @@ def _span_scratch_floats(dt: int, T: int, S: int, num_heads: int, num_kv_heads: 
     return n
 
 
-_span_counters = {}
-
-
-def _counters_of_spans(device: int, stream: int) -> torch.Tensor:
-    """The counters by which the blocks of an attention over whole requests find each other, zero before and after every launch.  Calls
-    on one stream follow one another and share them; a graph gets its own, since it may be replayed beside anything."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(lib().llb_span_counters(), dtype=torch.int32, device=f"cuda:{device}")
-    counters = _span_counters.get((device, stream))
-    if counters is None:
-        counters = torch.zeros(lib().llb_span_counters(), dtype=torch.int32, device=f"cuda:{device}")
-        _span_counters[(device, stream)] = counters
-        _reset_on_error.append(counters)
-    return counters
-
-
 def tree_mask(parents) -> torch.Tensor:
     """The masks of drafted trees for :func:`tree_attention`, int64 [nodes, words] on the CPU: ``parents`` holds a sequence of
     parents for every request, node 0 its root (-1), a parent always before its children.  A node sees itself and its ancestors."""
@@ -1461,8 +1445,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _check(lib().llb_tree_attention(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), dt, mask.data_ptr(), mask.shape[1], span_row.data_ptr(),
         span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, pages, page_size, slots, num_heads, num_kv_heads,
-        head_dim, scale, scratch.data_ptr(), _counters_of_spans(device, stream).data_ptr(),
-        async_error_flag(q.device).data_ptr(), stream))
+        head_dim, scale, scratch.data_ptr(), async_error_flag(q.device).data_ptr(), stream))
 
 
 def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, mass: torch.Tensor,
@@ -1494,8 +1477,7 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     _check(lib().llb_paged_attention_mass(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), dt, None if mass_in is None else mass_in.data_ptr(),
         mass.data_ptr(), span_row.data_ptr(), span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, max_len, pages,
-        page_size, slots, num_heads, num_kv_heads, head_dim, scale, scratch.data_ptr(), _counters_of_spans(device, stream).data_ptr(),
-        async_error_flag(q.device).data_ptr(), stream))
+        page_size, slots, num_heads, num_kv_heads, head_dim, scale, scratch.data_ptr(), async_error_flag(q.device).data_ptr(), stream))
 
 
 def _check_planes(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor):

@@ -1,5 +1,6 @@
 // Attention over whole requests on CUDA cores, in 32-bit floats: rows with a tree mask or causal ones (see span_attention.cuh), any
-// head size up to 256, group and page size, float or bf16 inputs; and the sums of the weights that keys receive.
+// head size up to 256, group and page size, float or bf16 inputs; the joining of cut jobs for this kernel and the tensor-core one;
+// and the sums of the weights that keys receive.
 //
 //     x_ij = scale * q_i . k_j,   m_i = max_j x_ij,   l_i = sum_j 2^(x_ij - m_i),   out_i = sum_j 2^(x_ij - m_i) v_j / l_i
 //
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
     float* v_s = k_s + KT * kp;                        // [KT][64 * NI]
     float* s_s = v_s + KT * 64 * NI;                   // [RB][SP]
     __shared__ float m_s[RB], l_s[RB], c_s[RB];
-    __shared__ int odd_s, flag_s;
+    __shared__ int odd_s;
     __shared__ LlbPiece piece_s;
     const int tid = threadIdx.x, ty = tid / CT, tx = tid % CT;
     llb_after_previous();
@@ -76,6 +77,7 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
     __syncthreads();
     const LlbPiece pc = piece_s;
     LlbJob job = pc.job;
+    if (tid == 0) llb_leave_open(a, pc, job, false);
     for (int t = pc.t0; t < pc.t1;) {
         const int rows = job.count(a) * a.group;
         const int k0 = t - job.begin, k1 = min(job.tiles, pc.t1 - job.begin);
@@ -213,7 +215,6 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
             }
         }
         const int part = llb_part_of(pc, job);
-        __syncthreads();                               // the scores have been read: their place serves the job's end
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = ty * 4 + i;
@@ -235,43 +236,179 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
                     float* ml = a.part_ml + ((size_t)(blockIdx.x * 2 + part) * a.rows + r) * 2;
                     ml[0] = m;
                     ml[1] = l;
-                } else {
-                    if (a.lse) a.lse[(size_t)row * a.Hq + head] = llb_lse(m, l);
-                    s_s[2 * r] = m;
-                    s_s[2 * r + 1] = l;
+                } else if (a.lse) {
+                    a.lse[(size_t)row * a.Hq + head] = llb_lse(m, l);
                 }
             }
         }
-        llb_finish_job<T, KT, NI == 1 ? 16 : 32>(a, pc, job, part, s_s, RB * SP, &flag_s, tid, [] { __syncthreads(); });
+        if (tid == 0 && part == 1) llb_leave_open(a, pc, job, true);
         __syncthreads();                               // the next job's Q, maxima and sums take the places of this one's
         t = job.begin + k1;
         if (t < pc.t1) job.next(a, KT);
     }
 }
 
-// What every key of requests of one row received: the sum of 2^(score - lse) over its kv head's query heads.  For requests of so many keys
-// that one block a kv head (llb_finish_job) would be slow at it.
-template <int TILE> __global__ void __launch_bounds__(THREADS) span_mass_of_scores_kernel(const LlbSpanArgs a) {
-    __shared__ int before_s;
-    llb_after_previous();
-    const int s = blockIdx.x / a.Hkv, kvh = blockIdx.x - s * a.Hkv;
+// out = sum_b 2^(m_b - M) O_b / sum_b 2^(m_b - M) l_b over the blocks that hold parts of a job, in their order, with a running maximum
+// so that O is asked for together with m and l: a trip to memory after the one for what there is to join.  TPR threads have a row, four
+// dimensions each; PB parts of RU rows are on their way at once.
+template <typename T, int TPR, int PB, int RU>
+__device__ __forceinline__ void join_rows(const LlbSpanArgs& a, const LlbOpen& job, int block, int y, int ny) {
+    constexpr int RPP = THREADS / TPR;
+    const int hd = a.hd, pieces = (hd + 3) / 4;
+    const bool whole = hd % 4 == 0;
+    for (int r0 = y * (RPP * RU) + threadIdx.x / TPR; r0 < job.rows; r0 += ny * (RPP * RU)) {
+        for (int piece = threadIdx.x % TPR; piece < pieces; piece += TPR) {
+            const int d = piece * 4;
+            float x[RU][4], M[RU], L[RU];
+#pragma unroll
+            for (int u = 0; u < RU; ++u) {
+                x[u][0] = x[u][1] = x[u][2] = x[u][3] = L[u] = 0.0f;
+                M[u] = -INFINITY;
+            }
+            for (int b0 = 0; b0 < job.parts; b0 += PB) {
+                float4 v[RU][PB];
+                float2 ml[RU][PB];
+#pragma unroll
+                for (int u = 0; u < RU; ++u)
+#pragma unroll
+                    for (int e = 0; e < PB; ++e) {
+                        const int r = r0 + u * RPP, b = b0 + e;
+                        ml[u][e] = make_float2(-INFINITY, 0.0f);
+                        v[u][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (r >= job.rows || b >= job.parts) continue;
+                        const size_t at = ((size_t)(block + b) * 2 + (b == 0 ? 1 : 0)) * a.rows + r;
+                        ml[u][e] = reinterpret_cast<const float2*>(a.part_ml)[at];
+                        const float* o = a.part_o + at * hd + d;
+                        if (whole) v[u][e] = *reinterpret_cast<const float4*>(o);
+                        else v[u][e] = make_float4(o[0], d + 1 < hd ? o[1] : 0.0f, d + 2 < hd ? o[2] : 0.0f, d + 3 < hd ? o[3] : 0.0f);
+                    }
+#pragma unroll
+                for (int u = 0; u < RU; ++u) {
+                    float top = M[u];
+#pragma unroll
+                    for (int e = 0; e < PB; ++e) top = fmaxf(top, ml[u][e].x);
+                    const float keep = M[u] == -INFINITY ? 1.0f : exp2f(M[u] - top);          // (nothing, or a NaN, which stays)
+                    x[u][0] *= keep; x[u][1] *= keep; x[u][2] *= keep; x[u][3] *= keep;
+                    L[u] *= keep;
+                    M[u] = top;
+#pragma unroll
+                    for (int e = 0; e < PB; ++e) {
+                        // (a part without visible keys has m = -infinity, l = 0 and O = 0; a NaN of another one stays)
+                        const float w = ml[u][e].x == -INFINITY ? 1.0f : exp2f(ml[u][e].x - top);
+                        L[u] = fmaf(w, ml[u][e].y, L[u]);
+                        x[u][0] = fmaf(w, v[u][e].x, x[u][0]);
+                        x[u][1] = fmaf(w, v[u][e].y, x[u][1]);
+                        x[u][2] = fmaf(w, v[u][e].z, x[u][2]);
+                        x[u][3] = fmaf(w, v[u][e].w, x[u][3]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < RU; ++u) {
+                const int r = r0 + u * RPP;
+                if (r >= job.rows) continue;
+                const int node = r / a.group, row = job.row + node, head = job.kvh * a.group + r - node * a.group;
+                const float inv = llb_inverse(M[u], L[u], job.pos);
+                if (a.lse && piece == 0) a.lse[(size_t)row * a.Hq + head] = llb_lse(M[u], L[u]);
+                T* dst = (T*)a.out + ((size_t)row * a.Hq + head) * hd + d;
+                if (whole && sizeof(T) == 2 && ((uintptr_t)dst & 7) == 0) {
+                    const __nv_bfloat162 lo = __floats2bfloat162_rn(x[u][0] * inv, x[u][1] * inv), hi = __floats2bfloat162_rn(x[u][2] * inv, x[u][3] * inv);
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const unsigned*>(&lo), *reinterpret_cast<const unsigned*>(&hi));
+                    continue;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < hd) dst[e] = llb_from_float<T>(x[u][e] * inv);
+            }
+        }
+    }
+}
+
+// What every key of a request of one row received: the sum of 2^(score - lse) over its kv head's query heads.  The row's lse is what the
+// attention kernel left, or, for a cut job, what its parts come to; which that is follows from the lengths, so that these blocks need
+// not wait for those that join.
+template <int TILE> __device__ __forceinline__ void mass_of_scores(const LlbSpanArgs& a, int grid, int least, int pair, int y, int ny) {
+    __shared__ int before_s, total_s;
+    __shared__ float lse_s[128];
+    const int s = pair / a.Hkv, kvh = pair - s * a.Hkv;
     const LlbSpan z = llb_span(a, s);
     if (z.len != 1) return;
-    if (threadIdx.x < 32) {          // tiles of the requests before
-        int n = 0;
-        for (int i = threadIdx.x; i < s; i += 32) n += llb_span_tiles(a, llb_span(a, i), TILE);
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (threadIdx.x == 0) before_s = n + kvh * ((z.pos + TILE) / TILE);
+    // the first key's cache row and what it had, on their way before anything is waited for
+    int key = y * THREADS + threadIdx.x;
+    int slot = key <= z.pos ? llb_span_slot(a, s, key) : -1;
+    float had = slot >= 0 && key < z.pos && a.mass_in ? a.mass_in[(size_t)kvh * a.num_slots + slot] : 0.0f;
+    if (threadIdx.x < 32) {
+        int before = 0, total = 0;
+        for (int i = threadIdx.x; i < a.S; i += 32) {
+            const int n = llb_span_tiles(a, llb_span(a, i), TILE);
+            total += n;
+            if (i < s) before += n;
+        }
+        before = __reduce_add_sync(0xffffffffu, before);
+        total = __reduce_add_sync(0xffffffffu, total);
+        if (threadIdx.x == 0) {
+            before_s = before;
+            total_s = total;
+        }
     }
     __syncthreads();
-    const float* lse = a.lse + (size_t)z.row * a.Hq + kvh * a.group;
-    for (int key = blockIdx.y * THREADS + threadIdx.x; key <= z.pos; key += gridDim.y * THREADS) {
-        const int tile = before_s + key / TILE;
-        float sum = 0.0f;
-        if (tile < a.score_tiles)
-            for (int g = 0; g < a.group; ++g) sum += exp2f(a.scores[((size_t)tile * a.group + g) * TILE + key % TILE] - lse[g]);
-        llb_add_mass(a, z, s, key, kvh, sum);
+    const int tiles = (z.pos + TILE) / TILE, begin = before_s + kvh * tiles;
+    LlbPiece pc;
+    pc.total = total_s;
+    pc.blocks = min(grid, (pc.total + least - 1) / least);
+    const int from = llb_piece_owner(pc, begin), parts = llb_piece_owner(pc, begin + tiles - 1) - from + 1;
+    for (int g = threadIdx.x; g < a.group; g += THREADS) {
+        float lse;
+        if (parts == 1) lse = a.lse[(size_t)z.row * a.Hq + kvh * a.group + g];
+        else {
+            const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)from * 2 * a.rows + g;
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll 8
+            for (int b = 0; b < parts; ++b) M = fmaxf(M, ml[(size_t)(b == 0 ? 1 : 2 * b) * a.rows].x);
+#pragma unroll 8
+            for (int b = 0; b < parts; ++b) {
+                const float2 x = ml[(size_t)(b == 0 ? 1 : 2 * b) * a.rows];
+                L = fmaf(x.x == -INFINITY ? 1.0f : exp2f(x.x - M), x.y, L);
+            }
+            lse = llb_lse(M, L);
+        }
+        lse_s[g] = lse;
     }
+    __syncthreads();
+    for (; key <= z.pos; key += ny * THREADS) {
+        if (slot >= 0) {
+            const int tile = begin + key / TILE;
+            float sum = 0.0f;
+            if (tile < a.score_tiles)
+#pragma unroll 8
+                for (int g = 0; g < a.group; ++g) sum += exp2f(a.scores[((size_t)tile * a.group + g) * TILE + key % TILE] - lse_s[g]);
+            a.mass[(size_t)kvh * a.num_slots + slot] = had + sum;
+        }
+        const int next = key + ny * THREADS;
+        slot = next <= z.pos ? llb_span_slot(a, s, next) : -1;
+        had = slot >= 0 && next < z.pos && a.mass_in ? a.mass_in[(size_t)kvh * a.num_slots + slot] : 0.0f;
+    }
+}
+
+// The first `blocks * ny` blocks join, the others add up weights, `mass_y` of them a request and kv head.
+template <typename T, int TPR, int TILE>
+__global__ void __launch_bounds__(THREADS) span_join_kernel(const LlbSpanArgs a, int blocks, int ny, int mass_y, int least) {
+    llb_after_previous();
+    const int i = blockIdx.x;
+    if (i >= blocks * ny) {
+        const int pair = (i - blocks * ny) / mass_y;
+        mass_of_scores<TILE>(a, blocks, least, pair, i - blocks * ny - pair * mass_y, mass_y);
+        return;
+    }
+    const int y = i / blocks, block = i - y * blocks;
+    LlbOpen job;
+    const int4* from = reinterpret_cast<const int4*>(a.open) + 2 * block;
+    const int4 lo = from[0];
+    job.pos = from[1].x;
+    job.parts = lo.x; job.row = lo.y; job.rows = lo.z; job.kvh = lo.w;
+    if (job.parts == 0) return;
+    if (job.parts <= 2) join_rows<T, TPR, 2, 4>(a, job, block, y, ny);
+    else join_rows<T, TPR, 8, 1>(a, job, block, y, ny);
 }
 
 // The same for requests of any number of rows: 64 keys of one request and kv head stay in shared memory, all rows that see any of them
@@ -367,6 +504,19 @@ __global__ void __launch_bounds__(THREADS) span_mass_kernel(const ColumnParams p
     }
 }
 
+template <typename T, int TPR, int TILE>
+int launch_join(const LlbSpanArgs& a, int blocks, int least, cudaStream_t stream) {
+    // a block of the first kind has 8 or 16 rows at a time: as many as the average job brings, up to four rounds
+    const int average = (int)max(1ll, min((long long)a.rows, (long long)a.T * a.group / max(1, a.S)));
+    const int ny = min(16, llb_ceil_div(average, THREADS / TPR));
+    int mass_y = 0;
+    if (a.scores) {
+        const long long keys = (long long)a.max_pages * a.page_size;
+        mass_y = (int)max(1ll, min((keys + THREADS - 1) / THREADS, (long long)llb_ceil_div(8 * llb_device_sms(), a.S * a.Hkv)));
+    }
+    llb_launch(span_join_kernel<T, TPR, TILE>, dim3(blocks * ny + a.S * a.Hkv * mass_y), dim3(THREADS), 0, stream, a, blocks, ny, mass_y, least);
+    return llb_check_launch("span_join");
+}
 template <typename T, int RB, int NI>
 int launch_attention(const SimtParams& p, int blocks, cudaStream_t stream) {
     const int hd4 = (p.a.hd + 3) & ~3;
@@ -386,15 +536,20 @@ int launch_attention_hd(const SimtParams& p, int blocks, cudaStream_t stream) {
 
 }  // namespace
 
+int llb_span_join(const LlbSpanArgs& a, int dtype, int blocks, int tile, int least, cudaStream_t stream) {
+    const bool narrow = a.hd <= 64;
+    if (dtype == LLB_F32) return narrow ? launch_join<float, 16, KT>(a, blocks, least, stream) : launch_join<float, 32, KT>(a, blocks, least, stream);
+    if (tile == KT)
+        return narrow ? launch_join<__nv_bfloat16, 16, KT>(a, blocks, least, stream) : launch_join<__nv_bfloat16, 32, KT>(a, blocks, least, stream);
+    return narrow ? launch_join<__nv_bfloat16, 16, 128>(a, blocks, least, stream) : launch_join<__nv_bfloat16, 32, 128>(a, blocks, least, stream);
+}
+
 namespace {
 
 // (row, head) pairs a job of the CUDA-core kernel holds: 16 where requests bring about that many or fewer on average.
 int simt_rows(int T, int S, int group) { return group <= 16 && (long long)T * group <= 16ll * S ? 16 : 64; }
 int simt_blocks() { return min(2 * llb_device_sms(), LLB_SPAN_BLOCKS); }
 int tc_blocks() { return min(llb_device_sms(), LLB_SPAN_BLOCKS); }
-// Up to so many keys a request (by its block table) the block that joins a job adds up the weights as well: 8,192 keys of six heads are
-// about 3 us of one block, a launch of its own costs the call as much.
-constexpr long long JOINED_MASS_KEYS = 8192;
 
 int check(const LlbSpanArgs& a, int dtype) {
     LLB_REQUIRE(dtype == LLB_F32 || dtype == LLB_BF16, "span_attention: unknown dtype %d", dtype);
@@ -414,13 +569,14 @@ bool tc_sizes(int dtype, int hd, int page_size) {
 // Scratch: the partial results, the partial sums of the weights, lse, scores.  (Requests share no pages, so that all tiles of one-row
 // requests hold no more keys than there are slots, and a piece of a tile each.)
 struct Layout {
-    long long part_o, part_ml, part_mass, lse, scores, score_tiles, floats;
+    long long part_o, part_ml, open, part_mass, lse, scores, score_tiles, floats;
 };
 Layout layout(int T, int S, int Hq, int group, int hd, int num_slots, int rows, int blocks, int tile, int mass) {
     Layout l;
     l.part_o = 0;
     l.part_ml = l.part_o + 2ll * blocks * rows * hd;
-    l.part_mass = l.part_ml + 2ll * blocks * rows * 2;
+    l.open = (l.part_ml + 2ll * blocks * rows * 2 + 3) & ~3ll;
+    l.part_mass = l.open + 8ll * blocks;
     l.lse = l.part_mass + (mass == 1 ? 2ll * blocks * 128 : 0);
     l.scores = (l.lse + (mass > 0 ? (long long)T * Hq : 0) + 3) & ~3ll;
     l.score_tiles = mass == 2 ? ((long long)num_slots / tile + S) * (Hq / group) : 0;
@@ -429,7 +585,7 @@ Layout layout(int T, int S, int Hq, int group, int hd, int num_slots, int rows, 
 }
 
 // mass as llb_span_scratch_floats; tc: on the tensor cores.
-int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtype, float* scratch, unsigned* counters, int mass, bool tc,
+int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtype, float* scratch, int mass, bool tc,
            float** part_mass, int* error_flag, cudaStream_t stream) {
     const int rows = tc ? 2 * llb_span_tc_pairs(a.group) * a.group : simt_rows(a.T, a.S, a.group);
     const int blocks = tc ? tc_blocks() : simt_blocks();
@@ -438,16 +594,21 @@ int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtyp
     a.nodes = rows / a.group;
     a.part_o = scratch + l.part_o;
     a.part_ml = scratch + l.part_ml;
-    a.arrived = counters;
+    a.open = (int*)(scratch + l.open);
     a.lse = mass > 0 ? scratch + l.lse : nullptr;
     a.scores = mass == 2 ? scratch + l.scores : nullptr;
     a.score_tiles = (int)min(l.score_tiles, 0x7fffffffll);
     *part_mass = scratch + l.part_mass;
-    if (tc) return llb_span_attention_tc(a, q, k, v, blocks, error_flag, stream);
+    int rc;
+    if (tc) {
+        rc = llb_span_attention_tc(a, q, k, v, blocks, error_flag, stream);
+        return rc ? rc : llb_span_join(a, dtype, blocks, 128, LLB_SPAN_TC_LEAST, stream);
+    }
     SimtParams p;
     p.a = a; p.q = q; p.k = k; p.v = v;
-    if (dtype == LLB_F32) return rows == 16 ? launch_attention_hd<float, 16>(p, blocks, stream) : launch_attention_hd<float, 64>(p, blocks, stream);
-    return rows == 16 ? launch_attention_hd<__nv_bfloat16, 16>(p, blocks, stream) : launch_attention_hd<__nv_bfloat16, 64>(p, blocks, stream);
+    if (dtype == LLB_F32) rc = rows == 16 ? launch_attention_hd<float, 16>(p, blocks, stream) : launch_attention_hd<float, 64>(p, blocks, stream);
+    else rc = rows == 16 ? launch_attention_hd<__nv_bfloat16, 16>(p, blocks, stream) : launch_attention_hd<__nv_bfloat16, 64>(p, blocks, stream);
+    return rc ? rc : llb_span_join(a, dtype, blocks, KT, 1, stream);
 }
 
 LlbSpanArgs span_args(const void* out, const int* span_row, const int* span_len, const int* span_pos, const int* table, int S, int T,
@@ -460,9 +621,6 @@ LlbSpanArgs span_args(const void* out, const int* span_row, const int* span_len,
 }
 
 }  // namespace
-
-// Counters that the calls below take, zero before and after each: calls that may run at the same time have their own.
-LLB_EXPORT int llb_span_counters() { return 2 * LLB_SPAN_BLOCKS; }
 
 // Floats of scratch that the calls below take; `mass` 0: a tree, 1: with the keys' weights, 2: the same where max_len is 1.
 LLB_EXPORT long long llb_span_scratch_floats(int dtype, int T, int S, int Hq, int Hkv, int hd, int page_size, int num_slots, int mass) {
@@ -480,45 +638,35 @@ LLB_EXPORT long long llb_span_scratch_floats(int dtype, int T, int S, int Hq, in
 LLB_EXPORT int llb_tree_attention(const void* q, const void* k, const void* v, void* out, int dtype, const unsigned long long* mask,
                                   int words, const int* span_row, const int* span_len, const int* span_pos, const int* table, int S, int T,
                                   int max_pages, int page_size, int num_slots, int Hq, int Hkv, int hd, float scale, float* scratch,
-                                  unsigned* counters, int* error_flag, cudaStream_t stream) {
+                                  int* error_flag, cudaStream_t stream) {
     LlbSpanArgs a = span_args(out, span_row, span_len, span_pos, table, S, T, max_pages, page_size, num_slots, Hq, Hkv, hd, scale, 0);
     if (int rc = check(a, dtype)) return rc;
-    LLB_REQUIRE(words > 0 && words <= (1 << 20) && mask && scratch && counters, "tree_attention: no mask or no scratch");
+    LLB_REQUIRE(words > 0 && words <= (1 << 20) && mask && scratch, "tree_attention: no mask or no scratch");
     if (S == 0 || T == 0) return 0;
     a.mask = mask;
     a.words = words;
     a.max_len = words * 64;
     float* unused;
-    return attend(a, q, k, v, dtype, scratch, counters, 0, tc_sizes(dtype, hd, page_size) && llb_span_tc_takes(a, q, k, v, out), &unused, error_flag, stream);
+    return attend(a, q, k, v, dtype, scratch, 0, tc_sizes(dtype, hd, page_size) && llb_span_tc_takes(a, q, k, v, out), &unused, error_flag, stream);
 }
 
 // Causal; mass_in (may be null) and mass [Hkv, num_slots] float, may be the same.
 LLB_EXPORT int llb_paged_attention_mass(const void* q, const void* k, const void* v, void* out, int dtype, const float* mass_in, float* mass,
                                         const int* span_row, const int* span_len, const int* span_pos, const int* table, int S, int T,
                                         int max_len, int max_pages, int page_size, int num_slots, int Hq, int Hkv, int hd, float scale,
-                                        float* scratch, unsigned* counters, int* error_flag, cudaStream_t stream) {
+                                        float* scratch, int* error_flag, cudaStream_t stream) {
     LlbSpanArgs a = span_args(out, span_row, span_len, span_pos, table, S, T, max_pages, page_size, num_slots, Hq, Hkv, hd, scale, max_len);
     if (int rc = check(a, dtype)) return rc;
-    LLB_REQUIRE(max_len > 0 && mass && scratch && counters, "paged_attention_mass: no weights, no scratch or rows");
+    LLB_REQUIRE(max_len > 0 && mass && scratch, "paged_attention_mass: no weights, no scratch or rows");
     LLB_REQUIRE((long long)S * Hkv < (1ll << 31), "paged_attention_mass: too many requests");
     if (S == 0 || T == 0) return 0;
     const bool single = max_len == 1;
     const bool tc = tc_sizes(dtype, hd, page_size) && llb_span_tc_takes(a, q, k, v, out);
-    const bool joined = (long long)max_pages * page_size <= JOINED_MASS_KEYS;
     float* part_mass;
     a.mass_in = mass_in;
-    a.mass = single && !joined ? nullptr : mass;
-    if (int rc = attend(a, q, k, v, dtype, scratch, counters, single ? 2 : 1, tc, &part_mass, error_flag, stream)) return rc;
-    if (single && joined) return 0;
     a.mass = mass;
-    const int sms = llb_device_sms();
-    if (single) {
-        const long long keys = (long long)max_pages * page_size;
-        const int y = (int)max(1ll, min((keys + THREADS - 1) / THREADS, (long long)llb_ceil_div(8 * sms, S * Hkv)));
-        llb_launch(tc ? span_mass_of_scores_kernel<128> : span_mass_of_scores_kernel<KT>, dim3(S * Hkv, y), dim3(THREADS), 0, stream, a);
-        return llb_check_launch("span_mass_of_scores");
-    }
-    a.arrived = counters + LLB_SPAN_BLOCKS;
+    if (int rc = attend(a, q, k, v, dtype, scratch, single ? 2 : 1, tc, &part_mass, error_flag, stream)) return rc;
+    if (single) return 0;
     if (tc) return llb_span_mass_tc(a, q, k, part_mass, tc_blocks(), error_flag, stream);
     ColumnParams p;
     p.a = a; p.q = q; p.k = k;
@@ -527,6 +675,6 @@ LLB_EXPORT int llb_paged_attention_mass(const void* q, const void* k, const void
     auto kernel = dtype == LLB_F32 ? span_mass_kernel<float> : span_mass_kernel<__nv_bfloat16>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return llb_fail("span_mass: cannot opt in to %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
-    llb_launch(kernel, dim3(2 * sms), dim3(THREADS), smem, stream, p);
+    llb_launch(kernel, dim3(2 * llb_device_sms()), dim3(THREADS), smem, stream, p);
     return llb_check_launch("span_mass");
 }

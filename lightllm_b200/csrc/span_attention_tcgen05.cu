@@ -130,7 +130,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     constexpr uint32_t TMEM_COLS = 512;              // S (and P) of the groups: 0.., 128..; O: 256.., 384..
     __shared__ __align__(8) uint64_t bar_q_full[2], bar_q_free[2], bar_kv_full[RING], bar_kv_free[RING], bar_s[2], bar_p[2], bar_o[2];
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_s, odd_s, join_s;
+    __shared__ int abort_s, odd_s;
     __shared__ LlbPiece piece_s;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -160,8 +160,11 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     griddep_wait();
     griddep_launch_dependents();
     if (warp == 0) {
-        const LlbPiece pc = llb_piece(a, BK, blockIdx.x, gridDim.x, 2, lane);
-        if (lane == 0) piece_s = pc;
+        const LlbPiece pc = llb_piece(a, BK, blockIdx.x, gridDim.x, LLB_SPAN_TC_LEAST, lane);
+        if (lane == 0) {
+            piece_s = pc;
+            llb_leave_open(a, pc, pc.job, false);
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -311,7 +314,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const unsigned long long* mask = a.mask ? a.mask + (size_t)(z.row + node) * a.words : nullptr;
             const int all = a.mask ? z.pos : z.pos + job.first + 1;         // keys that every row of the job sees
             const int own = a.mask ? z.pos : z.pos + node + 1;              // first keys that this row sees
-            const bool scores_of = a.scores && z.len == 1, scores = scores_of && mine;
+            const bool scores = a.scores && z.len == 1 && mine;
             const bool busy = (warp & 3) * 32 < pairs;                      // any pair in this warp's lanes
             float m_ref = -INFINITY, l_run = 0.0f;
             for (int j = g.two ? 0 : x; j < n; j += step) {
@@ -517,7 +520,6 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     }
                 }
             }
-            float* room = reinterpret_cast<float*>(q_s + buf * HALF);
             if (mine && ok && (g.two || x == 0)) {
                 if (g.part >= 0) {
                     float* ml = a.part_ml + ((size_t)(blockIdx.x * 2 + g.part) * a.rows + node0 * a.group + r) * 2;
@@ -527,20 +529,11 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     a.lse[(size_t)row * a.Hq + head] = llb_lse(m_ref, l_run);
                 }
             }
-            if (g.part >= 0 || scores_of) {
-                // (what the groups exchanged in the buffer has been read, and of a job of two tiles of pairs the first one's Q)
-                if (g.two) room = reinterpret_cast<float*>(q_s);
-                named_barrier(BAR_PAIR, 256);
-                if (g.part < 0 && mine && x == 0) {
-                    room[2 * r] = m_ref;
-                    room[2 * r + 1] = l_run;
-                }
-                llb_finish_job<__nv_bfloat16, BK, HD / 4>(a, pc, job, g.part, room, HALF / 4, &join_s, threadIdx.x, [] { named_barrier(BAR_PAIR, 256); });
-            }
+            if (g.part == 1 && threadIdx.x == 0) llb_leave_open(a, pc, job, true);
             // O and Q are free for the next job (the groups have read each other's O)
             tc_fence_before();
             fence_async_smem();
-            if (!g.two || g.part >= 0) named_barrier(BAR_PAIR, 256);
+            if (!g.two) named_barrier(BAR_PAIR, 256);
             else named_barrier(BAR_PAIR + 1 + x, 128);
             if (r == 0 && (g.two || x == 0)) mbar_arrive(&bar_q_free[buf]);
             tiles_before += n;
@@ -657,7 +650,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     constexpr uint32_t TMEM_COLS = 512;              // two score tiles of each group
     __shared__ __align__(8) uint64_t bar_k_full[2], bar_k_free[2], bar_q_full[RING], bar_q_free[RING], bar_s[4], bar_free[4];
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_s, join_s;
+    __shared__ int abort_s;
     __shared__ MassPiece piece_s;
     __shared__ __align__(16) float lse_s[2][2][128];
     __shared__ float sum_s[128];
@@ -696,7 +689,10 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     griddep_launch_dependents();
     if (warp == 0) {
         const MassPiece pc = mass_piece(a, pairs_nodes, blockIdx.x, gridDim.x, lane);
-        if (lane == 0) piece_s = pc;
+        if (lane == 0) {
+            piece_s = pc;
+            reinterpret_cast<int4*>(a.open)[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -840,25 +836,14 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             if (x == 0) {
                 sum += sum_s[r];
                 const int part = job.begin < pc.t0 ? 0 : job.begin + job.units > pc.t1 ? 1 : -1;
-                auto owner = [&](int at) { return (int)(((long long)(at + 1) * pc.blocks + pc.total - 1) / pc.total) - 1; };
-                bool joined = true;
                 if (part >= 0) {
-                    // the last block that leaves a part of the sums adds them up, in the blocks' order
-                    const int from = owner(job.begin), parts = owner(job.begin + job.units - 1) - from + 1;
                     m.part[(size_t)(blockIdx.x * 2 + part) * 128 + r] = sum;
-                    __threadfence();
-                    named_barrier(BAR_PAIR + 1, 128);
-                    if (r == 0) join_s = atomicInc(a.arrived + from, parts - 1) == (unsigned)parts - 1;
-                    named_barrier(BAR_PAIR + 1, 128);
-                    joined = join_s;
-                    if (joined) {
-                        __threadfence();
-                        sum = 0.0f;
-#pragma unroll 4
-                        for (int i = 0; i < parts; ++i) sum += __ldcg(m.part + (size_t)((from + i) * 2 + (i == 0 ? 1 : 0)) * 128 + r);
-                    }
+                    if (part == 1 && r == 0)
+                        reinterpret_cast<int4*>(a.open)[2 * blockIdx.x] =
+                            make_int4((int)(((long long)(job.begin + job.units) * pc.blocks + pc.total - 1) / pc.total) - blockIdx.x, job.s, job.tile, job.kvh);
+                } else if (ok) {
+                    llb_add_mass(a, z, job.s, key, job.kvh, sum);
                 }
-                if (joined && ok) llb_add_mass(a, z, job.s, key, job.kvh, sum);
             }
             named_barrier(BAR_PAIR, 256);
             if (threadIdx.x == 0) mbar_arrive(&bar_k_free[jobs & 1]);          // both groups have had all scores of the job
@@ -875,6 +860,18 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         tc_fence_after();
         tmem_dealloc(tmem_base, TMEM_COLS);
     }
+}
+
+// The sums of keys whose rows several blocks had, in the blocks' order.
+__global__ void __launch_bounds__(128) span_mass_join_kernel(const MassArgs m) {
+    llb_after_previous();
+    const LlbSpanArgs& a = m.p.a;
+    const int4 job = reinterpret_cast<const int4*>(a.open)[2 * blockIdx.x];          // blocks, request, tile, kv head
+    if (job.x == 0) return;
+    float sum = m.part[(size_t)(blockIdx.x * 2 + 1) * 128 + threadIdx.x];
+#pragma unroll 4
+    for (int b = 1; b < job.x; ++b) sum += m.part[(size_t)(blockIdx.x + b) * 2 * 128 + threadIdx.x];
+    llb_add_mass(a, llb_span(a, job.y), job.y, job.z * BK + threadIdx.x, job.w, sum);
 }
 
 // q [T, Hq, hd] in boxes of the group's heads of `nodes` rows.
@@ -939,5 +936,7 @@ int llb_span_mass_tc(const LlbSpanArgs& a, const void* q, const void* k, float* 
     int rc;
     if ((rc = make_map_q(q, a.T, a.Hq, a.hd, a.group, m.p.pairs_nodes, &mq))) return rc;
     if ((rc = make_map_bf16(k, a.num_slots, (long long)a.Hkv * a.hd, a.page_size, &mk))) return rc;
-    return a.hd == 64 ? launch_mass_tc<64>(mq, mk, m, blocks, stream) : launch_mass_tc<128>(mq, mk, m, blocks, stream);
+    if ((rc = a.hd == 64 ? launch_mass_tc<64>(mq, mk, m, blocks, stream) : launch_mass_tc<128>(mq, mk, m, blocks, stream))) return rc;
+    llb_launch(span_mass_join_kernel, dim3(blocks), dim3(128), 0, stream, m);
+    return llb_check_launch("span_mass_join");
 }
