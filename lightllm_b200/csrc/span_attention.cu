@@ -356,7 +356,7 @@ template <int TILE> __device__ __forceinline__ void mass_of_scores(const LlbSpan
     LlbPiece pc;
     pc.total = total_s;
     pc.blocks = min(grid, (pc.total + least - 1) / least);
-    const int from = llb_piece_owner(pc, begin), parts = llb_piece_owner(pc, begin + tiles - 1) - from + 1;
+    const int from = pc.owner(begin), parts = pc.owner(begin + tiles - 1) - from + 1;
     for (int g = threadIdx.x; g < a.group; g += THREADS) {
         float lse;
         if (parts == 1) lse = a.lse[(size_t)z.row * a.Hq + kvh * a.group + g];

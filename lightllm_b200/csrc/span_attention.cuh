@@ -92,6 +92,13 @@ struct LlbJob {
 struct LlbPiece {
     int t0, t1, total, blocks;
     LlbJob job;
+    // The first total % blocks pieces are a tile longer than the others.
+    __device__ __forceinline__ int start(int block) const { return block * (total / blocks) + min(block, total % blocks); }
+    // Which block has tile t of the line.
+    __device__ __forceinline__ int owner(int t) const {
+        const int each = total / blocks, longer = total % blocks, head = longer * (each + 1);
+        return t < head ? t / (each + 1) : longer + (t - head) / each;
+    }
 };
 __device__ __forceinline__ int llb_span_tiles(const LlbSpanArgs& a, const LlbSpan& z, int tile) {
     int n = 0;
@@ -114,8 +121,8 @@ __device__ __forceinline__ LlbPiece llb_piece(const LlbSpanArgs& a, int tile, in
     p.blocks = min(grid, (p.total + least - 1) / least);
     p.t0 = p.t1 = 0;
     if (block >= p.blocks) return p;
-    p.t0 = (int)((long long)p.total * block / p.blocks);
-    p.t1 = (int)((long long)p.total * (block + 1) / p.blocks);
+    p.t0 = p.start(block);
+    p.t1 = p.start(block + 1);
     int before = 0;
     for (int base = 0; base < a.S; base += 32) {
         if (a.S > 32) {
@@ -151,10 +158,6 @@ __device__ __forceinline__ LlbPiece llb_piece(const LlbSpanArgs& a, int tile, in
     p.job.begin += p.job.kvh * p.job.tiles;
     return p;
 }
-// Which block has tile t of the line.
-__device__ __forceinline__ int llb_piece_owner(const LlbPiece& p, int t) {
-    return (int)(((long long)(t + 1) * p.blocks + p.total - 1) / p.total) - 1;
-}
 // Where a job's partial result goes when the block [t0, t1) has not all of it: 0 or 1, or -1 when it has.
 __device__ __forceinline__ int llb_part_of(const LlbPiece& p, const LlbJob& j) {
     if (j.begin < p.t0) return 0;
@@ -181,7 +184,7 @@ struct LlbOpen {
 };
 __device__ __forceinline__ void llb_leave_open(const LlbSpanArgs& a, const LlbPiece& pc, const LlbJob& job, bool goes_on) {
     int4* to = reinterpret_cast<int4*>(a.open) + 2 * blockIdx.x;
-    to[0] = make_int4(goes_on ? llb_piece_owner(pc, job.begin + job.tiles - 1) - blockIdx.x + 1 : 0, job.z.row + job.first, job.count(a) * a.group,
+    to[0] = make_int4(goes_on ? pc.owner(job.begin + job.tiles - 1) - blockIdx.x + 1 : 0, job.z.row + job.first, job.count(a) * a.group,
                       job.kvh);
     to[1] = make_int4(job.z.pos, 0, 0, 0);
 }

@@ -47,9 +47,9 @@ struct TcParams {
 };
 
 // A block is launched with 3 x 168 registers a thread of its three groups; the third one needs few, the softmax groups hold a row
-// of 128 scores: 88 + 2 x 208 = 504.
-__device__ __forceinline__ void registers_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
-__device__ __forceinline__ void registers_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
+// of 128 scores: 104 + 2 x 200 = 504.
+__device__ __forceinline__ void registers_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 104;"); }
+__device__ __forceinline__ void registers_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 200;"); }
 __device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
     asm volatile(
@@ -80,23 +80,83 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&u)[32
           "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
         : "memory");
 }
+// The loads before this have completed; what uses their 32 registers stays behind it.
+__device__ __forceinline__ void tmem_wait_ld32(float (&r)[32]) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]), "+r"(u[8]), "+r"(u[9]),
+                   "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]), "+r"(u[14]), "+r"(u[15]), "+r"(u[16]), "+r"(u[17]), "+r"(u[18]),
+                   "+r"(u[19]), "+r"(u[20]), "+r"(u[21]), "+r"(u[22]), "+r"(u[23]), "+r"(u[24]), "+r"(u[25]), "+r"(u[26]), "+r"(u[27]),
+                   "+r"(u[28]), "+r"(u[29]), "+r"(u[30]), "+r"(u[31])::"memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 bits of a row's mask from node j0 on (which may be negative), those of nodes from len on cleared.
-__device__ __forceinline__ uint32_t mask_bits(const unsigned long long* row, int words, int j0, int len) {
-    if (j0 <= -32 || j0 >= len) return 0u;
-    uint32_t bits;
-    if (j0 < 0) bits = (uint32_t)row[0] << -j0;
-    else {
-        const int w = j0 >> 6, sh = j0 & 63;
-        unsigned long long x = row[w] >> sh;
-        if (sh > 32 && w + 1 < words) x |= row[w + 1] << (64 - sh);
-        bits = (uint32_t)x;
+// A row's mask.  The first two words (128 nodes) are asked for when the job begins, since a trip to memory in the last tile would be as long as
+// the rest of its work.
+struct RowMask {
+    const unsigned long long* row;
+    int words;
+    unsigned long long w0, w1;
+    __device__ __forceinline__ unsigned long long word(int w) const { return w == 0 ? w0 : w == 1 ? w1 : w < words ? row[w] : 0ull; }
+    // 32 bits from node j0 on (which may be negative), those of nodes from len on cleared
+    __device__ __forceinline__ uint32_t bits(int j0, int len) const {
+        if (j0 <= -32 || j0 >= len) return 0u;
+        uint32_t x;
+        if (j0 < 0) x = (uint32_t)w0 << -j0;
+        else {
+            const int w = j0 >> 6, sh = j0 & 63;
+            unsigned long long y = word(w) >> sh;
+            if (sh > 32) y |= word(w + 1) << (64 - sh);
+            x = (uint32_t)y;
+        }
+        return len - j0 < 32 ? x & ((1u << (len - j0)) - 1u) : x;
     }
-    return len - j0 < 32 ? bits & ((1u << (len - j0)) - 1u) : bits;
-}
+};
 __device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 __device__ __forceinline__ bool bf16_odd(uint32_t pair) { return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u; }
+
+// The largest of a lane's 128 scores.
+__device__ __forceinline__ float tile_max(uint32_t tmem) {
+    float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+#pragma unroll 1
+    for (int c = 0; c < 128; c += 32) {
+        float s[32];
+        tmem_ld32(tmem + c, s);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+            t0 = fmaxf(t0, s[i]);
+            t1 = fmaxf(t1, s[i + 1]);
+            t2 = fmaxf(t2, s[i + 2]);
+            t3 = fmaxf(t3, s[i + 3]);
+        }
+    }
+    return fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+}
+// 2^(score * scale + shift) of a lane's 128 scores as bf16 pairs, their sum (before the rounding) and the largest score, which tells
+// whether the shift was near enough: after the first tile it nearly always is, so that no pass for the maximum comes before this one.  The scores
+// stay where they are.
+__device__ __forceinline__ void tile_probs(uint32_t tmem, float scale, float shift, uint32_t (&probs)[64], float& sum, float& top) {
+    float l0 = 0.0f, l1 = 0.0f, t0 = -INFINITY, t1 = -INFINITY;
+    float s[2][32];
+    tmem_ld32_nowait(tmem, *reinterpret_cast<uint32_t(*)[32]>(&s[0][0]));
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        tmem_wait_ld32(s[c & 1]);
+        if (c < 3) tmem_ld32_nowait(tmem + 32 * (c + 1), *reinterpret_cast<uint32_t(*)[32]>(&s[(c + 1) & 1][0]));
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            const float a = s[c & 1][i], b = s[c & 1][i + 1];
+            t0 = fmaxf(t0, a);
+            t1 = fmaxf(t1, b);
+            const float p0 = fast_exp2(fmaf(a, scale, shift)), p1 = fast_exp2(fmaf(b, scale, shift));
+            l0 += p0;
+            l1 += p1;
+            probs[16 * c + i / 2] = wm::pack_bf16(p0, p1);
+        }
+    }
+    sum = l0 + l1;
+    top = fmaxf(t0, t1);
+}
 
 // Four bytes a page: the cache row that a page of a tile begins at, or num_slots (TMA reads zeros there) for one that holds no key of
 // the job or is none of the cache's.
@@ -312,9 +372,9 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const int node = job.first + node0 + (mine ? r / a.group : 0);
             const LlbSpan z = job.z;
             const unsigned long long* mask = a.mask ? a.mask + (size_t)(z.row + node) * a.words : nullptr;
+            const RowMask row_mask = {mask, a.words, mask && mine ? mask[0] : 0ull, mask && mine && a.words > 1 ? mask[1] : 0ull};
             const int all = a.mask ? z.pos : z.pos + job.first + 1;         // keys that every row of the job sees
             const int own = a.mask ? z.pos : z.pos + node + 1;              // first keys that this row sees
-            const bool scores = a.scores && z.len == 1 && mine;
             const bool busy = (warp & 3) * 32 < pairs;                      // any pair in this warp's lanes
             float m_ref = -INFINITY, l_run = 0.0f;
             for (int j = g.two ? 0 : x; j < n; j += step) {
@@ -363,47 +423,51 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     fence_async_smem();
                 }
                 if (busy) {
-                    float s[128];
-                    tmem_ld32_nowait(tmem_s, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-                    tmem_ld32_nowait(tmem_s + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
-                    tmem_ld32_nowait(tmem_s + 64, *reinterpret_cast<uint32_t(*)[32]>(&s[64]));
-                    tmem_ld32_nowait(tmem_s + 96, *reinterpret_cast<uint32_t(*)[32]>(&s[96]));
-                    tmem_wait_ld();
                     if (!interior) {
-#pragma unroll
+                        // what this row does not see becomes minus infinity where it stands
+#pragma unroll 1
                         for (int w = 0; w < 4; ++w) {
                             uint32_t bits = first_bits(own - key0 - 32 * w);
-                            if (mask && mine) bits |= mask_bits(mask, a.words, key0 + 32 * w - z.pos, z.len);
+                            if (mask && mine) bits |= row_mask.bits(key0 + 32 * w - z.pos, z.len);
+                            __syncwarp();
+                            float s[32];
+                            tmem_ld32(tmem_s + 32 * w, s);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) s[32 * w + i] = (bits >> i) & 1u ? s[32 * w + i] : -INFINITY;
+                            for (int i = 0; i < 32; ++i) s[i] = (bits >> i) & 1u ? s[i] : -INFINITY;
+                            tmem_st32(tmem_s + 32 * w, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
                         }
+                        tmem_wait_st();
                     }
-                    if (scores && job.begin + g.k0 + j < a.score_tiles) {
+                    if (a.scores && z.len == 1 && job.begin + g.k0 + j < a.score_tiles) {
                         float* to = a.scores + ((size_t)(job.begin + g.k0 + j) * a.group + r) * BK;
+#pragma unroll 1
+                        for (int c = 0; c < 128; c += 32) {
+                            float s[32];
+                            __syncwarp();
+                            tmem_ld32(tmem_s + c, s);
+                            if (mine) {
 #pragma unroll
-                        for (int c = 0; c < 128; c += 4)
-                            *reinterpret_cast<float4*>(to + c) = make_float4(s[c] * a.scale_log2e, s[c + 1] * a.scale_log2e,
-                                                                             s[c + 2] * a.scale_log2e, s[c + 3] * a.scale_log2e);
+                                for (int i = 0; i < 32; i += 4)
+                                    *reinterpret_cast<float4*>(to + c + i) = make_float4(s[i] * a.scale_log2e, s[i + 1] * a.scale_log2e,
+                                                                                         s[i + 2] * a.scale_log2e, s[i + 3] * a.scale_log2e);
+                            }
+                        }
+                        __syncwarp();
                     }
-                    float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
-#pragma unroll
-                    for (int i = 4; i < 128; i += 4) {
-                        t0 = fmaxf(t0, s[i]);
-                        t1 = fmaxf(t1, s[i + 1]);
-                        t2 = fmaxf(t2, s[i + 2]);
-                        t3 = fmaxf(t3, s[i + 3]);
-                    }
-                    const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * a.scale_log2e;
-                    __syncwarp();
-                    if (j < step) m_ref = top;              // (no O yet)
-                    else if (__any_sync(0xffffffffu, top > m_ref + RESCALE)) {
+                    if (j < step) m_ref = tile_max(tmem_s) * a.scale_log2e;              // (no O yet)
+                    uint32_t probs[64];
+                    float sum, top;
+                    tile_probs(tmem_s, a.scale_log2e, m_ref == -INFINITY ? 0.0f : -m_ref, probs, sum, top);
+                    top *= a.scale_log2e;
+                    if (__any_sync(0xffffffffu, top > m_ref + RESCALE)) {
                         float corr = 1.0f;
                         if (top > m_ref + RESCALE) {
                             corr = m_ref == -INFINITY ? 0.0f : fast_exp2(m_ref - top);
                             m_ref = top;
                         }
                         l_run *= corr;
-#pragma unroll
+                        __syncwarp();
+#pragma unroll 1
                         for (int c = 0; c < HD; c += 32) {
                             float o[32];
                             tmem_ld32(tmem_o + x * 128 + c, o);
@@ -411,29 +475,11 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             for (int i = 0; i < 32; ++i) o[i] *= corr;
                             tmem_st32(tmem_o + x * 128 + c, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
                         }
+                        tile_probs(tmem_s, a.scale_log2e, m_ref == -INFINITY ? 0.0f : -m_ref, probs, sum, top);
                     }
-                    __syncwarp();
-                    const float shift = m_ref == -INFINITY ? 0.0f : -m_ref;
-                    float l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
-#pragma unroll
-                    for (int c = 0; c < 128; c += 64) {
-                        uint32_t w[32];
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float p0 = fast_exp2(fmaf(s[c + 2 * i], a.scale_log2e, shift));
-                            const float p1 = fast_exp2(fmaf(s[c + 2 * i + 1], a.scale_log2e, shift));
-                            const float p2 = fast_exp2(fmaf(s[c + 2 * i + 2], a.scale_log2e, shift));
-                            const float p3 = fast_exp2(fmaf(s[c + 2 * i + 3], a.scale_log2e, shift));
-                            l0 += p0;
-                            l1 += p1;
-                            l2 += p2;
-                            l3 += p3;
-                            w[i] = wm::pack_bf16(p0, p1);
-                            w[i + 1] = wm::pack_bf16(p2, p3);
-                        }
-                        tmem_st32(tmem_s + c / 2, w);
-                    }
-                    l_run += (l0 + l1) + (l2 + l3);
+                    l_run += sum;
+                    tmem_st32(tmem_s, *reinterpret_cast<const uint32_t(*)[32]>(&probs[0]));
+                    tmem_st32(tmem_s + 32, *reinterpret_cast<const uint32_t(*)[32]>(&probs[32]));
                     tmem_wait_st();
                 }
                 tc_fence_before();
@@ -584,7 +630,7 @@ struct MassJob {
     }
 };
 struct MassPiece {
-    int t0, t1, total, blocks;
+    LlbPiece line;              // (its job is not used)
     MassJob job;
 };
 __device__ __forceinline__ int mass_units(const LlbSpanArgs& a, const LlbSpan& z, int pairs_nodes) {
@@ -595,7 +641,8 @@ __device__ __forceinline__ int mass_units(const LlbSpanArgs& a, const LlbSpan& z
     return n * a.Hkv;
 }
 __device__ __forceinline__ MassPiece mass_piece(const LlbSpanArgs& a, int pairs_nodes, int block, int grid, int lane) {
-    MassPiece p;
+    MassPiece m;
+    LlbPiece& p = m.line;
     int mine = 0;
     p.total = 0;
     for (int base = 0; base < a.S; base += 32) {
@@ -604,9 +651,9 @@ __device__ __forceinline__ MassPiece mass_piece(const LlbSpanArgs& a, int pairs_
     }
     p.blocks = min(grid, (p.total + 1) / 2);
     p.t0 = p.t1 = 0;
-    if (block >= p.blocks) return p;
-    p.t0 = (int)((long long)p.total * block / p.blocks);
-    p.t1 = (int)((long long)p.total * (block + 1) / p.blocks);
+    if (block >= p.blocks) return m;
+    p.t0 = p.start(block);
+    p.t1 = p.start(block + 1);
     int before = 0;
     for (int base = 0; base < a.S; base += 32) {
         if (a.S > 32) mine = base + lane < a.S ? mass_units(a, llb_span(a, base + lane), pairs_nodes) : 0;
@@ -619,23 +666,23 @@ __device__ __forceinline__ MassPiece mass_piece(const LlbSpanArgs& a, int pairs_
         const unsigned past = __ballot_sync(0xffffffffu, before + sum > p.t0);
         if (past) {
             const int at = __ffs(past) - 1;
-            p.job.s = base + at;
-            p.job.begin = before + __shfl_sync(0xffffffffu, sum - mine, at);
+            m.job.s = base + at;
+            m.job.begin = before + __shfl_sync(0xffffffffu, sum - mine, at);
             break;
         }
         before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    p.job.z = llb_span(a, p.job.s);
-    p.job.tile = 0;
+    m.job.z = llb_span(a, m.job.s);
+    m.job.tile = 0;
     for (;;) {
-        p.job.measure(pairs_nodes);
-        if (p.t0 < p.job.begin + p.job.units * a.Hkv) break;
-        p.job.begin += p.job.units * a.Hkv;
-        ++p.job.tile;
+        m.job.measure(pairs_nodes);
+        if (p.t0 < m.job.begin + m.job.units * a.Hkv) break;
+        m.job.begin += m.job.units * a.Hkv;
+        ++m.job.tile;
     }
-    p.job.kvh = (p.t0 - p.job.begin) / p.job.units;
-    p.job.begin += p.job.kvh * p.job.units;
-    return p;
+    m.job.kvh = (p.t0 - m.job.begin) / m.job.units;
+    m.job.begin += m.job.kvh * m.job.units;
+    return m;
 }
 template <int HD> struct MassShape {
     static constexpr int RING = HD == 64 ? 8 : 4;
@@ -698,8 +745,8 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = tmem_slot;
-    const MassPiece pc = piece_s;
-    MassJob job = pc.job;
+    const LlbPiece pc = piece_s.line;
+    MassJob job = piece_s.job;
     uint32_t jobs = 0, units_before = 0;
     constexpr uint32_t IDESC = idesc_bf16(BK, BQ, 0);
 
@@ -807,23 +854,23 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 const int upto = min(pairs_tile, (z.len - node0) * a.group);
                 const bool interior = job.tile * BK + BK - 1 - z.pos - node0 <= 0 && upto == pairs_tile;
                 const uint32_t tmem = tmem_base + place * 128 + lanes;
+                float s[2][32];
+                tmem_ld32_nowait(tmem, *reinterpret_cast<uint32_t(*)[32]>(&s[0][0]));
 #pragma unroll
-                for (int c = 0; c < 128; c += 64) {
-                    float s[64];
-                    tmem_ld32_nowait(tmem + c, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-                    tmem_ld32_nowait(tmem + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
-                    tmem_wait_ld();
+                for (int c = 0; c < 4; ++c) {
+                    tmem_wait_ld32(s[c & 1]);
+                    if (c < 3) tmem_ld32_nowait(tmem + 32 * (c + 1), *reinterpret_cast<uint32_t(*)[32]>(&s[(c + 1) & 1][0]));
                     if (!interior) {
 #pragma unroll
-                        for (int i = 0; i < 64; ++i) s[i] = c + i >= least && c + i < upto ? s[i] : -INFINITY;
+                        for (int i = 0; i < 32; ++i) s[c & 1][i] = 32 * c + i >= least && 32 * c + i < upto ? s[c & 1][i] : -INFINITY;
                     }
 #pragma unroll
-                    for (int i = 0; i < 64; i += 4) {
-                        const float4 e = *reinterpret_cast<const float4*>(lse_t + c + i);
-                        sum0 += fast_exp2(fmaf(s[i], a.scale_log2e, -e.x));
-                        sum1 += fast_exp2(fmaf(s[i + 1], a.scale_log2e, -e.y));
-                        sum2 += fast_exp2(fmaf(s[i + 2], a.scale_log2e, -e.z));
-                        sum3 += fast_exp2(fmaf(s[i + 3], a.scale_log2e, -e.w));
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 e = *reinterpret_cast<const float4*>(lse_t + 32 * c + i);
+                        sum0 += fast_exp2(fmaf(s[c & 1][i], a.scale_log2e, -e.x));
+                        sum1 += fast_exp2(fmaf(s[c & 1][i + 1], a.scale_log2e, -e.y));
+                        sum2 += fast_exp2(fmaf(s[c & 1][i + 2], a.scale_log2e, -e.z));
+                        sum3 += fast_exp2(fmaf(s[c & 1][i + 3], a.scale_log2e, -e.w));
                     }
                 }
                 tc_fence_before();
@@ -840,7 +887,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     m.part[(size_t)(blockIdx.x * 2 + part) * 128 + r] = sum;
                     if (part == 1 && r == 0)
                         reinterpret_cast<int4*>(a.open)[2 * blockIdx.x] =
-                            make_int4((int)(((long long)(job.begin + job.units) * pc.blocks + pc.total - 1) / pc.total) - blockIdx.x, job.s, job.tile, job.kvh);
+                            make_int4(pc.owner(job.begin + job.units - 1) - blockIdx.x + 1, job.s, job.tile, job.kvh);
                 } else if (ok) {
                     llb_add_mass(a, z, job.s, key, job.kvh, sum);
                 }
@@ -891,7 +938,7 @@ int make_map_q(const void* q, int T, int Hq, int hd, int group, int nodes, CUten
 // The softmax groups' registers come out of what the block was launched with: a build that gives a thread fewer is refused.
 template <int HD> bool registers_suffice() {
     cudaFuncAttributes at;
-    return cudaFuncGetAttributes(&at, span_attention_tc_kernel<HD>) == cudaSuccess && at.numRegs * 3 >= 88 + 2 * 208;
+    return cudaFuncGetAttributes(&at, span_attention_tc_kernel<HD>) == cudaSuccess && at.numRegs * 3 >= 104 + 2 * 200;
 }
 template <int HD>
 int launch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& p, int blocks, cudaStream_t stream) {
