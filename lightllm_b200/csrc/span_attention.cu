@@ -221,14 +221,14 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
             if (r >= rows) continue;
             const float l = l_s[r], m = m_s[r];
             const int node = job.first + r / a.group, row = job.z.row + node, head = job.kvh * a.group + r % a.group;
-            float* po = a.part_o + ((size_t)(blockIdx.x * 2 + max(part, 0)) * a.rows + r) * hd;
+            float* po = a.part_o + (size_t)(blockIdx.x * 2 + max(part, 0)) * (hd4 / 4) * a.rows * 4;
             const float inv = llb_inverse(m, l, job.z.pos);
             T* dst = (T*)a.out + ((size_t)row * a.Hq + head) * hd;
 #pragma unroll
             for (int d = 0; d < DPT; ++d) {
                 const int dim = RB == 64 ? (d >> 2) * 64 + tx * 4 + (d & 3) : d * 64 + tx;
                 if (dim >= hd) continue;
-                if (part >= 0) po[dim] = o[i][d];
+                if (part >= 0) po[((size_t)(dim >> 2) * a.rows + r) * 4 + (dim & 3)] = o[i][d];
                 else dst[dim] = llb_from_float<T>(o[i][d] * inv);
             }
             if (tx == 0) {
@@ -249,77 +249,73 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
 }
 
 // out = sum_b 2^(m_b - M) O_b / sum_b 2^(m_b - M) l_b over the blocks that hold parts of a job, in their order, with a running maximum
-// so that O is asked for together with m and l: a trip to memory after the one for what there is to join.  TPR threads have a row, four
-// dimensions each; PB parts of RU rows are on their way at once.
-template <typename T, int TPR, int PB, int RU>
+// so that O is asked for together with m and l: a trip to memory after the one for what there is to join.  A warp has 32 rows and four
+// dimensions of them; PB parts of PU groups of four dimensions are on their way at once.
+template <typename T, int PB, int PU>
 __device__ __forceinline__ void join_rows(const LlbSpanArgs& a, const LlbOpen& job, int block, int y, int ny) {
-    constexpr int RPP = THREADS / TPR;
-    const int hd = a.hd, pieces = (hd + 3) / 4;
-    const bool whole = hd % 4 == 0;
-    for (int r0 = y * (RPP * RU) + threadIdx.x / TPR; r0 < job.rows; r0 += ny * (RPP * RU)) {
-        for (int piece = threadIdx.x % TPR; piece < pieces; piece += TPR) {
-            const int d = piece * 4;
-            float x[RU][4], M[RU], L[RU];
+    const int hd = a.hd, pieces = (hd + 3) / 4, groups = (pieces + PU - 1) / PU;
+    const int row_groups = (job.rows + 31) / 32;
+    for (int i = y * (THREADS / 32) + (threadIdx.x >> 5); i < row_groups * groups; i += ny * (THREADS / 32)) {
+        const int r = i / groups * 32 + (threadIdx.x & 31), piece0 = i % groups * PU;
+        if (r >= job.rows) continue;
+        float x[PU][4], M = -INFINITY, L = 0.0f;
 #pragma unroll
-            for (int u = 0; u < RU; ++u) {
-                x[u][0] = x[u][1] = x[u][2] = x[u][3] = L[u] = 0.0f;
-                M[u] = -INFINITY;
+        for (int u = 0; u < PU; ++u) x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.0f;
+        for (int b0 = 0; b0 < job.parts; b0 += PB) {
+            float4 v[PU][PB];
+            float2 ml[PB];
+#pragma unroll
+            for (int e = 0; e < PB; ++e) {
+                const int b = b0 + e;
+                ml[e] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                for (int u = 0; u < PU; ++u) v[u][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (b >= job.parts) continue;
+                const size_t part = (size_t)(block + b) * 2 + (b == 0 ? 1 : 0);
+                ml[e] = reinterpret_cast<const float2*>(a.part_ml)[part * a.rows + r];
+#pragma unroll
+                for (int u = 0; u < PU; ++u)
+                    if (piece0 + u < pieces) v[u][e] = reinterpret_cast<const float4*>(a.part_o)[(part * pieces + piece0 + u) * a.rows + r];
             }
-            for (int b0 = 0; b0 < job.parts; b0 += PB) {
-                float4 v[RU][PB];
-                float2 ml[RU][PB];
+            float top = M;
 #pragma unroll
-                for (int u = 0; u < RU; ++u)
+            for (int e = 0; e < PB; ++e) top = fmaxf(top, ml[e].x);
+            const float keep = M == -INFINITY ? 1.0f : exp2f(M - top);          // (nothing, or a NaN, which stays)
+            L *= keep;
+            M = top;
 #pragma unroll
-                    for (int e = 0; e < PB; ++e) {
-                        const int r = r0 + u * RPP, b = b0 + e;
-                        ml[u][e] = make_float2(-INFINITY, 0.0f);
-                        v[u][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (r >= job.rows || b >= job.parts) continue;
-                        const size_t at = ((size_t)(block + b) * 2 + (b == 0 ? 1 : 0)) * a.rows + r;
-                        ml[u][e] = reinterpret_cast<const float2*>(a.part_ml)[at];
-                        const float* o = a.part_o + at * hd + d;
-                        if (whole) v[u][e] = *reinterpret_cast<const float4*>(o);
-                        else v[u][e] = make_float4(o[0], d + 1 < hd ? o[1] : 0.0f, d + 2 < hd ? o[2] : 0.0f, d + 3 < hd ? o[3] : 0.0f);
-                    }
+            for (int u = 0; u < PU; ++u) {
+                x[u][0] *= keep; x[u][1] *= keep; x[u][2] *= keep; x[u][3] *= keep;
+            }
 #pragma unroll
-                for (int u = 0; u < RU; ++u) {
-                    float top = M[u];
+            for (int e = 0; e < PB; ++e) {
+                // (a part without visible keys has m = -infinity, l = 0 and O = 0; a NaN of another one stays)
+                const float w = ml[e].x == -INFINITY ? 1.0f : exp2f(ml[e].x - top);
+                L = fmaf(w, ml[e].y, L);
 #pragma unroll
-                    for (int e = 0; e < PB; ++e) top = fmaxf(top, ml[u][e].x);
-                    const float keep = M[u] == -INFINITY ? 1.0f : exp2f(M[u] - top);          // (nothing, or a NaN, which stays)
-                    x[u][0] *= keep; x[u][1] *= keep; x[u][2] *= keep; x[u][3] *= keep;
-                    L[u] *= keep;
-                    M[u] = top;
-#pragma unroll
-                    for (int e = 0; e < PB; ++e) {
-                        // (a part without visible keys has m = -infinity, l = 0 and O = 0; a NaN of another one stays)
-                        const float w = ml[u][e].x == -INFINITY ? 1.0f : exp2f(ml[u][e].x - top);
-                        L[u] = fmaf(w, ml[u][e].y, L[u]);
-                        x[u][0] = fmaf(w, v[u][e].x, x[u][0]);
-                        x[u][1] = fmaf(w, v[u][e].y, x[u][1]);
-                        x[u][2] = fmaf(w, v[u][e].z, x[u][2]);
-                        x[u][3] = fmaf(w, v[u][e].w, x[u][3]);
-                    }
+                for (int u = 0; u < PU; ++u) {
+                    x[u][0] = fmaf(w, v[u][e].x, x[u][0]);
+                    x[u][1] = fmaf(w, v[u][e].y, x[u][1]);
+                    x[u][2] = fmaf(w, v[u][e].z, x[u][2]);
+                    x[u][3] = fmaf(w, v[u][e].w, x[u][3]);
                 }
             }
+        }
+        const int node = r / a.group, row = job.row + node, head = job.kvh * a.group + r - node * a.group;
+        const float inv = llb_inverse(M, L, job.pos);
+        if (a.lse && piece0 == 0) a.lse[(size_t)row * a.Hq + head] = llb_lse(M, L);
+        T* dst = (T*)a.out + ((size_t)row * a.Hq + head) * hd + piece0 * 4;
 #pragma unroll
-            for (int u = 0; u < RU; ++u) {
-                const int r = r0 + u * RPP;
-                if (r >= job.rows) continue;
-                const int node = r / a.group, row = job.row + node, head = job.kvh * a.group + r - node * a.group;
-                const float inv = llb_inverse(M[u], L[u], job.pos);
-                if (a.lse && piece == 0) a.lse[(size_t)row * a.Hq + head] = llb_lse(M[u], L[u]);
-                T* dst = (T*)a.out + ((size_t)row * a.Hq + head) * hd + d;
-                if (whole && sizeof(T) == 2 && ((uintptr_t)dst & 7) == 0) {
-                    const __nv_bfloat162 lo = __floats2bfloat162_rn(x[u][0] * inv, x[u][1] * inv), hi = __floats2bfloat162_rn(x[u][2] * inv, x[u][3] * inv);
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const unsigned*>(&lo), *reinterpret_cast<const unsigned*>(&hi));
-                    continue;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (d + e < hd) dst[e] = llb_from_float<T>(x[u][e] * inv);
+        for (int u = 0; u < PU; ++u) {
+            const int d = (piece0 + u) * 4;
+            if (hd % 4 == 0 && sizeof(T) == 2 && ((uintptr_t)a.out & 7) == 0 && d < hd) {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(x[u][0] * inv, x[u][1] * inv), hi = __floats2bfloat162_rn(x[u][2] * inv, x[u][3] * inv);
+                *reinterpret_cast<uint2*>(dst + 4 * u) = make_uint2(*reinterpret_cast<const unsigned*>(&lo), *reinterpret_cast<const unsigned*>(&hi));
+                continue;
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (d + e < hd) dst[4 * u + e] = llb_from_float<T>(x[u][e] * inv);
         }
     }
 }
@@ -391,7 +387,7 @@ template <int TILE> __device__ __forceinline__ void mass_of_scores(const LlbSpan
 }
 
 // The first `blocks * ny` blocks join, the others add up weights, `mass_y` of them a request and kv head.
-template <typename T, int TPR, int TILE>
+template <typename T, int TILE>
 __global__ void __launch_bounds__(THREADS) span_join_kernel(const LlbSpanArgs a, int blocks, int ny, int mass_y, int least) {
     llb_after_previous();
     const int i = blockIdx.x;
@@ -407,8 +403,8 @@ __global__ void __launch_bounds__(THREADS) span_join_kernel(const LlbSpanArgs a,
     job.pos = from[1].x;
     job.parts = lo.x; job.row = lo.y; job.rows = lo.z; job.kvh = lo.w;
     if (job.parts == 0) return;
-    if (job.parts <= 2) join_rows<T, TPR, 2, 4>(a, job, block, y, ny);
-    else join_rows<T, TPR, 8, 1>(a, job, block, y, ny);
+    if (job.parts <= 2) join_rows<T, 2, 4>(a, job, block, y, ny);
+    else join_rows<T, 8, 1>(a, job, block, y, ny);
 }
 
 // The same for requests of any number of rows: 64 keys of one request and kv head stay in shared memory, all rows that see any of them
@@ -504,17 +500,17 @@ __global__ void __launch_bounds__(THREADS) span_mass_kernel(const ColumnParams p
     }
 }
 
-template <typename T, int TPR, int TILE>
+template <typename T, int TILE>
 int launch_join(const LlbSpanArgs& a, int blocks, int least, cudaStream_t stream) {
-    // a block of the first kind has 8 or 16 rows at a time: as many as the average job brings, up to four rounds
+    // a warp of the first kind has 32 rows of four dimensions at a time: as many as the average job brings
     const int average = (int)max(1ll, min((long long)a.rows, (long long)a.T * a.group / max(1, a.S)));
-    const int ny = min(16, llb_ceil_div(average, THREADS / TPR));
+    const int ny = min(16, llb_ceil_div(llb_ceil_div(average, 32) * llb_ceil_div(a.hd, 4), THREADS / 32));
     int mass_y = 0;
     if (a.scores) {
         const long long keys = (long long)a.max_pages * a.page_size;
         mass_y = (int)max(1ll, min((keys + THREADS - 1) / THREADS, (long long)llb_ceil_div(8 * llb_device_sms(), a.S * a.Hkv)));
     }
-    llb_launch(span_join_kernel<T, TPR, TILE>, dim3(blocks * ny + a.S * a.Hkv * mass_y), dim3(THREADS), 0, stream, a, blocks, ny, mass_y, least);
+    llb_launch(span_join_kernel<T, TILE>, dim3(blocks * ny + a.S * a.Hkv * mass_y), dim3(THREADS), 0, stream, a, blocks, ny, mass_y, least);
     return llb_check_launch("span_join");
 }
 template <typename T, int RB, int NI>
@@ -537,11 +533,8 @@ int launch_attention_hd(const SimtParams& p, int blocks, cudaStream_t stream) {
 }  // namespace
 
 int llb_span_join(const LlbSpanArgs& a, int dtype, int blocks, int tile, int least, cudaStream_t stream) {
-    const bool narrow = a.hd <= 64;
-    if (dtype == LLB_F32) return narrow ? launch_join<float, 16, KT>(a, blocks, least, stream) : launch_join<float, 32, KT>(a, blocks, least, stream);
-    if (tile == KT)
-        return narrow ? launch_join<__nv_bfloat16, 16, KT>(a, blocks, least, stream) : launch_join<__nv_bfloat16, 32, KT>(a, blocks, least, stream);
-    return narrow ? launch_join<__nv_bfloat16, 16, 128>(a, blocks, least, stream) : launch_join<__nv_bfloat16, 32, 128>(a, blocks, least, stream);
+    if (dtype == LLB_F32) return launch_join<float, KT>(a, blocks, least, stream);
+    return tile == KT ? launch_join<__nv_bfloat16, KT>(a, blocks, least, stream) : launch_join<__nv_bfloat16, 128>(a, blocks, least, stream);
 }
 
 namespace {
@@ -574,7 +567,7 @@ struct Layout {
 Layout layout(int T, int S, int Hq, int group, int hd, int num_slots, int rows, int blocks, int tile, int mass) {
     Layout l;
     l.part_o = 0;
-    l.part_ml = l.part_o + 2ll * blocks * rows * hd;
+    l.part_ml = l.part_o + 2ll * blocks * rows * ((hd + 3) & ~3);
     l.open = (l.part_ml + 2ll * blocks * rows * 2 + 3) & ~3ll;
     l.part_mass = l.open + 8ll * blocks;
     l.lse = l.part_mass + (mass == 1 ? 2ll * blocks * 128 : 0);

@@ -34,7 +34,8 @@ struct LlbSpanArgs {
     int score_tiles;
     const float* mass_in;            // [Hkv, num_slots] or null: zeros
     float* mass;                     // [Hkv, num_slots]
-    float* part_o;                   // [2 * blocks, rows, hd]: what a block has of a job that began before it (0) and goes on after it (1)
+    float* part_o;                   // [2 * blocks, ceil(hd / 4), rows, 4]: what a block has of a job that began before it (0) and goes on after
+                                     // it (1); four dimensions of neighbouring rows side by side, as the threads that write and join them have them
     float* part_ml;                  // [2 * blocks, rows, 2]
     int* open;                       // [blocks, 8]: the job that begins in a block and goes on after it, see LlbOpen
     int nodes;                       // rows of a request that a job holds at most

@@ -60,7 +60,7 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
 __device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
 }
-// D[128 x N] += A B with A in tensor memory (bf16, two to a column).
+// D[128 x N] += A B with A in tensor memory (bf16, two to a column); the first product of a sum replaces D.
 __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t acc) {
     asm volatile(
         "{\n.reg .pred p;\n"
@@ -68,6 +68,25 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, u
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
         ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(acc)
         : "memory");
+}
+__device__ __forceinline__ void umma_bf16_ts_acc(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc) {
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "setp.eq.u32 p, 0, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc)
+        : "memory");
+}
+// A 128 x 128 tile of scores, both operands K-major in shared memory.  What a product costs the issuing warp is its instructions, beside
+// eight busy ones: the descriptors are made once and counted up.
+template <int KB> __device__ __forceinline__ void issue_scores(uint32_t tmem, uint32_t a_addr, uint32_t b_addr, uint32_t idesc) {
+    const uint64_t da = desc_kmajor(a_addr), db = desc_kmajor(b_addr);
+#pragma unroll
+    for (int k = 0; k < 4 * KB; ++k) {
+        const uint64_t step = (k >> 2) * (TILE_BYTES >> 4) + (k & 3) * 2;
+        if (k == 0) umma_bf16_first(tmem, da, db, idesc);
+        else umma_bf16_acc(tmem, da + step, db + step, idesc);
+    }
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&u)[32]) {
     asm volatile(
@@ -115,6 +134,29 @@ struct RowMask {
 __device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 __device__ __forceinline__ bool bf16_odd(uint32_t pair) { return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u; }
 
+// Two floats in a 64-bit register: an instruction for both (the schedulers' slots are what the softmax shares with the warp that issues
+// the products).
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // The largest of a lane's 128 scores.
 __device__ __forceinline__ float tile_max(uint32_t tmem) {
     float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
@@ -123,11 +165,11 @@ __device__ __forceinline__ float tile_max(uint32_t tmem) {
         float s[32];
         tmem_ld32(tmem + c, s);
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-            t0 = fmaxf(t0, s[i]);
-            t1 = fmaxf(t1, s[i + 1]);
-            t2 = fmaxf(t2, s[i + 2]);
-            t3 = fmaxf(t3, s[i + 3]);
+        for (int i = 0; i < 32; i += 8) {
+            t0 = max3(t0, s[i], s[i + 1]);
+            t1 = max3(t1, s[i + 2], s[i + 3]);
+            t2 = max3(t2, s[i + 4], s[i + 5]);
+            t3 = max3(t3, s[i + 6], s[i + 7]);
         }
     }
     return fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
@@ -136,7 +178,9 @@ __device__ __forceinline__ float tile_max(uint32_t tmem) {
 // whether the shift was near enough: after the first tile it nearly always is, so that no pass for the maximum comes before this one.  The scores
 // stay where they are.
 __device__ __forceinline__ void tile_probs(uint32_t tmem, float scale, float shift, uint32_t (&probs)[64], float& sum, float& top) {
-    float l0 = 0.0f, l1 = 0.0f, t0 = -INFINITY, t1 = -INFINITY;
+    float t0 = -INFINITY, t1 = -INFINITY;
+    uint64_t l0 = 0, l1 = 0;
+    const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
     float s[2][32];
     tmem_ld32_nowait(tmem, *reinterpret_cast<uint32_t(*)[32]>(&s[0][0]));
 #pragma unroll
@@ -144,17 +188,26 @@ __device__ __forceinline__ void tile_probs(uint32_t tmem, float scale, float shi
         tmem_wait_ld32(s[c & 1]);
         if (c < 3) tmem_ld32_nowait(tmem + 32 * (c + 1), *reinterpret_cast<uint32_t(*)[32]>(&s[(c + 1) & 1][0]));
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-            const float a = s[c & 1][i], b = s[c & 1][i + 1];
-            t0 = fmaxf(t0, a);
-            t1 = fmaxf(t1, b);
-            const float p0 = fast_exp2(fmaf(a, scale, shift)), p1 = fast_exp2(fmaf(b, scale, shift));
-            l0 += p0;
-            l1 += p1;
+        for (int i = 0; i < 32; i += 4) {
+            const float* v = &s[c & 1][i];
+            t0 = max3(t0, v[0], v[1]);
+            t1 = max3(t1, v[2], v[3]);
+            float p0, p1, p2, p3;
+            unpack2(fma2(pack2(v[0], v[1]), scale2, shift2), p0, p1);
+            unpack2(fma2(pack2(v[2], v[3]), scale2, shift2), p2, p3);
+            p0 = fast_exp2(p0);
+            p1 = fast_exp2(p1);
+            p2 = fast_exp2(p2);
+            p3 = fast_exp2(p3);
+            l0 = add2(l0, pack2(p0, p1));
+            l1 = add2(l1, pack2(p2, p3));
             probs[16 * c + i / 2] = wm::pack_bf16(p0, p1);
+            probs[16 * c + i / 2 + 1] = wm::pack_bf16(p2, p3);
         }
     }
-    sum = l0 + l1;
+    float a, b;
+    unpack2(add2(l0, l1), a, b);
+    sum = a + b;
     top = fmaxf(t0, t1);
 }
 
@@ -299,15 +352,8 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             tc_fence_after();
         };
         auto issue_s = [&](int x, int b, uint32_t half) {
-            if (lane == 0 && ok) {
-                const uint32_t qa = smem_u32(q_s + b * HALF), ka = smem_u32(ring + half % RING * HALF);
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_bf16(tmem_base + x * 128, desc_kmajor(qa + kb * TILE_BYTES + k * 32), desc_kmajor(ka + kb * TILE_BYTES + k * 32),
-                                  IDESC_S, (kb > 0 || k > 0) ? 1u : 0u);
-            }
+            if (lane == 0 && ok)
+                issue_scores<KB>(tmem_base + x * 128, smem_u32(q_s + b * HALF), smem_u32(ring + half % RING * HALF), IDESC_S);
             __syncwarp();
         };
         for (int t = pc.t0; t < pc.t1;) {
@@ -335,10 +381,11 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     tc_fence_after();
                     if (lane == 0 && ok) {
                         const uint32_t va = smem_u32(ring + (2 * (tiles_before + j) + 1) % RING * HALF);
+                        const uint64_t dv = desc_mnmajor(va, TILE_BYTES);
+                        const uint32_t to = tmem_base + 256 + x * 128, from = tmem_base + x * 128;
+                        umma_bf16_ts(to, from, dv, IDESC_PV, j0 > 0 ? 1u : 0u);
 #pragma unroll
-                        for (int k = 0; k < BK / 16; ++k)
-                            umma_bf16_ts(tmem_base + 256 + x * 128, tmem_base + x * 128 + k * 8, desc_mnmajor(va + k * 16 * 128, TILE_BYTES),
-                                         IDESC_PV, (j0 > 0 || k > 0) ? 1u : 0u);
+                        for (int k = 1; k < BK / 16; ++k) umma_bf16_ts_acc(to, from + k * 8, dv + k * (16 * 128 >> 4), IDESC_PV);
                     }
                     __syncwarp();
                     if (j + step < n) {
@@ -517,9 +564,8 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const bool both = !g.two && n > 1;
             const bool odd = *(volatile int*)&odd_s != 0;
             if (busy) {
-#pragma unroll
-                for (int c = 0; c < HD; c += 32) {
-                    if (c < d0 || c >= d1) continue;
+#pragma unroll 1
+                for (int c = d0; c < d1; c += 32) {
                     float o[32];
                     __syncwarp();
                     if (g.two) {
@@ -543,19 +589,20 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             const bool sees = mask ? (mask[jn >> 6] >> (jn & 63)) & 1ull : jn <= node;
                             const int slot = sees ? llb_span_slot(a, job.s, key) : -1;
                             if (slot < 0) continue;
-                            const __nv_bfloat16* vr = p.v + ((size_t)slot * a.Hkv + job.kvh) * HD + c;
+                            const uint32_t* vr = reinterpret_cast<const uint32_t*>(p.v + ((size_t)slot * a.Hkv + job.kvh) * HD + c);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const float f = __bfloat162float(vr[i]);
-                                if (!(fabsf(f) < INFINITY)) o[i] += f;
+                            for (int i = 0; i < 16; ++i) {
+                                const uint32_t w = vr[i];
+                                if ((w & 0x7f80u) == 0x7f80u) o[2 * i] += __uint_as_float(w << 16);
+                                if ((w & 0x7f800000u) == 0x7f800000u) o[2 * i + 1] += __uint_as_float(w & 0xffff0000u);
                             }
                         }
                     }
                     if (!mine || !ok) {
                     } else if (g.part >= 0) {
-                        float* po = a.part_o + ((size_t)(blockIdx.x * 2 + g.part) * a.rows + node0 * a.group + r) * HD + c;
+                        float4* po = reinterpret_cast<float4*>(a.part_o) + ((size_t)(blockIdx.x * 2 + g.part) * (HD / 4) + c / 4) * a.rows + node0 * a.group + r;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(po + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int i = 0; i < 32; i += 4) po[(size_t)(i / 4) * a.rows] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                     } else {
                         __nv_bfloat16* dst = (__nv_bfloat16*)a.out + ((size_t)row * a.Hq + head) * HD + c;
 #pragma unroll
@@ -807,13 +854,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (at >= 4) ok = mbar_wait(&bar_free[place], ((at >> 2) - 1) & 1, abort_flag) && ok;
                 tc_fence_after();
                 if (lane == 0 && ok) {
-                    const uint32_t ka = smem_u32(k_s + b * HALF), qa = smem_u32(ring + slot * HALF);
-#pragma unroll
-                    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            umma_bf16(tmem_base + place * 128, desc_kmajor(ka + kb * TILE_BYTES + k * 32), desc_kmajor(qa + kb * TILE_BYTES + k * 32),
-                                      IDESC, (kb > 0 || k > 0) ? 1u : 0u);
+                    issue_scores<KB>(tmem_base + place * 128, smem_u32(k_s + b * HALF), smem_u32(ring + slot * HALF), IDESC);
                     umma_commit(&bar_s[place]);
                 }
                 __syncwarp();
