@@ -407,97 +407,117 @@ __global__ void __launch_bounds__(THREADS) span_join_kernel(const LlbSpanArgs a,
     else join_rows<T, 8, 1>(a, job, block, y, ny);
 }
 
-// The same for requests of any number of rows: 64 keys of one request and kv head stay in shared memory, all rows that see any of them
-// go by, 64 (row, head) pairs at a time, and their scores are made once more.  A thread adds up four pairs by four keys; the threads of
-// a key meet at the end in a fixed order.
+// The same for requests of any number of rows: 64 keys of one request and kv head stay in shared memory, the rows that see any of them
+// go by, up to 64 (row, head) pairs at a time, and their scores are made once more.  A thread adds up four pairs by four keys; the threads
+// of a key meet at the end in a fixed order.
 struct ColumnParams {
     LlbSpanArgs a;
     const void* q;
     const void* k;
+    float* part;            // [2 * blocks, KT]
 };
 template <typename T>
 __global__ void __launch_bounds__(THREADS) span_mass_kernel(const ColumnParams p) {
     constexpr int RB = 64;
     const LlbSpanArgs& a = p.a;
-    const int hd = a.hd, hd4 = (hd + 3) & ~3, kp = hd4 + 4;
+    const int hd = a.hd, hd4 = (hd + 3) & ~3, kp = hd4 + 4, nodes = RB / a.group;
     extern __shared__ __align__(16) float sm[];
     float* q_s = sm;                     // [RB][hd4]
     float* k_s = q_s + RB * hd4;         // [KT][kp]
     __shared__ float lse_s[RB];
     __shared__ float sum_s[16][KT];
+    __shared__ LlbMassPiece piece_s;
     const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
     llb_after_previous();
-    // tiles of keys, one request after the other, dealt in turn
-    int tile = blockIdx.x;
-    for (int s = 0; s < a.S; ++s) {
-        const LlbSpan z = llb_span(a, s);
-        if (z.len == 0) continue;
-        const int keys = z.pos + z.len, tiles = (keys + KT - 1) / KT * a.Hkv;
-        for (; tile < tiles; tile += gridDim.x) {
-            const int kvh = tile % a.Hkv, key0 = tile / a.Hkv * KT;
+    if (tid < 32) {
+        const LlbMassPiece pc = llb_mass_piece(a, KT, nodes, blockIdx.x, gridDim.x, tid);
+        if (tid == 0) {
+            piece_s = pc;
+            llb_leave_open_mass(a, pc.line, pc.job, false);
+        }
+    }
+    __syncthreads();
+    const LlbPiece pc = piece_s.line;
+    LlbMassJob job = piece_s.job;
+    for (int t = pc.t0; t < pc.t1;) {
+        const int u0 = t - job.begin, u1 = min(job.units, pc.t1 - job.begin);
+        const LlbSpan z = job.z;
+        const int key0 = job.tile * KT, keys = z.pos + z.len;
+        for (int i = tid; i < KT * (hd4 / 4); i += THREADS) {
+            const int r = i / (hd4 / 4), d = (i - r * (hd4 / 4)) * 4;
+            const int slot = key0 + r < keys ? llb_span_slot(a, job.s, key0 + r) : -1;
+            *reinterpret_cast<float4*>(k_s + r * kp + d) =
+                slot >= 0 ? load4((const T*)p.k + ((size_t)slot * a.Hkv + job.kvh) * hd, d, hd) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int u = u0; u < u1; ++u) {
+            const int node0 = (job.from + u) * nodes, pairs = min(nodes, z.len - node0) * a.group;
             __syncthreads();
-            for (int i = tid; i < KT * (hd4 / 4); i += THREADS) {
+            for (int i = tid; i < RB * (hd4 / 4); i += THREADS) {
                 const int r = i / (hd4 / 4), d = (i - r * (hd4 / 4)) * 4;
-                const int slot = key0 + r < keys ? llb_span_slot(a, s, key0 + r) : -1;
-                *reinterpret_cast<float4*>(k_s + r * kp + d) =
-                    slot >= 0 ? load4((const T*)p.k + ((size_t)slot * a.Hkv + kvh) * hd, d, hd) : make_float4(0.f, 0.f, 0.f, 0.f);
+                *reinterpret_cast<float4*>(q_s + r * hd4 + d) =
+                    r < pairs ? load4((const T*)p.q + ((size_t)(z.row + node0 + r / a.group) * a.Hq + job.kvh * a.group + r % a.group) * hd, d, hd)
+                              : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            const int from = max(0, key0 - z.pos) * a.group, pairs = z.len * a.group;          // rows before see none of the tile
-            for (int r0 = from; r0 < pairs; r0 += RB) {
-                __syncthreads();
-                for (int i = tid; i < RB * (hd4 / 4); i += THREADS) {
-                    const int w = i / (hd4 / 4), d = (i - w * (hd4 / 4)) * 4, r = r0 + w;
-                    *reinterpret_cast<float4*>(q_s + w * hd4 + d) =
-                        r < pairs ? load4((const T*)p.q + ((size_t)(z.row + r / a.group) * a.Hq + kvh * a.group + r % a.group) * hd, d, hd)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
-                if (tid < RB) {
-                    const int r = r0 + tid;
-                    lse_s[tid] = r < pairs ? a.lse[(size_t)(z.row + r / a.group) * a.Hq + kvh * a.group + r % a.group] : INFINITY;
-                }
-                __syncthreads();
-                float x[4][4];
+            if (tid < RB)
+                lse_s[tid] = tid < pairs ? a.lse[(size_t)(z.row + node0 + tid / a.group) * a.Hq + job.kvh * a.group + tid % a.group] : INFINITY;
+            __syncthreads();
+            float x[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i][j] = 0.0f;
+            for (int d = 0; d < hd4; d += 4) {
+                float4 qv[4], kv[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(q_s + (ty * 4 + i) * hd4 + d);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * kp + d);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[i][j] = 0.0f;
-                for (int d = 0; d < hd4; d += 4) {
-                    float4 qv[4], kv[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(q_s + (ty * 4 + i) * hd4 + d);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * kp + d);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            x[i][j] = fmaf(qv[i].x, kv[j].x, x[i][j]);
-                            x[i][j] = fmaf(qv[i].y, kv[j].y, x[i][j]);
-                            x[i][j] = fmaf(qv[i].z, kv[j].z, x[i][j]);
-                            x[i][j] = fmaf(qv[i].w, kv[j].w, x[i][j]);
-                        }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int last = z.pos + (r0 + ty * 4 + i) / a.group;          // the last key that the row sees
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (key0 + tx + 16 * j <= last) sum[j] += exp2f(x[i][j] * a.scale_log2e - lse_s[ty * 4 + i]);
-                }
+                    for (int j = 0; j < 4; ++j) {
+                        x[i][j] = fmaf(qv[i].x, kv[j].x, x[i][j]);
+                        x[i][j] = fmaf(qv[i].y, kv[j].y, x[i][j]);
+                        x[i][j] = fmaf(qv[i].z, kv[j].z, x[i][j]);
+                        x[i][j] = fmaf(qv[i].w, kv[j].w, x[i][j]);
+                    }
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum_s[ty][tx + 16 * j] = sum[j];
-            __syncthreads();
-            if (tid < KT && key0 + tid < keys) {
-                float total = 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                const int last = z.pos + node0 + (ty * 4 + i) / a.group;          // the last key that the row sees
 #pragma unroll
-                for (int i = 0; i < 16; ++i) total += sum_s[i][tid];
-                llb_add_mass(a, z, s, key0 + tid, kvh, total);
+                for (int j = 0; j < 4; ++j)
+                    if (ty * 4 + i < pairs && key0 + tx + 16 * j <= last) sum[j] += exp2f(x[i][j] * a.scale_log2e - lse_s[ty * 4 + i]);
             }
         }
-        tile -= tiles;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum_s[ty][tx + 16 * j] = sum[j];
+        __syncthreads();
+        const int part = job.begin < pc.t0 ? 0 : job.begin + job.units > pc.t1 ? 1 : -1;
+        if (tid < KT) {
+            float total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) total += sum_s[i][tid];
+            if (part >= 0) p.part[(size_t)(blockIdx.x * 2 + part) * KT + tid] = total;
+            else llb_add_mass(a, z, job.s, key0 + tid, job.kvh, total);
+        }
+        if (tid == 0 && part == 1) llb_leave_open_mass(a, pc, job, true);
+        __syncthreads();
+        t = job.begin + u1;
+        if (t < pc.t1) job.next(a, KT, nodes);
     }
+}
+
+// The sums of keys whose rows several blocks had, in the blocks' order.
+template <int TILE> __global__ void __launch_bounds__(TILE) span_mass_join_kernel(const LlbSpanArgs a, const float* part) {
+    llb_after_previous();
+    const int4 job = reinterpret_cast<const int4*>(a.open)[2 * blockIdx.x];          // blocks, request, tile, kv head
+    if (job.x == 0) return;
+    float sum = part[(size_t)(blockIdx.x * 2 + 1) * TILE + threadIdx.x];
+#pragma unroll 4
+    for (int b = 1; b < job.x; ++b) sum += part[(size_t)(blockIdx.x + b) * 2 * TILE + threadIdx.x];
+    llb_add_mass(a, llb_span(a, job.y), job.y, job.z * TILE + threadIdx.x, job.w, sum);
 }
 
 template <typename T, int TILE>
@@ -513,6 +533,7 @@ int launch_join(const LlbSpanArgs& a, int blocks, int least, cudaStream_t stream
     llb_launch(span_join_kernel<T, TILE>, dim3(blocks * ny + a.S * a.Hkv * mass_y), dim3(THREADS), 0, stream, a, blocks, ny, mass_y, least);
     return llb_check_launch("span_join");
 }
+
 template <typename T, int RB, int NI>
 int launch_attention(const SimtParams& p, int blocks, cudaStream_t stream) {
     const int hd4 = (p.a.hd + 3) & ~3;
@@ -660,14 +681,20 @@ LLB_EXPORT int llb_paged_attention_mass(const void* q, const void* k, const void
     a.mass = mass;
     if (int rc = attend(a, q, k, v, dtype, scratch, single ? 2 : 1, tc, &part_mass, error_flag, stream)) return rc;
     if (single) return 0;
-    if (tc) return llb_span_mass_tc(a, q, k, part_mass, tc_blocks(), error_flag, stream);
+    if (tc) {
+        if (int rc = llb_span_mass_tc(a, q, k, part_mass, tc_blocks(), error_flag, stream)) return rc;
+        llb_launch(span_mass_join_kernel<128>, dim3(tc_blocks()), dim3(128), 0, stream, a, (const float*)part_mass);
+        return llb_check_launch("span_mass_join");
+    }
     ColumnParams p;
-    p.a = a; p.q = q; p.k = k;
+    p.a = a; p.q = q; p.k = k; p.part = part_mass;
     const int hd4 = (hd + 3) & ~3;
     const size_t smem = sizeof(float) * ((size_t)64 * hd4 + KT * (hd4 + 4));
     auto kernel = dtype == LLB_F32 ? span_mass_kernel<float> : span_mass_kernel<__nv_bfloat16>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return llb_fail("span_mass: cannot opt in to %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
-    llb_launch(kernel, dim3(2 * llb_device_sms()), dim3(THREADS), smem, stream, p);
-    return llb_check_launch("span_mass");
+    llb_launch(kernel, dim3(simt_blocks()), dim3(THREADS), smem, stream, p);
+    if (int rc = llb_check_launch("span_mass")) return rc;
+    llb_launch(span_mass_join_kernel<KT>, dim3(simt_blocks()), dim3(KT), 0, stream, a, (const float*)part_mass);
+    return llb_check_launch("span_mass_join");
 }

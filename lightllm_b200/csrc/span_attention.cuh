@@ -81,6 +81,7 @@ struct LlbJob {
         if (++kvh < a.Hkv) return;
         kvh = 0;
         first += a.nodes;
+#pragma unroll 1
         while (first >= z.len) {
             ++s;
             z = llb_span(a, s);
@@ -105,6 +106,7 @@ __device__ __forceinline__ int llb_span_tiles(const LlbSpanArgs& a, const LlbSpa
     int n = 0;
     if (z.len > 0 && a.mask) n = (z.len + a.nodes - 1) / a.nodes * ((z.pos + z.len + tile - 1) / tile);
     else
+#pragma unroll 1
         for (int c = 0; c < z.len; c += a.nodes) n += (llb_span_keys(a, z, c + a.nodes) + tile - 1) / tile;
     return n * a.Hkv;
 }
@@ -114,6 +116,7 @@ __device__ __forceinline__ LlbPiece llb_piece(const LlbSpanArgs& a, int tile, in
     LlbSpan z = {0, 0, 0};
     int mine = 0;
     p.total = 0;
+#pragma unroll 1
     for (int base = 0; base < a.S; base += 32) {
         z = base + lane < a.S ? llb_span(a, base + lane) : LlbSpan{0, 0, 0};
         mine = llb_span_tiles(a, z, tile);
@@ -125,6 +128,7 @@ __device__ __forceinline__ LlbPiece llb_piece(const LlbSpanArgs& a, int tile, in
     p.t0 = p.start(block);
     p.t1 = p.start(block + 1);
     int before = 0;
+#pragma unroll 1
     for (int base = 0; base < a.S; base += 32) {
         if (a.S > 32) {
             z = base + lane < a.S ? llb_span(a, base + lane) : LlbSpan{0, 0, 0};
@@ -149,6 +153,7 @@ __device__ __forceinline__ LlbPiece llb_piece(const LlbSpanArgs& a, int tile, in
         before += __shfl_sync(0xffffffffu, sum, 31);
     }
     p.job.first = 0;
+#pragma unroll 1
     for (;;) {
         p.job.measure(a, tile);
         if (p.t0 < p.job.begin + p.job.tiles * a.Hkv) break;
@@ -193,6 +198,96 @@ __device__ __forceinline__ void llb_leave_open(const LlbSpanArgs& a, const LlbPi
 // Joins the parts of cut jobs and, for requests of one row (a.scores), adds up the weights that their keys received; `blocks` is the grid
 // of the attention kernel, `tile` its keys a tile, `least` what it gave llb_piece.
 int llb_span_join(const LlbSpanArgs& a, int dtype, int blocks, int tile, int least, cudaStream_t stream);
+
+// ---- the weights that keys receive, of requests of several rows ------------------------------------------------------------------
+// A job is a tile of keys of one request and kv head; the tiles of `nodes` rows that see any of them make the line that is cut among the
+// blocks.  A job that a cut falls into leaves partial sums, which a second kernel adds up in the blocks' order.
+struct LlbMassJob {
+    LlbSpan z;
+    int s, tile, kvh;
+    int from, units, begin;     // first tile of rows that sees the keys, how many do, the job's place in the line
+    __device__ __forceinline__ void measure(int keys, int nodes) {
+        from = max(0, tile * keys - z.pos) / nodes;
+        units = (z.len + nodes - 1) / nodes - from;
+    }
+    __device__ __forceinline__ int tiles(int keys) const { return z.len > 0 ? (z.pos + z.len + keys - 1) / keys : 0; }
+    __device__ __forceinline__ void next(const LlbSpanArgs& a, int keys, int nodes) {
+        begin += units;
+        if (++kvh < a.Hkv) return;
+        kvh = 0;
+        ++tile;
+#pragma unroll 1
+        while (tile >= tiles(keys)) {
+            z = llb_span(a, ++s);
+            tile = 0;
+        }
+        measure(keys, nodes);
+    }
+};
+struct LlbMassPiece {
+    LlbPiece line;              // (its job is not used)
+    LlbMassJob job;
+};
+__device__ __forceinline__ int llb_mass_units(const LlbSpanArgs& a, const LlbSpan& z, int keys, int nodes) {
+    if (z.len == 0) return 0;
+    const int rows = (z.len + nodes - 1) / nodes, whole = z.pos / keys + 1, tiles = (z.pos + z.len + keys - 1) / keys;
+    int n = whole * rows;          // (whole <= tiles: the first row sees key pos)
+#pragma unroll 1
+    for (int i = whole; i < tiles; ++i) n += rows - (i * keys - z.pos) / nodes;
+    return n * a.Hkv;
+}
+__device__ __forceinline__ LlbMassPiece llb_mass_piece(const LlbSpanArgs& a, int keys, int nodes, int block, int grid, int lane) {
+    LlbMassPiece m;
+    LlbPiece& p = m.line;
+    int mine = 0;
+    p.total = 0;
+#pragma unroll 1
+    for (int base = 0; base < a.S; base += 32) {
+        mine = base + lane < a.S ? llb_mass_units(a, llb_span(a, base + lane), keys, nodes) : 0;
+        p.total += __reduce_add_sync(0xffffffffu, mine);
+    }
+    p.blocks = min(grid, (p.total + 1) / 2);
+    p.t0 = p.t1 = 0;
+    if (block >= p.blocks) return m;
+    p.t0 = p.start(block);
+    p.t1 = p.start(block + 1);
+    int before = 0;
+#pragma unroll 1
+    for (int base = 0; base < a.S; base += 32) {
+        if (a.S > 32) mine = base + lane < a.S ? llb_mass_units(a, llb_span(a, base + lane), keys, nodes) : 0;
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, before + sum > p.t0);
+        if (past) {
+            const int at = __ffs(past) - 1;
+            m.job.s = base + at;
+            m.job.begin = before + __shfl_sync(0xffffffffu, sum - mine, at);
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    m.job.z = llb_span(a, m.job.s);
+    m.job.tile = 0;
+#pragma unroll 1
+    for (;;) {
+        m.job.measure(keys, nodes);
+        if (p.t0 < m.job.begin + m.job.units * a.Hkv) break;
+        m.job.begin += m.job.units * a.Hkv;
+        ++m.job.tile;
+    }
+    m.job.kvh = (p.t0 - m.job.begin) / m.job.units;
+    m.job.begin += m.job.kvh * m.job.units;
+    return m;
+}
+// What the block that a job begins in leaves of it: how many blocks have parts (0: it has no such job), request, tile and kv head.
+__device__ __forceinline__ void llb_leave_open_mass(const LlbSpanArgs& a, const LlbPiece& line, const LlbMassJob& job, bool goes_on) {
+    reinterpret_cast<int4*>(a.open)[2 * blockIdx.x] =
+        goes_on ? make_int4(line.owner(job.begin + job.units - 1) - blockIdx.x + 1, job.s, job.tile, job.kvh) : make_int4(0, 0, 0, 0);
+}
 
 // The tensor-core kernels (span_attention_tcgen05.cu): whether they take a call, how many rows of a request fill 128 pairs, the attention
 // (a.nodes twice that many, a.rows 2 x 128), and the weights of keys (part: 2 * blocks * 128 floats).

@@ -298,8 +298,10 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const uint32_t q_bytes = (uint32_t)p.pairs_nodes * a.group * 128 * KB;
         const int ppt = BK / a.page_size;
         uint32_t loaded = 0;
+#pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const Segment g = segment_of(p, pc, job, t);
+#pragma unroll 1
             for (int x = 0; x < (g.two ? 2 : 1); ++x) {
                 const int b = g.two ? x : q_next;
                 if (q_uses[b] > 0) ok = mbar_wait(&bar_q_free[b], (q_uses[b] - 1) & 1, abort_flag) && ok;
@@ -313,6 +315,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 ++q_uses[b];
             }
             if (!g.two) q_next ^= 1;
+#pragma unroll 1
             for (int k = g.k0; k < g.k1; ++k) {
                 const int row = lane < ppt ? page_row(a, job.s, k * ppt + lane, job.keys) : a.num_slots;
 #pragma unroll
@@ -356,10 +359,12 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 issue_scores<KB>(tmem_base + x * 128, smem_u32(q_s + b * HALF), smem_u32(ring + half % RING * HALF), IDESC_S);
             __syncwarp();
         };
+#pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const Segment g = segment_of(p, pc, job, t);
             const int n = g.k1 - g.k0, step = g.two ? 1 : 2;
             int buf[2];
+#pragma unroll 1
             for (int x = 0; x < 2; ++x) {
                 const int b = g.two ? x : q_next;
                 buf[x] = b;
@@ -372,7 +377,9 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 __syncwarp();
             }
             if (!g.two) q_next ^= 1;
+#pragma unroll 1
             for (int j0 = 0; j0 < n; j0 += step) {
+#pragma unroll 1
                 for (int x = 0; x < 2; ++x) {
                     const int j = g.two ? j0 : j0 + x;
                     if (j >= n) continue;
@@ -410,6 +417,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const uint32_t tmem_s = tmem_base + x * 128 + lanes, tmem_o = tmem_base + 256 + lanes;
         bool ok = true;
         uint32_t n_s = 0, n_o = 0;
+#pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const Segment g = segment_of(p, pc, job, t);
             const int n = g.k1 - g.k0, step = g.two ? 1 : 2;
@@ -424,6 +432,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const int own = a.mask ? z.pos : z.pos + node + 1;              // first keys that this row sees
             const bool busy = (warp & 3) * 32 < pairs;                      // any pair in this warp's lanes
             float m_ref = -INFINITY, l_run = 0.0f;
+#pragma unroll 1
             for (int j = g.two ? 0 : x; j < n; j += step) {
                 const int key0 = (g.k0 + j) * BK;
                 const uint32_t half = 2 * (tiles_before + j);
@@ -443,9 +452,9 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     const int key = key0 + r;
                     if (key >= all && ok) {
                         uint8_t* row = ring + (half + 1) % RING * HALF + (uint32_t)r * 128;
-#pragma unroll
+#pragma unroll 1
                         for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
+#pragma unroll 1
                             for (int c = 0; c < 8; ++c) {
                                 // (neighbouring threads begin at other chunks: their rows lie in the same banks)
                                 uint4* at = reinterpret_cast<uint4*>(row + kb * TILE_BYTES + ((c ^ r) & 7) * 16);
@@ -584,6 +593,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         }
                     }
                     if (odd && mine) {
+#pragma unroll 1
                         for (int key = max(all, g.k0 * BK); key < min(job.keys, g.k1 * BK); ++key) {
                             const int jn = key - z.pos;
                             const bool sees = mask ? (mask[jn >> 6] >> (jn & 63)) & 1ull : jn <= node;
@@ -655,82 +665,7 @@ struct MassArgs {
     TcParams p;
     float* part;                // [2 * blocks, 128]
 };
-struct MassJob {
-    LlbSpan z;
-    int s, tile, kvh;
-    int from, units, begin;     // first tile of rows that sees the keys, how many do, the job's place in the line
-    __device__ __forceinline__ void measure(int pairs_nodes) {
-        from = max(0, tile * BK - z.pos) / pairs_nodes;
-        units = (z.len + pairs_nodes - 1) / pairs_nodes - from;
-    }
-    __device__ __forceinline__ int tiles() const { return z.len > 0 ? (z.pos + z.len + BK - 1) / BK : 0; }
-    __device__ __forceinline__ void next(const LlbSpanArgs& a, int pairs_nodes) {
-        begin += units;
-        if (++kvh < a.Hkv) return;
-        kvh = 0;
-        ++tile;
-        while (tile >= tiles()) {
-            z = llb_span(a, ++s);
-            tile = 0;
-        }
-        measure(pairs_nodes);
-    }
-};
-struct MassPiece {
-    LlbPiece line;              // (its job is not used)
-    MassJob job;
-};
-__device__ __forceinline__ int mass_units(const LlbSpanArgs& a, const LlbSpan& z, int pairs_nodes) {
-    if (z.len == 0) return 0;
-    const int rows = (z.len + pairs_nodes - 1) / pairs_nodes, whole = z.pos / BK + 1, tiles = (z.pos + z.len + BK - 1) / BK;
-    int n = whole * rows;          // (whole <= tiles: the first row sees key pos)
-    for (int i = whole; i < tiles; ++i) n += rows - (i * BK - z.pos) / pairs_nodes;
-    return n * a.Hkv;
-}
-__device__ __forceinline__ MassPiece mass_piece(const LlbSpanArgs& a, int pairs_nodes, int block, int grid, int lane) {
-    MassPiece m;
-    LlbPiece& p = m.line;
-    int mine = 0;
-    p.total = 0;
-    for (int base = 0; base < a.S; base += 32) {
-        mine = base + lane < a.S ? mass_units(a, llb_span(a, base + lane), pairs_nodes) : 0;
-        p.total += __reduce_add_sync(0xffffffffu, mine);
-    }
-    p.blocks = min(grid, (p.total + 1) / 2);
-    p.t0 = p.t1 = 0;
-    if (block >= p.blocks) return m;
-    p.t0 = p.start(block);
-    p.t1 = p.start(block + 1);
-    int before = 0;
-    for (int base = 0; base < a.S; base += 32) {
-        if (a.S > 32) mine = base + lane < a.S ? mass_units(a, llb_span(a, base + lane), pairs_nodes) : 0;
-        int sum = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += x;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, before + sum > p.t0);
-        if (past) {
-            const int at = __ffs(past) - 1;
-            m.job.s = base + at;
-            m.job.begin = before + __shfl_sync(0xffffffffu, sum - mine, at);
-            break;
-        }
-        before += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    m.job.z = llb_span(a, m.job.s);
-    m.job.tile = 0;
-    for (;;) {
-        m.job.measure(pairs_nodes);
-        if (p.t0 < m.job.begin + m.job.units * a.Hkv) break;
-        m.job.begin += m.job.units * a.Hkv;
-        ++m.job.tile;
-    }
-    m.job.kvh = (p.t0 - m.job.begin) / m.job.units;
-    m.job.begin += m.job.kvh * m.job.units;
-    return m;
-}
+
 template <int HD> struct MassShape {
     static constexpr int RING = HD == 64 ? 8 : 4;
     static constexpr size_t SMEM = (size_t)(2 + RING) * Shape<HD>::HALF + 1024;
@@ -745,7 +680,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     __shared__ __align__(8) uint64_t bar_k_full[2], bar_k_free[2], bar_q_full[RING], bar_q_free[RING], bar_s[4], bar_free[4];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_s;
-    __shared__ MassPiece piece_s;
+    __shared__ LlbMassPiece piece_s;
     __shared__ __align__(16) float lse_s[2][2][128];
     __shared__ float sum_s[128];
     extern __shared__ uint8_t smem_raw[];
@@ -782,10 +717,10 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     griddep_wait();
     griddep_launch_dependents();
     if (warp == 0) {
-        const MassPiece pc = mass_piece(a, pairs_nodes, blockIdx.x, gridDim.x, lane);
+        const LlbMassPiece pc = llb_mass_piece(a, BK, pairs_nodes, blockIdx.x, gridDim.x, lane);
         if (lane == 0) {
             piece_s = pc;
-            reinterpret_cast<int4*>(a.open)[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+            llb_leave_open_mass(a, pc.line, pc.job, false);
         }
     }
     tc_fence_before();
@@ -793,7 +728,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     tc_fence_after();
     const uint32_t tmem_base = tmem_slot;
     const LlbPiece pc = piece_s.line;
-    MassJob job = piece_s.job;
+    LlbMassJob job = piece_s.job;
     uint32_t jobs = 0, units_before = 0;
     constexpr uint32_t IDESC = idesc_bf16(BK, BQ, 0);
 
@@ -802,6 +737,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const uint32_t q_bytes = (uint32_t)pairs_tile * 128 * KB;
         const int ppt = BK / a.page_size;
         uint32_t loaded = 0;
+#pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const int u0 = t - job.begin, u1 = min(job.units, pc.t1 - job.begin), b = jobs & 1;
             const int row = lane < ppt ? page_row(a, job.s, job.tile * ppt + lane, job.z.pos + job.z.len) : a.num_slots;
@@ -816,6 +752,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 }
             }
             __syncwarp();
+#pragma unroll 1
             for (int u = u0; u < u1; ++u) {
                 const uint32_t slot = loaded % RING;
                 if (loaded >= RING) ok = mbar_wait(&bar_q_free[slot], (loaded / RING - 1) & 1, abort_flag) && ok;
@@ -833,7 +770,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             }
             ++jobs;
             t = job.begin + u1;
-            if (t < pc.t1) job.next(a, pairs_nodes);
+            if (t < pc.t1) job.next(a, BK, pairs_nodes);
         }
         if (!ok) {
             for (uint32_t i = loaded > RING ? loaded - RING : 0; i < loaded; ++i) {
@@ -844,9 +781,11 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
     } else if (warp == MMA_WARP) {
         bool ok = true;
+#pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const int u0 = t - job.begin, u1 = min(job.units, pc.t1 - job.begin), b = jobs & 1;
             ok = mbar_wait(&bar_k_full[b], (jobs >> 1) & 1, abort_flag) && ok;
+#pragma unroll 1
             for (int u = u0; u < u1; ++u) {
                 const uint32_t at = units_before + (u - u0);          // the block's tiles of rows go to four score tiles in turn
                 const uint32_t slot = at % RING, place = at & 3;
@@ -862,12 +801,13 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             units_before += u1 - u0;
             ++jobs;
             t = job.begin + u1;
-            if (t < pc.t1) job.next(a, pairs_nodes);
+            if (t < pc.t1) job.next(a, BK, pairs_nodes);
         }
     } else if (warp < MMA_WARP) {
         const int x = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         bool ok = true;
+#pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const int u0 = t - job.begin, u1 = min(job.units, pc.t1 - job.begin), n = u1 - u0;
             const LlbSpan z = job.z;
@@ -880,6 +820,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             };
             const int first = (int)((x - units_before) & 1);          // the group's first tile of the job
             float lse = lse_of(first);
+#pragma unroll 1
             for (int j = first; j < n; j += 2) {
                 const uint32_t at = units_before + j, place = at & 3;
                 float* lse_t = lse_s[x][place >> 1];
@@ -926,9 +867,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 const int part = job.begin < pc.t0 ? 0 : job.begin + job.units > pc.t1 ? 1 : -1;
                 if (part >= 0) {
                     m.part[(size_t)(blockIdx.x * 2 + part) * 128 + r] = sum;
-                    if (part == 1 && r == 0)
-                        reinterpret_cast<int4*>(a.open)[2 * blockIdx.x] =
-                            make_int4(pc.owner(job.begin + job.units - 1) - blockIdx.x + 1, job.s, job.tile, job.kvh);
+                    if (part == 1 && r == 0) llb_leave_open_mass(a, pc, job, true);
                 } else if (ok) {
                     llb_add_mass(a, z, job.s, key, job.kvh, sum);
                 }
@@ -938,7 +877,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             units_before += n;
             ++jobs;
             t = job.begin + u1;
-            if (t < pc.t1) job.next(a, pairs_nodes);
+            if (t < pc.t1) job.next(a, BK, pairs_nodes);
         }
     }
     tc_fence_before();
@@ -948,18 +887,6 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         tc_fence_after();
         tmem_dealloc(tmem_base, TMEM_COLS);
     }
-}
-
-// The sums of keys whose rows several blocks had, in the blocks' order.
-__global__ void __launch_bounds__(128) span_mass_join_kernel(const MassArgs m) {
-    llb_after_previous();
-    const LlbSpanArgs& a = m.p.a;
-    const int4 job = reinterpret_cast<const int4*>(a.open)[2 * blockIdx.x];          // blocks, request, tile, kv head
-    if (job.x == 0) return;
-    float sum = m.part[(size_t)(blockIdx.x * 2 + 1) * 128 + threadIdx.x];
-#pragma unroll 4
-    for (int b = 1; b < job.x; ++b) sum += m.part[(size_t)(blockIdx.x + b) * 2 * 128 + threadIdx.x];
-    llb_add_mass(a, llb_span(a, job.y), job.y, job.z * BK + threadIdx.x, job.w, sum);
 }
 
 // q [T, Hq, hd] in boxes of the group's heads of `nodes` rows.
@@ -1024,7 +951,5 @@ int llb_span_mass_tc(const LlbSpanArgs& a, const void* q, const void* k, float* 
     int rc;
     if ((rc = make_map_q(q, a.T, a.Hq, a.hd, a.group, m.p.pairs_nodes, &mq))) return rc;
     if ((rc = make_map_bf16(k, a.num_slots, (long long)a.Hkv * a.hd, a.page_size, &mk))) return rc;
-    if ((rc = a.hd == 64 ? launch_mass_tc<64>(mq, mk, m, blocks, stream) : launch_mass_tc<128>(mq, mk, m, blocks, stream))) return rc;
-    llb_launch(span_mass_join_kernel, dim3(blocks), dim3(128), 0, stream, m);
-    return llb_check_launch("span_mass_join");
+    return a.hd == 64 ? launch_mass_tc<64>(mq, mk, m, blocks, stream) : launch_mass_tc<128>(mq, mk, m, blocks, stream);
 }
