@@ -115,10 +115,12 @@ __global__ void __launch_bounds__(COMMIT_THREADS) tree_commit_kernel(const Commi
 // order) take the keys, values, weights and positions of those that stay beyond it (in rising order).  Attention does not ask for
 // the order of its keys (they carry their rotation), so nothing else moves: as many rows as there are holes instead of nearly all.
 //
-// A block takes one (layer, request, kv head).  The worth of all places as whole numbers in the floats' order is kept in shared
-// memory (or read again where there are too many); the budget's threshold is found digit by digit from the top, 11, 11 and 10 bits,
-// by counting, the dropping of a single place by one search for the least.  The places that stay become a bit each, which
-// gives holes and fillers their numbers by counting bits; the moves are then dealt evenly to all threads, 16 bytes at a time.
+// A block takes one (layer, request, kv head).  A thread has up to 8 or 32 places, all asked for at once (what a block's time is made of is
+// trips to memory, 0.6 us each): their cache rows and their worth as whole numbers in the floats' order stay in registers.  The
+// budget's threshold is found digit by digit from the top, 11, 11 and 10 bits, by counting, the dropping of a single place by one search for
+// the least.  The places that stay become a bit each, which gives holes and fillers their numbers by counting bits; the moves
+// are then dealt evenly to all threads, 16 bytes at a time.  Tables of more places go through a kernel that keeps the worths that fit in
+// shared memory and reads the rest again.
 constexpr int EV_THREADS = 512;
 constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_BINS = 2048;
@@ -145,14 +147,259 @@ __device__ __forceinline__ unsigned order_of(float f) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+// The listed moves of one (layer, kv head): rows of K and V, 16 bytes a thread and AHEAD of them on their way, then weights and positions.
 template <typename U>
-__global__ void __launch_bounds__(EV_THREADS) cache_evict_kernel(const EvictParams p) {
+__device__ __forceinline__ void move_rows(const EvictParams& p, size_t plane, int layer, int h, const unsigned (&list)[2][EV_LIST], unsigned count) {
+    constexpr int AHEAD = 8;
+    const unsigned units = 2 * p.head_units, total = count * units;
+    const size_t stride = (size_t)p.Hkv * p.head_units, base = (size_t)layer * p.num_slots * stride + (size_t)h * p.head_units;
+    const int shift = (units & (units - 1)) == 0 ? 31 - __clz(units) : -1;          // (heads of 64 and 128: no division)
+    for (unsigned i0 = threadIdx.x; i0 < total; i0 += EV_THREADS * AHEAD) {
+        U x[AHEAD];
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            const unsigned i = i0 + e * EV_THREADS;
+            if (i >= total) continue;
+            const unsigned m = shift >= 0 ? i >> shift : i / units, u = i - m * units;
+            const int src = (int)list[1][m];
+            const U* from = (const U*)(u < (unsigned)p.head_units ? p.k : p.v) + base + (u < (unsigned)p.head_units ? u : u - p.head_units);
+            if (src >= 0) x[e] = from[(size_t)src * stride];
+        }
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            const unsigned i = i0 + e * EV_THREADS;
+            if (i >= total) continue;
+            const unsigned m = shift >= 0 ? i >> shift : i / units, u = i - m * units;
+            const int src = (int)list[1][m], dst = (int)list[0][m];
+            U* to = (U*)(u < (unsigned)p.head_units ? p.k : p.v) + base + (u < (unsigned)p.head_units ? u : u - p.head_units);
+            if (src >= 0 && dst >= 0) to[(size_t)dst * stride] = x[e];
+        }
+    }
+    for (unsigned m = threadIdx.x; m < count; m += EV_THREADS) {
+        const int src = (int)list[1][m], dst = (int)list[0][m];
+        if (src < 0 || dst < 0) continue;
+        p.mass_out[plane + dst] = p.mass[plane + src];
+        p.positions_out[plane + dst] = p.positions[plane + src];
+    }
+}
+
+// Where `wanted` of those whose digits above this one are `prefix` end, counted from the top: hist holds how many have each value of
+// the digit.  found: the prefix with this digit, how many of its bearers are wanted, how many there are.
+__device__ __forceinline__ void find_digit(const unsigned (&hist)[EV_BINS], unsigned prefix, unsigned wanted, int shift, unsigned (&warp_s)[EV_WARPS][2],
+                                           unsigned (&found)[3]) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int PER = EV_BINS / EV_THREADS;
+    const int top = EV_BINS - 1 - tid * PER;
+    unsigned mine = 0;
+#pragma unroll
+    for (int b = 0; b < PER; ++b) mine += hist[top - b];
+    unsigned sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+    }
+    if (lane == 31) warp_s[warp][0] = sum;
+    __syncthreads();
+    unsigned above = sum - mine;
+    for (int w = 0; w < warp; ++w) above += warp_s[w][0];
+    if (above < wanted && above + mine >= wanted) {
+#pragma unroll
+        for (int b = 0; b < PER; ++b) {
+            const unsigned c = hist[top - b];
+            if (above < wanted && above + c >= wanted) {
+                found[0] = prefix | ((unsigned)(top - b) << shift);
+                found[1] = wanted - above;
+                found[2] = c;
+            }
+            above += c;
+        }
+    }
+    __syncthreads();
+}
+
+// Exclusive sums of `words` counts (two to a word: low and high half) by the first warp; everyone has them and the totals afterwards.
+template <int WORDS> __device__ __forceinline__ void scan_words(unsigned (&count)[WORDS], unsigned& total_s, int words) {
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        unsigned before = 0;
+        for (int w0 = 0; w0 < words; w0 += 32) {
+            const int w = w0 + threadIdx.x;
+            const unsigned mine = w < words ? count[w] : 0u;
+            unsigned sum = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned x = __shfl_up_sync(0xffffffffu, sum, o);
+                if ((int)threadIdx.x >= o) sum += x;
+            }
+            if (w < words) count[w] = before + sum - mine;
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (threadIdx.x == 0) total_s = before;
+    }
+    __syncthreads();
+}
+
+template <typename U, int PER>
+__global__ void __launch_bounds__(EV_THREADS, PER <= 8 ? 2 : 1) cache_evict_kernel(const EvictParams p) {
+    constexpr int WORDS = PER * EV_WARPS;
+    __shared__ unsigned hist[EV_BINS];
+    __shared__ unsigned list_s[2][EV_LIST];
+    __shared__ unsigned warp_s[EV_WARPS][2], word_s[WORDS];
+    __shared__ unsigned long long least_s[EV_WARPS];
+    __shared__ unsigned found_s[3], total_s;
+    llb_after_previous();
+    const int s = blockIdx.x / p.Hkv, h = blockIdx.x - s * p.Hkv, layer = blockIdx.y;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int n = max(0, min(p.lengths[s], p.max_pages * p.page_size)), budget = p.budget;
+    const int from = p.ends[s] - p.latest;
+    const int* table = p.table + (size_t)s * p.max_pages;
+    const size_t plane = ((size_t)layer * p.Hkv + h) * p.num_slots;
+    const bool apart = p.mass_out != p.mass;
+    const int page_shift = (p.page_size & (p.page_size - 1)) == 0 ? 31 - __clz(p.page_size) : -1;
+    if (n <= budget && !apart) return;
+    // place k * EV_THREADS + tid: word k * EV_WARPS + warp of the bits, bit `lane`
+    int slot[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int i = k * EV_THREADS + tid;
+        slot[k] = -1;
+        if (i < n) {
+            const int page_of = page_shift >= 0 ? i >> page_shift : i / p.page_size;
+            const int page = table[page_of];
+            const long long at = (long long)page * p.page_size + (i - page_of * p.page_size);
+            if (page >= 0 && at < p.num_slots) slot[k] = (int)at;
+        }
+    }
+    // the weights and positions of the places that stay where they are
+    auto copy = [&](auto stays) {
+        if (!apart) return;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            if (k * EV_THREADS >= min(n, budget) || slot[k] < 0 || !stays(k)) continue;
+            p.mass_out[plane + slot[k]] = p.mass[plane + slot[k]];
+            p.positions_out[plane + slot[k]] = p.positions[plane + slot[k]];
+        }
+    };
+    if (n <= budget) {
+        copy([&](int) { return true; });
+        return;
+    }
+    unsigned worth[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        worth[k] = 0u;
+        if (slot[k] < 0) continue;
+        const int pos = p.positions[plane + slot[k]];
+        worth[k] = pos < p.first || pos >= from ? 0xffffffffu : order_of(p.mass[plane + slot[k]]);
+    }
+
+    if (n == budget + 1) {
+        // one place goes: the least worth, of equal ones the highest place
+        unsigned long long least = ~0ull;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int i = k * EV_THREADS + tid;
+            const unsigned long long x = ((unsigned long long)worth[k] << 32) | (unsigned)(n - 1 - i);
+            if (i < n && x < least) least = x;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const unsigned long long x = __shfl_xor_sync(0xffffffffu, least, o);
+            least = x < least ? x : least;
+        }
+        if (lane == 0) least_s[warp] = least;
+        __syncthreads();
+        least = least_s[0];
+#pragma unroll
+        for (int w = 1; w < EV_WARPS; ++w) least = least_s[w] < least ? least_s[w] : least;
+        const int hole = n - 1 - (int)(unsigned)least;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int i = k * EV_THREADS + tid;
+            if (i == hole) list_s[0][0] = slot[k];
+            if (i == n - 1) list_s[1][0] = slot[k];
+        }
+        __syncthreads();
+        if (hole != n - 1) move_rows<U>(p, plane, layer, h, list_s, 1);
+        copy([&](int k) { return k * EV_THREADS + tid < budget && k * EV_THREADS + tid != hole; });
+        return;
+    }
+
+    // the threshold: the budget-th largest worth, and how many of its equals stay
+    unsigned prefix = 0, wanted = budget;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
+        for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            // (64 bits: a shift by 32 would be none)
+            if (k * EV_THREADS + tid < n && ((unsigned long long)(worth[k] ^ prefix) >> (shift + width)) == 0)
+                atomicAdd(&hist[(worth[k] >> shift) & ((1u << width) - 1u)], 1u);
+        __syncthreads();
+        find_digit(hist, prefix, wanted, shift, warp_s, found_s);
+        prefix = found_s[0];
+        wanted = found_s[1];
+    }
+    const int words = (n + 31) / 32;
+    unsigned stays = 0;          // a bit for each of the thread's places
+    if (found_s[2] == wanted) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) stays |= (unsigned)(k * EV_THREADS + tid < n && worth[k] >= prefix) << k;
+    } else {
+        // of equals the lowest places stay: they are numbered
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const unsigned same = __ballot_sync(0xffffffffu, k * EV_THREADS + tid < n && worth[k] == prefix);
+            if (lane == 0) word_s[k * EV_WARPS + warp] = __popc(same);
+        }
+        scan_words(word_s, total_s, words);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const bool held = k * EV_THREADS + tid < n;
+            const unsigned same = __ballot_sync(0xffffffffu, held && worth[k] == prefix);
+            const bool on = held && (worth[k] > prefix ||
+                                     (worth[k] == prefix && word_s[k * EV_WARPS + warp] + __popc(same & ((1u << lane) - 1u)) < wanted));
+            stays |= (unsigned)on << k;
+        }
+        __syncthreads();
+    }
+    // numbers of the holes (low half of a count) and of those that fill them (high half)
+    auto is_hole = [&](int k) { return k * EV_THREADS + tid < budget && !((stays >> k) & 1u); };
+    auto fills = [&](int k) { return k * EV_THREADS + tid >= budget && ((stays >> k) & 1u); };
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const unsigned a = __ballot_sync(0xffffffffu, is_hole(k)), b = __ballot_sync(0xffffffffu, fills(k));
+        if (lane == 0) word_s[k * EV_WARPS + warp] = __popc(a) | (__popc(b) << 16);
+    }
+    scan_words(word_s, total_s, words);
+    const unsigned moves = total_s & 0xffffu;
+    for (unsigned m0 = 0; m0 < moves; m0 += EV_LIST) {
+        const unsigned count = min((unsigned)EV_LIST, moves - m0);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const unsigned a = __ballot_sync(0xffffffffu, is_hole(k)), b = __ballot_sync(0xffffffffu, fills(k));
+            const unsigned under = (1u << lane) - 1u, before = word_s[k * EV_WARPS + warp];
+            const unsigned hr = (before & 0xffffu) + __popc(a & under) - m0, fr = (before >> 16) + __popc(b & under) - m0;
+            if (is_hole(k) && hr < count) list_s[0][hr] = slot[k];
+            if (fills(k) && fr < count) list_s[1][fr] = slot[k];
+        }
+        __syncthreads();
+        move_rows<U>(p, plane, layer, h, list_s, count);
+        __syncthreads();
+    }
+    copy([&](int k) { return k * EV_THREADS + tid < budget && ((stays >> k) & 1u); });
+}
+
+template <typename U>
+__global__ void __launch_bounds__(EV_THREADS) cache_evict_any_kernel(const EvictParams p) {
     extern __shared__ unsigned ev_sm[];
     __shared__ unsigned hist[EV_BINS];
     __shared__ unsigned list_s[2][EV_LIST];
     __shared__ unsigned warp_s[EV_WARPS][2];
-    __shared__ unsigned long long least_s[EV_WARPS];
-    __shared__ unsigned found_s[2];
+    __shared__ unsigned found_s[3];
     llb_after_previous();
     const int s = blockIdx.x / p.Hkv, h = blockIdx.x - s * p.Hkv, layer = blockIdx.y;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -184,46 +431,6 @@ __global__ void __launch_bounds__(EV_THREADS) cache_evict_kernel(const EvictPara
     const bool cached = n <= p.cache_places;
     auto worth = [&](int i) -> unsigned { return cached ? worth_s[i] : compute(i); };
 
-    if (n == budget + 1) {
-        // one place goes: the least worth, of equal ones the highest place
-        unsigned long long least = ~0ull;
-        for (int i = tid; i < n; i += EV_THREADS) {
-            const unsigned long long x = ((unsigned long long)compute(i) << 32) | (unsigned)(n - 1 - i);
-            least = x < least ? x : least;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long x = __shfl_xor_sync(0xffffffffu, least, o);
-            least = x < least ? x : least;
-        }
-        if (lane == 0) least_s[warp] = least;
-        __syncthreads();
-        least = least_s[0];
-#pragma unroll
-        for (int w = 1; w < EV_WARPS; ++w) least = least_s[w] < least ? least_s[w] : least;
-        const int hole = n - 1 - (int)(unsigned)least;
-        if (apart)
-            for (int i = tid; i < budget; i += EV_THREADS) {
-                const int slot = slot_of(table, p.page_size, p.num_slots, i);
-                if (slot < 0 || i == hole) continue;
-                p.mass_out[plane + slot] = p.mass[plane + slot];
-                p.positions_out[plane + slot] = p.positions[plane + slot];
-            }
-        if (hole == n - 1) return;
-        const int dst = slot_of(table, p.page_size, p.num_slots, hole), src = slot_of(table, p.page_size, p.num_slots, n - 1);
-        if (dst < 0 || src < 0) return;
-        for (int u = tid; u < 2 * p.head_units; u += EV_THREADS) {
-            const int e = u < p.head_units ? u : u - p.head_units;
-            U* base = (U*)(u < p.head_units ? p.k : p.v) + ((size_t)layer * p.num_slots * p.Hkv + h) * p.head_units + e;
-            base[(size_t)dst * p.Hkv * p.head_units] = base[(size_t)src * p.Hkv * p.head_units];
-        }
-        if (tid == 0) {
-            p.mass_out[plane + dst] = p.mass[plane + src];
-            p.positions_out[plane + dst] = p.positions[plane + src];
-        }
-        return;
-    }
-
     // the threshold: the budget-th largest worth, and how many of its equals stay
     unsigned prefix = 0, wanted = budget;
 #pragma unroll 1
@@ -238,34 +445,7 @@ __global__ void __launch_bounds__(EV_THREADS) cache_evict_kernel(const EvictPara
             if (((unsigned long long)(x ^ prefix) >> (shift + width)) == 0) atomicAdd(&hist[(x >> shift) & ((1u << width) - 1u)], 1u);
         }
         __syncthreads();
-        // how many lie above each thread's four bins, counted from the top
-        constexpr int PER = EV_BINS / EV_THREADS;
-        unsigned mine = 0;
-        const int top = EV_BINS - 1 - tid * PER;
-#pragma unroll
-        for (int b = 0; b < PER; ++b) mine += hist[top - b];
-        unsigned sum = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned x = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += x;
-        }
-        if (lane == 31) warp_s[warp][0] = sum;
-        __syncthreads();
-        unsigned above = sum - mine;
-        for (int w = 0; w < warp; ++w) above += warp_s[w][0];
-        if (above < wanted && above + mine >= wanted) {
-#pragma unroll
-            for (int b = 0; b < PER; ++b) {
-                const unsigned c = hist[top - b];
-                if (above < wanted && above + c >= wanted) {
-                    found_s[0] = prefix | ((unsigned)(top - b) << shift);
-                    found_s[1] = wanted - above;
-                }
-                above += c;
-            }
-        }
-        __syncthreads();
+        find_digit(hist, prefix, wanted, shift, warp_s, found_s);
         prefix = found_s[0];
         wanted = found_s[1];
     }
@@ -345,36 +525,7 @@ __global__ void __launch_bounds__(EV_THREADS) cache_evict_kernel(const EvictPara
                 if (fr - m0 < count) list_s[1][fr - m0] = slot_of(table, p.page_size, p.num_slots, w * 32 + __ffs(x) - 1);
         }
         __syncthreads();
-        const unsigned units = 2 * p.head_units, total = count * units;
-        const size_t stride = (size_t)p.Hkv * p.head_units, base = (size_t)layer * p.num_slots * stride + (size_t)h * p.head_units;
-        constexpr int AHEAD = 4;
-        for (unsigned i0 = tid; i0 < total; i0 += EV_THREADS * AHEAD) {
-            U x[AHEAD];
-#pragma unroll
-            for (int e = 0; e < AHEAD; ++e) {
-                const unsigned i = i0 + e * EV_THREADS;
-                if (i >= total) continue;
-                const unsigned m = i / units, u = i - m * units;
-                const int src = (int)list_s[1][m];
-                const U* from_row = (const U*)(u < (unsigned)p.head_units ? p.k : p.v) + base + (u < (unsigned)p.head_units ? u : u - p.head_units);
-                if (src >= 0) x[e] = from_row[(size_t)src * stride];
-            }
-#pragma unroll
-            for (int e = 0; e < AHEAD; ++e) {
-                const unsigned i = i0 + e * EV_THREADS;
-                if (i >= total) continue;
-                const unsigned m = i / units, u = i - m * units;
-                const int src = (int)list_s[1][m], dst = (int)list_s[0][m];
-                U* to_row = (U*)(u < (unsigned)p.head_units ? p.k : p.v) + base + (u < (unsigned)p.head_units ? u : u - p.head_units);
-                if (src >= 0 && dst >= 0) to_row[(size_t)dst * stride] = x[e];
-            }
-        }
-        for (unsigned m = tid; m < count; m += EV_THREADS) {
-            const int src = (int)list_s[1][m], dst = (int)list_s[0][m];
-            if (src < 0 || dst < 0) continue;
-            p.mass_out[plane + dst] = p.mass[plane + src];
-            p.positions_out[plane + dst] = p.positions[plane + src];
-        }
+        move_rows<U>(p, plane, layer, h, list_s, count);
         __syncthreads();
     }
 }
@@ -391,13 +542,20 @@ template <typename U> int launch_commit(const CommitParams& p, cudaStream_t stre
 }
 template <typename U> int launch_evict(EvictParams p, int L, cudaStream_t stream) {
     const int places = p.max_pages * p.page_size, bit_words = (places + 31) / 32;
+    // 32 places a thread leave an SM one block, which pays while there are no more blocks than SMs (us, 16,000 places thinned to 1,024, heads
+    // of 128: 20 blocks 57, the general kernel 62; 560 blocks 341 and 220)
+    if (places <= 8 * EV_THREADS || (places <= 32 * EV_THREADS && (long long)p.S * p.Hkv * L <= llb_device_sms())) {
+        if (places <= 8 * EV_THREADS) llb_launch(cache_evict_kernel<U, 8>, dim3(p.S * p.Hkv, L), dim3(EV_THREADS), 0, stream, p);
+        else llb_launch(cache_evict_kernel<U, 32>, dim3(p.S * p.Hkv, L), dim3(EV_THREADS), 0, stream, p);
+        return llb_check_launch("cache_evict");
+    }
     // two blocks an SM have room for 20,000 worths each; places beyond that are read again in every pass
     p.cache_places = places < 20000 ? places : 20000;
     if (bit_words > 8192) p.cache_places = 8192;
     const size_t smem = sizeof(unsigned) * ((size_t)bit_words + p.cache_places);
-    cudaError_t e = cudaFuncSetAttribute(cache_evict_kernel<U>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(cache_evict_any_kernel<U>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return llb_fail("cache_evict: cannot opt in to %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
-    llb_launch(cache_evict_kernel<U>, dim3(p.S * p.Hkv, L), dim3(EV_THREADS), smem, stream, p);
+    llb_launch(cache_evict_any_kernel<U>, dim3(p.S * p.Hkv, L), dim3(EV_THREADS), smem, stream, p);
     return llb_check_launch("cache_evict");
 }
 

@@ -1344,16 +1344,30 @@ def paged_decode_mma(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
 
 # ---- a cache that is drafted into and thinned out (csrc/span_attention.cu, csrc/cache_rows.cu) ---------------------------
-def _check_here(what: str, *tensors) -> int:
-    """The current device, which the launch goes to: every tensor is there, and contiguous."""
-    device = tensors[0].get_device()
+# These calls come once a layer and step, and the host's part of one is longer than the small ones' kernels: the checks look at every
+# property of a tensor once and no more.
+_INT32, _INT64, _FLOAT32 = torch.int32, torch.int64, torch.float32
+
+
+def _elsewhere(what: str, device: int, *tensors) -> None:
+    """Raises for the tensor that is not contiguous or not on the current device, which the launch goes to."""
     for t in tensors:
-        if t is not None and (t.get_device() != device or device < 0 or not t.is_contiguous()):
+        if t is not None and (t.get_device() < 0 or t.get_device() != device or not t.is_contiguous()):
             raise KernelError(f"{what}: a tensor of shape {tuple(t.shape)} on {t.device} must be contiguous and on the device of "
                               "the others, a CUDA device; there is no CPU path")
-    if device != torch.cuda.current_device():
-        raise KernelError(f"{what}: the tensors are on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
-    return device
+    raise KernelError(f"{what}: the tensors are on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _check_here(what: str, *tensors) -> int:
+    """The current device: every tensor is there, and contiguous."""
+    device = tensors[0].get_device()
+    if device >= 0 and device == torch._C._cuda_getDevice():
+        for t in tensors:
+            if t is not None and (t.get_device() != device or not t.is_contiguous()):
+                break
+        else:
+            return device
+    return _elsewhere(what, device, *tensors)
 
 
 def _stream_on(device: int) -> int:
@@ -1361,32 +1375,35 @@ def _stream_on(device: int) -> int:
     return _scoped_stream if _scoped_stream is not None else torch._C._cuda_getCurrentRawStream(device)
 
 
-def _check_spans(what: str, span_row, span_len, span_pos, block_table, page_size: int):
-    """(requests, pages a request) of a call over whole requests: the index arrays are int32 of one length."""
-    S = span_len.shape[0]
-    for t, shape in ((span_row, (S,)), (span_len, (S,)), (span_pos, (S,))):
-        if t is not None and (t.dtype != torch.int32 or t.shape != shape):
-            raise KernelError(f"{what}: the index arrays are int32 [{S}], got {t.dtype} {tuple(t.shape)}")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != S:
-        raise KernelError(f"{what}: block_table must be int32 [{S}, pages], got {block_table.dtype} {tuple(block_table.shape)}")
+def _check_ints(what: str, shape, *arrays) -> None:
+    for t in arrays:
+        if t.dtype is not _INT32 or t.shape != shape:
+            raise KernelError(f"{what}: the index arrays are int32 {list(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _check_table(what: str, S: int, block_table, page_size: int) -> int:
+    """Pages a request."""
+    shape = block_table.shape
+    if block_table.dtype is not _INT32 or len(shape) != 2 or shape[0] != S:
+        raise KernelError(f"{what}: block_table must be int32 [{S}, pages], got {block_table.dtype} {tuple(shape)}")
     if page_size <= 0:
         raise KernelError(f"{what}: page size {page_size}")
-    return S, block_table.shape[1]
+    return shape[1]
 
 
-def _check_span_attention(what, q, k_cache, v_cache, out, num_heads, num_kv_heads, head_dim) -> int:
-    """The dtype code of an attention over whole requests, after the checks of its operands."""
-    T = q.shape[0]
+def _check_span_attention(what, q, k_cache, v_cache, out, num_heads, num_kv_heads, head_dim):
+    """(rows, slots) of an attention over whole requests, after the checks of its operands."""
     if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
         raise KernelError(f"{what}: {num_heads} query heads are not a multiple of {num_kv_heads} kv heads")
-    if q.numel() != T * num_heads * head_dim or out.shape != q.shape or out.dtype != q.dtype:
-        raise KernelError(f"{what}: q and out are [T, {num_heads * head_dim}] of one dtype, got {tuple(q.shape)} {q.dtype}, "
+    dtype, shape, cache = q.dtype, q.shape, k_cache.shape
+    if shape.numel() != shape[0] * num_heads * head_dim or out.shape != shape or out.dtype is not dtype:
+        raise KernelError(f"{what}: q and out are [T, {num_heads * head_dim}] of one dtype, got {tuple(shape)} {dtype}, "
                           f"{tuple(out.shape)} {out.dtype}")
-    shape = (k_cache.shape[0], num_kv_heads, head_dim)
-    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype or k_cache.shape != shape or v_cache.shape != shape:
-        raise KernelError(f"{what}: the caches are {q.dtype} [slots, {num_kv_heads}, {head_dim}], got {k_cache.dtype} "
-                          f"{tuple(k_cache.shape)}, {v_cache.dtype} {tuple(v_cache.shape)}")
-    return _dt(q)
+    if (k_cache.dtype is not dtype or v_cache.dtype is not dtype or v_cache.shape != cache or len(cache) != 3
+            or cache[1] != num_kv_heads or cache[2] != head_dim):
+        raise KernelError(f"{what}: the caches are {dtype} [slots, {num_kv_heads}, {head_dim}], got {k_cache.dtype} "
+                          f"{tuple(cache)}, {v_cache.dtype} {tuple(v_cache.shape)}")
+    return shape[0], cache[0]
 
 
 _span_scratch = {}
@@ -1433,17 +1450,20 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     q, out [T, heads * head_dim], caches [slots, kv heads, head_dim], all float32 or all bfloat16; mask int64 [T, words]; span arrays
     int32 [requests], block_table int32 [requests, pages].  Nothing is read on the host: a captured graph serves other trees,
     lengths and tables of the same sizes.  Rows of no request are left as they were."""
-    S, pages = _check_spans("tree_attention", span_row, span_len, span_pos, block_table, page_size)
-    dt = _check_span_attention("tree_attention", q, k_cache, v_cache, out, num_heads, num_kv_heads, head_dim)
-    T, slots = q.shape[0], k_cache.shape[0]
-    if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != T or mask.shape[1] == 0:
-        raise KernelError(f"tree_attention: mask must be int64 [{T}, words], got {mask.dtype} {tuple(mask.shape)}")
+    T, slots = _check_span_attention("tree_attention", q, k_cache, v_cache, out, num_heads, num_kv_heads, head_dim)
+    each, words = span_len.shape, mask.shape
+    S = each[0]
+    _check_ints("tree_attention", each, span_row, span_len, span_pos)
+    pages = _check_table("tree_attention", S, block_table, page_size)
+    if mask.dtype is not _INT64 or len(words) != 2 or words[0] != T or words[1] == 0:
+        raise KernelError(f"tree_attention: mask must be int64 [{T}, words], got {mask.dtype} {tuple(words)}")
+    dt = _dt(q)
     device = _check_here("tree_attention", q, k_cache, v_cache, out, mask, span_row, span_len, span_pos, block_table)
     stream = _stream_on(device)
     scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, slots, 0, device),
                           dtype=torch.float32, device=q.device)
     _check(lib().llb_tree_attention(
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), dt, mask.data_ptr(), mask.shape[1], span_row.data_ptr(),
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), dt, mask.data_ptr(), words[1], span_row.data_ptr(),
         span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, pages, page_size, slots, num_heads, num_kv_heads,
         head_dim, scale, scratch.data_ptr(), async_error_flag(q.device).data_ptr(), stream))
 
@@ -1462,11 +1482,14 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     from zero).  ``mass`` float32 [kv heads, slots].  ``max_len``: the most rows that a request brings (longer ones
     are cut to it); 1 takes the form for single tokens, which reads every key once.  The other arguments as
     :func:`tree_attention`.  Sums are made in one order: equal calls give equal bits."""
-    S, pages = _check_spans("paged_attention_mass", span_row, span_len, span_pos, block_table, page_size)
-    dt = _check_span_attention("paged_attention_mass", q, k_cache, v_cache, out, num_heads, num_kv_heads, head_dim)
-    T, slots = q.shape[0], k_cache.shape[0]
+    T, slots = _check_span_attention("paged_attention_mass", q, k_cache, v_cache, out, num_heads, num_kv_heads, head_dim)
+    each = span_len.shape
+    S = each[0]
+    _check_ints("paged_attention_mass", each, span_row, span_len, span_pos)
+    pages = _check_table("paged_attention_mass", S, block_table, page_size)
+    dt, plane = _dt(q), (num_kv_heads, slots)
     for t in (mass, mass_in):
-        if t is not None and (t.dtype != torch.float32 or t.shape != (num_kv_heads, slots)):
+        if t is not None and (t.dtype is not _FLOAT32 or t.shape != plane):
             raise KernelError(f"paged_attention_mass: weights are float32 [{num_kv_heads}, {slots}], got {t.dtype} {tuple(t.shape)}")
     if max_len <= 0:
         raise KernelError(f"paged_attention_mass: max_len is {max_len}")
@@ -1482,13 +1505,14 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
 
 def _check_planes(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor):
     """(layers, slots, kv heads, head size) of planes [slots, kv heads, head_dim] or [layers, slots, kv heads, head_dim]."""
-    if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype or k_cache.dim() not in (3, 4) or k_cache.numel() == 0:
+    shape = k_cache.shape
+    if v_cache.shape != shape or k_cache.dtype is not v_cache.dtype or len(shape) not in (3, 4) or shape.numel() == 0:
         raise KernelError(f"{what}: keys and values are [slots, kv heads, head_dim] or [layers, ...] of one shape and dtype, got "
                           f"{tuple(k_cache.shape)} {k_cache.dtype}, {tuple(v_cache.shape)} {v_cache.dtype}")
     _dt(k_cache)
     if k_cache.data_ptr() == v_cache.data_ptr():
         raise KernelError(f"{what}: keys and values must be planes of their own")
-    return (1, *k_cache.shape) if k_cache.dim() == 3 else tuple(k_cache.shape)
+    return (1, *shape) if len(shape) == 3 else shape
 
 
 def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, targets: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -1506,19 +1530,19 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, targets: torch.Tens
     ``span_pos[s] + path[s, d]`` to ``span_pos[s] + d`` in every layer: the request then holds ``span_pos[s] + count[s]`` keys, what lies
     behind them is left over.  tokens, parents, targets int32 [T]; caches [slots, kv heads, head_dim] or [layers, ...]; path int32
     [requests, width], width up to 1,024; count, next_token int32 [requests]."""
-    S, pages = _check_spans("tree_commit", span_row, span_len, span_pos, block_table, page_size)
     L, slots, heads, hd = _check_planes("tree_commit", k_cache, v_cache)
-    T = tokens.shape[0]
-    for t, shape in ((tokens, (T,)), (parents, (T,)), (targets, (T,)), (count, (S,)), (next_token, (S,))):
-        if t.dtype != torch.int32 or t.shape != shape:
-            raise KernelError(f"tree_commit: tokens, parents, targets are int32 [{T}], count and next_token int32 [{S}], got {t.dtype} {tuple(t.shape)}")
-    if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != S:
-        raise KernelError(f"tree_commit: path must be int32 [{S}, width], got {path.dtype} {tuple(path.shape)}")
+    each, rows, room = span_len.shape, tokens.shape, path.shape
+    S = each[0]
+    _check_ints("tree_commit (tokens, parents, targets)", rows, tokens, parents, targets)
+    _check_ints("tree_commit (spans, count, next_token)", each, span_row, span_len, span_pos, count, next_token)
+    pages = _check_table("tree_commit", S, block_table, page_size)
+    if path.dtype is not _INT32 or len(room) != 2 or room[0] != S:
+        raise KernelError(f"tree_commit: path must be int32 [{S}, width], got {path.dtype} {tuple(room)}")
     device = _check_here("tree_commit", tokens, parents, targets, k_cache, v_cache, span_row, span_len, span_pos, block_table, path, count, next_token)
     _check(lib().llb_tree_commit(
         tokens.data_ptr(), parents.data_ptr(), targets.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), span_row.data_ptr(),
-        span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, L, pages, page_size, slots,
-        heads * hd * k_cache.element_size(), path.data_ptr(), path.shape[1], count.data_ptr(), next_token.data_ptr(),
+        span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, rows[0], L, pages, page_size, slots,
+        heads * hd * k_cache.element_size(), path.data_ptr(), room[1], count.data_ptr(), next_token.data_ptr(),
         _stream_on(device)))
 
 
@@ -1538,8 +1562,11 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor
     Caches [slots, kv heads, head_dim] or [layers, ...]; mass float32 and positions int32 [kv heads, slots] or [layers, ...];
     lengths, ends int32 [requests].  ``mass_out`` and ``positions_out`` (both or neither): planes that receive the mass and position
     of every place that is held afterwards, in the place of the planes that are read; nothing else in them is written."""
-    S, pages = _check_spans("cache_evict", ends, lengths, None, block_table, page_size)
     L, slots, heads, hd = _check_planes("cache_evict", k_cache, v_cache)
+    each = lengths.shape
+    S = each[0]
+    _check_ints("cache_evict", each, lengths, ends)
+    pages = _check_table("cache_evict", S, block_table, page_size)
     shape = (heads, slots) if k_cache.dim() == 3 else (L, heads, slots)
     if (mass_out is None) != (positions_out is None):
         raise KernelError("cache_evict: mass_out and positions_out are given both or neither")
@@ -1547,8 +1574,8 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor
         mass_out, positions_out = mass, positions
     elif (mass_out.data_ptr() == mass.data_ptr()) != (positions_out.data_ptr() == positions.data_ptr()):
         raise KernelError("cache_evict: mass_out and positions_out are both the planes that are read, or neither is")
-    for t, dtype in ((mass, torch.float32), (mass_out, torch.float32), (positions, torch.int32), (positions_out, torch.int32)):
-        if t.dtype != dtype or t.shape != shape:
+    for t, dtype in ((mass, _FLOAT32), (mass_out, _FLOAT32), (positions, _INT32), (positions_out, _INT32)):
+        if t.dtype is not dtype or t.shape != shape:
             raise KernelError(f"cache_evict: mass is float32 and positions int32 {shape}, got {t.dtype} {tuple(t.shape)}")
     if budget <= 0 or first < 0 or latest < 0 or first + latest > budget:
         raise KernelError(f"cache_evict: a budget of {budget} places does not hold the first {first} and the latest {latest}")
