@@ -60,8 +60,16 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
 __device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
 }
-// D[128 x N] += A B with A in tensor memory (bf16, two to a column); the first product of a sum replaces D.
-__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t acc) {
+// One lane of the warp, chosen by the hardware's own election: the compiler then knows that a single lane runs what follows, and keeps
+// descriptors and addresses in the uniform registers that a product takes.  Under `lane == 0` it brings each of them there first, and
+// beside eight busy warps a 128 x 128 x 16 product costs the issuing one 83 to 350 cycles instead of 65 (64 is the tensor cores' own time).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
+}
+// D[128 x N] += A B with A in tensor memory (bf16, two to a column).
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t acc) {
     asm volatile(
         "{\n.reg .pred p;\n"
         "setp.ne.b32 p, %4, 0;\n"
@@ -69,23 +77,14 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, u
         ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ void umma_bf16_ts_acc(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc) {
-    asm volatile(
-        "{\n.reg .pred p;\n"
-        "setp.eq.u32 p, 0, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc)
-        : "memory");
-}
-// A 128 x 128 tile of scores, both operands K-major in shared memory.  What a product costs the issuing warp is its instructions, beside
-// eight busy ones: the descriptors are made once and counted up.
+// A 128 x 128 tile of scores, both operands K-major in shared memory.
 template <int KB> __device__ __forceinline__ void issue_scores(uint32_t tmem, uint32_t a_addr, uint32_t b_addr, uint32_t idesc) {
     const uint64_t da = desc_kmajor(a_addr), db = desc_kmajor(b_addr);
+    umma_bf16_first(tmem, da, db, idesc);
 #pragma unroll
-    for (int k = 0; k < 4 * KB; ++k) {
+    for (int k = 1; k < 4 * KB; ++k) {
         const uint64_t step = (k >> 2) * (TILE_BYTES >> 4) + (k & 3) * 2;
-        if (k == 0) umma_bf16_first(tmem, da, db, idesc);
-        else umma_bf16_acc(tmem, da + step, db + step, idesc);
+        umma_bf16_acc(tmem, da + step, db + step, idesc);
     }
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&u)[32]) {
@@ -287,7 +286,6 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     LlbJob job = pc.job;
     constexpr uint32_t IDESC_S = idesc_bf16(BQ, BK, 0), IDESC_PV = idesc_bf16(BQ, HD, 1);
     // Q buffers: jobs of two pair tiles take both, others one after the other
-    uint32_t q_uses[2] = {0, 0};
     int q_next = 0;
     uint32_t tiles_before = 0;                       // tiles of the block's jobs before this one
 
@@ -297,14 +295,18 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         bool ok = true;
         const uint32_t q_bytes = (uint32_t)p.pairs_nodes * a.group * 128 * KB;
         const int ppt = BK / a.page_size;
-        uint32_t loaded = 0;
+        uint32_t loaded = 0, q_phases = 0;           // of bar_q_free (bits 0, 1), and which buffers have been used (bits 2, 3)
 #pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const Segment g = segment_of(p, pc, job, t);
 #pragma unroll 1
             for (int x = 0; x < (g.two ? 2 : 1); ++x) {
                 const int b = g.two ? x : q_next;
-                if (q_uses[b] > 0) ok = mbar_wait(&bar_q_free[b], (q_uses[b] - 1) & 1, abort_flag) && ok;
+                if ((q_phases >> (2 + b)) & 1) {
+                    ok = mbar_wait(&bar_q_free[b], (q_phases >> b) & 1, abort_flag) && ok;
+                    q_phases ^= 1u << b;
+                }
+                q_phases |= 4u << b;
                 if (lane == 0 && ok) {
                     mbar_expect_tx(&bar_q_full[b], q_bytes);
 #pragma unroll
@@ -312,7 +314,6 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         tma_load_3d(q_s + b * HALF + kb * TILE_BYTES, &map_q, kb * 64, job.kvh * a.group,
                                     job.z.row + job.first + x * p.pairs_nodes, &bar_q_full[b]);
                 }
-                ++q_uses[b];
             }
             if (!g.two) q_next ^= 1;
 #pragma unroll 1
@@ -347,34 +348,33 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
             }
         }
-    } else if (warp == MMA_WARP) {
+    } else if (warp == MMA_WARP && elect_one()) {
         bool ok = true;
-        uint32_t n_p[2] = {0, 0};
+        uint32_t phases = 0;                         // the next phase of bar_p (bits 0, 1) and bar_q_full (bits 2, 3)
         auto full = [&](uint32_t half) {             // half tile number `half` of the block has arrived
             ok = mbar_wait(&bar_kv_full[half % RING], (half / RING) & 1, abort_flag) && ok;
             tc_fence_after();
         };
         auto issue_s = [&](int x, int b, uint32_t half) {
-            if (lane == 0 && ok)
-                issue_scores<KB>(tmem_base + x * 128, smem_u32(q_s + b * HALF), smem_u32(ring + half % RING * HALF), IDESC_S);
-            __syncwarp();
+            if (ok) issue_scores<KB>(tmem_base + x * 128, smem_u32(q_s + b * HALF), smem_u32(ring + half % RING * HALF), IDESC_S);
         };
 #pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const Segment g = segment_of(p, pc, job, t);
             const int n = g.k1 - g.k0, step = g.two ? 1 : 2;
-            int buf[2];
+            const int buf0 = g.two ? 0 : q_next, buf1 = g.two ? 1 : q_next;
 #pragma unroll 1
             for (int x = 0; x < 2; ++x) {
-                const int b = g.two ? x : q_next;
-                buf[x] = b;
-                if (g.two || x == 0) ok = mbar_wait(&bar_q_full[b], q_uses[b]++ & 1, abort_flag) && ok;
+                const int b = x == 0 ? buf0 : buf1;
+                if (g.two || x == 0) {
+                    ok = mbar_wait(&bar_q_full[b], (phases >> (2 + b)) & 1, abort_flag) && ok;
+                    phases ^= 4u << b;
+                }
                 const int first = g.two ? 0 : x;
                 if (first >= n) continue;
                 full(2 * (tiles_before + first));
                 issue_s(x, b, 2 * (tiles_before + first));
-                if (lane == 0 && ok) umma_commit(&bar_s[x]);
-                __syncwarp();
+                if (ok) umma_commit(&bar_s[x]);
             }
             if (!g.two) q_next ^= 1;
 #pragma unroll 1
@@ -384,25 +384,23 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     const int j = g.two ? j0 : j0 + x;
                     if (j >= n) continue;
                     full(2 * (tiles_before + j) + 1);
-                    ok = mbar_wait(&bar_p[x], n_p[x]++ & 1, abort_flag) && ok;
+                    ok = mbar_wait(&bar_p[x], (phases >> x) & 1, abort_flag) && ok;
+                    phases ^= 1u << x;
                     tc_fence_after();
-                    if (lane == 0 && ok) {
-                        const uint32_t va = smem_u32(ring + (2 * (tiles_before + j) + 1) % RING * HALF);
-                        const uint64_t dv = desc_mnmajor(va, TILE_BYTES);
-                        const uint32_t to = tmem_base + 256 + x * 128, from = tmem_base + x * 128;
-                        umma_bf16_ts(to, from, dv, IDESC_PV, j0 > 0 ? 1u : 0u);
+                    const uint64_t dv = desc_mnmajor(smem_u32(ring + (2 * (tiles_before + j) + 1) % RING * HALF), TILE_BYTES);
+                    const uint32_t to = tmem_base + 256 + x * 128, from = tmem_base + x * 128;
+                    if (ok) {
 #pragma unroll
-                        for (int k = 1; k < BK / 16; ++k) umma_bf16_ts_acc(to, from + k * 8, dv + k * (16 * 128 >> 4), IDESC_PV);
+                        for (int k = 0; k < BK / 16; ++k)
+                            umma_ts(to, from + k * 8, dv + k * (16 * 128 >> 4), IDESC_PV, (j0 > 0 || k > 0) ? 1u : 0u);
                     }
-                    __syncwarp();
                     if (j + step < n) {
                         full(2 * (tiles_before + j + step));
-                        issue_s(x, buf[x], 2 * (tiles_before + j + step));
-                        if (lane == 0 && ok) umma_commit(&bar_s[x]);       // this P V and the next S
-                    } else if (lane == 0 && ok) {
-                        umma_commit(&bar_o[x]);
+                        issue_s(x, x == 0 ? buf0 : buf1, 2 * (tiles_before + j + step));
+                        if (ok) umma_commit(&bar_s[x]);       // this P V and the next S
+                    } else {
+                        if (ok) umma_commit(&bar_o[x]);
                     }
-                    __syncwarp();
                 }
             }
             tiles_before += n;
@@ -644,6 +642,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (t < pc.t1) job.next(a, BK);
         }
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (*abort_flag && threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 4);
@@ -779,7 +778,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 }
             }
         }
-    } else if (warp == MMA_WARP) {
+    } else if (warp == MMA_WARP && elect_one()) {
         bool ok = true;
 #pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
@@ -792,11 +791,10 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 ok = mbar_wait(&bar_q_full[slot], (at / RING) & 1, abort_flag) && ok;
                 if (at >= 4) ok = mbar_wait(&bar_free[place], ((at >> 2) - 1) & 1, abort_flag) && ok;
                 tc_fence_after();
-                if (lane == 0 && ok) {
+                if (ok) {
                     issue_scores<KB>(tmem_base + place * 128, smem_u32(k_s + b * HALF), smem_u32(ring + slot * HALF), IDESC);
                     umma_commit(&bar_s[place]);
                 }
-                __syncwarp();
             }
             units_before += u1 - u0;
             ++jobs;
@@ -880,6 +878,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             if (t < pc.t1) job.next(a, BK, pairs_nodes);
         }
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (*abort_flag && threadIdx.x == 0 && m.p.error_flag) atomicExch(m.p.error_flag, 5);
