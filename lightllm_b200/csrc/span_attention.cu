@@ -81,6 +81,11 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
     for (int t = pc.t0; t < pc.t1;) {
         const int rows = job.count(a) * a.group;
         const int k0 = t - job.begin, k1 = min(job.tiles, pc.t1 - job.begin);
+        if (k0 >= job.tiles) {
+            t = job.begin + job.tiles + a.extra;
+            if (t < pc.t1) job.next(a, KT);
+            continue;
+        }
         const T* qb = (const T*)p.q + ((size_t)(job.z.row + job.first) * a.Hq + job.kvh * a.group) * hd;
         for (int i = tid; i < RB * (hd4 / 4); i += THREADS) {
             const int r = i / (hd4 / 4), d = (i - r * (hd4 / 4)) * 4;
@@ -243,7 +248,7 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
         }
         if (tid == 0 && part == 1) llb_leave_open(a, pc, job, true);
         __syncthreads();                               // the next job's Q, maxima and sums take the places of this one's
-        t = job.begin + k1;
+        t = job.begin + job.tiles + a.extra;
         if (t < pc.t1) job.next(a, KT);
     }
 }
@@ -348,7 +353,7 @@ template <int TILE> __device__ __forceinline__ void mass_of_scores(const LlbSpan
         }
     }
     __syncthreads();
-    const int tiles = (z.pos + TILE) / TILE, begin = before_s + kvh * tiles;
+    const int tiles = (z.pos + TILE) / TILE, begin = before_s + kvh * (tiles + a.extra);
     LlbPiece pc;
     pc.total = total_s;
     pc.blocks = min(grid, (pc.total + least - 1) / least);
@@ -571,7 +576,7 @@ int check(const LlbSpanArgs& a, int dtype) {
     LLB_REQUIRE(a.hd > 0 && a.hd <= 256, "span_attention: head size %d, up to 256 are supported", a.hd);
     LLB_REQUIRE(a.S >= 0 && a.T >= 0 && a.page_size > 0 && a.max_pages >= 0 && a.num_slots > 0 && (long long)a.max_pages * a.page_size <= (1 << 30),
                 "span_attention: bad sizes");
-    LLB_REQUIRE(((long long)a.T / max(1, 64 / a.group) + a.S) * a.Hkv * (((long long)a.max_pages * a.page_size + KT - 1) / KT) < (1ll << 31),
+    LLB_REQUIRE(((long long)a.T / max(1, 64 / a.group) + a.S) * a.Hkv * (((long long)a.max_pages * a.page_size + KT - 1) / KT + 3) < (1ll << 31),
                 "span_attention: %d rows over up to %d keys a request are more tiles than one call takes", a.T, a.max_pages * a.page_size);
     return 0;
 }
@@ -585,7 +590,7 @@ bool tc_sizes(int dtype, int hd, int page_size) {
 struct Layout {
     long long part_o, part_ml, open, part_mass, lse, scores, score_tiles, floats;
 };
-Layout layout(int T, int S, int Hq, int group, int hd, int num_slots, int rows, int blocks, int tile, int mass) {
+Layout layout(int T, int S, int Hq, int group, int hd, int num_slots, int rows, int blocks, int tile, int extra, int mass) {
     Layout l;
     l.part_o = 0;
     l.part_ml = l.part_o + 2ll * blocks * rows * ((hd + 3) & ~3);
@@ -593,7 +598,7 @@ Layout layout(int T, int S, int Hq, int group, int hd, int num_slots, int rows, 
     l.part_mass = l.open + 8ll * blocks;
     l.lse = l.part_mass + (mass == 1 ? 2ll * blocks * 128 : 0);
     l.scores = (l.lse + (mass > 0 ? (long long)T * Hq : 0) + 3) & ~3ll;
-    l.score_tiles = mass == 2 ? ((long long)num_slots / tile + S) * (Hq / group) : 0;
+    l.score_tiles = mass == 2 ? ((long long)num_slots / tile + (long long)S * (1 + extra)) * (Hq / group) : 0;
     l.floats = l.scores + l.score_tiles * group * tile;
     return l;
 }
@@ -603,7 +608,8 @@ int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtyp
            float** part_mass, int* error_flag, cudaStream_t stream) {
     const int rows = tc ? 2 * llb_span_tc_pairs(a.group) * a.group : simt_rows(a.T, a.S, a.group);
     const int blocks = tc ? tc_blocks() : simt_blocks();
-    const Layout l = layout(a.T, a.S, a.Hq, a.group, a.hd, a.num_slots, rows, blocks, tc ? 128 : KT, mass);
+    a.extra = tc ? LLB_SPAN_TC_EXTRA : LLB_SPAN_EXTRA;
+    const Layout l = layout(a.T, a.S, a.Hq, a.group, a.hd, a.num_slots, rows, blocks, tc ? 128 : KT, a.extra, mass);
     a.rows = rows;
     a.nodes = rows / a.group;
     a.part_o = scratch + l.part_o;
@@ -640,9 +646,9 @@ LlbSpanArgs span_args(const void* out, const int* span_row, const int* span_len,
 LLB_EXPORT long long llb_span_scratch_floats(int dtype, int T, int S, int Hq, int Hkv, int hd, int page_size, int num_slots, int mass) {
     if (Hkv <= 0 || Hq < Hkv || S <= 0) return 1;
     const int group = Hq / Hkv;
-    long long n = layout(T, S, Hq, group, hd, num_slots, simt_rows(T, S, group), simt_blocks(), KT, mass).floats;
+    long long n = layout(T, S, Hq, group, hd, num_slots, simt_rows(T, S, group), simt_blocks(), KT, LLB_SPAN_EXTRA, mass).floats;
     if (tc_sizes(dtype, hd, page_size) && group <= 128) {
-        const long long tc = layout(T, S, Hq, group, hd, num_slots, 2 * llb_span_tc_pairs(group) * group, tc_blocks(), 128, mass).floats;
+        const long long tc = layout(T, S, Hq, group, hd, num_slots, 2 * llb_span_tc_pairs(group) * group, tc_blocks(), 128, LLB_SPAN_TC_EXTRA, mass).floats;
         n = tc > n ? tc : n;
     }
     return n;

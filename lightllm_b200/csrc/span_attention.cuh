@@ -17,6 +17,9 @@
 
 constexpr int LLB_SPAN_BLOCKS = 512;          // blocks of a kernel at most
 constexpr int LLB_SPAN_TC_LEAST = 2;          // tiles a block of the tensor-core kernel has at least: one for each of its groups
+// What beginning and ending a job costs a block, in tiles: every job is so much longer in the line, or blocks with several short jobs would be the
+// last ones (27 trees of 65 to 4,001 keys: 39 -> 33 us).
+constexpr int LLB_SPAN_TC_EXTRA = 3, LLB_SPAN_EXTRA = 1;
 
 struct LlbSpanArgs {
     const int* span_row;             // [S]
@@ -38,6 +41,7 @@ struct LlbSpanArgs {
                                      // it (1); four dimensions of neighbouring rows side by side, as the threads that write and join them have them
     float* part_ml;                  // [2 * blocks, rows, 2]
     int* open;                       // [blocks, 8]: the job that begins in a block and goes on after it, see LlbOpen
+    int extra;                       // what a job takes of the line besides its tiles
     int nodes;                       // rows of a request that a job holds at most
     int rows;                        // nodes * group, rounded up: (row, head) pairs of a job in the partial results
 };
@@ -65,7 +69,8 @@ __device__ __forceinline__ int llb_span_slot(const LlbSpanArgs& a, int s, int ke
     return page >= 0 && slot < a.num_slots ? (int)slot : -1;
 }
 
-// A job and its tiles' place in the line of all tiles.
+// A job and its tiles' place in the line of all tiles: begin .. begin + tiles - 1, then what it costs besides (no tile, and nothing to do for
+// a block whose piece begins there).
 struct LlbJob {
     LlbSpan z;
     int s, first, kvh;       // first: its first row in its request
@@ -77,7 +82,7 @@ struct LlbJob {
     __device__ __forceinline__ int count(const LlbSpanArgs& a) const { return min(a.nodes, z.len - first); }
     // the next job of the line (there is one)
     __device__ __forceinline__ void next(const LlbSpanArgs& a, int tile) {
-        begin += tiles;
+        begin += tiles + a.extra;
         if (++kvh < a.Hkv) return;
         kvh = 0;
         first += a.nodes;
@@ -104,10 +109,10 @@ struct LlbPiece {
 };
 __device__ __forceinline__ int llb_span_tiles(const LlbSpanArgs& a, const LlbSpan& z, int tile) {
     int n = 0;
-    if (z.len > 0 && a.mask) n = (z.len + a.nodes - 1) / a.nodes * ((z.pos + z.len + tile - 1) / tile);
+    if (z.len > 0 && a.mask) n = (z.len + a.nodes - 1) / a.nodes * ((z.pos + z.len + tile - 1) / tile + a.extra);
     else
 #pragma unroll 1
-        for (int c = 0; c < z.len; c += a.nodes) n += (llb_span_keys(a, z, c + a.nodes) + tile - 1) / tile;
+        for (int c = 0; c < z.len; c += a.nodes) n += (llb_span_keys(a, z, c + a.nodes) + tile - 1) / tile + a.extra;
     return n * a.Hkv;
 }
 // By one whole warp; every lane gets the answer.  A block has `least` tiles or more where there are enough.
@@ -156,12 +161,12 @@ __device__ __forceinline__ LlbPiece llb_piece(const LlbSpanArgs& a, int tile, in
 #pragma unroll 1
     for (;;) {
         p.job.measure(a, tile);
-        if (p.t0 < p.job.begin + p.job.tiles * a.Hkv) break;
-        p.job.begin += p.job.tiles * a.Hkv;
+        if (p.t0 < p.job.begin + (p.job.tiles + a.extra) * a.Hkv) break;
+        p.job.begin += (p.job.tiles + a.extra) * a.Hkv;
         p.job.first += a.nodes;
     }
-    p.job.kvh = (p.t0 - p.job.begin) / p.job.tiles;
-    p.job.begin += p.job.kvh * p.job.tiles;
+    p.job.kvh = (p.t0 - p.job.begin) / (p.job.tiles + a.extra);
+    p.job.begin += p.job.kvh * (p.job.tiles + a.extra);
     return p;
 }
 // Where a job's partial result goes when the block [t0, t1) has not all of it: 0 or 1, or -1 when it has.

@@ -8,9 +8,9 @@
 //     up to 128 pairs         both have the same pairs, the first sees the even tiles and the second the odd ones; they are joined at
 //                             the end through tensor memory (the same pair has the same lane in both)
 // While one group works on its scores the tensor cores work for the other.  For every tile of 128 keys of a group:
-//     S = Q K^T               tcgen05.mma, 128 columns of tensor memory
-//     m, p = 2^(S - m), l     a thread reads its lane's 128 scores once, keeps them in registers; p goes back to tensor memory as bf16
-//                             (over S) and is the A operand of the next product without a way through shared memory
+//     S = Q K^T               tcgen05.mma, 128 columns of tensor memory, in two halves of 64 keys
+//     m, p = 2^(S - m), l     a thread reads its lane's 128 scores once; p goes back to tensor memory as bf16 (over the second half of S)
+//                             and is the A operand of the next product without a way through shared memory
 //     O += P V                in tensor memory; it is scaled only when a lane's maximum has grown by more than 2^8 since its last
 //                             scaling (any reference works for a softmax, and 2^8 leaves floats and bf16 their accuracy)
 // K and V tiles go through a ring of half tiles (128 keys of K, or of V) that TMA fills page by page, several ahead, across jobs.
@@ -77,7 +77,7 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64
         ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(acc)
         : "memory");
 }
-// A 128 x 128 tile of scores, both operands K-major in shared memory.
+// A 128 x N tile of scores, both operands K-major in shared memory.
 template <int KB> __device__ __forceinline__ void issue_scores(uint32_t tmem, uint32_t a_addr, uint32_t b_addr, uint32_t idesc) {
     const uint64_t da = desc_kmajor(a_addr), db = desc_kmajor(b_addr);
     umma_bf16_first(tmem, da, db, idesc);
@@ -175,8 +175,10 @@ __device__ __forceinline__ float tile_max(uint32_t tmem) {
 }
 // 2^(score * scale + shift) of a lane's 128 scores as bf16 pairs, their sum (before the rounding) and the largest score, which tells
 // whether the shift was near enough: after the first tile it nearly always is, so that no pass for the maximum comes before this one.  The scores
-// stay where they are.
-__device__ __forceinline__ void tile_probs(uint32_t tmem, float scale, float shift, uint32_t (&probs)[64], float& sum, float& top) {
+// stay where they are.  second_half() is called when the second 64 of them are wanted.
+template <typename SecondHalf>
+__device__ __forceinline__ void tile_probs(uint32_t tmem, float scale, float shift, uint32_t (&probs)[64], float& sum, float& top,
+                                           const SecondHalf& second_half) {
     float t0 = -INFINITY, t1 = -INFINITY;
     uint64_t l0 = 0, l1 = 0;
     const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
@@ -185,6 +187,10 @@ __device__ __forceinline__ void tile_probs(uint32_t tmem, float scale, float shi
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         tmem_wait_ld32(s[c & 1]);
+        if (c == 1) {
+            second_half();
+            __syncwarp();
+        }
         if (c < 3) tmem_ld32_nowait(tmem + 32 * (c + 1), *reinterpret_cast<uint32_t(*)[32]>(&s[(c + 1) & 1][0]));
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
@@ -233,6 +239,14 @@ __device__ __forceinline__ Segment segment_of(const TcParams& p, const LlbPiece&
     return g;
 }
 
+// On to the next job, if the piece goes on.
+__device__ __forceinline__ bool next_job(const LlbSpanArgs& a, const LlbPiece& pc, LlbJob& job, int& t) {
+    t = job.begin + job.tiles + a.extra;
+    if (t >= pc.t1) return false;
+    job.next(a, BK);
+    return true;
+}
+
 template <int HD>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -240,7 +254,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     constexpr int KB = Shape<HD>::KB, RING = Shape<HD>::RING;
     constexpr uint32_t HALF = Shape<HD>::HALF;
     constexpr uint32_t TMEM_COLS = 512;              // S (and P) of the groups: 0.., 128..; O: 256.., 384..
-    __shared__ __align__(8) uint64_t bar_q_full[2], bar_q_free[2], bar_kv_full[RING], bar_kv_free[RING], bar_s[2], bar_p[2], bar_o[2];
+    __shared__ __align__(8) uint64_t bar_q_full[2], bar_q_free[2], bar_kv_full[RING], bar_kv_free[RING], bar_s[4], bar_p[2], bar_o[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_s, odd_s;
     __shared__ LlbPiece piece_s;
@@ -257,6 +271,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             mbar_init(&bar_q_full[i], 1);
             mbar_init(&bar_q_free[i], 1);
             mbar_init(&bar_s[i], 1);
+            mbar_init(&bar_s[2 + i], 1);
             mbar_init(&bar_p[i], 4);
             mbar_init(&bar_o[i], 1);
         }
@@ -284,7 +299,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const uint32_t tmem_base = tmem_slot;
     const LlbPiece pc = piece_s;
     LlbJob job = pc.job;
-    constexpr uint32_t IDESC_S = idesc_bf16(BQ, BK, 0), IDESC_PV = idesc_bf16(BQ, HD, 1);
+    constexpr uint32_t IDESC_S = idesc_bf16(BQ, BK / 2, 0), IDESC_PV = idesc_bf16(BQ, HD, 1);
     // Q buffers: jobs of two pair tiles take both, others one after the other
     int q_next = 0;
     uint32_t tiles_before = 0;                       // tiles of the block's jobs before this one
@@ -299,6 +314,10 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const Segment g = segment_of(p, pc, job, t);
+            if (g.k0 >= job.tiles) {
+                if (!next_job(a, pc, job, t)) break;
+                continue;
+            }
 #pragma unroll 1
             for (int x = 0; x < (g.two ? 2 : 1); ++x) {
                 const int b = g.two ? x : q_next;
@@ -337,8 +356,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     __syncwarp();
                 }
             }
-            t = job.begin + g.k1;
-            if (t < pc.t1) job.next(a, BK);
+            if (!next_job(a, pc, job, t)) break;
         }
         // after a wait has run out: what was asked for arrives before the block ends
         if (!ok) {
@@ -355,12 +373,20 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             ok = mbar_wait(&bar_kv_full[half % RING], (half / RING) & 1, abort_flag) && ok;
             tc_fence_after();
         };
-        auto issue_s = [&](int x, int b, uint32_t half) {
-            if (ok) issue_scores<KB>(tmem_base + x * 128, smem_u32(q_s + b * HALF), smem_u32(ring + half % RING * HALF), IDESC_S);
+        // The scores come in two halves: the first one of the next tile goes ahead of this tile's P V, so that the softmax goes on with it
+        // meanwhile; the second one, which takes the place of P, follows it.
+        auto issue_s = [&](int x, int b, uint32_t half, int which) {
+            if (!ok) return;
+            issue_scores<KB>(tmem_base + x * 128 + which * 64, smem_u32(q_s + b * HALF), smem_u32(ring + half % RING * HALF) + which * 64 * 128, IDESC_S);
+            umma_commit(&bar_s[2 * which + x]);
         };
 #pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const Segment g = segment_of(p, pc, job, t);
+            if (g.k0 >= job.tiles) {
+                if (!next_job(a, pc, job, t)) break;
+                continue;
+            }
             const int n = g.k1 - g.k0, step = g.two ? 1 : 2;
             const int buf0 = g.two ? 0 : q_next, buf1 = g.two ? 1 : q_next;
 #pragma unroll 1
@@ -373,8 +399,8 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const int first = g.two ? 0 : x;
                 if (first >= n) continue;
                 full(2 * (tiles_before + first));
-                issue_s(x, b, 2 * (tiles_before + first));
-                if (ok) umma_commit(&bar_s[x]);
+                issue_s(x, b, 2 * (tiles_before + first), 0);
+                issue_s(x, b, 2 * (tiles_before + first), 1);
             }
             if (!g.two) q_next ^= 1;
 #pragma unroll 1
@@ -383,29 +409,27 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 for (int x = 0; x < 2; ++x) {
                     const int j = g.two ? j0 : j0 + x;
                     if (j >= n) continue;
-                    full(2 * (tiles_before + j) + 1);
+                    const uint32_t half = 2 * (tiles_before + j);
+                    const bool more = j + step < n;
+                    if (more) full(half + 2 * step);
                     ok = mbar_wait(&bar_p[x], (phases >> x) & 1, abort_flag) && ok;
                     phases ^= 1u << x;
                     tc_fence_after();
-                    const uint64_t dv = desc_mnmajor(smem_u32(ring + (2 * (tiles_before + j) + 1) % RING * HALF), TILE_BYTES);
-                    const uint32_t to = tmem_base + 256 + x * 128, from = tmem_base + x * 128;
+                    if (more) issue_s(x, x == 0 ? buf0 : buf1, half + 2 * step, 0);
+                    full(half + 1);
                     if (ok) {
+                        const uint64_t dv = desc_mnmajor(smem_u32(ring + (half + 1) % RING * HALF), TILE_BYTES);
+                        const uint32_t to = tmem_base + 256 + x * 128, from = tmem_base + x * 128 + 64;
 #pragma unroll
                         for (int k = 0; k < BK / 16; ++k)
                             umma_ts(to, from + k * 8, dv + k * (16 * 128 >> 4), IDESC_PV, (j0 > 0 || k > 0) ? 1u : 0u);
                     }
-                    if (j + step < n) {
-                        full(2 * (tiles_before + j + step));
-                        issue_s(x, x == 0 ? buf0 : buf1, 2 * (tiles_before + j + step));
-                        if (ok) umma_commit(&bar_s[x]);       // this P V and the next S
-                    } else {
-                        if (ok) umma_commit(&bar_o[x]);
-                    }
+                    if (more) issue_s(x, x == 0 ? buf0 : buf1, half + 2 * step, 1);          // (its commit is behind P V, too)
+                    else if (ok) umma_commit(&bar_o[x]);
                 }
             }
             tiles_before += n;
-            t = job.begin + g.k1;
-            if (t < pc.t1) job.next(a, BK);
+            if (!next_job(a, pc, job, t)) break;
         }
     }
     } else {
@@ -418,6 +442,10 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const Segment g = segment_of(p, pc, job, t);
+            if (g.k0 >= job.tiles) {
+                if (!next_job(a, pc, job, t)) break;
+                continue;
+            }
             const int n = g.k1 - g.k0, step = g.two ? 1 : 2;
             const int node0 = g.two ? x * p.pairs_nodes : 0;
             const int pairs = min(p.pairs_nodes, job.count(a) - node0) * a.group;
@@ -434,14 +462,23 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             for (int j = g.two ? 0 : x; j < n; j += step) {
                 const int key0 = (g.k0 + j) * BK;
                 const uint32_t half = 2 * (tiles_before + j);
-                ok = mbar_wait(&bar_s[x], n_s++ & 1, abort_flag) && ok;
+                ok = mbar_wait(&bar_s[x], n_s & 1, abort_flag) && ok;
                 tc_fence_after();
-                if (r == 0) {
-                    // S has read K, and the product before it V
-                    mbar_arrive_n(&bar_kv_free[half % RING], g.two ? 1 : 2);
-                    if (j >= step) mbar_arrive_n(&bar_kv_free[(half + 1 - 2 * step) % RING], g.two ? 1 : 2);
-                }
+                // The second half of S: it has read K, and the product before it V; Q, if this is the job's last tile.
+                bool whole = false;
+                auto second_half = [&]() {
+                    if (whole) return;
+                    whole = true;
+                    ok = mbar_wait(&bar_s[2 + x], n_s & 1, abort_flag) && ok;
+                    tc_fence_after();
+                    if (r == 0) {
+                        mbar_arrive_n(&bar_kv_free[half % RING], g.two ? 1 : 2);
+                        if (j >= step) mbar_arrive_n(&bar_kv_free[(half + 1 - 2 * step) % RING], g.two ? 1 : 2);
+                        if (g.two && j + 1 == n) mbar_arrive(&bar_q_free[x]);
+                    }
+                };
                 const bool interior = key0 + BK <= all;
+                if (!interior || j < step || a.scores || !busy) second_half();
                 if (!interior) {
                     // Values that no row or not every row sees: what earlier owners left behind the last key, and numbers that are
                     // none in rows that see them, would reach the other rows as 0 * inf.  They become zeros here; rows that see the
@@ -511,7 +548,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     if (j < step) m_ref = tile_max(tmem_s) * a.scale_log2e;              // (no O yet)
                     uint32_t probs[64];
                     float sum, top;
-                    tile_probs(tmem_s, a.scale_log2e, m_ref == -INFINITY ? 0.0f : -m_ref, probs, sum, top);
+                    tile_probs(tmem_s, a.scale_log2e, m_ref == -INFINITY ? 0.0f : -m_ref, probs, sum, top, second_half);
                     top *= a.scale_log2e;
                     if (__any_sync(0xffffffffu, top > m_ref + RESCALE)) {
                         float corr = 1.0f;
@@ -529,13 +566,14 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             for (int i = 0; i < 32; ++i) o[i] *= corr;
                             tmem_st32(tmem_o + x * 128 + c, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
                         }
-                        tile_probs(tmem_s, a.scale_log2e, m_ref == -INFINITY ? 0.0f : -m_ref, probs, sum, top);
+                        tile_probs(tmem_s, a.scale_log2e, m_ref == -INFINITY ? 0.0f : -m_ref, probs, sum, top, second_half);
                     }
                     l_run += sum;
-                    tmem_st32(tmem_s, *reinterpret_cast<const uint32_t(*)[32]>(&probs[0]));
-                    tmem_st32(tmem_s + 32, *reinterpret_cast<const uint32_t(*)[32]>(&probs[32]));
+                    tmem_st32(tmem_s + 64, *reinterpret_cast<const uint32_t(*)[32]>(&probs[0]));
+                    tmem_st32(tmem_s + 96, *reinterpret_cast<const uint32_t(*)[32]>(&probs[32]));
                     tmem_wait_st();
                 }
+                ++n_s;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_p[x]);
@@ -631,15 +669,14 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
             }
             if (g.part == 1 && threadIdx.x == 0) llb_leave_open(a, pc, job, true);
-            // O and Q are free for the next job (the groups have read each other's O)
+            // O is free for the next job, and Q where the groups met in it (they have read each other's O)
             tc_fence_before();
             fence_async_smem();
             if (!g.two) named_barrier(BAR_PAIR, 256);
             else named_barrier(BAR_PAIR + 1 + x, 128);
-            if (r == 0 && (g.two || x == 0)) mbar_arrive(&bar_q_free[buf]);
+            if (!g.two && r == 0 && x == 0) mbar_arrive(&bar_q_free[buf]);
             tiles_before += n;
-            t = job.begin + g.k1;
-            if (t < pc.t1) job.next(a, BK);
+            if (!next_job(a, pc, job, t)) break;
         }
     }
     __syncwarp();
@@ -680,7 +717,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_s;
     __shared__ LlbMassPiece piece_s;
-    __shared__ __align__(16) float lse_s[2][2][128];
+    __shared__ __align__(16) float lse_s[8][2][128];          // a warp's own, so that no group has to meet
     __shared__ float sum_s[128];
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -810,21 +847,27 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const int u0 = t - job.begin, u1 = min(job.units, pc.t1 - job.begin), n = u1 - u0;
             const LlbSpan z = job.z;
             const int key = job.tile * BK + r;
-            float sum0 = 0.0f, sum1 = 0.0f, sum2 = 0.0f, sum3 = 0.0f;
-            // the lse of a tile's pair r, +infinity where there is none
-            auto lse_of = [&](int j) -> float {
-                const int node = (job.from + u0 + j) * pairs_nodes + r / a.group;
-                return j < n && r < pairs_tile && node < z.len ? a.lse[(size_t)(z.row + node) * a.Hq + job.kvh * a.group + r % a.group] : INFINITY;
+            uint64_t sum0 = 0, sum1 = 0;
+            // minus the lse of four pairs of a tile, minus infinity where there is none
+            auto lse_of = [&](int j) -> float4 {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int pair = lane * 4 + e, node = (job.from + u0 + j) * pairs_nodes + pair / a.group;
+                    v[e] = j < n && pair < pairs_tile && node < z.len ? -a.lse[(size_t)(z.row + node) * a.Hq + job.kvh * a.group + pair % a.group] : -INFINITY;
+                }
+                return make_float4(v[0], v[1], v[2], v[3]);
             };
+            const uint64_t scale2 = pack2(a.scale_log2e, a.scale_log2e);
             const int first = (int)((x - units_before) & 1);          // the group's first tile of the job
-            float lse = lse_of(first);
+            float4 lse = lse_of(first);
 #pragma unroll 1
             for (int j = first; j < n; j += 2) {
                 const uint32_t at = units_before + j, place = at & 3;
-                float* lse_t = lse_s[x][place >> 1];
-                lse_t[r] = lse;
+                float* lse_t = lse_s[warp][place >> 1];
+                *reinterpret_cast<float4*>(lse_t + lane * 4) = lse;
+                __syncwarp();
                 lse = lse_of(j + 2);
-                named_barrier(BAR_PAIR + 1 + x, 128);
                 ok = mbar_wait(&bar_s[place], (at >> 2) & 1, abort_flag) && ok;
                 tc_fence_after();
                 if (r == 0) mbar_arrive(&bar_q_free[at % RING]);
@@ -847,17 +890,21 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         const float4 e = *reinterpret_cast<const float4*>(lse_t + 32 * c + i);
-                        sum0 += fast_exp2(fmaf(s[c & 1][i], a.scale_log2e, -e.x));
-                        sum1 += fast_exp2(fmaf(s[c & 1][i + 1], a.scale_log2e, -e.y));
-                        sum2 += fast_exp2(fmaf(s[c & 1][i + 2], a.scale_log2e, -e.z));
-                        sum3 += fast_exp2(fmaf(s[c & 1][i + 3], a.scale_log2e, -e.w));
+                        const float* v = &s[c & 1][i];
+                        float p0, p1, p2, p3;
+                        unpack2(fma2(pack2(v[0], v[1]), scale2, pack2(e.x, e.y)), p0, p1);
+                        unpack2(fma2(pack2(v[2], v[3]), scale2, pack2(e.z, e.w)), p2, p3);
+                        sum0 = add2(sum0, pack2(fast_exp2(p0), fast_exp2(p1)));
+                        sum1 = add2(sum1, pack2(fast_exp2(p2), fast_exp2(p3)));
                     }
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_free[place]);
             }
-            float sum = (sum0 + sum1) + (sum2 + sum3);
+            float sum, sum_b;
+            unpack2(add2(sum0, sum1), sum, sum_b);
+            sum += sum_b;
             if (x == 1) sum_s[r] = sum;
             named_barrier(BAR_PAIR, 256);
             if (x == 0) {
