@@ -30,7 +30,8 @@ constexpr int NUM_THREADS = 384;               // two softmax groups of 128; a t
 constexpr int MMA_WARP = 8, LOAD_WARP = 9;
 constexpr uint32_t TILE_BYTES = 128 * 128;     // [128 rows][64 elements]
 constexpr float RESCALE = 8.0f;                // how far (powers of two) a lane's maximum may pass its reference
-constexpr int BAR_PAIR = 1;                    // both softmax groups
+constexpr int BAR_PAIR = 1;                    // both softmax groups; 2 and 3: each of them
+constexpr int BAR_TURN = 4;                    // and 5: a group's turn at the exponentials
 
 template <int HD> struct Shape {
     static constexpr int KB = HD / 64;
@@ -51,6 +52,7 @@ struct TcParams {
 __device__ __forceinline__ void registers_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 104;"); }
 __device__ __forceinline__ void registers_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 200;"); }
 __device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void named_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -439,6 +441,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const uint32_t tmem_s = tmem_base + x * 128 + lanes, tmem_o = tmem_base + 256 + lanes;
         bool ok = true;
         uint32_t n_s = 0, n_o = 0;
+        if (x == 1) named_arrive(BAR_TURN, 256);
 #pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const Segment g = segment_of(p, pc, job, t);
@@ -458,6 +461,9 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const int own = a.mask ? z.pos : z.pos + node + 1;              // first keys that this row sees
             const bool busy = (warp & 3) * 32 < pairs;                      // any pair in this warp's lanes
             float m_ref = -INFINITY, l_run = 0.0f;
+            // In longer jobs the groups take turns at the exponentials, which bound them: one makes them while the other waits for its
+            // scores (both at once leave the unit idle while both wait: 3,600 cycles a pair of tiles, in turns 2,700).
+            const bool turns = n >= 4 * step;
 #pragma unroll 1
             for (int j = g.two ? 0 : x; j < n; j += step) {
                 const int key0 = (g.k0 + j) * BK;
@@ -479,6 +485,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 };
                 const bool interior = key0 + BK <= all;
                 if (!interior || j < step || a.scores || !busy) second_half();
+                if (turns) named_barrier(BAR_TURN + x, 256);
                 if (!interior) {
                     // Values that no row or not every row sees: what earlier owners left behind the last key, and numbers that are
                     // none in rows that see them, would reach the other rows as 0 * inf.  They become zeros here; rows that see the
@@ -568,15 +575,22 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         }
                         tile_probs(tmem_s, a.scale_log2e, m_ref == -INFINITY ? 0.0f : -m_ref, probs, sum, top, second_half);
                     }
+                    if (turns) named_arrive(BAR_TURN + (x ^ 1), 256);
                     l_run += sum;
                     tmem_st32(tmem_s + 64, *reinterpret_cast<const uint32_t(*)[32]>(&probs[0]));
                     tmem_st32(tmem_s + 96, *reinterpret_cast<const uint32_t(*)[32]>(&probs[32]));
                     tmem_wait_st();
+                } else if (turns) {
+                    named_arrive(BAR_TURN + (x ^ 1), 256);
                 }
                 ++n_s;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_p[x]);
+            }
+            if (turns && !g.two && x == 1 && (n & 1)) {          // the first group has a tile more
+                named_barrier(BAR_TURN + 1, 256);
+                named_arrive(BAR_TURN, 256);
             }
             const bool any = g.two || x < n;
             if (any) {
@@ -679,6 +693,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (!next_job(a, pc, job, t)) break;
         }
     }
+    if (warp < 4) named_barrier(BAR_TURN, 256);          // (the turn that was left)
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -842,6 +857,13 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const int x = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         bool ok = true;
+        int lse_node[4], lse_at[4];          // of the lane's four pairs of a tile: row, and place behind the tile's first
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int pair = lane * 4 + e;
+            lse_node[e] = pair < pairs_tile ? pair / a.group : 0x7fffffff;
+            lse_at[e] = pair / a.group * a.Hq + pair % a.group;
+        }
 #pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const int u0 = t - job.begin, u1 = min(job.units, pc.t1 - job.begin), n = u1 - u0;
@@ -850,12 +872,11 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             uint64_t sum0 = 0, sum1 = 0;
             // minus the lse of four pairs of a tile, minus infinity where there is none
             auto lse_of = [&](int j) -> float4 {
+                const int node0 = (job.from + u0 + j) * pairs_nodes, left = j < n ? z.len - node0 : 0;
+                const float* from = a.lse + (size_t)(z.row + node0) * a.Hq + job.kvh * a.group;
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int pair = lane * 4 + e, node = (job.from + u0 + j) * pairs_nodes + pair / a.group;
-                    v[e] = j < n && pair < pairs_tile && node < z.len ? -a.lse[(size_t)(z.row + node) * a.Hq + job.kvh * a.group + pair % a.group] : -INFINITY;
-                }
+                for (int e = 0; e < 4; ++e) v[e] = lse_node[e] < left ? -from[lse_at[e]] : -INFINITY;
                 return make_float4(v[0], v[1], v[2], v[3]);
             };
             const uint64_t scale2 = pack2(a.scale_log2e, a.scale_log2e);
