@@ -1,5 +1,6 @@
 // Kernels that move rows of the paged cache: the commit of confirmed drafted tokens, and eviction by accumulated attention weight.
 // Both work on all layers of a group of planes at once: keys and values [layers, slots, kv heads, head size].
+#include "cache_calls.h"
 #include "common.cuh"
 
 namespace {
@@ -561,21 +562,17 @@ template <typename U> int launch_evict(EvictParams p, int L, cudaStream_t stream
 
 }  // namespace
 
-// tokens, parents, targets int [T]; caches [L, num_slots, row_bytes]; path [S, width], count [S], next [S].
-LLB_EXPORT int llb_tree_commit(const int* tokens, const int* parents, const int* targets, void* k, void* v, const int* span_row,
-                               const int* span_len, const int* span_pos, const int* table, int S, int T, int L, int max_pages,
-                               int page_size, int num_slots, int row_bytes, int* path, int width, int* count, int* next,
-                               cudaStream_t stream) {
-    if (S == 0) return 0;
-    LLB_REQUIRE(S > 0 && T >= 0 && L > 0 && L <= 65535 && max_pages >= 0 && page_size > 0 && num_slots > 0 && row_bytes > 0 && row_bytes % 2 == 0 &&
-                (long long)max_pages * page_size <= 0x7fffffff, "tree_commit: bad sizes");
-    LLB_REQUIRE(width > 0 && width <= COMMIT_MAX_PATH, "tree_commit: path has room for %d nodes, 1 to %d are possible", width, COMMIT_MAX_PATH);
+LLB_EXPORT int llb_tree_commit(const LlbTreeCommit* c, cudaStream_t stream) {
+    if (c->S == 0) return 0;
+    LLB_REQUIRE(c->S > 0 && c->T >= 0 && c->L > 0 && c->L <= 65535 && c->max_pages >= 0 && c->page_size > 0 && c->num_slots > 0 && c->row_bytes > 0 &&
+                c->row_bytes % 2 == 0 && (long long)c->max_pages * c->page_size <= (1 << 30), "tree_commit: bad sizes");
+    LLB_REQUIRE(c->width > 0 && c->width <= COMMIT_MAX_PATH, "tree_commit: path has room for %d nodes, 1 to %d are possible", c->width, COMMIT_MAX_PATH);
     CommitParams p;
-    p.tokens = tokens; p.parents = parents; p.targets = targets; p.k = (char*)k; p.v = (char*)v; p.span_row = span_row;
-    p.span_len = span_len; p.span_pos = span_pos; p.table = table; p.S = S; p.T = T; p.L = L; p.max_pages = max_pages;
-    p.page_size = page_size; p.num_slots = num_slots; p.path = path; p.width = width; p.count = count; p.next = next;
-    const int unit = unit_bytes(k, v, row_bytes);
-    p.row_units = row_bytes / unit;
+    p.tokens = c->tokens; p.parents = c->parents; p.targets = c->targets; p.k = (char*)c->k; p.v = (char*)c->v; p.span_row = c->span_row;
+    p.span_len = c->span_len; p.span_pos = c->span_pos; p.table = c->table; p.S = c->S; p.T = c->T; p.L = c->L; p.max_pages = c->max_pages;
+    p.page_size = c->page_size; p.num_slots = c->num_slots; p.path = c->path; p.width = c->width; p.count = c->count; p.next = c->next;
+    const int unit = unit_bytes(c->k, c->v, c->row_bytes);
+    p.row_units = c->row_bytes / unit;
     p.layers_a_block = COMMIT_THREADS / (2 * p.row_units) > 1 ? COMMIT_THREADS / (2 * p.row_units) : 1;
     if (unit == 16) return launch_commit<uint4>(p, stream);
     if (unit == 8) return launch_commit<uint2>(p, stream);
@@ -583,25 +580,22 @@ LLB_EXPORT int llb_tree_commit(const int* tokens, const int* parents, const int*
     return launch_commit<unsigned short>(p, stream);
 }
 
-// caches [L, num_slots, Hkv, head_bytes]; mass, positions and their outputs [L, Hkv, num_slots] (the outputs may be the inputs).
-LLB_EXPORT int llb_cache_evict(void* k, void* v, const float* mass, const int* positions, float* mass_out, int* positions_out,
-                               const int* lengths, const int* ends, const int* table, int S, int L, int Hkv, int max_pages, int page_size,
-                               int num_slots, int head_bytes, int budget, int first, int latest, cudaStream_t stream) {
-    if (S == 0) return 0;
-    LLB_REQUIRE(S > 0 && L > 0 && L <= 65535 && Hkv > 0 && (long long)S * Hkv < (1ll << 31) && page_size > 0 && max_pages >= 0 && num_slots > 0 &&
-                head_bytes > 0 && head_bytes % 2 == 0, "cache_evict: bad sizes");
-    LLB_REQUIRE((long long)max_pages * page_size <= EV_MAX_PLACES, "cache_evict: a block table of %d pages of %d names more than %d places", max_pages,
-                page_size, EV_MAX_PLACES);
-    LLB_REQUIRE(budget > 0 && first >= 0 && latest >= 0 && (long long)first + latest <= budget,
-                "cache_evict: a budget of %d places does not hold the first %d and the latest %d", budget, first, latest);
+LLB_EXPORT int llb_cache_evict(const LlbCacheEvict* c, cudaStream_t stream) {
+    if (c->S == 0) return 0;
+    LLB_REQUIRE(c->S > 0 && c->L > 0 && c->L <= 65535 && c->Hkv > 0 && (long long)c->S * c->Hkv < (1ll << 31) && c->page_size > 0 && c->max_pages >= 0 &&
+                c->num_slots > 0 && c->head_bytes > 0 && c->head_bytes % 2 == 0, "cache_evict: bad sizes");
+    LLB_REQUIRE((long long)c->max_pages * c->page_size <= EV_MAX_PLACES, "cache_evict: a block table of %d pages of %d names more than %d places",
+                c->max_pages, c->page_size, EV_MAX_PLACES);
+    LLB_REQUIRE(c->budget > 0 && c->first >= 0 && c->latest >= 0 && (long long)c->first + c->latest <= c->budget,
+                "cache_evict: a budget of %d places does not hold the first %d and the latest %d", c->budget, c->first, c->latest);
     EvictParams p;
-    p.k = (char*)k; p.v = (char*)v; p.mass = mass; p.positions = positions; p.mass_out = mass_out; p.positions_out = positions_out;
-    p.lengths = lengths; p.ends = ends; p.table = table; p.S = S; p.max_pages = max_pages; p.page_size = page_size; p.num_slots = num_slots;
-    p.Hkv = Hkv; p.budget = budget; p.first = first; p.latest = latest; p.cache_places = 0;
-    const int unit = unit_bytes(k, v, head_bytes);
-    p.head_units = head_bytes / unit;
-    if (unit == 16) return launch_evict<uint4>(p, L, stream);
-    if (unit == 8) return launch_evict<uint2>(p, L, stream);
-    if (unit == 4) return launch_evict<unsigned>(p, L, stream);
-    return launch_evict<unsigned short>(p, L, stream);
+    p.k = (char*)c->k; p.v = (char*)c->v; p.mass = c->mass; p.positions = c->positions; p.mass_out = c->mass_out; p.positions_out = c->positions_out;
+    p.lengths = c->lengths; p.ends = c->ends; p.table = c->table; p.S = c->S; p.max_pages = c->max_pages; p.page_size = c->page_size;
+    p.num_slots = c->num_slots; p.Hkv = c->Hkv; p.budget = c->budget; p.first = c->first; p.latest = c->latest; p.cache_places = 0;
+    const int unit = unit_bytes(c->k, c->v, c->head_bytes);
+    p.head_units = c->head_bytes / unit;
+    if (unit == 16) return launch_evict<uint4>(p, c->L, stream);
+    if (unit == 8) return launch_evict<uint2>(p, c->L, stream);
+    if (unit == 4) return launch_evict<unsigned>(p, c->L, stream);
+    return launch_evict<unsigned short>(p, c->L, stream);
 }

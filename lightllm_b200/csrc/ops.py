@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import struct
 from typing import Optional
 
 import torch
@@ -1347,6 +1348,12 @@ def paged_decode_mma(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 # These calls come once a layer and step, and the host's part of one is longer than the small ones' kernels: the checks look at every
 # property of a tensor once and no more.
 _INT32, _INT64, _FLOAT32 = torch.int32, torch.int64, torch.float32
+# the C structs of csrc/cache_calls.h
+_SPAN_CALL = "10P9if"
+_TREE_ATTENTION = struct.Struct("@" + _SPAN_CALL + "Pii").pack
+_ATTENTION_MASS = struct.Struct("@" + _SPAN_CALL + "PPii").pack
+_TREE_COMMIT = struct.Struct("@12P8i").pack
+_CACHE_EVICT = struct.Struct("@9P10i").pack
 
 
 def _elsewhere(what: str, device: int, *tensors) -> None:
@@ -1462,10 +1469,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     stream = _stream_on(device)
     scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, slots, 0, device),
                           dtype=torch.float32, device=q.device)
-    _check(lib().llb_tree_attention(
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), dt, mask.data_ptr(), words[1], span_row.data_ptr(),
-        span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, pages, page_size, slots, num_heads, num_kv_heads,
-        head_dim, scale, scratch.data_ptr(), async_error_flag(q.device).data_ptr(), stream))
+    _check(lib().llb_tree_attention(_TREE_ATTENTION(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), span_row.data_ptr(), span_len.data_ptr(), span_pos.data_ptr(),
+        block_table.data_ptr(), scratch.data_ptr(), async_error_flag(q.device).data_ptr(), dt, S, T, pages, page_size, slots, num_heads,
+        num_kv_heads, head_dim, scale, mask.data_ptr(), words[1], 0), stream))
 
 
 def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, mass: torch.Tensor,
@@ -1497,10 +1504,10 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     stream = _stream_on(device)
     scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, slots, 2 if max_len == 1 else 1, device),
                           dtype=torch.float32, device=q.device)
-    _check(lib().llb_paged_attention_mass(
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), dt, None if mass_in is None else mass_in.data_ptr(),
-        mass.data_ptr(), span_row.data_ptr(), span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, T, max_len, pages,
-        page_size, slots, num_heads, num_kv_heads, head_dim, scale, scratch.data_ptr(), async_error_flag(q.device).data_ptr(), stream))
+    _check(lib().llb_paged_attention_mass(_ATTENTION_MASS(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), span_row.data_ptr(), span_len.data_ptr(), span_pos.data_ptr(),
+        block_table.data_ptr(), scratch.data_ptr(), async_error_flag(q.device).data_ptr(), dt, S, T, pages, page_size, slots, num_heads,
+        num_kv_heads, head_dim, scale, 0 if mass_in is None else mass_in.data_ptr(), mass.data_ptr(), max_len, 0), stream))
 
 
 def _check_planes(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor):
@@ -1539,11 +1546,10 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, targets: torch.Tens
     if path.dtype is not _INT32 or len(room) != 2 or room[0] != S:
         raise KernelError(f"tree_commit: path must be int32 [{S}, width], got {path.dtype} {tuple(room)}")
     device = _check_here("tree_commit", tokens, parents, targets, k_cache, v_cache, span_row, span_len, span_pos, block_table, path, count, next_token)
-    _check(lib().llb_tree_commit(
+    _check(lib().llb_tree_commit(_TREE_COMMIT(
         tokens.data_ptr(), parents.data_ptr(), targets.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), span_row.data_ptr(),
-        span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), S, rows[0], L, pages, page_size, slots,
-        heads * hd * k_cache.element_size(), path.data_ptr(), room[1], count.data_ptr(), next_token.data_ptr(),
-        _stream_on(device)))
+        span_len.data_ptr(), span_pos.data_ptr(), block_table.data_ptr(), path.data_ptr(), count.data_ptr(), next_token.data_ptr(),
+        S, rows[0], L, pages, page_size, slots, heads * hd * k_cache.element_size(), room[1]), _stream_on(device)))
 
 
 def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor,
@@ -1580,10 +1586,10 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor
     if budget <= 0 or first < 0 or latest < 0 or first + latest > budget:
         raise KernelError(f"cache_evict: a budget of {budget} places does not hold the first {first} and the latest {latest}")
     device = _check_here("cache_evict", k_cache, v_cache, mass, positions, lengths, ends, block_table, mass_out, positions_out)
-    _check(lib().llb_cache_evict(
+    _check(lib().llb_cache_evict(_CACHE_EVICT(
         k_cache.data_ptr(), v_cache.data_ptr(), mass.data_ptr(), positions.data_ptr(), mass_out.data_ptr(), positions_out.data_ptr(),
         lengths.data_ptr(), ends.data_ptr(), block_table.data_ptr(), S, L, heads, pages, page_size, slots, hd * k_cache.element_size(),
-        budget, first, latest, _stream_on(device)))
+        budget, first, latest), _stream_on(device)))
 
 
 # Where the blocks that share a long row of logits meet (a 64-bit slot and a counter per row), per device.

@@ -8,6 +8,7 @@
 // and walks 64 keys at a time: the tile's K and V go to shared memory as floats, the scores to shared memory for the softmax (whole
 // rows are needed there), O stays in registers.  Every thread has 4 rows of the scores and of O, so that a float4 from shared memory
 // feeds 16 products or more.  RB is 64, or 16 where requests bring so few rows that most of 64 would stay empty.
+#include "cache_calls.h"
 #include "span_attention.cuh"
 
 #include <math.h>
@@ -393,7 +394,7 @@ template <int TILE> __device__ __forceinline__ void mass_of_scores(const LlbSpan
 
 // The first `blocks * ny` blocks join, the others add up weights, `mass_y` of them a request and kv head.
 template <typename T, int TILE>
-__global__ void __launch_bounds__(THREADS) span_join_kernel(const LlbSpanArgs a, int blocks, int ny, int mass_y, int least) {
+__global__ void __launch_bounds__(THREADS, 5) span_join_kernel(const LlbSpanArgs a, int blocks, int ny, int mass_y, int least) {
     llb_after_previous();
     const int i = blockIdx.x;
     if (i >= blocks * ny) {
@@ -408,8 +409,8 @@ __global__ void __launch_bounds__(THREADS) span_join_kernel(const LlbSpanArgs a,
     job.pos = from[1].x;
     job.parts = lo.x; job.row = lo.y; job.rows = lo.z; job.kvh = lo.w;
     if (job.parts == 0) return;
-    if (job.parts <= 2) join_rows<T, 2, 4>(a, job, block, y, ny);
-    else join_rows<T, 8, 1>(a, job, block, y, ny);
+    if (job.parts <= 2) join_rows<T, 2, 2>(a, job, block, y, ny);
+    else join_rows<T, 5, 1>(a, job, block, y, ny);
 }
 
 // The same for requests of any number of rows: 64 keys of one request and kv head stay in shared memory, the rows that see any of them
@@ -529,7 +530,7 @@ template <typename T, int TILE>
 int launch_join(const LlbSpanArgs& a, int blocks, int least, cudaStream_t stream) {
     // a warp of the first kind has 32 rows of four dimensions at a time: as many as the average job brings
     const int average = (int)max(1ll, min((long long)a.rows, (long long)a.T * a.group / max(1, a.S)));
-    const int ny = min(16, llb_ceil_div(llb_ceil_div(average, 32) * llb_ceil_div(a.hd, 4), THREADS / 32));
+    const int ny = min(16, llb_ceil_div(llb_ceil_div(average, 32) * llb_ceil_div(a.hd, 8), THREADS / 32));
     int mass_y = 0;
     if (a.scores) {
         const long long keys = (long long)a.max_pages * a.page_size;
@@ -631,13 +632,15 @@ int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtyp
     return rc ? rc : llb_span_join(a, dtype, blocks, KT, 1, stream);
 }
 
-LlbSpanArgs span_args(const void* out, const int* span_row, const int* span_len, const int* span_pos, const int* table, int S, int T,
-                      int max_pages, int page_size, int num_slots, int Hq, int Hkv, int hd, float scale, int max_len) {
+LlbSpanArgs span_args(const LlbSpanCall& s, int max_len) {
     LlbSpanArgs a = {};
-    a.out = const_cast<void*>(out); a.span_row = span_row; a.span_len = span_len; a.span_pos = span_pos; a.table = table;
-    a.S = S; a.T = T; a.max_pages = max_pages; a.page_size = page_size; a.num_slots = num_slots; a.Hq = Hq; a.Hkv = Hkv; a.hd = hd;
-    a.group = Hkv > 0 ? Hq / Hkv : 0; a.scale_log2e = scale * 1.4426950408889634f; a.max_len = max_len;
+    a.out = s.out; a.span_row = s.span_row; a.span_len = s.span_len; a.span_pos = s.span_pos; a.table = s.table;
+    a.S = s.S; a.T = s.T; a.max_pages = s.max_pages; a.page_size = s.page_size; a.num_slots = s.num_slots; a.Hq = s.Hq; a.Hkv = s.Hkv; a.hd = s.hd;
+    a.group = s.Hkv > 0 ? s.Hq / s.Hkv : 0; a.scale_log2e = s.scale * 1.4426950408889634f; a.max_len = max_len;
     return a;
+}
+bool takes_tc(const LlbSpanArgs& a, const LlbSpanCall& s) {
+    return tc_sizes(s.dtype, a.hd, a.page_size) && llb_span_tc_takes(a, s.q, s.k, s.v, s.out);
 }
 
 }  // namespace
@@ -654,49 +657,42 @@ LLB_EXPORT long long llb_span_scratch_floats(int dtype, int T, int S, int Hq, in
     return n;
 }
 
-// q, out [T, Hq, hd]; caches [num_slots, Hkv, hd]; span arrays [S]; table [S, max_pages]; mask [T, words] 64-bit words.
-LLB_EXPORT int llb_tree_attention(const void* q, const void* k, const void* v, void* out, int dtype, const unsigned long long* mask,
-                                  int words, const int* span_row, const int* span_len, const int* span_pos, const int* table, int S, int T,
-                                  int max_pages, int page_size, int num_slots, int Hq, int Hkv, int hd, float scale, float* scratch,
-                                  int* error_flag, cudaStream_t stream) {
-    LlbSpanArgs a = span_args(out, span_row, span_len, span_pos, table, S, T, max_pages, page_size, num_slots, Hq, Hkv, hd, scale, 0);
-    if (int rc = check(a, dtype)) return rc;
-    LLB_REQUIRE(words > 0 && words <= (1 << 20) && mask && scratch, "tree_attention: no mask or no scratch");
-    if (S == 0 || T == 0) return 0;
-    a.mask = mask;
-    a.words = words;
-    a.max_len = words * 64;
+// The calls take one C struct: what a caller from Python pays for an argument of its own (0.12 us) is a tenth of a small call's time.
+LLB_EXPORT int llb_tree_attention(const LlbTreeAttention* c, cudaStream_t stream) {
+    const LlbSpanCall& s = c->span;
+    LlbSpanArgs a = span_args(s, c->words > 0 && c->words <= (1 << 20) ? c->words * 64 : 0);
+    if (int rc = check(a, s.dtype)) return rc;
+    LLB_REQUIRE(a.max_len > 0 && c->mask && s.scratch, "tree_attention: no mask or no scratch");
+    if (a.S == 0 || a.T == 0) return 0;
+    a.mask = c->mask;
+    a.words = c->words;
     float* unused;
-    return attend(a, q, k, v, dtype, scratch, 0, tc_sizes(dtype, hd, page_size) && llb_span_tc_takes(a, q, k, v, out), &unused, error_flag, stream);
+    return attend(a, s.q, s.k, s.v, s.dtype, s.scratch, 0, takes_tc(a, s), &unused, s.error_flag, stream);
 }
 
-// Causal; mass_in (may be null) and mass [Hkv, num_slots] float, may be the same.
-LLB_EXPORT int llb_paged_attention_mass(const void* q, const void* k, const void* v, void* out, int dtype, const float* mass_in, float* mass,
-                                        const int* span_row, const int* span_len, const int* span_pos, const int* table, int S, int T,
-                                        int max_len, int max_pages, int page_size, int num_slots, int Hq, int Hkv, int hd, float scale,
-                                        float* scratch, int* error_flag, cudaStream_t stream) {
-    LlbSpanArgs a = span_args(out, span_row, span_len, span_pos, table, S, T, max_pages, page_size, num_slots, Hq, Hkv, hd, scale, max_len);
-    if (int rc = check(a, dtype)) return rc;
-    LLB_REQUIRE(max_len > 0 && mass && scratch, "paged_attention_mass: no weights, no scratch or rows");
-    LLB_REQUIRE((long long)S * Hkv < (1ll << 31), "paged_attention_mass: too many requests");
-    if (S == 0 || T == 0) return 0;
-    const bool single = max_len == 1;
-    const bool tc = tc_sizes(dtype, hd, page_size) && llb_span_tc_takes(a, q, k, v, out);
+LLB_EXPORT int llb_paged_attention_mass(const LlbAttentionMass* c, cudaStream_t stream) {
+    const LlbSpanCall& s = c->span;
+    LlbSpanArgs a = span_args(s, c->max_len);
+    if (int rc = check(a, s.dtype)) return rc;
+    LLB_REQUIRE(a.max_len > 0 && c->mass && s.scratch, "paged_attention_mass: no weights, no scratch or rows");
+    LLB_REQUIRE((long long)a.S * a.Hkv < (1ll << 24), "paged_attention_mass: too many requests");
+    if (a.S == 0 || a.T == 0) return 0;
+    const bool single = a.max_len == 1, tc = takes_tc(a, s);
     float* part_mass;
-    a.mass_in = mass_in;
-    a.mass = mass;
-    if (int rc = attend(a, q, k, v, dtype, scratch, single ? 2 : 1, tc, &part_mass, error_flag, stream)) return rc;
+    a.mass_in = c->mass_in;
+    a.mass = c->mass;
+    if (int rc = attend(a, s.q, s.k, s.v, s.dtype, s.scratch, single ? 2 : 1, tc, &part_mass, s.error_flag, stream)) return rc;
     if (single) return 0;
     if (tc) {
-        if (int rc = llb_span_mass_tc(a, q, k, part_mass, tc_blocks(), error_flag, stream)) return rc;
+        if (int rc = llb_span_mass_tc(a, s.q, s.k, part_mass, tc_blocks(), s.error_flag, stream)) return rc;
         llb_launch(span_mass_join_kernel<128>, dim3(tc_blocks()), dim3(128), 0, stream, a, (const float*)part_mass);
         return llb_check_launch("span_mass_join");
     }
     ColumnParams p;
-    p.a = a; p.q = q; p.k = k; p.part = part_mass;
-    const int hd4 = (hd + 3) & ~3;
+    p.a = a; p.q = s.q; p.k = s.k; p.part = part_mass;
+    const int hd4 = (a.hd + 3) & ~3;
     const size_t smem = sizeof(float) * ((size_t)64 * hd4 + KT * (hd4 + 4));
-    auto kernel = dtype == LLB_F32 ? span_mass_kernel<float> : span_mass_kernel<__nv_bfloat16>;
+    auto kernel = s.dtype == LLB_F32 ? span_mass_kernel<float> : span_mass_kernel<__nv_bfloat16>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return llb_fail("span_mass: cannot opt in to %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
     llb_launch(kernel, dim3(simt_blocks()), dim3(THREADS), smem, stream, p);

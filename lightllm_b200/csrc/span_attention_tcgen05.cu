@@ -7,7 +7,8 @@
 //     more than 128 pairs     each group has 128 pairs of its own, both see every tile
 //     up to 128 pairs         both have the same pairs, the first sees the even tiles and the second the odd ones; they are joined at
 //                             the end through tensor memory (the same pair has the same lane in both)
-// While one group works on its scores the tensor cores work for the other.  For every tile of 128 keys of a group:
+// While one group works on its scores the tensor cores work for the other.  (Strict turns at the exponentials were built: a pair of tiles took
+// 4,200 cycles instead of 3,600.)  For every tile of 128 keys of a group:
 //     S = Q K^T               tcgen05.mma, 128 columns of tensor memory, in two halves of 64 keys
 //     m, p = 2^(S - m), l     a thread reads its lane's 128 scores once; p goes back to tensor memory as bf16 (over the second half of S)
 //                             and is the A operand of the next product without a way through shared memory
@@ -31,7 +32,6 @@ constexpr int MMA_WARP = 8, LOAD_WARP = 9;
 constexpr uint32_t TILE_BYTES = 128 * 128;     // [128 rows][64 elements]
 constexpr float RESCALE = 8.0f;                // how far (powers of two) a lane's maximum may pass its reference
 constexpr int BAR_PAIR = 1;                    // both softmax groups; 2 and 3: each of them
-constexpr int BAR_TURN = 4;                    // and 5: a group's turn at the exponentials
 
 template <int HD> struct Shape {
     static constexpr int KB = HD / 64;
@@ -52,7 +52,6 @@ struct TcParams {
 __device__ __forceinline__ void registers_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 104;"); }
 __device__ __forceinline__ void registers_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 200;"); }
 __device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-__device__ __forceinline__ void named_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -441,7 +440,6 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const uint32_t tmem_s = tmem_base + x * 128 + lanes, tmem_o = tmem_base + 256 + lanes;
         bool ok = true;
         uint32_t n_s = 0, n_o = 0;
-        if (x == 1) named_arrive(BAR_TURN, 256);
 #pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const Segment g = segment_of(p, pc, job, t);
@@ -461,9 +459,6 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const int own = a.mask ? z.pos : z.pos + node + 1;              // first keys that this row sees
             const bool busy = (warp & 3) * 32 < pairs;                      // any pair in this warp's lanes
             float m_ref = -INFINITY, l_run = 0.0f;
-            // In longer jobs the groups take turns at the exponentials, which bound them: one makes them while the other waits for its
-            // scores (both at once leave the unit idle while both wait: 3,600 cycles a pair of tiles, in turns 2,700).
-            const bool turns = n >= 4 * step;
 #pragma unroll 1
             for (int j = g.two ? 0 : x; j < n; j += step) {
                 const int key0 = (g.k0 + j) * BK;
@@ -485,7 +480,6 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 };
                 const bool interior = key0 + BK <= all;
                 if (!interior || j < step || a.scores || !busy) second_half();
-                if (turns) named_barrier(BAR_TURN + x, 256);
                 if (!interior) {
                     // Values that no row or not every row sees: what earlier owners left behind the last key, and numbers that are
                     // none in rows that see them, would reach the other rows as 0 * inf.  They become zeros here; rows that see the
@@ -575,22 +569,15 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         }
                         tile_probs(tmem_s, a.scale_log2e, m_ref == -INFINITY ? 0.0f : -m_ref, probs, sum, top, second_half);
                     }
-                    if (turns) named_arrive(BAR_TURN + (x ^ 1), 256);
                     l_run += sum;
                     tmem_st32(tmem_s + 64, *reinterpret_cast<const uint32_t(*)[32]>(&probs[0]));
                     tmem_st32(tmem_s + 96, *reinterpret_cast<const uint32_t(*)[32]>(&probs[32]));
                     tmem_wait_st();
-                } else if (turns) {
-                    named_arrive(BAR_TURN + (x ^ 1), 256);
                 }
                 ++n_s;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_p[x]);
-            }
-            if (turns && !g.two && x == 1 && (n & 1)) {          // the first group has a tile more
-                named_barrier(BAR_TURN + 1, 256);
-                named_arrive(BAR_TURN, 256);
             }
             const bool any = g.two || x < n;
             if (any) {
@@ -693,7 +680,6 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (!next_job(a, pc, job, t)) break;
         }
     }
-    if (warp < 4) named_barrier(BAR_TURN, 256);          // (the turn that was left)
     __syncwarp();
     tc_fence_before();
     __syncthreads();

@@ -7,7 +7,7 @@ from lightllm_b200.csrc import build, ops
 
 # the number -> what callers of that number were built for (see :func:`interface`).  Changed arguments or structs take the next number
 # in csrc/common.cu, csrc/ops.py and csrc/host/generate.cpp, and a line here.
-KNOWN = {25: "5eeac51547ca62c7", 26: "2619e82c8415ad5b", 27: "8651f0f98d98b681"}
+KNOWN = {25: "5eeac51547ca62c7", 26: "2619e82c8415ad5b", 27: "0f7f06b9314ad8b9"}
 
 
 def interface() -> str:
