@@ -151,7 +151,7 @@ __device__ __forceinline__ unsigned order_of(float f) {
 // The listed moves of one (layer, kv head): rows of K and V, 16 bytes a thread and AHEAD of them on their way, then weights and positions.
 template <typename U>
 __device__ __forceinline__ void move_rows(const EvictParams& p, size_t plane, int layer, int h, const unsigned (&list)[2][EV_LIST], unsigned count) {
-    constexpr int AHEAD = 8;
+    constexpr int AHEAD = 4;
     const unsigned units = 2 * p.head_units, total = count * units;
     const size_t stride = (size_t)p.Hkv * p.head_units, base = (size_t)layer * p.num_slots * stride + (size_t)h * p.head_units;
     const int shift = (units & (units - 1)) == 0 ? 31 - __clz(units) : -1;          // (heads of 64 and 128: no division)
@@ -242,7 +242,7 @@ template <int WORDS> __device__ __forceinline__ void scan_words(unsigned (&count
 }
 
 template <typename U, int PER>
-__global__ void __launch_bounds__(EV_THREADS, PER <= 8 ? 2 : 1) cache_evict_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(EV_THREADS, PER <= 8 ? 3 : 1) cache_evict_kernel(const EvictParams p) {
     constexpr int WORDS = PER * EV_WARPS;
     __shared__ unsigned hist[EV_BINS];
     __shared__ unsigned list_s[2][EV_LIST];

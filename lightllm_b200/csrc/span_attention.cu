@@ -311,12 +311,21 @@ __device__ __forceinline__ void join_rows(const LlbSpanArgs& a, const LlbOpen& j
         const float inv = llb_inverse(M, L, job.pos);
         if (a.lse && piece0 == 0) a.lse[(size_t)row * a.Hq + head] = llb_lse(M, L);
         T* dst = (T*)a.out + ((size_t)row * a.Hq + head) * hd + piece0 * 4;
+        unsigned held0 = 0, held1 = 0;          // two groups of four dimensions leave together
 #pragma unroll
         for (int u = 0; u < PU; ++u) {
             const int d = (piece0 + u) * 4;
-            if (hd % 4 == 0 && sizeof(T) == 2 && ((uintptr_t)a.out & 7) == 0 && d < hd) {
+            if (sizeof(T) == 2 && ((uintptr_t)a.out & 15) == 0 && hd % 8 == 0 && d < hd) {
                 const __nv_bfloat162 lo = __floats2bfloat162_rn(x[u][0] * inv, x[u][1] * inv), hi = __floats2bfloat162_rn(x[u][2] * inv, x[u][3] * inv);
-                *reinterpret_cast<uint2*>(dst + 4 * u) = make_uint2(*reinterpret_cast<const unsigned*>(&lo), *reinterpret_cast<const unsigned*>(&hi));
+                const unsigned w0 = *reinterpret_cast<const unsigned*>(&lo), w1 = *reinterpret_cast<const unsigned*>(&hi);
+                if (PU == 1) {
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(w0, w1);
+                } else if (u & 1) {
+                    *reinterpret_cast<uint4*>(dst + 4 * (u - 1)) = make_uint4(held0, held1, w0, w1);
+                } else {
+                    held0 = w0;
+                    held1 = w1;
+                }
                 continue;
             }
 #pragma unroll
@@ -394,7 +403,7 @@ template <int TILE> __device__ __forceinline__ void mass_of_scores(const LlbSpan
 
 // The first `blocks * ny` blocks join, the others add up weights, `mass_y` of them a request and kv head.
 template <typename T, int TILE>
-__global__ void __launch_bounds__(THREADS, 5) span_join_kernel(const LlbSpanArgs a, int blocks, int ny, int mass_y, int least) {
+__global__ void __launch_bounds__(THREADS, 4) span_join_kernel(const LlbSpanArgs a, int blocks, int ny, int mass_y, int least) {
     llb_after_previous();
     const int i = blockIdx.x;
     if (i >= blocks * ny) {
@@ -409,8 +418,8 @@ __global__ void __launch_bounds__(THREADS, 5) span_join_kernel(const LlbSpanArgs
     job.pos = from[1].x;
     job.parts = lo.x; job.row = lo.y; job.rows = lo.z; job.kvh = lo.w;
     if (job.parts == 0) return;
-    if (job.parts <= 2) join_rows<T, 2, 2>(a, job, block, y, ny);
-    else join_rows<T, 5, 1>(a, job, block, y, ny);
+    if (job.parts <= 2) join_rows<T, 2, 4>(a, job, block, y, ny);
+    else join_rows<T, 8, 1>(a, job, block, y, ny);
 }
 
 // The same for requests of any number of rows: 64 keys of one request and kv head stay in shared memory, the rows that see any of them
@@ -530,7 +539,8 @@ template <typename T, int TILE>
 int launch_join(const LlbSpanArgs& a, int blocks, int least, cudaStream_t stream) {
     // a warp of the first kind has 32 rows of four dimensions at a time: as many as the average job brings
     const int average = (int)max(1ll, min((long long)a.rows, (long long)a.T * a.group / max(1, a.S)));
-    const int ny = min(16, llb_ceil_div(llb_ceil_div(average, 32) * llb_ceil_div(a.hd, 8), THREADS / 32));
+    // (small jobs are cut into many parts, of which it takes few groups of dimensions at once)
+    const int ny = min(16, llb_ceil_div(llb_ceil_div(average, 32) * llb_ceil_div(a.hd, average <= 128 ? 4 : 16), THREADS / 32));
     int mass_y = 0;
     if (a.scores) {
         const long long keys = (long long)a.max_pages * a.page_size;
