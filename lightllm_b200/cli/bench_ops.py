@@ -515,6 +515,41 @@ def main(argv=None) -> int:
         run("paged_decode_mma_and_merge", lambda: ops.paged_decode_mma(qd, kcd, vcd, od, rows, zero, B, rows, pos, btd, pages_per,
                                                                        page, Hq, Hkv, hd, 0, 1 / math.sqrt(hd), big, scratch),
             kv_bytes + 2 * B * Hq * big * (hd + 2) * 4)
+    # ---- a cache that is drafted into and thinned out: trees of 16 nodes, keys' weights, commit and eviction ----------------
+    nodes, layers_c = 16, 4
+    pages_t = -(-(C + nodes) // page)
+    slots_t = B * pages_t * page
+    btt = torch.randperm(B * pages_t, generator=g, device=dev).to(torch.int32).reshape(B, pages_t)
+    tree = [-1] + [(i - 1) // 3 for i in range(1, nodes)]
+    mask_t = ops.tree_mask([tree] * B).to(dev)
+    row_t, len_t, pos_t, each_t = i32([nodes * i for i in range(B)]), i32([nodes] * B), i32([C] * B), i32([1] * B)
+    for dt, label in ((torch.bfloat16, ""), (torch.float32, "_float32")):
+        e = 2 if dt == torch.bfloat16 else 4
+        kct, vct = rn(slots_t, Hkv, hd, dtype=dt), rn(slots_t, Hkv, hd, dtype=dt)
+        qt = rn(B * nodes, Hq * hd, dtype=dt)
+        ot = torch.empty_like(qt)
+        mass_t = torch.zeros((Hkv, slots_t), device=dev)
+        run("tree_attention" + label,
+            lambda: ops.tree_attention(qt, kct, vct, ot, mask_t, row_t, len_t, pos_t, btt, page, Hq, Hkv, hd, 1 / math.sqrt(hd)),
+            2 * B * (nodes * Hq + (C + nodes) * Hkv) * hd * e, 4 * B * nodes * Hq * hd * C)
+        run("paged_attention_mass_one_token" + label,
+            lambda: ops.paged_attention_mass(qt[:B], kct, vct, ot[:B], mass_t, rows, each_t, pos, btt, page, Hq, Hkv, hd,
+                                             1 / math.sqrt(hd), 1, mass_in=mass_t), B * (C + 1) * Hkv * (2 * hd * e + 8))
+        run("paged_attention_mass_portions" + label,
+            lambda: ops.paged_attention_mass(qt, kct, vct, ot, mass_t, row_t, len_t, pos_t, btt, page, Hq, Hkv, hd, 1 / math.sqrt(hd),
+                                             nodes, mass_in=mass_t), B * (C + nodes) * Hkv * (2 * hd * e + 8), 4 * B * nodes * Hq * hd * C)
+    kcl, vcl = rn(layers_c, slots_t, Hkv, hd, dtype=torch.bfloat16), rn(layers_c, slots_t, Hkv, hd, dtype=torch.bfloat16)
+    tok_t, par_t = i32([7] * (B * nodes)), i32(tree * B)
+    path_t, cnt_t, nxt_t = i32([[0] * nodes] * B), i32([0] * B), i32([0] * B)
+    run("tree_commit", lambda: ops.tree_commit(tok_t, par_t, tok_t, kcl, vcl, row_t, len_t, pos_t, btt, page, path_t, cnt_t, nxt_t),
+        B * nodes * 12 + 4 * layers_c * B * 3 * Hkv * hd * 2)
+    mass_l = torch.rand((layers_c, Hkv, slots_t), generator=g, device=dev)
+    pos_l = torch.zeros((layers_c, Hkv, slots_t), dtype=torch.int32, device=dev)
+    mass_o, pos_o, ends_t = torch.zeros_like(mass_l), torch.zeros_like(pos_l), i32([2 * C] * B)
+    for label, budget in (("one", C - 1), ("half", max(1, C // 2))):
+        run(f"cache_evict_{label}", lambda: ops.cache_evict(kcl, vcl, mass_l, pos_l, pos, ends_t, btt, page, budget, 0, 0, mass_out=mass_o,
+                                                            positions_out=pos_o),
+            layers_c * B * Hkv * (8 * C + 8 * budget + (C - budget) * budget // C * 8 * hd))
     logits = rn(B, V, s=3.0)
     tok = torch.empty(B, dtype=torch.int32, device=dev)
     run("argmax", lambda: ops.argmax(logits, tok), B * V * 4)

@@ -554,8 +554,8 @@ template <typename T, int RB, int NI>
 int launch_attention(const SimtParams& p, int blocks, cudaStream_t stream) {
     const int hd4 = (p.a.hd + 3) & ~3;
     const size_t smem = sizeof(float) * ((size_t)RB * hd4 + KT * (hd4 + 4) + KT * 64 * NI + RB * SP);
-    // (set every time: the attribute belongs to the current device)
-    cudaError_t e = cudaFuncSetAttribute(span_attention_kernel<T, RB, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static LlbSharedMemory room;
+    cudaError_t e = room.allow(span_attention_kernel<T, RB, NI>, smem);
     if (e != cudaSuccess) return llb_fail("span_attention: cannot opt in to %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
     llb_launch(span_attention_kernel<T, RB, NI>, dim3(blocks), dim3(THREADS), smem, stream, p);
     return llb_check_launch("span_attention");
@@ -702,8 +702,9 @@ LLB_EXPORT int llb_paged_attention_mass(const LlbAttentionMass* c, cudaStream_t 
     p.a = a; p.q = s.q; p.k = s.k; p.part = part_mass;
     const int hd4 = (a.hd + 3) & ~3;
     const size_t smem = sizeof(float) * ((size_t)64 * hd4 + KT * (hd4 + 4));
+    static LlbSharedMemory room_f32, room_bf16;
     auto kernel = s.dtype == LLB_F32 ? span_mass_kernel<float> : span_mass_kernel<__nv_bfloat16>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = (s.dtype == LLB_F32 ? room_f32 : room_bf16).allow(kernel, smem);
     if (e != cudaSuccess) return llb_fail("span_mass: cannot opt in to %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
     llb_launch(kernel, dim3(simt_blocks()), dim3(THREADS), smem, stream, p);
     if (int rc = llb_check_launch("span_mass")) return rc;

@@ -965,13 +965,15 @@ template <int HD>
 int launch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TcParams& p, int blocks, cudaStream_t stream) {
     static const bool suffice = registers_suffice<HD>();
     LLB_REQUIRE(suffice, "span_attention_tcgen05: the kernel was built with too few registers a thread");
-    cudaError_t e = cudaFuncSetAttribute(span_attention_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<HD>::SMEM);
+    static LlbSharedMemory room;
+    cudaError_t e = room.allow(span_attention_tc_kernel<HD>, Shape<HD>::SMEM);
     if (e == cudaSuccess) e = launch_pdl(span_attention_tc_kernel<HD>, dim3(blocks), dim3(NUM_THREADS), Shape<HD>::SMEM, stream, mq, mk, mv, p);
     if (e != cudaSuccess) return llb_fail("span_attention_tcgen05: launch failed: %s", cudaGetErrorString(e));
     return llb_check_launch("span_attention_tcgen05");
 }
 template <int HD> int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const MassArgs& m, int blocks, cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(span_mass_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MassShape<HD>::SMEM);
+    static LlbSharedMemory room;
+    cudaError_t e = room.allow(span_mass_tc_kernel<HD>, MassShape<HD>::SMEM);
     if (e == cudaSuccess) e = launch_pdl(span_mass_tc_kernel<HD>, dim3(blocks), dim3(NUM_THREADS), MassShape<HD>::SMEM, stream, mq, mk, m);
     if (e != cudaSuccess) return llb_fail("span_mass_tcgen05: launch failed: %s", cudaGetErrorString(e));
     return llb_check_launch("span_mass_tcgen05");

@@ -58,7 +58,7 @@ class Requests:
         self.scale = self.hd ** -0.5
 
     def spans(self):
-        return i32(self.first), i32(self.rows), i32(self.held), i32(self.table).reshape(len(self.held), -1)
+        return i32(self.first), i32(self.rows), i32(self.held), i32(self.table).reshape(len(self.held), len(self.table[0]) if self.table else 1)
 
     def args(self):
         return (*self.spans(), self.page, self.hq, self.hkv, self.hd, self.scale)
@@ -560,3 +560,151 @@ def test_a_run_of_them(ops):
                     pos[:, slot(s, held[s] + d)] = ends[s] + d
                 held[s], ends[s] = held[s] + len(took), ends[s] + len(took)
             rows = [1, 1, 1]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (12, 2, 128)], ids=str)
+@pytest.mark.parametrize("page", [4, 24, 32, 128])
+def test_other_pages(ops, dtype, heads, page):
+    """Pages that a tile of keys holds a part of, one of, or no whole number of."""
+    held, rows = [0, 5, 131, 400, 23], [3, 1, 20, 7, 64]
+    r = Requests(held, rows, heads, dtype, page, 91)
+    mask = spread_mask(ops, r, trees(random.Random(6), rows))
+    check_rows(r, run_tree(ops, r, mask), tree_sees(r, mask))
+    mass_in = torch.rand((r.hkv, r.num_slots), generator=torch.Generator().manual_seed(92))
+    got, mass = run_mass(ops, r, mass_in)
+    check_mass(r, got, mass, mass_in, torch.full_like(mass_in, -5.0))
+    r = Requests(held, [1] * 5, heads, dtype, page, 93)
+    got, mass = run_mass(ops, r, None)
+    check_mass(r, got, mass, None, torch.full((r.hkv, r.num_slots), -5.0))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+def test_many_requests(ops, dtype):
+    """More requests than a warp has lanes, and more jobs than there are blocks."""
+    rng = random.Random(7)
+    held, rows = [rng.randrange(0, 90) for _ in range(333)], [rng.choice([0, 1, 1, 2, 5, 11]) for _ in range(333)]
+    r = Requests(held, rows, (14, 2, 64), dtype, 16, 94, gap=0)
+    mask = spread_mask(ops, r, trees(rng, rows))
+    check_rows(r, run_tree(ops, r, mask), tree_sees(r, mask))
+    for n in (rows, [1] * 333):
+        r = Requests(held, n, (14, 2, 64), dtype, 16, 95, gap=0)
+        got, mass = run_mass(ops, r, None)
+        check_mass(r, got, mass, None, torch.full((2, r.num_slots), -5.0))
+
+
+def test_nothing_to_do(ops):
+    for dtype in DTYPES:
+        r = Requests([7, 9], [0, 0], (4, 2, 64), dtype, 16, 96)
+        mask = torch.zeros((r.T, 1), dtype=torch.int64)
+        assert bool((run_tree(ops, r, mask) == 7.0).all())
+        got, mass = run_mass(ops, r, None, max_len=1)
+        assert bool((got == 7.0).all()) and bool((mass == -5.0).all())
+        got, mass = run_mass(ops, r, None, max_len=4)
+        assert bool((got == 7.0).all()) and bool((mass == -5.0).all())
+        r = Requests([], [], (4, 2, 64), dtype, 16, 97)
+        assert run_tree(ops, r, torch.zeros((r.T, 1), dtype=torch.int64)).shape[0] == r.T
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+def test_spans_beyond_their_tensors(ops, dtype):
+    """Lengths that the rows, the mask, max_len or the block table have no room for are cut to what there is."""
+    heads = (4, 2, 64)
+    r = Requests([20], [12], heads, dtype, 16, 98, gap=0)
+    mask = spread_mask(ops, r, trees(random.Random(1), r.rows))
+    want, sees = run_tree(ops, r, mask), tree_sees(r, mask)
+    r.rows = [4000]
+    assert torch.equal(run_tree(ops, r, mask), want)
+    r.rows, r.held = [12], [40]          # (two pages and one that is not there: 48 places)
+    got = run_tree(ops, r, mask)
+    assert bool((got[8:] == 7.0).all()) and bool((got[:8] != 7.0).any())
+    r.rows, r.held = [12], [20]
+    full, mass = run_mass(ops, r, None)
+    r2 = Requests([20], [12], heads, dtype, 16, 98, gap=0)
+    cut, mass_cut = run_mass(ops, r2, None, max_len=5)
+    assert bool((cut[5:] == 7.0).all()) and bool((cut[:5] != 7.0).any())
+    assert bool((mass_cut[:, r2.slots[0][25:]] == -5.0).all()) and bool((mass_cut[:, r2.slots[0][:25]] > 0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+def test_two_calls_at_once(ops, dtype):
+    """Calls on two streams, and on another stream than the current one was, have scratch of their own."""
+    rs = [Requests([900, 33], [20, 5], (12, 2, 128), dtype, 16, 101), Requests([1500, 77], [9, 40], (12, 2, 128), dtype, 16, 102)]
+    masks = [spread_mask(ops, r, trees(random.Random(2), r.rows)) for r in rs]
+    want = [run_tree(ops, r, m) for r, m in zip(rs, masks)]
+    want_mass = [run_mass(ops, r, None) for r in rs]
+    streams = [torch.cuda.Stream() for _ in rs]
+    on = [[x.to(dev()) for x in (r.q.reshape(r.T, -1), r.k, r.v, m)] for r, m in zip(rs, masks)]
+    args = [r.args() for r in rs]
+    outs = [[torch.full((r.T, r.hq * r.hd), 7.0, dtype=dtype, device=dev()) for _ in range(2)] for r in rs]
+    sums = [torch.full((r.hkv, r.num_slots), -5.0, device=dev()) for r in rs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                q, k, v, m = on[i]
+                ops.tree_attention(q, k, v, outs[i][0], m, *args[i])
+                ops.paged_attention_mass(q, k, v, outs[i][1], sums[i], *args[i], max(rs[i].rows))
+    torch.cuda.synchronize()
+    ops.check_async_errors(dev())
+    for i, r in enumerate(rs):
+        assert torch.equal(outs[i][0].cpu().reshape(want[i].shape), want[i])
+        assert torch.equal(outs[i][1].cpu().reshape(want[i].shape), want_mass[i][0]) and torch.equal(sums[i].cpu(), want_mass[i][1])
+
+
+def test_one_request_twice(ops):
+    """Requests that share their pages, as two drafts of one sequence do: reading is no matter."""
+    r = Requests([300, 300], [9, 9], (14, 2, 64), torch.bfloat16, 16, 103)
+    r.table[1], r.slots[1] = r.table[0], r.slots[0]
+    rng = random.Random(3)
+    mask = spread_mask(ops, r, trees(rng, r.rows))
+    check_rows(r, run_tree(ops, r, mask), tree_sees(r, mask))
+
+
+def test_strided_tensors_are_refused(ops):
+    r = Requests([30], [4], (4, 2, 64), torch.bfloat16, 16, 104, gap=0)
+    q, k, v = (x.to(dev()) for x in (r.q.reshape(4, -1), r.k, r.v))
+    mask = ops.tree_mask([[-1, 0, 0, 1]]).to(dev())
+    out = torch.empty((8, 256), dtype=torch.bfloat16, device=dev())[::2]
+    with pytest.raises(ops.KernelError, match="contiguous"):
+        ops.tree_attention(q, k, v, out, mask, *r.args())
+    with pytest.raises(ops.KernelError, match="contiguous"):
+        ops.cache_evict(k, v, torch.zeros((r.num_slots, 2), device=dev()).t(), torch.zeros((2, r.num_slots), dtype=torch.int32, device=dev()), i32([34]), i32([34]),
+                        r.spans()[3], 16, 8, 0, 0)
+    with pytest.raises(ops.KernelError, match="query heads a kv head"):
+        ops.tree_attention(torch.zeros((4, 65 * 16), device=dev()), torch.zeros((r.num_slots, 1, 16), device=dev()), torch.zeros((r.num_slots, 1, 16), device=dev()),
+                           torch.zeros((4, 65 * 16), device=dev()), mask, *r.spans(), 16, 65, 1, 16, 1.0)
+    with pytest.raises(ops.KernelError, match="head size 260"):
+        ops.tree_attention(torch.zeros((4, 260), device=dev()), torch.zeros((r.num_slots, 1, 260), device=dev()), torch.zeros((r.num_slots, 1, 260), device=dev()),
+                           torch.zeros((4, 260), device=dev()), mask, *r.spans(), 16, 1, 1, 260, 1.0)
+
+
+def test_caches_of_more_than_2_to_the_31_numbers(ops):
+    """Pages at the end of planes whose offsets pass 32 bits."""
+    hq, hkv, hd, page, dtype = 16, 8, 128, 16, torch.bfloat16
+    r = Requests([300, 40], [9, 1], (hq, hkv, hd), dtype, page, 105)
+    slots = (1 << 21) + (1 << 14)          # 2.2e9 numbers a plane
+    move = slots // page - r.num_slots // page
+    k, v = (torch.empty((slots, hkv, hd), dtype=dtype, device=dev()) for _ in range(2))
+    k[-r.num_slots:], v[-r.num_slots:] = r.k.to(dev()), r.v.to(dev())
+    table = i32([[p + move if p >= 0 else -1 for p in row] for row in r.table])
+    args = (*r.spans()[:3], table, page, hq, hkv, hd, r.scale)
+    q, out = r.q.reshape(r.T, -1).to(dev()), torch.full((r.T, hq * hd), 7.0, dtype=dtype, device=dev())
+    parents = trees(random.Random(4), r.rows)
+    mask = spread_mask(ops, r, parents)
+    ops.tree_attention(q, k, v, out, mask.to(dev()), *args)
+    check_rows(r, out.cpu().reshape(r.T, hq, hd), tree_sees(r, mask))
+    mass, out = torch.full((hkv, slots), -5.0, device=dev()), torch.full_like(out, 7.0)
+    ops.paged_attention_mass(q, k, v, out, mass, *args, 9)
+    check_mass(r, out.cpu().reshape(r.T, hq, hd), mass[:, -r.num_slots:].cpu(), None, torch.full((hkv, r.num_slots), -5.0))
+    held, ends = [309, 41], [400, 41]
+    pos = torch.arange(slots, dtype=torch.int32, device=dev()).expand(hkv, slots).contiguous() % 300
+    kr, vr, mr, pr = k[-r.num_slots:].cpu(), v[-r.num_slots:].cpu(), mass[:, -r.num_slots:].cpu(), pos[:, -r.num_slots:].cpu()
+    ops.cache_evict(k, v, mass, pos, i32(held), i32(ends), table, page, 100, 4, 20)
+    for h in range(hkv):
+        for s, n in enumerate(held):
+            at = r.slots[s][:n]
+            for a, b in P.evict(mr[h, at].tolist(), pr[h, at].tolist(), ends[s], 100, 4, 20):
+                for c in (kr, vr):
+                    c[at[a], h] = c[at[b], h].clone()
+    assert torch.equal(k[-r.num_slots:].cpu().nan_to_num(9.0), kr.nan_to_num(9.0)) and torch.equal(v[-r.num_slots:].cpu().nan_to_num(9.0), vr.nan_to_num(9.0))
