@@ -5,6 +5,10 @@
 
 namespace {
 
+// The kernel before has completed.  The next one is not let in early, as other kernels of the library do: these move keys that are not new,
+// and decode attention reads such keys before it waits.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // The cache row of a place of a request, or -1 for a page that is none of the cache's: such a place is neither read nor written.
 __device__ __forceinline__ int slot_of(const int* table, int page_size, int num_slots, int place) {
     const int page = table[place / page_size];
@@ -46,7 +50,7 @@ __global__ void __launch_bounds__(COMMIT_THREADS) tree_commit_kernel(const Commi
     __shared__ int path_s[COMMIT_MAX_PATH];
     __shared__ int slot_s[2][COMMIT_MAX_PATH];
     __shared__ int count_s;
-    llb_after_previous();
+    after_previous();
     const int s = blockIdx.x, lane = threadIdx.x & 31;
     const int row = p.span_row[s], pos = max(p.span_pos[s], 0);
     int n = min(min(p.span_len[s], p.T - row), p.max_pages * p.page_size - pos);
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(EV_THREADS, PER <= 8 ? 3 : 1) cache_evict_kern
     __shared__ unsigned warp_s[EV_WARPS][2], word_s[WORDS];
     __shared__ unsigned long long least_s[EV_WARPS];
     __shared__ unsigned found_s[3], total_s;
-    llb_after_previous();
+    after_previous();
     const int s = blockIdx.x / p.Hkv, h = blockIdx.x - s * p.Hkv, layer = blockIdx.y;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int n = max(0, min(p.lengths[s], p.max_pages * p.page_size)), budget = p.budget;
@@ -401,7 +405,7 @@ __global__ void __launch_bounds__(EV_THREADS) cache_evict_any_kernel(const Evict
     __shared__ unsigned list_s[2][EV_LIST];
     __shared__ unsigned warp_s[EV_WARPS][2];
     __shared__ unsigned found_s[3];
-    llb_after_previous();
+    after_previous();
     const int s = blockIdx.x / p.Hkv, h = blockIdx.x - s * p.Hkv, layer = blockIdx.y;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int n = max(0, min(p.lengths[s], p.max_pages * p.page_size)), budget = p.budget;
