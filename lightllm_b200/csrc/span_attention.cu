@@ -587,8 +587,6 @@ int check(const LlbSpanArgs& a, int dtype) {
     LLB_REQUIRE(a.hd > 0 && a.hd <= 256, "span_attention: head size %d, up to 256 are supported", a.hd);
     LLB_REQUIRE(a.S >= 0 && a.T >= 0 && a.page_size > 0 && a.max_pages >= 0 && a.num_slots > 0 && (long long)a.max_pages * a.page_size <= (1 << 30),
                 "span_attention: bad sizes");
-    LLB_REQUIRE(((long long)a.T / max(1, 64 / a.group) + a.S) * a.Hkv * (((long long)a.max_pages * a.page_size + KT - 1) / KT + 3) < (1ll << 31),
-                "span_attention: %d rows over up to %d keys a request are more tiles than one call takes", a.T, a.max_pages * a.page_size);
     return 0;
 }
 
@@ -623,6 +621,10 @@ int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtyp
     const Layout l = layout(a.T, a.S, a.Hq, a.group, a.hd, a.num_slots, rows, blocks, tc ? 128 : KT, a.extra, mass);
     a.rows = rows;
     a.nodes = rows / a.group;
+    // (an int numbers the tiles, whatever the lengths on the device say)
+    const long long most = min(a.T, a.max_len), keys = (long long)a.max_pages * a.page_size, each = tc ? 128 : KT;
+    LLB_REQUIRE(((most + a.nodes - 1) / a.nodes) * a.S * a.Hkv * ((keys + each - 1) / each + a.extra) < (1ll << 31),
+                "span_attention: %d requests of up to %lld rows over up to %lld keys are more tiles than one call takes", a.S, most, keys);
     a.part_o = scratch + l.part_o;
     a.part_ml = scratch + l.part_ml;
     a.open = (int*)(scratch + l.open);
