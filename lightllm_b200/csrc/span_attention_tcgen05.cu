@@ -890,19 +890,21 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 for (int c = 0; c < 4; ++c) {
                     tmem_wait_ld32(s[c & 1]);
                     if (c < 3) tmem_ld32_nowait(tmem + 32 * (c + 1), *reinterpret_cast<uint32_t(*)[32]>(&s[(c + 1) & 1][0]));
-                    if (!interior) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) s[c & 1][i] = 32 * c + i >= least && 32 * c + i < upto ? s[c & 1][i] : -INFINITY;
-                    }
+                    float* v = s[c & 1];
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         const float4 e = *reinterpret_cast<const float4*>(lse_t + 32 * c + i);
-                        const float* v = &s[c & 1][i];
-                        float p0, p1, p2, p3;
-                        unpack2(fma2(pack2(v[0], v[1]), scale2, pack2(e.x, e.y)), p0, p1);
-                        unpack2(fma2(pack2(v[2], v[3]), scale2, pack2(e.z, e.w)), p2, p3);
-                        sum0 = add2(sum0, pack2(fast_exp2(p0), fast_exp2(p1)));
-                        sum1 = add2(sum1, pack2(fast_exp2(p2), fast_exp2(p3)));
+                        unpack2(fma2(pack2(v[i], v[i + 1]), scale2, pack2(e.x, e.y)), v[i], v[i + 1]);
+                        unpack2(fma2(pack2(v[i + 2], v[i + 3]), scale2, pack2(e.z, e.w)), v[i + 2], v[i + 3]);
+                    }
+                    if (!interior) {          // (behind the lse: that of a row which is NaN is nothing to keys that the row does not see)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = 32 * c + i >= least && 32 * c + i < upto ? v[i] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        sum0 = add2(sum0, pack2(fast_exp2(v[i]), fast_exp2(v[i + 1])));
+                        sum1 = add2(sum1, pack2(fast_exp2(v[i + 2]), fast_exp2(v[i + 3])));
                     }
                 }
                 tc_fence_before();

@@ -21,7 +21,7 @@ def attention(q, k, v, sees, scale):
     q, k, v = q.double(), k.double(), v.double()
     Hq, Hkv = q.shape[1], k.shape[1]
     out, weights = torch.zeros_like(q), torch.zeros((Hq, q.shape[0], k.shape[0]), dtype=torch.float64)
-    if bool(k.isfinite().all()) and bool(v.isfinite().all()):          # all rows at once
+    if all(bool(x.isfinite().all()) for x in (q, k, v)):          # all rows at once
         kk, vv = (x.repeat_interleave(Hq // Hkv, 1).transpose(0, 1) for x in (k, v))
         x = torch.where(sees, q.transpose(0, 1) @ kk.transpose(1, 2) * scale, -math.inf)
         weights = torch.where(sees.any(1)[:, None], torch.softmax(x, -1), 0.0)

@@ -708,3 +708,30 @@ def test_caches_of_more_than_2_to_the_31_numbers(ops):
                 for c in (kr, vr):
                     c[at[a], h] = c[at[b], h].clone()
     assert torch.equal(k[-r.num_slots:].cpu().nan_to_num(9.0), kr.nan_to_num(9.0)) and torch.equal(v[-r.num_slots:].cpu().nan_to_num(9.0), vr.nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (12, 2, 128), (3, 1, 32)], ids=str)
+@pytest.mark.parametrize("what", ["query", "key"])
+def test_weights_beside_a_row_of_nan(ops, dtype, heads, what):
+    """A row whose scores are no numbers gives none to the keys that it sees, and leaves the other keys alone."""
+    held, n, at = 90, 150, 77
+    r = Requests([held, 20], [n, 3], heads, dtype, 16, 111)
+    if what == "query":
+        r.q[r.first[0] + at, 0] = math.nan
+    else:
+        r.k[r.slots[0][held + at], 0] = math.nan          # seen by the rows from its own on
+    got, mass = run_mass(ops, r, None)
+    for s in range(2):
+        q, k, v = r.of(s)
+        sees = torch.cat([torch.ones((r.rows[s], r.held[s]), dtype=torch.bool), torch.ones((r.rows[s],) * 2, dtype=torch.bool).tril()], 1)
+        out, w = P.attention(q, k, v, sees, r.scale)
+        sums = w.reshape(r.hkv, -1, w.shape[-1]).sum(1)
+        have = mass[:, r.slots[s]].double()
+        assert torch.equal(have.isnan(), sums.isnan()) and bool(have.isnan().any()) == (s == 0)
+        fine = ~sums.isnan()
+        # (the bound of the tests above, with the rows' number for the terms of a sum)
+        rel = 2 * P.score_error(q, k, r.scale) + (r.rows[s] * r.hq // r.hkv + len(r.slots[s]) + 16) * 2.0 ** -24 + 2.0 ** -20
+        assert bool(((have - sums).abs()[fine] <= rel * sums[fine]).all())
+        rows = got[r.first[s]:r.first[s] + r.rows[s]].double()
+        assert torch.equal(rows.isnan(), out.isnan())
