@@ -45,14 +45,6 @@ struct SimtParams {
     const void* v;
 };
 
-// Whether row `node` of the request sees key `key` (of those below the request's end).
-__device__ __forceinline__ bool sees(const LlbSpanArgs& a, const LlbSpan& z, int node, int key) {
-    const int j = key - z.pos;
-    if (j < 0) return true;
-    if (!a.mask) return j <= node;
-    return (a.mask[(size_t)(z.row + node) * a.words + (j >> 6)] >> (j & 63)) & 1ull;
-}
-
 template <typename T, int RB, int NI>
 __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParams p) {
     constexpr int RG = RB / 4, CT = THREADS / RG;      // groups of four rows; threads that share a group's columns
@@ -102,6 +94,16 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int d = 0; d < DPT; ++d) o[i][d] = 0.0f;
+        // the first so many keys each of the thread's rows sees (-1: it is none of the job's), and where its mask for the others begins
+        const unsigned long long* bits = a.mask;
+        int own[4];
+        size_t mask_at[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = ty * 4 + i, node = job.first + r / a.group;
+            own[i] = r >= rows ? -1 : bits ? job.z.pos : job.z.pos + node + 1;
+            mask_at[i] = (size_t)(job.z.row + node) * a.words;
+        }
         for (int kt = k0; kt < k1; ++kt) {
             const int key0 = kt * KT;
             __syncthreads();                           // the tile before has been read
@@ -120,35 +122,33 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
             }
             __syncthreads();
             // scores: four rows by KPT keys (CT apart, so that neighbouring threads read neighbouring rows of K)
-            float x[4][KPT];
+            unsigned long long x[4][KPT];          // sums of even and of odd dimensions
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < KPT; ++j) x[i][j] = 0.0f;
+                for (int j = 0; j < KPT; ++j) x[i][j] = 0ull;
             for (int d = 0; d < hd4; d += 4) {
-                float4 qv[4], kv[KPT];
+                ulonglong2 qv[4], kv[KPT];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(q_s + (ty * 4 + i) * hd4 + d);
+                for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const ulonglong2*>(q_s + (ty * 4 + i) * hd4 + d);
 #pragma unroll
-                for (int j = 0; j < KPT; ++j) kv[j] = *reinterpret_cast<const float4*>(k_s + (tx + CT * j) * kp + d);
+                for (int j = 0; j < KPT; ++j) kv[j] = *reinterpret_cast<const ulonglong2*>(k_s + (tx + CT * j) * kp + d);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < KPT; ++j) {
-                        x[i][j] = fmaf(qv[i].x, kv[j].x, x[i][j]);
-                        x[i][j] = fmaf(qv[i].y, kv[j].y, x[i][j]);
-                        x[i][j] = fmaf(qv[i].z, kv[j].z, x[i][j]);
-                        x[i][j] = fmaf(qv[i].w, kv[j].w, x[i][j]);
-                    }
+                    for (int j = 0; j < KPT; ++j) x[i][j] = llb_fma2(qv[i].y, kv[j].y, llb_fma2(qv[i].x, kv[j].x, x[i][j]));
             }
             const bool inner = key0 + KT <= job.z.pos;          // every row sees the whole tile
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < KPT; ++j) {
-                    const int r = ty * 4 + i, key = key0 + tx + CT * j;
-                    const bool on = r < rows && key < job.keys && (inner || sees(a, job.z, job.first + r / a.group, key));
-                    s_s[r * SP + tx + CT * j] = on ? x[i][j] * a.scale_log2e : -INFINITY;
+                    const int key = key0 + tx + CT * j;
+                    bool on = key < own[i];
+                    if (!inner && bits && own[i] > -1 && !on && key < job.keys) on = (bits[mask_at[i] + ((key - job.z.pos) >> 6)] >> ((key - job.z.pos) & 63)) & 1ull;
+                    float lo, hi;
+                    llb_unpack2(x[i][j], lo, hi);
+                    s_s[(ty * 4 + i) * SP + tx + CT * j] = on ? (lo + hi) * a.scale_log2e : -INFINITY;
                 }
             // values of keys that some rows do not see: what is no finite number there must not reach those rows (0 * inf)
             if (!inner)
@@ -211,6 +211,14 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
                         for (int i = 0; i < 4; ++i)
 #pragma unroll
                             for (int d = 0; d < DPT; ++d) o[i][d] = pr[i][e] == 0.0f ? o[i][d] : fmaf(pr[i][e], vv[d], o[i][d]);
+                    } else if (DPT % 2 == 0) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const unsigned long long pp = llb_pack2(pr[i][e], pr[i][e]);
+#pragma unroll
+                            for (int d = 0; d + 1 < DPT; d += 2)
+                                llb_unpack2(llb_fma2(pp, llb_pack2(vv[d], vv[d + 1]), llb_pack2(o[i][d], o[i][d + 1])), o[i][d], o[i][d + 1]);
+                        }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
@@ -230,12 +238,27 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
             float* po = a.part_o + (size_t)(blockIdx.x * 2 + max(part, 0)) * (hd4 / 4) * a.rows * 4;
             const float inv = llb_inverse(m, l, job.z.pos);
             T* dst = (T*)a.out + ((size_t)row * a.Hq + head) * hd;
+            if (RB == 64 && hd % 4 == 0 && (sizeof(T) == 4 ? ((uintptr_t)a.out & 15) == 0 : ((uintptr_t)a.out & 7) == 0)) {
 #pragma unroll
-            for (int d = 0; d < DPT; ++d) {
-                const int dim = RB == 64 ? (d >> 2) * 64 + tx * 4 + (d & 3) : d * 64 + tx;
-                if (dim >= hd) continue;
-                if (part >= 0) po[((size_t)(dim >> 2) * a.rows + r) * 4 + (dim & 3)] = o[i][d];
-                else dst[dim] = llb_from_float<T>(o[i][d] * inv);
+                for (int n = 0; n < NI; ++n) {
+                    const int dim = n * 64 + tx * 4;
+                    if (dim >= hd) continue;
+                    const float* v = o[i] + (RB == 64 ? 4 * n : 0);
+                    if (part >= 0) *reinterpret_cast<float4*>(po + ((size_t)(dim >> 2) * a.rows + r) * 4) = make_float4(v[0], v[1], v[2], v[3]);
+                    else if (sizeof(T) == 4) *reinterpret_cast<float4*>(dst + dim) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                    else {
+                        const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0] * inv, v[1] * inv), hi = __floats2bfloat162_rn(v[2] * inv, v[3] * inv);
+                        *reinterpret_cast<uint2*>(dst + dim) = make_uint2(*reinterpret_cast<const unsigned*>(&lo), *reinterpret_cast<const unsigned*>(&hi));
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int d = 0; d < DPT; ++d) {
+                    const int dim = RB == 64 ? (d >> 2) * 64 + tx * 4 + (d & 3) : d * 64 + tx;
+                    if (dim >= hd) continue;
+                    if (part >= 0) po[((size_t)(dim >> 2) * a.rows + r) * 4 + (dim & 3)] = o[i][d];
+                    else dst[dim] = llb_from_float<T>(o[i][d] * inv);
+                }
             }
             if (tx == 0) {
                 if (part >= 0) {
@@ -477,33 +500,32 @@ __global__ void __launch_bounds__(THREADS) span_mass_kernel(const ColumnParams p
             if (tid < RB)
                 lse_s[tid] = tid < pairs ? a.lse[(size_t)(z.row + node0 + tid / a.group) * a.Hq + job.kvh * a.group + tid % a.group] : INFINITY;
             __syncthreads();
-            float x[4][4];
+            unsigned long long x[4][4];          // sums of even and of odd dimensions
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[i][j] = 0.0f;
+                for (int j = 0; j < 4; ++j) x[i][j] = 0ull;
             for (int d = 0; d < hd4; d += 4) {
-                float4 qv[4], kv[4];
+                ulonglong2 qv[4], kv[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(q_s + (ty * 4 + i) * hd4 + d);
+                for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const ulonglong2*>(q_s + (ty * 4 + i) * hd4 + d);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * kp + d);
+                for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const ulonglong2*>(k_s + (tx + 16 * j) * kp + d);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        x[i][j] = fmaf(qv[i].x, kv[j].x, x[i][j]);
-                        x[i][j] = fmaf(qv[i].y, kv[j].y, x[i][j]);
-                        x[i][j] = fmaf(qv[i].z, kv[j].z, x[i][j]);
-                        x[i][j] = fmaf(qv[i].w, kv[j].w, x[i][j]);
-                    }
+                    for (int j = 0; j < 4; ++j) x[i][j] = llb_fma2(qv[i].y, kv[j].y, llb_fma2(qv[i].x, kv[j].x, x[i][j]));
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int last = z.pos + node0 + (ty * 4 + i) / a.group;          // the last key that the row sees
+                const int last = ty * 4 + i < pairs ? z.pos + node0 + (ty * 4 + i) / a.group : -1;          // the last key that the row sees
+                const float lse = lse_s[ty * 4 + i];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (ty * 4 + i < pairs && key0 + tx + 16 * j <= last) sum[j] += exp2f(x[i][j] * a.scale_log2e - lse_s[ty * 4 + i]);
+                for (int j = 0; j < 4; ++j) {
+                    float lo, hi;
+                    llb_unpack2(x[i][j], lo, hi);
+                    if (key0 + tx + 16 * j <= last) sum[j] += exp2f((lo + hi) * a.scale_log2e - lse);
+                }
             }
         }
 #pragma unroll
@@ -648,6 +670,7 @@ LlbSpanArgs span_args(const LlbSpanCall& s, int max_len) {
     LlbSpanArgs a = {};
     a.out = s.out; a.span_row = s.span_row; a.span_len = s.span_len; a.span_pos = s.span_pos; a.table = s.table;
     a.S = s.S; a.T = s.T; a.max_pages = s.max_pages; a.page_size = s.page_size; a.num_slots = s.num_slots; a.Hq = s.Hq; a.Hkv = s.Hkv; a.hd = s.hd;
+    a.page_shift = s.page_size > 0 && (s.page_size & (s.page_size - 1)) == 0 ? __builtin_ctz(s.page_size) : -1;
     a.group = s.Hkv > 0 ? s.Hq / s.Hkv : 0; a.scale_log2e = s.scale * 1.4426950408889634f; a.max_len = max_len;
     return a;
 }

@@ -42,6 +42,7 @@ struct LlbSpanArgs {
     const int* span_pos;
     const int* table;                // [S, max_pages]
     int S, T, max_pages, page_size, max_len, num_slots;
+    int page_shift;                  // log2 of the page size, or -1
     int Hq, Hkv, hd, group;
     const unsigned long long* mask;  // tree: [T, words]; null: causal
     int words;
@@ -79,9 +80,28 @@ __device__ __forceinline__ int llb_span_keys(const LlbSpanArgs& a, const LlbSpan
 }
 // The cache row of a key, or -1 for a page that is none of the cache's: such a key reads as zeros.
 __device__ __forceinline__ int llb_span_slot(const LlbSpanArgs& a, int s, int key) {
-    const int page = a.table[(size_t)s * a.max_pages + key / a.page_size];
-    const long long slot = (long long)page * a.page_size + key % a.page_size;
+    const int page_of = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+    const int page = a.table[(size_t)s * a.max_pages + page_of];
+    const long long slot = (long long)page * a.page_size + (key - page_of * a.page_size);
     return page >= 0 && slot < a.num_slots ? (int)slot : -1;
+}
+
+// Two floats in a 64-bit register: an instruction for both.
+__device__ __forceinline__ unsigned long long llb_pack2(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void llb_unpack2(unsigned long long v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ unsigned long long llb_fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long llb_add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 // A job and its tiles' place in the line of all tiles: begin .. begin + tiles - 1, then what it costs besides (no tile, and nothing to do for

@@ -134,24 +134,6 @@ struct RowMask {
 __device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 __device__ __forceinline__ bool bf16_odd(uint32_t pair) { return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u; }
 
-// Two floats in a 64-bit register: an instruction for both (the schedulers' slots are what the softmax shares with the warp that issues
-// the products).
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -181,8 +163,8 @@ template <typename SecondHalf>
 __device__ __forceinline__ void tile_probs(uint32_t tmem, float scale, float shift, uint32_t (&probs)[64], float& sum, float& top,
                                            const SecondHalf& second_half) {
     float t0 = -INFINITY, t1 = -INFINITY;
-    uint64_t l0 = 0, l1 = 0;
-    const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
+    unsigned long long l0 = 0, l1 = 0;          // (sums two by two: the schedulers' slots are shared with the warp that issues the products)
+    const unsigned long long scale2 = llb_pack2(scale, scale), shift2 = llb_pack2(shift, shift);
     float s[2][32];
     tmem_ld32_nowait(tmem, *reinterpret_cast<uint32_t(*)[32]>(&s[0][0]));
 #pragma unroll
@@ -199,20 +181,20 @@ __device__ __forceinline__ void tile_probs(uint32_t tmem, float scale, float shi
             t0 = max3(t0, v[0], v[1]);
             t1 = max3(t1, v[2], v[3]);
             float p0, p1, p2, p3;
-            unpack2(fma2(pack2(v[0], v[1]), scale2, shift2), p0, p1);
-            unpack2(fma2(pack2(v[2], v[3]), scale2, shift2), p2, p3);
+            llb_unpack2(llb_fma2(llb_pack2(v[0], v[1]), scale2, shift2), p0, p1);
+            llb_unpack2(llb_fma2(llb_pack2(v[2], v[3]), scale2, shift2), p2, p3);
             p0 = fast_exp2(p0);
             p1 = fast_exp2(p1);
             p2 = fast_exp2(p2);
             p3 = fast_exp2(p3);
-            l0 = add2(l0, pack2(p0, p1));
-            l1 = add2(l1, pack2(p2, p3));
+            l0 = llb_add2(l0, llb_pack2(p0, p1));
+            l1 = llb_add2(l1, llb_pack2(p2, p3));
             probs[16 * c + i / 2] = wm::pack_bf16(p0, p1);
             probs[16 * c + i / 2 + 1] = wm::pack_bf16(p2, p3);
         }
     }
     float a, b;
-    unpack2(add2(l0, l1), a, b);
+    llb_unpack2(llb_add2(l0, l1), a, b);
     sum = a + b;
     top = fmaxf(t0, t1);
 }
@@ -855,7 +837,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const int u0 = t - job.begin, u1 = min(job.units, pc.t1 - job.begin), n = u1 - u0;
             const LlbSpan z = job.z;
             const int key = job.tile * BK + r;
-            uint64_t sum0 = 0, sum1 = 0;
+            unsigned long long sum0 = 0, sum1 = 0;
             // minus the lse of four pairs of a tile, minus infinity where there is none
             auto lse_of = [&](int j) -> float4 {
                 const int node0 = (job.from + u0 + j) * pairs_nodes, left = j < n ? z.len - node0 : 0;
@@ -865,7 +847,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 for (int e = 0; e < 4; ++e) v[e] = lse_node[e] < left ? -from[lse_at[e]] : -INFINITY;
                 return make_float4(v[0], v[1], v[2], v[3]);
             };
-            const uint64_t scale2 = pack2(a.scale_log2e, a.scale_log2e);
+            const unsigned long long scale2 = llb_pack2(a.scale_log2e, a.scale_log2e);
             const int first = (int)((x - units_before) & 1);          // the group's first tile of the job
             float4 lse = lse_of(first);
 #pragma unroll 1
@@ -894,8 +876,8 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         const float4 e = *reinterpret_cast<const float4*>(lse_t + 32 * c + i);
-                        unpack2(fma2(pack2(v[i], v[i + 1]), scale2, pack2(e.x, e.y)), v[i], v[i + 1]);
-                        unpack2(fma2(pack2(v[i + 2], v[i + 3]), scale2, pack2(e.z, e.w)), v[i + 2], v[i + 3]);
+                        llb_unpack2(llb_fma2(llb_pack2(v[i], v[i + 1]), scale2, llb_pack2(e.x, e.y)), v[i], v[i + 1]);
+                        llb_unpack2(llb_fma2(llb_pack2(v[i + 2], v[i + 3]), scale2, llb_pack2(e.z, e.w)), v[i + 2], v[i + 3]);
                     }
                     if (!interior) {          // (behind the lse: that of a row which is NaN is nothing to keys that the row does not see)
 #pragma unroll
@@ -903,8 +885,8 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
-                        sum0 = add2(sum0, pack2(fast_exp2(v[i]), fast_exp2(v[i + 1])));
-                        sum1 = add2(sum1, pack2(fast_exp2(v[i + 2]), fast_exp2(v[i + 3])));
+                        sum0 = llb_add2(sum0, llb_pack2(fast_exp2(v[i]), fast_exp2(v[i + 1])));
+                        sum1 = llb_add2(sum1, llb_pack2(fast_exp2(v[i + 2]), fast_exp2(v[i + 3])));
                     }
                 }
                 tc_fence_before();
@@ -912,7 +894,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (lane == 0) mbar_arrive(&bar_free[place]);
             }
             float sum, sum_b;
-            unpack2(add2(sum0, sum1), sum, sum_b);
+            llb_unpack2(llb_add2(sum0, sum1), sum, sum_b);
             sum += sum_b;
             if (x == 1) sum_s[r] = sum;
             named_barrier(BAR_PAIR, 256);
