@@ -598,7 +598,9 @@ int llb_span_join(const LlbSpanArgs& a, int dtype, int blocks, int tile, int lea
 
 namespace {
 
-// (row, head) pairs a job of the CUDA-core kernel holds: 16 where requests bring about that many or fewer on average.
+// (row, head) pairs a job of the CUDA-core kernel holds: 16 where requests bring that many or fewer on average.  (float32, 14/2 heads of 64, 5
+// requests of 77 to 1,103 keys, us with 16 | 64: a row each 15 | 20, two 15.4 | 20.5, four 18.5 | 21.5, eight 25 | 22, 64 rows 103 | 48;
+// 27 requests: two 26 | 31, four 37 | 33.)
 int simt_rows(int T, int S, int group) { return group <= 16 && (long long)T * group <= 16ll * S ? 16 : 64; }
 int simt_blocks() { return min(2 * llb_device_sms(), LLB_SPAN_BLOCKS); }
 int tc_blocks() { return min(llb_device_sms(), LLB_SPAN_BLOCKS); }
@@ -612,7 +614,8 @@ int check(const LlbSpanArgs& a, int dtype) {
     return 0;
 }
 
-// Whether the tensor-core kernels take these sizes (they may still pass a call on, see llb_span_tc_takes).
+// Whether the tensor-core kernels take these sizes (they may still pass a call on, see llb_span_tc_takes).  Where they can they do: 2 rows behind
+// 60 keys 9.3 us instead of 11.1 on the CUDA cores, 8 behind 2,048 12.4 instead of 20.7, 27 trees of up to 26 rows 33 instead of 270.
 bool tc_sizes(int dtype, int hd, int page_size) {
     return dtype == LLB_BF16 && (hd == 64 || hd == 128) && page_size % 8 == 0 && page_size <= 128 && 128 % page_size == 0;
 }

@@ -33,7 +33,9 @@ struct LlbSharedMemory {
 constexpr int LLB_SPAN_BLOCKS = 512;          // blocks of a kernel at most
 constexpr int LLB_SPAN_TC_LEAST = 2;          // tiles a block of the tensor-core kernel has at least: one for each of its groups
 // What beginning and ending a job costs a block, in tiles: every job is so much longer in the line, or blocks with several short jobs would be the
-// last ones (27 trees of 65 to 4,001 keys: 39 -> 33 us).
+// last ones (tensor cores, 27 trees of up to 26 rows behind 65 to 4,001 keys, 12/2 heads of 128: 45 us with nothing, 39 with one tile, 33 with 3
+// or 5; 64 trees behind 30 to 300 keys, 28/4 heads: 38.5, 38, 37 with 3, 41 with 5.  CUDA cores, 5 trees of 64 rows: 51 with nothing, 48 with
+// one, 53 with 3).
 constexpr int LLB_SPAN_TC_EXTRA = 3, LLB_SPAN_EXTRA = 1;
 
 struct LlbSpanArgs {
