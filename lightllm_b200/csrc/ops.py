@@ -1393,7 +1393,7 @@ def _check_table(what: str, S: int, block_table, page_size: int) -> int:
     shape = block_table.shape
     if block_table.dtype is not _INT32 or len(shape) != 2 or shape[0] != S:
         raise KernelError(f"{what}: block_table must be int32 [{S}, pages], got {block_table.dtype} {tuple(shape)}")
-    if page_size <= 0:
+    if not 0 < page_size <= 1 << 30:
         raise KernelError(f"{what}: page size {page_size}")
     return shape[1]
 
@@ -1406,6 +1406,8 @@ def _check_span_attention(what, q, k_cache, v_cache, out, num_heads, num_kv_head
     if shape.numel() != shape[0] * num_heads * head_dim or out.shape != shape or out.dtype is not dtype:
         raise KernelError(f"{what}: q and out are [T, {num_heads * head_dim}] of one dtype, got {tuple(shape)} {dtype}, "
                           f"{tuple(out.shape)} {out.dtype}")
+    if abs(q.data_ptr() - out.data_ptr()) < q.nbytes:          # (several blocks read a row of q, and not at once)
+        raise KernelError(f"{what}: out must not lie over q")
     if (k_cache.dtype is not dtype or v_cache.dtype is not dtype or v_cache.shape != cache or len(cache) != 3
             or cache[1] != num_kv_heads or cache[2] != head_dim):
         raise KernelError(f"{what}: the caches are {dtype} [slots, {num_kv_heads}, {head_dim}], got {k_cache.dtype} "
@@ -1486,7 +1488,7 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
 
     for every key of the requests that bring rows (:func:`cache_evict` goes by these sums).  ``mass_in`` may be ``mass`` itself
     (sums go on from step to step; a new key starts from zero whatever an earlier owner left in its slot) or ``None`` (all start
-    from zero).  ``mass`` float32 [kv heads, slots].  ``max_len``: the most rows that a request brings (longer ones
+    from zero).  ``mass`` float32 [kv heads, slots].  No two requests share a page: a key's sum belongs to one request.  ``max_len``: the most rows that a request brings (longer ones
     are cut to it); 1 takes the form for single tokens, which reads every key once.  The other arguments as
     :func:`tree_attention`.  Sums are made in one order: equal calls give equal bits."""
     T, slots = _check_span_attention("paged_attention_mass", q, k_cache, v_cache, out, num_heads, num_kv_heads, head_dim)
@@ -1500,6 +1502,7 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
             raise KernelError(f"paged_attention_mass: weights are float32 [{num_kv_heads}, {slots}], got {t.dtype} {tuple(t.shape)}")
     if max_len <= 0:
         raise KernelError(f"paged_attention_mass: max_len is {max_len}")
+    max_len = max(1, min(max_len, T))
     device = _check_here("paged_attention_mass", q, k_cache, v_cache, out, mass, mass_in, span_row, span_len, span_pos, block_table)
     stream = _stream_on(device)
     scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, slots, 2 if max_len == 1 else 1, device),
@@ -1563,7 +1566,7 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor
     equal ones the lowest place (NaN counts as the largest).  The i-th place below the budget that does not stay takes the key, value, mass and
     position of the i-th place beyond it that does; all others stay where they are.  So the order of the places says nothing of the
     keys' positions afterwards: for attention that does not go by it (no window, no bias by distance).  A request then holds
-    ``min(lengths[s], budget)`` places; one of no more than the budget is left as it is.
+    ``min(lengths[s], budget)`` places; one of no more than the budget is left as it is.  No two requests share a page.
 
     Caches [slots, kv heads, head_dim] or [layers, ...]; mass float32 and positions int32 [kv heads, slots] or [layers, ...];
     lengths, ends int32 [requests].  ``mass_out`` and ``positions_out`` (both or neither): planes that receive the mass and position
@@ -1585,6 +1588,8 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor
             raise KernelError(f"cache_evict: mass is float32 and positions int32 {shape}, got {t.dtype} {tuple(t.shape)}")
     if budget <= 0 or first < 0 or latest < 0 or first + latest > budget:
         raise KernelError(f"cache_evict: a budget of {budget} places does not hold the first {first} and the latest {latest}")
+    if budget >= 1 << 31:
+        raise KernelError(f"cache_evict: a budget of {budget} places; places are numbered in 32 bits")
     device = _check_here("cache_evict", k_cache, v_cache, mass, positions, lengths, ends, block_table, mass_out, positions_out)
     _check(lib().llb_cache_evict(_CACHE_EVICT(
         k_cache.data_ptr(), v_cache.data_ptr(), mass.data_ptr(), positions.data_ptr(), mass_out.data_ptr(), positions_out.data_ptr(),

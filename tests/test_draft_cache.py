@@ -74,6 +74,29 @@ def test_shared_planes_are_refused():
         ops.cache_evict(*evict_args(k=k, v=k))
 
 
+@pytest.mark.parametrize("call,args", [(ops.tree_attention, tree_args), (ops.paged_attention_mass, mass_args)])
+def test_results_over_the_queries_are_refused(call, args):
+    """Blocks read a job's queries at different times, some of them when others have written its results."""
+    both = torch.zeros(7, 64)
+    for q, out in ((both[:6], both[:6]), (both[:6], both[1:]), (both[1:], both[:6])):
+        with pytest.raises(ops.KernelError, match="must not lie over q"):
+            call(*args(q=q, out=out))
+    twice = torch.zeros(12, 64)
+    with pytest.raises(ops.KernelError, match="no CPU path"):          # side by side is fine
+        call(*args(q=twice[:6], out=twice[6:]))
+
+
+@pytest.mark.parametrize("call,args,word", [
+    (ops.tree_attention, tree_args(page=1 << 40), "page size"), (ops.paged_attention_mass, mass_args(page=1 << 40), "page size"),
+    (ops.tree_commit, commit_args(page=1 << 40), "page size"), (ops.cache_evict, evict_args(page=1 << 40), "page size"),
+    (ops.cache_evict, evict_args(budget=1 << 40), "32 bits"), (ops.paged_attention_mass, mass_args(max_len=1 << 40), "no CPU path"),
+])
+def test_numbers_of_more_than_32_bits(call, args, word):
+    """No count is cut to 32 bits: it is refused, or (rows a request) means no more than the rows that there are."""
+    with pytest.raises(ops.KernelError, match=word):
+        call(*args)
+
+
 def test_tree_masks():
     trees = [[-1], [-1, 0, 0, 1, 3], [], [-1] + list(range(129))]
     mask = ops.tree_mask(trees)
