@@ -2,6 +2,7 @@
 // Both work on all layers of a group of planes at once: keys and values [layers, slots, kv heads, head size].
 #include "cache_calls.h"
 #include "common.cuh"
+#include "tcgen05_common.cuh"
 
 namespace {
 
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(COMMIT_THREADS) tree_commit_kernel(const Commi
 // order) take the keys, values, weights and positions of those that stay beyond it (in rising order).  Attention does not ask for
 // the order of its keys (they carry their rotation), so nothing else moves: as many rows as there are holes instead of nearly all.
 //
-// A block takes one (layer, request, kv head).  A thread has up to 8 or 32 places, all asked for at once (what a block's time is made of is
+// A block takes one (layer, request, kv head), or as many as fill the device share its moves.  A thread has up to 8 or 32 places, all asked for at once (what a block's time is made of is
 // trips to memory, 0.6 us each): their cache rows and their worth as whole numbers in the floats' order stay in registers.  The
 // budget's threshold is found digit by digit from the top, 11, 11 and 10 bits, by counting, the dropping of a single place by one search for
 // the least.  The places that stay become a bit each, which gives holes and fillers their numbers by counting bits; the moves
@@ -144,6 +145,7 @@ struct EvictParams {
     int S, max_pages, page_size, num_slots, Hkv, budget, first, latest;
     int head_units;                       // of one head's row of K (or V), in units of the copies
     int cache_places;                     // as many worths as shared memory holds
+    int parts;                            // blocks that share the moves of one (layer, request, kv head), a power of two
 };
 
 __device__ __forceinline__ unsigned order_of(float f) {
@@ -152,14 +154,14 @@ __device__ __forceinline__ unsigned order_of(float f) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// The listed moves of one (layer, kv head): rows of K and V, 16 bytes a thread and AHEAD of them on their way, then weights and positions.
+// The listed moves begin .. end - 1 of one (layer, kv head): rows of K and V, 16 bytes a thread and AHEAD of them on their way, then weights and positions.
 template <typename U>
-__device__ __forceinline__ void move_rows(const EvictParams& p, size_t plane, int layer, int h, const unsigned (&list)[2][EV_LIST], unsigned count) {
+__device__ __forceinline__ void move_rows(const EvictParams& p, size_t plane, int layer, int h, const unsigned (&list)[2][EV_LIST], unsigned begin, unsigned end) {
     constexpr int AHEAD = 4;
-    const unsigned units = 2 * p.head_units, total = count * units;
+    const unsigned units = 2 * p.head_units, total = end * units;
     const size_t stride = (size_t)p.Hkv * p.head_units, base = (size_t)layer * p.num_slots * stride + (size_t)h * p.head_units;
     const int shift = (units & (units - 1)) == 0 ? 31 - __clz(units) : -1;          // (heads of 64 and 128: no division)
-    for (unsigned i0 = threadIdx.x; i0 < total; i0 += EV_THREADS * AHEAD) {
+    for (unsigned i0 = begin * units + threadIdx.x; i0 < total; i0 += EV_THREADS * AHEAD) {
         U x[AHEAD];
 #pragma unroll
         for (int e = 0; e < AHEAD; ++e) {
@@ -180,7 +182,7 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, size_t plane, in
             if (src >= 0 && dst >= 0) to[(size_t)dst * stride] = x[e];
         }
     }
-    for (unsigned m = threadIdx.x; m < count; m += EV_THREADS) {
+    for (unsigned m = begin + threadIdx.x; m < end; m += EV_THREADS) {
         const int src = (int)list[1][m], dst = (int)list[0][m];
         if (src < 0 || dst < 0) continue;
         p.mass_out[plane + dst] = p.mass[plane + src];
@@ -245,7 +247,8 @@ template <int WORDS> __device__ __forceinline__ void scan_words(unsigned (&count
     __syncthreads();
 }
 
-template <typename U, int PER>
+// SHARED: the p.parts blocks of a cluster take one (layer, request, kv head).
+template <typename U, int PER, bool SHARED>
 __global__ void __launch_bounds__(EV_THREADS, PER <= 8 ? 3 : 1) cache_evict_kernel(const EvictParams p) {
     constexpr int WORDS = PER * EV_WARPS;
     __shared__ unsigned hist[EV_BINS];
@@ -254,7 +257,8 @@ __global__ void __launch_bounds__(EV_THREADS, PER <= 8 ? 3 : 1) cache_evict_kern
     __shared__ unsigned long long least_s[EV_WARPS];
     __shared__ unsigned found_s[3], total_s;
     after_previous();
-    const int s = blockIdx.x / p.Hkv, h = blockIdx.x - s * p.Hkv, layer = blockIdx.y;
+    const int parts = SHARED ? p.parts : 1, part = blockIdx.x & (parts - 1), both = blockIdx.x / parts;
+    const int s = both / p.Hkv, h = both - s * p.Hkv, layer = blockIdx.y;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int n = max(0, min(p.lengths[s], p.max_pages * p.page_size)), budget = p.budget;
     const int from = p.ends[s] - p.latest;
@@ -281,7 +285,7 @@ __global__ void __launch_bounds__(EV_THREADS, PER <= 8 ? 3 : 1) cache_evict_kern
         if (!apart) return;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-            if (k * EV_THREADS >= min(n, budget) || slot[k] < 0 || !stays(k)) continue;
+            if (k * EV_THREADS >= min(n, budget) || (k & (parts - 1)) != part || slot[k] < 0 || !stays(k)) continue;
             p.mass_out[plane + slot[k]] = p.mass[plane + slot[k]];
             p.positions_out[plane + slot[k]] = p.positions[plane + slot[k]];
         }
@@ -301,6 +305,7 @@ __global__ void __launch_bounds__(EV_THREADS, PER <= 8 ? 3 : 1) cache_evict_kern
 
     if (n == budget + 1) {
         // one place goes: the least worth, of equal ones the highest place
+        if (part > 0 && !apart) return;          // (a single move, and it may write what this block reads)
         unsigned long long least = ~0ull;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
@@ -326,10 +331,13 @@ __global__ void __launch_bounds__(EV_THREADS, PER <= 8 ? 3 : 1) cache_evict_kern
             if (i == n - 1) list_s[1][0] = slot[k];
         }
         __syncthreads();
-        if (hole != n - 1) move_rows<U>(p, plane, layer, h, list_s, 1);
+        if (hole != n - 1 && part == 0) move_rows<U>(p, plane, layer, h, list_s, 0, 1);
         copy([&](int k) { return k * EV_THREADS + tid < budget && k * EV_THREADS + tid != hole; });
         return;
     }
+
+    // the blocks of a cluster write, in place, what the others have read
+    if (SHARED && !apart) t5::cluster_sync_all();
 
     // the threshold: the budget-th largest worth, and how many of its equals stay
     unsigned prefix = 0, wanted = budget;
@@ -392,7 +400,7 @@ __global__ void __launch_bounds__(EV_THREADS, PER <= 8 ? 3 : 1) cache_evict_kern
             if (fills(k) && fr < count) list_s[1][fr] = slot[k];
         }
         __syncthreads();
-        move_rows<U>(p, plane, layer, h, list_s, count);
+        move_rows<U>(p, plane, layer, h, list_s, count * part / parts, count * (part + 1) / parts);
         __syncthreads();
     }
     copy([&](int k) { return k * EV_THREADS + tid < budget && ((stays >> k) & 1u); });
@@ -530,7 +538,7 @@ __global__ void __launch_bounds__(EV_THREADS) cache_evict_any_kernel(const Evict
                 if (fr - m0 < count) list_s[1][fr - m0] = slot_of(table, p.page_size, p.num_slots, w * 32 + __ffs(x) - 1);
         }
         __syncthreads();
-        move_rows<U>(p, plane, layer, h, list_s, count);
+        move_rows<U>(p, plane, layer, h, list_s, 0, count);
         __syncthreads();
     }
 }
@@ -547,11 +555,31 @@ template <typename U> int launch_commit(const CommitParams& p, cudaStream_t stre
 }
 template <typename U> int launch_evict(EvictParams p, int L, cudaStream_t stream) {
     const int places = p.max_pages * p.page_size, bit_words = (places + 31) / 32;
-    // 32 places a thread leave an SM one block, which pays while there are no more blocks than SMs (us, 16,000 places thinned to 1,024, heads
-    // of 128: 20 blocks 57, the general kernel 62; 560 blocks 341 and 220)
+    // 32 places a thread leave an SM one block, which pays while there are no more triples than SMs (us, 16,000 places thinned to 1,024, heads
+    // of 128: 20 triples 57, shared 42, the general kernel 62; 560 triples 341, the general kernel 220)
     if (places <= 8 * EV_THREADS || (places <= 32 * EV_THREADS && (long long)p.S * p.Hkv * L <= llb_device_sms())) {
-        if (places <= 8 * EV_THREADS) llb_launch(cache_evict_kernel<U, 8>, dim3(p.S * p.Hkv, L), dim3(EV_THREADS), 0, stream, p);
-        else llb_launch(cache_evict_kernel<U, 32>, dim3(p.S * p.Hkv, L), dim3(EV_THREADS), 0, stream, p);
+        // Where there are fewer (layer, request, kv head) triples than SMs, the blocks of a cluster share a triple's moves (each finds all of them:
+        // trips that all have to make anyway).  us with one block | shared: 4,001 places thinned to 1,024, heads of 128: 20 triples 31 | 18;
+        // heads of 64: 2 triples 22 | 13, 48 triples 23 | 18; 16,000 places to 8,000: 20 triples 155 | 74.  One key of each goes: 5.3 | 5.3.
+        // (Up to three blocks an SM: 48 triples 18 -> 22, 80 of 128 33 -> 29, one key 5.4 -> 7.4.)
+        const long long blocks = (long long)p.S * p.Hkv * L;
+        while (p.parts < 8 && 2 * p.parts * blocks <= llb_device_sms()) p.parts *= 2;
+        const bool few = places <= 8 * EV_THREADS;
+        auto kernel = p.parts > 1 ? (few ? cache_evict_kernel<U, 8, true> : cache_evict_kernel<U, 32, true>)
+                                  : (few ? cache_evict_kernel<U, 8, false> : cache_evict_kernel<U, 32, false>);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(p.S * p.Hkv * p.parts, L);
+        cfg.blockDim = dim3(EV_THREADS);
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = p.parts;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = p.parts > 1 ? 2 : 1;
+        cudaLaunchKernelEx(&cfg, kernel, p);          // (a failure is the runtime's last error, which llb_check_launch reads)
         return llb_check_launch("cache_evict");
     }
     // two blocks an SM have room for 20,000 worths each; places beyond that are read again in every pass
@@ -595,7 +623,7 @@ LLB_EXPORT int llb_cache_evict(const LlbCacheEvict* c, cudaStream_t stream) {
     EvictParams p;
     p.k = (char*)c->k; p.v = (char*)c->v; p.mass = c->mass; p.positions = c->positions; p.mass_out = c->mass_out; p.positions_out = c->positions_out;
     p.lengths = c->lengths; p.ends = c->ends; p.table = c->table; p.S = c->S; p.max_pages = c->max_pages; p.page_size = c->page_size;
-    p.num_slots = c->num_slots; p.Hkv = c->Hkv; p.budget = c->budget; p.first = c->first; p.latest = c->latest; p.cache_places = 0;
+    p.num_slots = c->num_slots; p.Hkv = c->Hkv; p.budget = c->budget; p.first = c->first; p.latest = c->latest; p.cache_places = 0; p.parts = 1;
     const int unit = unit_bytes(c->k, c->v, c->head_bytes);
     p.head_units = c->head_bytes / unit;
     if (unit == 16) return launch_evict<uint4>(p, c->L, stream);

@@ -362,6 +362,31 @@ def test_evict(ops, dtype, heads, held, budget, first, latest, apart, ties):
         assert torch.equal(pd.cpu(), pick(pos))
 
 
+@pytest.mark.parametrize("layers", [1, 4, 8, 15, 30])          # 8, 4, 2 blocks a (layer, request, kv head), and one
+@pytest.mark.parametrize("held", [[900, 1500, 601], [513, 513, 40], [9000, 5000, 1]], ids=str)
+@pytest.mark.parametrize("apart", [False, True])
+def test_evict_shared_by_blocks(ops, layers, held, apart):
+    """Few (layer, request, kv head) triples: several blocks share the moves of one."""
+    r, k, v, mass, pos, ends = evict_case(held, (4, 2, 16), torch.bfloat16, 16, layers, 43)
+    kd, vd, md, pd = (x.to(dev()) for x in (k, v, mass, pos))
+    mo, po = (torch.full_like(md, -3.0), torch.full_like(pd, -3)) if apart else (None, None)
+    ops.cache_evict(kd, vd, md, pd, i32(held), i32(ends), r.spans()[3], r.page, 512, 4, 100, mass_out=mo, positions_out=po)
+    want_m, want_p = (torch.full_like(mass, -3.0), torch.full_like(pos, -3)) if apart else (mass.clone(), pos.clone())
+    for l in range(layers):
+        for h in range(r.hkv):
+            for s, n in enumerate(held):
+                at = r.slots[s]
+                moves = P.evict(mass[l, h, at].tolist(), pos[l, h, at].tolist(), ends[s], 512, 4, 100)
+                stay = at[:min(n, 512)]
+                want_m[l, h, stay], want_p[l, h, stay] = mass[l, h, stay], pos[l, h, stay]
+                if moves:
+                    a, b = (torch.tensor([at[m[i]] for m in moves]) for i in (0, 1))
+                    k[l, a, h], v[l, a, h] = k[l, b, h], v[l, b, h]
+                    want_m[l, h, a], want_p[l, h, a] = mass[l, h, b], pos[l, h, b]
+    for got, want in ((kd, k), (vd, v), (mo if apart else md, want_m), (po if apart else pd, want_p)):
+        assert torch.equal(got.cpu(), want)
+
+
 def test_evict_more_places_than_shared_memory_holds(ops):
     held = [30000, 20001]
     r, k, v, mass, pos, ends = evict_case(held, (2, 1, 4), torch.float32, 16, 1, 42)
