@@ -648,7 +648,8 @@ int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtyp
     a.nodes = rows / a.group;
     // (an int numbers the tiles, whatever the lengths on the device say)
     const long long most = min(a.T, a.max_len), keys = (long long)a.max_pages * a.page_size, each = tc ? 128 : KT;
-    LLB_REQUIRE(((most + a.nodes - 1) / a.nodes) * a.S * a.Hkv * ((keys + each - 1) / each + a.extra) < (1ll << 31),
+    // (the kernel of portions' weights on the tensor cores has half as many rows a tile)
+    LLB_REQUIRE(((most + a.nodes - 1) / a.nodes) * a.S * a.Hkv * ((keys + each - 1) / each + a.extra) * (tc && mass == 1 ? 2 : 1) < (1ll << 31),
                 "span_attention: %d requests of up to %lld rows over up to %lld keys are more tiles than one call takes", a.S, most, keys);
     a.part_o = scratch + l.part_o;
     a.part_ml = scratch + l.part_ml;
