@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
         }
         if (tid < RB) {
             m_s[tid] = -INFINITY;
-            l_s[tid] = 0.0f;
+            l_s[tid] = tid < rows ? llb_first_sum(a, job.z, job.first + tid / a.group) : 0.0f;
         }
         float o[4][DPT];
 #pragma unroll
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
                 for (int w = TPR / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
                 __syncwarp();
                 if (c == 0) {
-                    const float corr = m_old == -INFINITY ? 0.0f : exp2f(m_old - use);
+                    const float corr = m_old == -INFINITY ? 1.0f : exp2f(m_old - use);          // (nothing so far, or llb_first_sum)
                     c_s[r] = corr;
                     l_s[r] = l_s[r] * corr + sum;
                     m_s[r] = m_new;
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
             const float l = l_s[r], m = m_s[r];
             const int node = job.first + r / a.group, row = job.z.row + node, head = job.kvh * a.group + r % a.group;
             float* po = a.part_o + (size_t)(blockIdx.x * 2 + max(part, 0)) * (hd4 / 4) * a.rows * 4;
-            const float inv = llb_inverse(m, l, job.z.pos);
+            const float inv = 1.0f / l;
             T* dst = (T*)a.out + ((size_t)row * a.Hq + head) * hd;
             if (RB == 64 && hd % 4 == 0 && (sizeof(T) == 4 ? ((uintptr_t)a.out & 15) == 0 : ((uintptr_t)a.out & 7) == 0)) {
 #pragma unroll
@@ -318,7 +318,7 @@ __device__ __forceinline__ void join_rows(const LlbSpanArgs& a, const LlbOpen& j
             }
 #pragma unroll
             for (int e = 0; e < PB; ++e) {
-                // (a part without visible keys has m = -infinity, l = 0 and O = 0; a NaN of another one stays)
+                // (a part without visible keys has m = -infinity, l = 0 or llb_first_sum and O = 0; a NaN of another one stays)
                 const float w = ml[e].x == -INFINITY ? 1.0f : exp2f(ml[e].x - top);
                 L = fmaf(w, ml[e].y, L);
 #pragma unroll
@@ -331,7 +331,7 @@ __device__ __forceinline__ void join_rows(const LlbSpanArgs& a, const LlbOpen& j
             }
         }
         const int node = r / a.group, row = job.row + node, head = job.kvh * a.group + r - node * a.group;
-        const float inv = llb_inverse(M, L, job.pos);
+        const float inv = 1.0f / L;
         if (a.lse && piece0 == 0) a.lse[(size_t)row * a.Hq + head] = llb_lse(M, L);
         T* dst = (T*)a.out + ((size_t)row * a.Hq + head) * hd + piece0 * 4;
         unsigned held0 = 0, held1 = 0;          // two groups of four dimensions leave together
@@ -436,10 +436,8 @@ __global__ void __launch_bounds__(THREADS, 4) span_join_kernel(const LlbSpanArgs
     }
     const int y = i / blocks, block = i - y * blocks;
     LlbOpen job;
-    const int4* from = reinterpret_cast<const int4*>(a.open) + 2 * block;
-    const int4 lo = from[0];
-    job.pos = from[1].x;
-    job.parts = lo.x; job.row = lo.y; job.rows = lo.z; job.kvh = lo.w;
+    const int4 open = reinterpret_cast<const int4*>(a.open)[block];
+    job.parts = open.x; job.row = open.y; job.rows = open.z; job.kvh = open.w;
     if (job.parts == 0) return;
     if (job.parts <= 2) join_rows<T, 2, 4>(a, job, block, y, ny);
     else join_rows<T, 8, 1>(a, job, block, y, ny);
@@ -549,7 +547,7 @@ __global__ void __launch_bounds__(THREADS) span_mass_kernel(const ColumnParams p
 // The sums of keys whose rows several blocks had, in the blocks' order.
 template <int TILE> __global__ void __launch_bounds__(TILE) span_mass_join_kernel(const LlbSpanArgs a, const float* part) {
     llb_after_previous();
-    const int4 job = reinterpret_cast<const int4*>(a.open)[2 * blockIdx.x];          // blocks, request, tile, kv head
+    const int4 job = reinterpret_cast<const int4*>(a.open)[blockIdx.x];          // blocks, request, tile, kv head
     if (job.x == 0) return;
     float sum = part[(size_t)(blockIdx.x * 2 + 1) * TILE + threadIdx.x];
 #pragma unroll 4
@@ -629,7 +627,7 @@ Layout layout(int T, int S, int Hq, int group, int hd, int num_slots, int rows, 
     l.part_o = 0;
     l.part_ml = l.part_o + 2ll * blocks * rows * ((hd + 3) & ~3);
     l.open = (l.part_ml + 2ll * blocks * rows * 2 + 3) & ~3ll;
-    l.part_mass = l.open + 8ll * blocks;
+    l.part_mass = l.open + 4ll * blocks;
     l.lse = l.part_mass + (mass == 1 ? 2ll * blocks * 128 : 0);
     l.scores = (l.lse + (mass > 0 ? (long long)T * Hq : 0) + 3) & ~3ll;
     l.score_tiles = mass == 2 ? ((long long)num_slots / tile + (long long)S * (1 + extra)) * (Hq / group) : 0;

@@ -50,7 +50,7 @@ struct LlbSpanArgs {
     int words;
     float scale_log2e;               // scores are kept in base-2 units
     void* out;                       // [T, Hq, hd]
-    float* lse;                      // [T, Hq] or null: log2 of the sum of 2^score; +infinity in a row that sees nothing
+    float* lse;                      // [T, Hq] or null (causal rows): log2 of the sum of 2^score
     float* scores;                   // [score_tiles, group, keys a tile] or null: the scores of requests of one row, tile by tile of the line
     int score_tiles;
     const float* mass_in;            // [Hkv, num_slots] or null: zeros
@@ -58,7 +58,7 @@ struct LlbSpanArgs {
     float* part_o;                   // [2 * blocks, ceil(hd / 4), rows, 4]: what a block has of a job that began before it (0) and goes on after
                                      // it (1); four dimensions of neighbouring rows side by side, as the threads that write and join them have them
     float* part_ml;                  // [2 * blocks, rows, 2]
-    int* open;                       // [blocks, 8]: the job that begins in a block and goes on after it, see LlbOpen
+    int* open;                       // [blocks, 4]: the job that begins in a block and goes on after it, see LlbOpen
     int extra;                       // what a job takes of the line besides its tiles
     int nodes;                       // rows of a request that a job holds at most
     int rows;                        // nodes * group, rounded up: (row, head) pairs of a job in the partial results
@@ -220,21 +220,28 @@ __device__ __forceinline__ void llb_add_mass(const LlbSpanArgs& a, const LlbSpan
     a.mass[at] = key < z.pos && a.mass_in ? a.mass_in[at] + sum : sum;
 }
 
-__device__ __forceinline__ float llb_lse(float m, float l) { return l == 0.0f ? INFINITY : m + log2f(l); }
-// What a row's sum of weighted values is multiplied by: 0 in a row that sees nothing; where everything that it sees scores minus infinity
-// it is 1 / 0, and the row is NaN.
-__device__ __forceinline__ float llb_inverse(float m, float l, int pos) { return l > 0.0f || m != -INFINITY || pos > 0 ? 1.0f / l : 0.0f; }
+// (Minus infinity where everything that the row sees scores minus infinity: the weights are then 2^(-inf + inf), NaN, like the row's result.)
+__device__ __forceinline__ float llb_lse(float m, float l) { return m + log2f(l); }
+// What a row's sum of weights begins with, so that 1 / sum is what its weighted values are multiplied by: infinity, which the sum then
+// stays, in a row that sees nothing (one of a tree's whose mask names none of the nodes, in a request that holds no keys) and gets zeros; 0 in
+// all others, and where everything that such a row sees scores minus infinity 1 / 0 makes it NaN.
+__device__ __forceinline__ float llb_first_sum(const LlbSpanArgs& a, const LlbSpan& z, int node) {
+    if (!a.mask || z.pos > 0) return 0.0f;
+    const unsigned long long* mask = a.mask + (size_t)(z.row + node) * a.words;
+    int left = z.len;
+#pragma unroll 1
+    for (; left >= 64; left -= 64)
+        if (*mask++) return 0.0f;
+    return left > 0 && *mask << (64 - left) ? 0.0f : INFINITY;
+}
 
 // A job whose parts are to be joined, as the block that it begins in leaves it (parts 0: it has none).
 struct LlbOpen {
     int parts, row, rows, kvh;      // blocks that have parts; first row of q, (row, head) pairs, kv head
-    int pos, unused[3];
 };
 __device__ __forceinline__ void llb_leave_open(const LlbSpanArgs& a, const LlbPiece& pc, const LlbJob& job, bool goes_on) {
-    int4* to = reinterpret_cast<int4*>(a.open) + 2 * blockIdx.x;
-    to[0] = make_int4(goes_on ? pc.owner(job.begin + job.tiles - 1) - blockIdx.x + 1 : 0, job.z.row + job.first, job.count(a) * a.group,
-                      job.kvh);
-    to[1] = make_int4(job.z.pos, 0, 0, 0);
+    reinterpret_cast<int4*>(a.open)[blockIdx.x] = make_int4(goes_on ? pc.owner(job.begin + job.tiles - 1) - blockIdx.x + 1 : 0,
+                                                            job.z.row + job.first, job.count(a) * a.group, job.kvh);
 }
 
 // Joins the parts of cut jobs and, for requests of one row (a.scores), adds up the weights that their keys received; `blocks` is the grid
@@ -327,7 +334,7 @@ __device__ __forceinline__ LlbMassPiece llb_mass_piece(const LlbSpanArgs& a, int
 }
 // What the block that a job begins in leaves of it: how many blocks have parts (0: it has no such job), request, tile and kv head.
 __device__ __forceinline__ void llb_leave_open_mass(const LlbSpanArgs& a, const LlbPiece& line, const LlbMassJob& job, bool goes_on) {
-    reinterpret_cast<int4*>(a.open)[2 * blockIdx.x] =
+    reinterpret_cast<int4*>(a.open)[blockIdx.x] =
         goes_on ? make_int4(line.owner(job.begin + job.units - 1) - blockIdx.x + 1, job.s, job.tile, job.kvh) : make_int4(0, 0, 0, 0);
 }
 

@@ -440,7 +440,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const int all = a.mask ? z.pos : z.pos + job.first + 1;         // keys that every row of the job sees
             const int own = a.mask ? z.pos : z.pos + node + 1;              // first keys that this row sees
             const bool busy = (warp & 3) * 32 < pairs;                      // any pair in this warp's lanes
-            float m_ref = -INFINITY, l_run = 0.0f;
+            float m_ref = -INFINITY, l_run = mine ? llb_first_sum(a, z, node) : 0.0f;
 #pragma unroll 1
             for (int j = g.two ? 0 : x; j < n; j += step) {
                 const int key0 = (g.k0 + j) * BK;
@@ -588,7 +588,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
             const int head = job.kvh * a.group + (mine ? r % a.group : 0), row = z.row + node;
             const int d0 = g.two ? 0 : x * (HD / 2), d1 = g.two ? HD : d0 + HD / 2;
-            const float inv = llb_inverse(m_ref, l_run, z.pos);
+            const float inv = 1.0f / l_run;
             const bool both = !g.two && n > 1;
             const bool odd = *(volatile int*)&odd_s != 0;
             if (busy) {

@@ -1,0 +1,72 @@
+"""Edges of the operators of a cache that is drafted into and thinned out, against plain forms in 64 bits."""
+import math
+import random
+
+import pytest
+import torch
+
+from tests import test_draft_cache_gpu as G
+from tests.plain import draft_cache_plain as P
+from tests.test_draft_cache_gpu import DTYPES, Requests, check_rows, dev, i32, run_mass, run_tree, spread_mask, tree_sees, trees
+
+pytestmark = pytest.mark.gpu
+ops = G.ops
+
+
+def same_mass(r, mass):
+    """Sums of weights, NaN and infinite ones among them, against 64 bits (the bound of check_mass)."""
+    for s, n in enumerate(r.rows):
+        q, k, v = r.of(s)
+        sees = torch.cat([torch.ones((n, r.held[s]), dtype=torch.bool), torch.ones((n, n), dtype=torch.bool).tril()], 1)
+        _, w = P.attention(q, k, v, sees, r.scale)
+        sums = w.reshape(r.hkv, -1, w.shape[-1]).sum(1)
+        have = mass[:, r.slots[s]].double()
+        assert torch.equal(have.isnan(), sums.isnan()), (s, have.isnan().sum(), sums.isnan().sum())
+        fine = ~sums.isnan()
+        rel = 2 * P.score_error(q, k, r.scale) + (n * r.hq // r.hkv + len(r.slots[s]) + 16) * 2.0 ** -24 + 2.0 ** -20
+        assert bool(((have - sums).abs()[fine] <= rel * sums[fine]).all()), s
+
+
+def causal(r):
+    return [torch.cat([torch.ones((n, h), dtype=torch.bool), torch.ones((n, n), dtype=torch.bool).tril()], 1) for h, n in zip(r.held, r.rows)]
+
+
+HEADS = [(14, 2, 64), (12, 2, 128), (3, 1, 32), (8, 8, 64)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("rows", [[1, 1, 1, 1], [1, 37, 200, 3]], ids=["single", "portions"])
+def test_rows_that_score_minus_infinity_everywhere(ops, dtype, heads, rows):
+    """A row that sees keys and scores minus infinity with all of them has no softmax: NaN in its result and in what its keys receive, as
+    in 64 bits.  The others are as ever; a head of queries that looks the other way sees plus infinity, which is NaN as well."""
+    held = [0, 5, 700, 130]
+    r = Requests(held, rows, heads, dtype, 16, 201)
+    r.q[:, :, 0] = r.q[:, :, 0].abs() + 0.5
+    for s in (0, 2):
+        r.k[r.slots[s], 0, 0] = -math.inf          # the first kv head of two requests
+    got, mass = run_mass(ops, r, None)
+    check_rows(r, got, causal(r))
+    same_mass(r, mass)
+    nan = mass[:, r.slots[2]].isnan()
+    assert bool(nan[0].all()) and not bool(nan[1:].any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+def test_drafted_rows_that_score_minus_infinity_everywhere(ops, dtype, heads):
+    """In a tree, too, whether its request holds keys or not; a row without any key to see is zeros beside them."""
+    r = Requests([0, 0, 900, 31], [7, 150, 20, 5], heads, dtype, 16, 202)
+    mask = spread_mask(ops, r, trees(random.Random(1), r.rows))
+    empty = [r.first[0] + 3, r.first[1] + 9, r.first[1] + 140]
+    mask[empty] = 0
+    r.q[:, :, 0] = r.q[:, :, 0].abs() + 0.5
+    for s in (0, 1, 2):
+        r.k[r.slots[s], 0, 0] = -math.inf
+    got = run_tree(ops, r, mask)
+    check_rows(r, got, tree_sees(r, mask))
+    group = r.hq // r.hkv
+    for s in (0, 1, 2):
+        rows = [i for i in range(r.first[s], r.first[s] + r.rows[s]) if i not in empty]
+        assert bool(got[rows, :group].isnan().all())
+    assert bool((got[empty] == 0).all())
