@@ -70,3 +70,19 @@ def test_drafted_rows_that_score_minus_infinity_everywhere(ops, dtype, heads):
         rows = [i for i in range(r.first[s], r.first[s] + r.rows[s]) if i not in empty]
         assert bool(got[rows, :group].isnan().all())
     assert bool((got[empty] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", HEADS + [(28, 4, 128), (5, 1, 64), (43, 1, 64)], ids=str)
+@pytest.mark.parametrize("held,n", [(0, 300), (500, 130), (900, 1)])
+def test_a_key_that_scores_minus_infinity(ops, dtype, heads, held, n):
+    """It receives nothing from any row (nothing, not a NaN), and changes nothing else."""
+    r = Requests([held, 40], [n, 3 if n > 1 else 1], heads, dtype, 16, 203)
+    r.q[:, :, 1] = r.q[:, :, 1].abs() + 0.5
+    at = [2 if n > 1 or held else 0, (held + n) // 2] if held + n > 3 else []
+    r.k[[r.slots[0][j] for j in at], :, 1] = -math.inf
+    got, mass = run_mass(ops, r, None)
+    # (a portion's rows that see only such keys have none here: key 0 is a common one)
+    check_rows(r, got, causal(r))
+    same_mass(r, mass)
+    assert bool((mass[:, [r.slots[0][j] for j in at]] == 0).all())
