@@ -361,7 +361,7 @@ __device__ __forceinline__ void join_rows(const LlbSpanArgs& a, const LlbOpen& j
 // What every key of a request of one row received: the sum of 2^(score - lse) over its kv head's query heads.  The row's lse is what the
 // attention kernel left, or, for a cut job, what its parts come to; which that is follows from the lengths, so that these blocks need
 // not wait for those that join.
-template <int TILE> __device__ __forceinline__ void mass_of_scores(const LlbSpanArgs& a, int grid, int least, int pair, int y, int ny) {
+template <typename T, int TILE> __device__ __forceinline__ void mass_of_scores(const LlbSpanArgs& a, int grid, int least, int pair, int y, int ny) {
     __shared__ int before_s, total_s;
     __shared__ float lse_s[128];
     const int s = pair / a.Hkv, kvh = pair - s * a.Hkv;
@@ -413,9 +413,21 @@ template <int TILE> __device__ __forceinline__ void mass_of_scores(const LlbSpan
         if (slot >= 0) {
             const int tile = begin + key / TILE;
             float sum = 0.0f;
-            if (tile < a.score_tiles)
+            if (tile < a.score_tiles) {
 #pragma unroll 8
                 for (int g = 0; g < a.group; ++g) sum += exp2f(a.scores[((size_t)tile * a.group + g) * TILE + key % TILE] - lse_s[g]);
+            } else {
+                // the line is longer than the cache's keys make it (pages outside the cache): there was no place for this one's scores
+                const T* q = (const T*)a.q + ((size_t)z.row * a.Hq + kvh * a.group) * a.hd;
+                const T* k = (const T*)a.k + ((size_t)slot * a.Hkv + kvh) * a.hd;
+#pragma unroll 1
+                for (int g = 0; g < a.group; ++g, q += a.hd) {
+                    float x = 0.0f;
+#pragma unroll 1
+                    for (int d = 0; d < a.hd; ++d) x = fmaf(llb_to_float(q[d]), llb_to_float(k[d]), x);
+                    sum += exp2f(x * a.scale_log2e - lse_s[g]);
+                }
+            }
             a.mass[(size_t)kvh * a.num_slots + slot] = had + sum;
         }
         const int next = key + ny * THREADS;
@@ -431,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, 4) span_join_kernel(const LlbSpanArgs
     const int i = blockIdx.x;
     if (i >= blocks * ny) {
         const int pair = (i - blocks * ny) / mass_y;
-        mass_of_scores<TILE>(a, blocks, least, pair, i - blocks * ny - pair * mass_y, mass_y);
+        mass_of_scores<T, TILE>(a, blocks, least, pair, i - blocks * ny - pair * mass_y, mass_y);
         return;
     }
     const int y = i / blocks, block = i - y * blocks;
@@ -618,7 +630,7 @@ bool tc_sizes(int dtype, int hd, int page_size) {
     return dtype == LLB_BF16 && (hd == 64 || hd == 128) && page_size % 8 == 0 && page_size <= 128 && 128 % page_size == 0;
 }
 // Scratch: the partial results, the partial sums of the weights, lse, scores.  (Requests share no pages, so that all tiles of one-row
-// requests hold no more keys than there are slots, and a piece of a tile each.)
+// requests hold no more keys than there are slots, and a piece of a tile each; mass_of_scores makes the others' scores once more.)
 struct Layout {
     long long part_o, part_ml, open, part_mass, lse, scores, score_tiles, floats;
 };
@@ -656,6 +668,7 @@ int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtyp
     a.scores = mass == 2 ? scratch + l.scores : nullptr;
     a.score_tiles = (int)min(l.score_tiles, 0x7fffffffll);
     *part_mass = scratch + l.part_mass;
+    a.q = q; a.k = k;
     int rc;
     if (tc) {
         rc = llb_span_attention_tc(a, q, k, v, blocks, error_flag, stream);

@@ -49,10 +49,12 @@ struct LlbSpanArgs {
     const unsigned long long* mask;  // tree: [T, words]; null: causal
     int words;
     float scale_log2e;               // scores are kept in base-2 units
+    const void* q;                   // [T, Hq, hd], keys [num_slots, Hkv, hd]
+    const void* k;
     void* out;                       // [T, Hq, hd]
     float* lse;                      // [T, Hq] or null (causal rows): log2 of the sum of 2^score
     float* scores;                   // [score_tiles, group, keys a tile] or null: the scores of requests of one row, tile by tile of the line
-    int score_tiles;
+    int score_tiles;                 // as many as the keys of the cache fill (tables that name pages outside the cache may make more)
     const float* mass_in;            // [Hkv, num_slots] or null: zeros
     float* mass;                     // [Hkv, num_slots]
     float* part_o;                   // [2 * blocks, ceil(hd / 4), rows, 4]: what a block has of a job that began before it (0) and goes on after

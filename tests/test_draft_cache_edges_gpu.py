@@ -86,3 +86,44 @@ def test_a_key_that_scores_minus_infinity(ops, dtype, heads, held, n):
     check_rows(r, got, causal(r))
     same_mass(r, mass)
     assert bool((mass[:, [r.slots[0][j] for j in at]] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(3, 1, 64), (4, 2, 128), (5, 1, 20)], ids=str)
+def test_single_tokens_behind_many_bad_pages(ops, dtype, heads):
+    """A table may name more places outside the cache than the cache has rows: the keys that there are receive their weights all the same."""
+    hq, hkv, hd = heads
+    page, S, held = 16, 3, [1500, 77, 2303]
+    g = torch.Generator().manual_seed(204)
+    slots = 8 * page
+    k, v = (torch.randn((slots, hkv, hd), generator=g).to(dtype) for _ in range(2))
+    q = torch.randn((S, hq, hd), generator=g).to(dtype)
+    table = [[-1] * 150 for _ in range(S)]
+    good = {0: {3: 5, 80: 0, 93: 7}, 1: {0: 1, 4: 2}, 2: {60: 3, 143: 6, 142: 4}}
+    for s, pages in good.items():
+        for at, p in pages.items():
+            table[s][at] = p
+    mass_in = torch.rand((hkv, slots), generator=g)
+    mass, out = torch.full((hkv, slots), -5.0, device=dev()), torch.full((S, hq * hd), 7.0, dtype=dtype, device=dev())
+    ops.paged_attention_mass(q.reshape(S, -1).to(dev()), k.to(dev()), v.to(dev()), out, mass, i32([0, 1, 2]), i32([1] * S), i32(held), i32(table), page,
+                             hq, hkv, hd, hd ** -0.5, 1, mass_in=mass_in.to(dev()))
+    ops.check_async_errors(dev())
+    have, out = mass.cpu().double(), out.cpu().double().reshape(S, hq, hd)
+    for s in range(S):
+        kk, vv = (torch.zeros((held[s] + 1, hkv, hd), dtype=dtype) for _ in range(2))
+        here = {}
+        for at, p in good[s].items():
+            for o in range(page):
+                if at * page + o <= held[s]:
+                    kk[at * page + o], vv[at * page + o] = k[p * page + o], v[p * page + o]
+                    here[at * page + o] = p * page + o
+        want, w = P.attention(q[s:s + 1], kk, vv, torch.ones((1, held[s] + 1), dtype=torch.bool), hd ** -0.5)
+        sums = w.reshape(hkv, -1, w.shape[-1]).sum(1)
+        rel = 2 * P.score_error(q[s:s + 1], kk, hd ** -0.5) + (hq // hkv + held[s] + 17) * 2.0 ** -24 + 2.0 ** -20
+        for j, slot in here.items():
+            before = mass_in[:, slot].double() if j < held[s] else 0.0
+            assert bool(((have[:, slot] - before - sums[:, j]).abs() <= rel * sums[:, j] + 2.0 ** -23 * before).all()), (s, j)
+        # (a bf16 result's bound as in Requests.tolerance)
+        top = float(vv.double().abs().max())
+        step = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+        assert bool(((out[s] - want[0]).abs() <= (rel + (step if dtype == torch.bfloat16 else 0.0)) * top + step * want[0].abs()).all())
