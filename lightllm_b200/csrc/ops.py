@@ -1418,9 +1418,9 @@ def _check_span_attention(what, q, k_cache, v_cache, out, num_heads, num_kv_head
 _span_scratch = {}
 
 
-def _span_scratch_floats(dt: int, T: int, S: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, num_slots: int,
+def _span_scratch_floats(dt: int, T: int, S: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, keys: int,
                          mass: int, device: int) -> int:
-    key = (dt, T, S, num_heads, num_kv_heads, head_dim, page_size, num_slots, mass, device)
+    key = (dt, T, S, num_heads, num_kv_heads, head_dim, page_size, keys, mass, device)
     n = _span_scratch.get(key)
     if n is None:
         if len(_span_scratch) > 4096:
@@ -1469,7 +1469,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     dt = _dt(q)
     device = _check_here("tree_attention", q, k_cache, v_cache, out, mask, span_row, span_len, span_pos, block_table)
     stream = _stream_on(device)
-    scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, slots, 0, device),
+    scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, 0, 0, device),
                           dtype=torch.float32, device=q.device)
     _check(lib().llb_tree_attention(_TREE_ATTENTION(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), span_row.data_ptr(), span_len.data_ptr(), span_pos.data_ptr(),
@@ -1505,7 +1505,8 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     max_len = max(1, min(max_len, T))
     device = _check_here("paged_attention_mass", q, k_cache, v_cache, out, mass, mass_in, span_row, span_len, span_pos, block_table)
     stream = _stream_on(device)
-    scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, slots, 2 if max_len == 1 else 1, device),
+    keys, mass_of = (min(slots, S * pages * page_size), 2) if max_len == 1 else (0, 1)
+    scratch = torch.empty(_span_scratch_floats(dt, T, S, num_heads, num_kv_heads, head_dim, page_size, keys, mass_of, device),
                           dtype=torch.float32, device=q.device)
     _check(lib().llb_paged_attention_mass(_ATTENTION_MASS(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), span_row.data_ptr(), span_len.data_ptr(), span_pos.data_ptr(),

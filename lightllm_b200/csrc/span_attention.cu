@@ -631,10 +631,11 @@ bool tc_sizes(int dtype, int hd, int page_size) {
 }
 // Scratch: the partial results, the partial sums of the weights, lse, scores.  (Requests share no pages, so that all tiles of one-row
 // requests hold no more keys than there are slots, and a piece of a tile each; mass_of_scores makes the others' scores once more.)
+// keys: what the requests hold together at most, the cache's rows or their tables' places: a pool may be many times what a call can see.
 struct Layout {
     long long part_o, part_ml, open, part_mass, lse, scores, score_tiles, floats;
 };
-Layout layout(int T, int S, int Hq, int group, int hd, int num_slots, int rows, int blocks, int tile, int extra, int mass) {
+Layout layout(int T, int S, int Hq, int group, int hd, long long keys, int rows, int blocks, int tile, int extra, int mass) {
     Layout l;
     l.part_o = 0;
     l.part_ml = l.part_o + 2ll * blocks * rows * ((hd + 3) & ~3);
@@ -642,7 +643,7 @@ Layout layout(int T, int S, int Hq, int group, int hd, int num_slots, int rows, 
     l.part_mass = l.open + 4ll * blocks;
     l.lse = l.part_mass + (mass == 1 ? 2ll * blocks * 128 : 0);
     l.scores = (l.lse + (mass > 0 ? (long long)T * Hq : 0) + 3) & ~3ll;
-    l.score_tiles = mass == 2 ? ((long long)num_slots / tile + (long long)S * (1 + extra)) * (Hq / group) : 0;
+    l.score_tiles = mass == 2 ? (keys / tile + (long long)S * (1 + extra)) * (Hq / group) : 0;
     l.floats = l.scores + l.score_tiles * group * tile;
     return l;
 }
@@ -653,7 +654,8 @@ int attend(LlbSpanArgs& a, const void* q, const void* k, const void* v, int dtyp
     const int rows = tc ? 2 * llb_span_tc_pairs(a.group) * a.group : simt_rows(a.T, a.S, a.group);
     const int blocks = tc ? tc_blocks() : simt_blocks();
     a.extra = tc ? LLB_SPAN_TC_EXTRA : LLB_SPAN_EXTRA;
-    const Layout l = layout(a.T, a.S, a.Hq, a.group, a.hd, a.num_slots, rows, blocks, tc ? 128 : KT, a.extra, mass);
+    const long long places = min((long long)a.num_slots, (long long)a.S * a.max_pages * a.page_size);
+    const Layout l = layout(a.T, a.S, a.Hq, a.group, a.hd, places, rows, blocks, tc ? 128 : KT, a.extra, mass);
     a.rows = rows;
     a.nodes = rows / a.group;
     // (an int numbers the tiles, whatever the lengths on the device say)
@@ -695,13 +697,14 @@ bool takes_tc(const LlbSpanArgs& a, const LlbSpanCall& s) {
 
 }  // namespace
 
-// Floats of scratch that the calls below take; `mass` 0: a tree, 1: with the keys' weights, 2: the same where max_len is 1.
-LLB_EXPORT long long llb_span_scratch_floats(int dtype, int T, int S, int Hq, int Hkv, int hd, int page_size, int num_slots, int mass) {
+// Floats of scratch that the calls below take; `keys`: the smaller of num_slots and S * max_pages * page_size (or more); `mass` 0: a tree, 1: with
+// the keys' weights, 2: the same where max_len is 1.
+LLB_EXPORT long long llb_span_scratch_floats(int dtype, int T, int S, int Hq, int Hkv, int hd, int page_size, int keys, int mass) {
     if (Hkv <= 0 || Hq < Hkv || S <= 0) return 1;
     const int group = Hq / Hkv;
-    long long n = layout(T, S, Hq, group, hd, num_slots, simt_rows(T, S, group), simt_blocks(), KT, LLB_SPAN_EXTRA, mass).floats;
+    long long n = layout(T, S, Hq, group, hd, keys, simt_rows(T, S, group), simt_blocks(), KT, LLB_SPAN_EXTRA, mass).floats;
     if (tc_sizes(dtype, hd, page_size) && group <= 128) {
-        const long long tc = layout(T, S, Hq, group, hd, num_slots, 2 * llb_span_tc_pairs(group) * group, tc_blocks(), 128, LLB_SPAN_TC_EXTRA, mass).floats;
+        const long long tc = layout(T, S, Hq, group, hd, keys, 2 * llb_span_tc_pairs(group) * group, tc_blocks(), 128, LLB_SPAN_TC_EXTRA, mass).floats;
         n = tc > n ? tc : n;
     }
     return n;

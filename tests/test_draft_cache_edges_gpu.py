@@ -127,3 +127,30 @@ def test_single_tokens_behind_many_bad_pages(ops, dtype, heads):
         top = float(vv.double().abs().max())
         step = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
         assert bool(((out[s] - want[0]).abs() <= (rel + (step if dtype == torch.bfloat16 else 0.0)) * top + step * want[0].abs()).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+def test_scratch_goes_by_what_the_requests_can_hold(ops, dtype):
+    """One token behind few keys in a pool of two million rows: its call asks for no memory in proportion to the pool."""
+    hq, hkv, hd, page, slots = 16, 1, 64 if dtype == torch.bfloat16 else 8, 16, 1 << 21
+    k, v = (torch.zeros((slots, hkv, hd), dtype=dtype, device=dev()) for _ in range(2))
+    q, out = torch.ones((1, hq * hd), dtype=dtype, device=dev()), torch.zeros((1, hq * hd), dtype=dtype, device=dev())
+    mass = torch.full((hkv, slots), -5.0, device=dev())
+    table = i32([[slots // page - 1 - i for i in range(40)]])
+    args = (i32([0]), i32([1]), i32([600]), table, page, hq, hkv, hd, hd ** -0.5, 1)
+    ops.paged_attention_mass(q, k, v, out, mass, *args)          # (the flag of errors and the like are there afterwards)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    ops.paged_attention_mass(q, k, v, out, mass, *args)
+    torch.cuda.synchronize()
+    # scores of at most 640 places and the pieces' ends, partial results of up to 512 blocks of two parts of 128 rows (of bf16 heads; 16
+    # rows of float32) and their maxima
+    rows = 256 if dtype == torch.bfloat16 else 64
+    bound = 4 * (2 * 512 * rows * (hd + 4) + 2 * 512 * 128 + (640 + 4 * 128 * 5) * hq + 65536)
+    assert torch.cuda.max_memory_allocated() - before <= bound
+    assert torch.cuda.max_memory_allocated() - before < 4 * slots * hq // 2
+    slots_of = torch.tensor([int(table[0, j // page]) * page + j % page for j in range(601)])
+    weights = mass.cpu()[0, slots_of].double()
+    assert torch.allclose(weights, torch.full_like(weights, hq / 601), rtol=1e-5)
+    assert int((mass != -5.0).sum()) == 601
