@@ -2,6 +2,7 @@
 // Both work on all layers of a group of planes at once: keys and values [layers, slots, kv heads, head size].
 #include "cache_calls.h"
 #include "common.cuh"
+#include "memory_ranges.h"
 #include "tcgen05_common.cuh"
 
 namespace {
@@ -599,6 +600,13 @@ LLB_EXPORT int llb_tree_commit(const LlbTreeCommit* c, cudaStream_t stream) {
     LLB_REQUIRE(c->S > 0 && c->T >= 0 && c->L > 0 && c->L <= 65535 && c->max_pages >= 0 && c->page_size > 0 && c->num_slots > 0 && c->row_bytes > 0 &&
                 c->row_bytes % 2 == 0 && (long long)c->max_pages * c->page_size <= (1 << 30), "tree_commit: bad sizes");
     LLB_REQUIRE(c->width > 0 && c->width <= COMMIT_MAX_PATH, "tree_commit: path has room for %d nodes, 1 to %d are possible", c->width, COMMIT_MAX_PATH);
+    const long long rows = 4ll * c->T, spans = 4ll * c->S, planes = (long long)c->L * c->num_slots * c->row_bytes;
+    if (int rc = llb_refuse_overlap("tree_commit", {{"k_cache", c->k, planes}, {"v_cache", c->v, planes}, {"path", c->path, spans * c->width},
+                                                    {"count", c->count, spans}, {"next_token", c->next, spans}},
+                                    {{"tokens", c->tokens, rows}, {"parents", c->parents, rows}, {"targets", c->targets, rows},
+                                     {"span_row", c->span_row, spans}, {"span_len", c->span_len, spans}, {"span_pos", c->span_pos, spans},
+                                     {"block_table", c->table, spans * c->max_pages}}))
+        return rc;
     CommitParams p;
     p.tokens = c->tokens; p.parents = c->parents; p.targets = c->targets; p.k = (char*)c->k; p.v = (char*)c->v; p.span_row = c->span_row;
     p.span_len = c->span_len; p.span_pos = c->span_pos; p.table = c->table; p.S = c->S; p.T = c->T; p.L = c->L; p.max_pages = c->max_pages;
@@ -620,6 +628,13 @@ LLB_EXPORT int llb_cache_evict(const LlbCacheEvict* c, cudaStream_t stream) {
                 c->max_pages, c->page_size, EV_MAX_PLACES);
     LLB_REQUIRE(c->budget > 0 && c->first >= 0 && c->latest >= 0 && (long long)c->first + c->latest <= c->budget,
                 "cache_evict: a budget of %d places does not hold the first %d and the latest %d", c->budget, c->first, c->latest);
+    const long long spans = 4ll * c->S, heads = (long long)c->L * c->Hkv * c->num_slots, planes = heads * c->head_bytes;
+    const bool apart = c->mass_out != c->mass || c->positions_out != c->positions;
+    if (int rc = llb_refuse_overlap("cache_evict", {{"k_cache", c->k, planes}, {"v_cache", c->v, planes}, {"mass_out", c->mass_out, 4 * heads},
+                                                    {"positions_out", c->positions_out, 4 * heads}},
+                                    {{"mass", apart ? c->mass : nullptr, 4 * heads}, {"positions", apart ? c->positions : nullptr, 4 * heads},
+                                     {"lengths", c->lengths, spans}, {"ends", c->ends, spans}, {"block_table", c->table, spans * c->max_pages}}))
+        return rc;
     EvictParams p;
     p.k = (char*)c->k; p.v = (char*)c->v; p.mass = c->mass; p.positions = c->positions; p.mass_out = c->mass_out; p.positions_out = c->positions_out;
     p.lengths = c->lengths; p.ends = c->ends; p.table = c->table; p.S = c->S; p.max_pages = c->max_pages; p.page_size = c->page_size;

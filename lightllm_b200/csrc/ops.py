@@ -1458,7 +1458,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 
     q, out [T, heads * head_dim], caches [slots, kv heads, head_dim], all float32 or all bfloat16; mask int64 [T, words]; span arrays
     int32 [requests], block_table int32 [requests, pages].  Nothing is read on the host: a captured graph serves other trees,
-    lengths and tables of the same sizes.  Rows of no request are left as they were."""
+    lengths and tables of the same sizes.  Rows of no request are left as they were.  ``out`` lies over nothing that the call reads."""
     T, slots = _check_span_attention("tree_attention", q, k_cache, v_cache, out, num_heads, num_kv_heads, head_dim)
     each, words = span_len.shape, mask.shape
     S = each[0]
@@ -1490,7 +1490,7 @@ def paged_attention_mass(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     (sums go on from step to step; a new key starts from zero whatever an earlier owner left in its slot) or ``None`` (all start
     from zero).  ``mass`` float32 [kv heads, slots].  No two requests share a page: a key's sum belongs to one request.  ``max_len``: the most rows that a request brings (longer ones
     are cut to it); 1 takes the form for single tokens, which reads every key once.  The other arguments as
-    :func:`tree_attention`.  Sums are made in one order: equal calls give equal bits."""
+    :func:`tree_attention`.  Sums are made in one order: equal calls give equal bits.  ``out`` and ``mass`` lie over nothing else of the call."""
     T, slots = _check_span_attention("paged_attention_mass", q, k_cache, v_cache, out, num_heads, num_kv_heads, head_dim)
     each = span_len.shape
     S = each[0]

@@ -9,6 +9,7 @@
 // rows are needed there), O stays in registers.  Every thread has 4 rows of the scores and of O, so that a float4 from shared memory
 // feeds 16 products or more.  RB is 64, or 16 where requests bring so few rows that most of 64 would stay empty.
 #include "cache_calls.h"
+#include "memory_ranges.h"
 #include "span_attention.cuh"
 
 #include <math.h>
@@ -691,6 +692,15 @@ LlbSpanArgs span_args(const LlbSpanCall& s, int max_len) {
     a.group = s.Hkv > 0 ? s.Hq / s.Hkv : 0; a.scale_log2e = s.scale * 1.4426950408889634f; a.max_len = max_len;
     return a;
 }
+// Nothing that the call reads lies under what it writes: the result, and the weights (null: a tree).
+int check_apart(const char* what, const LlbSpanCall& s, const unsigned long long* mask, int words, const float* mass, const float* mass_in) {
+    const long long e = s.dtype == LLB_F32 ? 4 : 2, rows = (long long)s.T * s.Hq * s.hd * e, plane = (long long)s.num_slots * s.Hkv * s.hd * e;
+    const long long spans = 4ll * s.S, weights = 4ll * s.num_slots * s.Hkv;
+    return llb_refuse_overlap(what, {{"out", s.out, rows}, {"mass", mass, weights}},
+                              {{"q", s.q, rows}, {"k_cache", s.k, plane}, {"v_cache", s.v, plane}, {"mask", mask, 8ll * s.T * words},
+                               {"mass_in", mass_in == mass ? nullptr : mass_in, weights}, {"span_row", s.span_row, spans},
+                               {"span_len", s.span_len, spans}, {"span_pos", s.span_pos, spans}, {"block_table", s.table, spans * s.max_pages}});
+}
 bool takes_tc(const LlbSpanArgs& a, const LlbSpanCall& s) {
     return tc_sizes(s.dtype, a.hd, a.page_size) && llb_span_tc_takes(a, s.q, s.k, s.v, s.out);
 }
@@ -717,6 +727,7 @@ LLB_EXPORT int llb_tree_attention(const LlbTreeAttention* c, cudaStream_t stream
     if (int rc = check(a, s.dtype)) return rc;
     LLB_REQUIRE(a.max_len > 0 && c->mask && s.scratch, "tree_attention: no mask or no scratch");
     if (a.S == 0 || a.T == 0) return 0;
+    if (int rc = check_apart("tree_attention", s, c->mask, c->words, nullptr, nullptr)) return rc;
     a.mask = c->mask;
     a.words = c->words;
     float* unused;
@@ -730,6 +741,7 @@ LLB_EXPORT int llb_paged_attention_mass(const LlbAttentionMass* c, cudaStream_t 
     LLB_REQUIRE(a.max_len > 0 && c->mass && s.scratch, "paged_attention_mass: no weights, no scratch or rows");
     LLB_REQUIRE((long long)a.S * a.Hkv < (1ll << 24), "paged_attention_mass: too many requests");
     if (a.S == 0 || a.T == 0) return 0;
+    if (int rc = check_apart("paged_attention_mass", s, nullptr, 0, c->mass, c->mass_in)) return rc;
     const bool single = a.max_len == 1, tc = takes_tc(a, s);
     float* part_mass;
     a.mass_in = c->mass_in;

@@ -1,0 +1,91 @@
+"""The library's own refusals of the operators of a cache that is drafted into and thinned out; no GPU needed."""
+import pytest
+import torch
+
+from lightllm_b200.csrc import ops
+
+T, S, L, SLOTS, HQ, HKV, HD, PAGES, PAGE, WIDTH = 6, 2, 3, 32, 4, 2, 16, 3, 8, 4
+
+
+def refusal(call, pack, *numbers):
+    """What the library says to a call that it refuses before anything is launched."""
+    assert call(pack(*numbers), 0) != 0
+    return ops.lib().llb_last_error().decode()
+
+
+NAMES = ("q", "k_cache", "v_cache", "out", "mass", "mass_in", "span_row", "span_len", "span_pos", "block_table", "scratch", "flag", "tokens", "parents",
+        "targets", "path", "count", "next_token", "lengths", "ends", "positions", "positions_out")
+SIZES = dict(q=T * HQ * HD * 4, out=T * HQ * HD * 4, k_cache=SLOTS * HKV * HD * 4, v_cache=SLOTS * HKV * HD * 4, mass=HKV * SLOTS * 4, mass_in=HKV * SLOTS * 4,
+             span_row=S * 4, span_len=S * 4, span_pos=S * 4, block_table=S * PAGES * 4)
+ARENA = torch.zeros(1 << 21, dtype=torch.uint8)
+
+
+def memory():
+    """An address for every range of the calls, by name, all far from each other."""
+    return {name: ARENA.data_ptr() + 65536 * (i + 1) for i, name in enumerate(NAMES + ("mask",))}
+
+
+def attention_call(at, mass):
+    span = [at[x] for x in ("q", "k_cache", "v_cache", "out", "span_row", "span_len", "span_pos", "block_table", "scratch", "flag")]
+    span += [ops.F32, S, T, PAGES, PAGE, SLOTS, HQ, HKV, HD, 0.25]
+    if mass:
+        return ops.lib().llb_paged_attention_mass, ops._ATTENTION_MASS, *span, at["mass_in"], at["mass"], 3, 0
+    return ops.lib().llb_tree_attention, ops._TREE_ATTENTION, *span, at["mask"], 1, 0
+
+
+@pytest.mark.parametrize("mass", [False, True])
+@pytest.mark.parametrize("under", ["q", "k_cache", "v_cache", "span_row", "span_len", "span_pos", "block_table"])
+def test_attention_refuses_results_over_what_it_reads(mass, under):
+    at = memory()
+    for written in ["out", "mass"] if mass else ["out"]:
+        for moved in (0, 4, SIZES[under] - 4, 4 - SIZES[written]):
+            there = dict(at, **{written: at[under] + moved})
+            assert refusal(*attention_call(there, mass)).endswith(f"{written} must not lie over {under}")
+
+
+def test_trees_refuse_results_over_their_masks():
+    at = memory()
+    assert refusal(*attention_call(dict(at, out=at["mask"]), False)).endswith("out must not lie over mask")
+
+
+def test_weights_go_on_in_the_same_plane_or_in_one_of_its_own():
+    """Blocks add a key's sum to what another key's place may already have lost, if the two planes are some places apart."""
+    at = memory()
+    for moved in (4, -4, SIZES["mass"] - 4):
+        assert refusal(*attention_call(dict(at, mass=at["mass_in"] + moved), True)).endswith("mass must not lie over mass_in")
+    assert refusal(*attention_call(dict(at, mass=at["out"]), True)).endswith("out must not lie over mass")
+
+
+def commit_call(at):
+    order = ("tokens", "parents", "targets", "k_cache", "v_cache", "span_row", "span_len", "span_pos", "block_table", "path", "count", "next_token")
+    return ops.lib().llb_tree_commit, ops._TREE_COMMIT, *(at[x] for x in order), S, T, 1, PAGES, PAGE, SLOTS, HKV * HD * 4, WIDTH
+
+
+@pytest.mark.parametrize("written", ["k_cache", "v_cache", "path", "count", "next_token"])
+@pytest.mark.parametrize("under", ["tokens", "parents", "targets", "span_row", "span_len", "span_pos", "block_table", "v_cache", "path"])
+def test_commit_refuses_results_over_what_it_reads(written, under):
+    """Every block finds the path for itself, some when others have written theirs."""
+    if written == under or (written, under) == ("path", "v_cache"):
+        return
+    at = memory()
+    said = refusal(*commit_call(dict(at, **{written: at[under]})))
+    assert said.endswith(f"{written} must not lie over {under}") or said.endswith(f"{under} must not lie over {written}")
+
+
+def evict_call(at, apart):
+    ints = (S, 1, HKV, PAGES, PAGE, SLOTS, HD * 4, 8, 2, 4)
+    order = ("k_cache", "v_cache", "mass_in", "positions", "mass", "positions_out", "lengths", "ends", "block_table")
+    at = dict(at) if apart else dict(at, mass=at["mass_in"], positions_out=at["positions"])
+    return ops.lib().llb_cache_evict, ops._CACHE_EVICT, *(at[x] for x in order), *ints
+
+
+@pytest.mark.parametrize("written,under,moved", [
+    ("mass", "mass_in", 4), ("mass", "mass_in", -4), ("positions_out", "positions", 4), ("mass", "positions", 0), ("positions_out", "mass_in", 0),
+    ("mass", "positions_out", 0), ("k_cache", "v_cache", 4), ("k_cache", "mass_in", 0), ("v_cache", "positions", 0), ("k_cache", "block_table", 0),
+    ("mass", "lengths", 0), ("positions_out", "ends", 0), ("mass", "k_cache", 8)])
+def test_eviction_refuses_planes_that_overlap(written, under, moved):
+    """Holes' weights are written while other places' are read: planes are the same or have nothing in common."""
+    at = memory()
+    assert "must not lie over" in refusal(*evict_call(dict(at, **{written: at[under] + moved}), True))
+    if written in ("k_cache", "v_cache"):
+        assert "must not lie over" in refusal(*evict_call(dict(at, **{written: at[under] + moved}), False))

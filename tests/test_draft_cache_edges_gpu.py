@@ -154,3 +154,40 @@ def test_scratch_goes_by_what_the_requests_can_hold(ops, dtype):
     weights = mass.cpu()[0, slots_of].double()
     assert torch.allclose(weights, torch.full_like(weights, hq / 601), rtol=1e-5)
     assert int((mass != -5.0).sum()) == 601
+
+
+def test_results_over_other_memory_of_a_call(ops):
+    """Refused, with nothing written; memory that lies side by side is fine."""
+    r = Requests([40, 7], [3, 5], (4, 2, 64), torch.float32, 16, 205)
+    q, k, v = r.q.reshape(r.T, -1).to(dev()), r.k.to(dev()), r.v.to(dev())
+    want, sums = run_mass(ops, r, None)
+    planes = torch.full((3 * r.hkv * r.num_slots,), -5.0, device=dev())
+    plane = lambda at: planes[at:at + r.hkv * r.num_slots].view(r.hkv, r.num_slots)  # noqa: E731
+    n = r.hkv * r.num_slots
+    out = torch.full_like(q, 7.0)
+    for at in (1, n - 1):
+        with pytest.raises(ops.KernelError, match="mass must not lie over mass_in"):
+            ops.paged_attention_mass(q, k, v, out, plane(at), *r.args(), 5, mass_in=plane(0))
+    with pytest.raises(ops.KernelError, match="out must not lie over k_cache"):
+        ops.paged_attention_mass(q, k, v, k.view(-1)[:q.numel()].view_as(q), plane(0), *r.args(), 5)
+    mask = spread_mask(ops, r, trees(random.Random(1), r.rows)).to(dev())
+    with pytest.raises(ops.KernelError, match="out must not lie over v_cache"):
+        ops.tree_attention(q, k, v, v.view(-1)[-q.numel():].view_as(q), mask, *r.args())
+    assert bool((out == 7.0).all()) and bool((planes == -5.0).all())
+    plane(0).zero_()
+    ops.paged_attention_mass(q, k, v, out, plane(n), *r.args(), 5, mass_in=plane(0))          # side by side
+    assert torch.equal(out.cpu().view_as(want), want) and torch.equal(plane(n).cpu(), sums) and bool((planes[2 * n:] == -5.0).all())
+    # two layers of weights, written one layer further on
+    kl, vl = (x.expand(2, *x.shape).contiguous() for x in (k, v))
+    mass, pos = torch.rand((3, r.hkv, r.num_slots), device=dev()), torch.zeros((3, r.hkv, r.num_slots), dtype=torch.int32, device=dev())
+    spans = r.spans()
+    before = [x.clone() for x in (kl, vl, mass, pos)]
+    with pytest.raises(ops.KernelError, match="mass_out must not lie over mass"):
+        ops.cache_evict(kl, vl, mass[:2], pos[:2], i32([43, 12]), i32([43, 12]), spans[3], 16, 10, 0, 0, mass_out=mass[1:], positions_out=pos[1:])
+    ids = i32([0] * r.T)
+    path, count = i32([[0] * 4] * 2), i32([0, 0])
+    with pytest.raises(ops.KernelError, match="next_token must not lie over tokens"):
+        ops.tree_commit(ids, ids.clone(), ids.clone(), kl, vl, *spans, 16, path, count, ids[:2])
+    with pytest.raises(ops.KernelError, match="k_cache must not lie over v_cache"):
+        ops.tree_commit(ids, ids.clone(), ids.clone(), kl.view(-1, 2, 64)[:-1], kl.view(-1, 2, 64)[1:], *spans, 16, path, count, i32([0, 0]))
+    assert all(torch.equal(a.nan_to_num(9.0), b.nan_to_num(9.0)) for a, b in zip((kl, vl, mass, pos), before))
