@@ -8,8 +8,11 @@
 namespace {
 
 // The kernel before has completed.  The next one is not let in early, as other kernels of the library do: these move keys that are not new,
-// and decode attention reads such keys before it waits.
+// and decode attention reads such keys before it waits.  It may be the next one and begin as soon as the last block here has ended, when only
+// its own wait would promise it what was written: so a thread that has moved rows ends with before_next().
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// What this thread has written is in the memory that all multiprocessors read.
+__device__ __forceinline__ void before_next() { __threadfence(); }
 
 // The cache row of a place of a request, or -1 for a page that is none of the cache's: such a place is neither read nor written.
 __device__ __forceinline__ int slot_of(const int* table, int page_size, int num_slots, int place) {
@@ -113,6 +116,7 @@ __global__ void __launch_bounds__(COMMIT_THREADS) tree_commit_kernel(const Commi
                 if (d0 + e < count && slot_s[0][d0 + e] >= 0 && slot_s[1][d0 + e] >= 0) base[(size_t)slot_s[1][d0 + e] * p.row_units] = x[e];
         }
     }
+    before_next();
 }
 
 // ---- eviction ------------------------------------------------------------------------------------------------------------------
@@ -334,6 +338,7 @@ __global__ void __launch_bounds__(EV_THREADS, PER <= 8 ? 3 : 1) cache_evict_kern
         __syncthreads();
         if (hole != n - 1 && part == 0) move_rows<U>(p, plane, layer, h, list_s, 0, 1);
         copy([&](int k) { return k * EV_THREADS + tid < budget && k * EV_THREADS + tid != hole; });
+        before_next();
         return;
     }
 
@@ -405,6 +410,7 @@ __global__ void __launch_bounds__(EV_THREADS, PER <= 8 ? 3 : 1) cache_evict_kern
         __syncthreads();
     }
     copy([&](int k) { return k * EV_THREADS + tid < budget && ((stays >> k) & 1u); });
+    before_next();
 }
 
 template <typename U>
@@ -542,6 +548,7 @@ __global__ void __launch_bounds__(EV_THREADS) cache_evict_any_kernel(const Evict
         move_rows<U>(p, plane, layer, h, list_s, 0, count);
         __syncthreads();
     }
+    before_next();
 }
 
 // The widest unit that divides a row's bytes and every address that rows begin at.

@@ -1539,7 +1539,7 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, targets: torch.Tens
 
     (count 0 and next_token -1 where a request brings no rows; a path ends at its width).  The row of node ``path[s, d]`` moves from place
     ``span_pos[s] + path[s, d]`` to ``span_pos[s] + d`` in every layer: the request then holds ``span_pos[s] + count[s]`` keys, what lies
-    behind them is left over.  tokens, parents, targets int32 [T]; caches [slots, kv heads, head_dim] or [layers, ...]; path int32
+    behind them is left over.  (:func:`paged_decode_mma` may be the next launch, with ``fresh``: moved keys are there.)  tokens, parents, targets int32 [T]; caches [slots, kv heads, head_dim] or [layers, ...]; path int32
     [requests, width], width up to 1,024; count, next_token int32 [requests]."""
     L, slots, heads, hd = _check_planes("tree_commit", k_cache, v_cache)
     each, rows, room = span_len.shape, tokens.shape, path.shape
@@ -1567,7 +1567,8 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor
     equal ones the lowest place (NaN counts as the largest).  The i-th place below the budget that does not stay takes the key, value, mass and
     position of the i-th place beyond it that does; all others stay where they are.  So the order of the places says nothing of the
     keys' positions afterwards: for attention that does not go by it (no window, no bias by distance).  A request then holds
-    ``min(lengths[s], budget)`` places; one of no more than the budget is left as it is.  No two requests share a page.
+    ``min(lengths[s], budget)`` places; one of no more than the budget is left as it is.  No two requests share a page.  A decode step may follow
+    at once, as behind :func:`tree_commit`.
 
     Caches [slots, kv heads, head_dim] or [layers, ...]; mass float32 and positions int32 [kv heads, slots] or [layers, ...];
     lengths, ends int32 [requests].  ``mass_out`` and ``positions_out`` (both or neither): planes that receive the mass and position

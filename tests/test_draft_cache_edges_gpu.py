@@ -191,3 +191,100 @@ def test_results_over_other_memory_of_a_call(ops):
     with pytest.raises(ops.KernelError, match="k_cache must not lie over v_cache"):
         ops.tree_commit(ids, ids.clone(), ids.clone(), kl.view(-1, 2, 64)[:-1], kl.view(-1, 2, 64)[1:], *spans, 16, path, count, i32([0, 0]))
     assert all(torch.equal(a.nan_to_num(9.0), b.nan_to_num(9.0)) for a, b in zip((kl, vl, mass, pos), before))
+
+
+def decode(ops, q, k, v, out, pos, table, page, heads, fresh, nsplit=4):
+    hq, hkv, hd = heads
+    S = q.shape[0]
+    iota, zeros = i32(list(range(S))), i32([0] * S)
+    return lambda f=fresh: ops.paged_decode_mma(q, k, v, out, iota, zeros, S, iota, pos, table, table.shape[1], page, hq, hkv, hd, 0, hd ** -0.5, nsplit, None,
+                                                fresh=f)
+
+
+@pytest.mark.parametrize("held", [1500, 5000], ids=["registers", "large tables"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128)], ids=str)
+def test_a_decode_step_right_behind_an_eviction(ops, heads, held):
+    """Decode attention asks for the keys of earlier steps before it waits for the launch before it: the moved ones are there, eager and
+    from a graph."""
+    hq, hkv, hd = heads
+    S, page, budget = 24, 16, 1024
+    r, k, v, mass, pos, ends = evict_inputs(held, S, heads, page)
+    k0, v0, m0, p0 = (x.to(dev()) for x in (k, v, mass, pos))
+    k1, v1, m1, p1 = (torch.empty_like(x) for x in (k0, v0, m0, p0))
+    q = torch.randn((S, hq * hd), generator=torch.Generator().manual_seed(207)).bfloat16().to(dev())
+    out, table, lengths, end = torch.zeros_like(q), r.spans()[3], i32([held] * S), i32(ends)
+    step = decode(ops, q, k1, v1, out, i32([budget - 1] * S), table, page, heads, 1)
+
+    def run():
+        for a, b in ((k1, k0), (v1, v0), (m1, m0), (p1, p0)):
+            a.copy_(b)
+        ops.cache_evict(k1, v1, m1, p1, lengths, end, table, page, budget, 4, 100)
+
+    run()
+    torch.cuda.synchronize()
+    step(0)
+    torch.cuda.synchronize()
+    want, rows = out.clone(), k1.clone()
+    assert not torch.equal(rows, k0)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        run()
+        step()
+    for i in range(40):
+        out.zero_()
+        if i % 2:
+            graph.replay()
+        else:
+            run()
+            step()
+        torch.cuda.synchronize()
+        assert torch.equal(k1, rows) and torch.equal(out, want), i
+
+
+def evict_inputs(held, S, heads, page):
+    r, k, v, mass, pos, ends = G.evict_case([held] * S, heads, torch.bfloat16, page, 0, 206)
+    return r, k[0].contiguous(), v[0].contiguous(), mass[0].contiguous(), pos[0].contiguous(), ends
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128)], ids=str)
+def test_a_decode_step_right_behind_a_commit(ops, heads):
+    """The same of confirmed drafted tokens: every other node of a long chain moves up, over several tiles of keys."""
+    hq, hkv, hd = heads
+    S, page, n, held = 24, 16, 400, 300
+    r = Requests([held] * S, [n] * S, heads, torch.bfloat16, page, 208, gap=0)
+    parents = [-1] + [max(0, i - 2) for i in range(1, n)]
+    tokens, targets = [i % 2 for i in range(n)], [0] * n          # (even nodes go on with even ones)
+    flat = [i32(x * S) for x in (tokens, parents, targets)]
+    k0, v0 = r.k.to(dev()), r.v.to(dev())
+    k1, v1 = torch.empty_like(k0), torch.empty_like(v0)
+    path, count, nxt = i32([[0] * n] * S), i32([0] * S), i32([0] * S)
+    took, _ = P.commit(tokens, parents, targets, n)
+    assert len(took) == n // 2
+    q = r.q[:S].reshape(S, -1).to(dev())
+    out, spans = torch.zeros_like(q), r.spans()
+    step = decode(ops, q, k1, v1, out, i32([held + len(took) - 1] * S), spans[3], page, heads, 1)
+
+    def run():
+        k1.copy_(k0), v1.copy_(v0)
+        ops.tree_commit(*flat, k1, v1, *spans, page, path, count, nxt)
+
+    run()
+    torch.cuda.synchronize()
+    assert count.tolist() == [len(took)] * S
+    step(0)
+    torch.cuda.synchronize()
+    want = out.clone()
+    assert bool(want.isfinite().all())
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        run()
+        step()
+    for i in range(40):
+        out.zero_()
+        if i % 2:
+            graph.replay()
+        else:
+            run()
+            step()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
