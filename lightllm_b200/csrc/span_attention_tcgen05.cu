@@ -110,6 +110,19 @@ __device__ __forceinline__ void tmem_wait_ld32(float (&r)[32]) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// What the loader has asked for arrives before its block ends, whoever gave up on a wait: of every barrier that loads complete on, the last of
+// the `loads` that it had (they take turns: a barrier has one at a time).  With a limit, as every wait.
+__device__ __forceinline__ void loads_arrive(uint64_t* bar, uint32_t loads) {
+    if (loads == 0) return;
+    const long long since = clock64();
+    while (!mbar_try_wait(bar, (loads - 1) & 1) && clock64() - since < WAIT_LIMIT_CYCLES / 64) {
+    }
+}
+// Of those that `loaded` loads went through one after the other.
+template <int RING> __device__ __forceinline__ void ring_arrives(uint64_t (&bar)[RING], uint32_t loaded) {
+    for (uint32_t i = 0; i < RING; ++i) loads_arrive(&bar[i], (loaded + RING - 1 - i) / RING);
+}
+
 // A row's mask.  The first two words (128 nodes) are asked for when the job begins, since a trip to memory in the last tile would be as long as
 // the rest of its work.
 struct RowMask {
@@ -294,6 +307,7 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const uint32_t q_bytes = (uint32_t)p.pairs_nodes * a.group * 128 * KB;
         const int ppt = BK / a.page_size;
         uint32_t loaded = 0, q_phases = 0;           // of bar_q_free (bits 0, 1), and which buffers have been used (bits 2, 3)
+        uint32_t q_loaded[2] = {0, 0};
 #pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const Segment g = segment_of(p, pc, job, t);
@@ -309,12 +323,15 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     q_phases ^= 1u << b;
                 }
                 q_phases |= 4u << b;
-                if (lane == 0 && ok) {
-                    mbar_expect_tx(&bar_q_full[b], q_bytes);
+                if (ok) {
+                    if (lane == 0) {
+                        mbar_expect_tx(&bar_q_full[b], q_bytes);
 #pragma unroll
-                    for (int kb = 0; kb < KB; ++kb)
-                        tma_load_3d(q_s + b * HALF + kb * TILE_BYTES, &map_q, kb * 64, job.kvh * a.group,
-                                    job.z.row + job.first + x * p.pairs_nodes, &bar_q_full[b]);
+                        for (int kb = 0; kb < KB; ++kb)
+                            tma_load_3d(q_s + b * HALF + kb * TILE_BYTES, &map_q, kb * 64, job.kvh * a.group,
+                                        job.z.row + job.first + x * p.pairs_nodes, &bar_q_full[b]);
+                    }
+                    ++(b == 0 ? q_loaded[0] : q_loaded[1]);
                 }
             }
             if (!g.two) q_next ^= 1;
@@ -341,14 +358,9 @@ span_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
             if (!next_job(a, pc, job, t)) break;
         }
-        // after a wait has run out: what was asked for arrives before the block ends
-        if (!ok) {
-            for (uint32_t i = loaded > RING ? loaded - RING : 0; i < loaded; ++i) {
-                const long long since = clock64();
-                while (!mbar_try_wait(&bar_kv_full[i % RING], (i / RING) & 1) && clock64() - since < WAIT_LIMIT_CYCLES / 64) {
-                }
-            }
-        }
+        ring_arrives(bar_kv_full, loaded);
+        loads_arrive(&bar_q_full[0], q_loaded[0]);
+        loads_arrive(&bar_q_full[1], q_loaded[1]);
     } else if (warp == MMA_WARP && elect_one()) {
         bool ok = true;
         uint32_t phases = 0;                         // the next phase of bar_p (bits 0, 1) and bar_q_full (bits 2, 3)
@@ -755,7 +767,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         bool ok = true;
         const uint32_t q_bytes = (uint32_t)pairs_tile * 128 * KB;
         const int ppt = BK / a.page_size;
-        uint32_t loaded = 0;
+        uint32_t loaded = 0, k_loaded = 0;
 #pragma unroll 1
         for (int t = pc.t0; t < pc.t1;) {
             const int u0 = t - job.begin, u1 = min(job.units, pc.t1 - job.begin), b = jobs & 1;
@@ -769,6 +781,7 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                     for (int kb = 0; kb < KB; ++kb) tma_load_2d(dst + kb * TILE_BYTES, &map_k, job.kvh * HD + kb * 64, row, &bar_k_full[b]);
                 }
+                ++k_loaded;
             }
             __syncwarp();
 #pragma unroll 1
@@ -791,13 +804,8 @@ span_mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             t = job.begin + u1;
             if (t < pc.t1) job.next(a, BK, pairs_nodes);
         }
-        if (!ok) {
-            for (uint32_t i = loaded > RING ? loaded - RING : 0; i < loaded; ++i) {
-                const long long since = clock64();
-                while (!mbar_try_wait(&bar_q_full[i % RING], (i / RING) & 1) && clock64() - since < WAIT_LIMIT_CYCLES / 64) {
-                }
-            }
-        }
+        ring_arrives(bar_q_full, loaded);
+        ring_arrives(bar_k_full, k_loaded);
     } else if (warp == MMA_WARP && elect_one()) {
         bool ok = true;
 #pragma unroll 1

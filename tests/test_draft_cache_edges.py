@@ -1,8 +1,11 @@
 """The library's own refusals of the operators of a cache that is drafted into and thinned out; no GPU needed."""
+import os
+import re
+
 import pytest
 import torch
 
-from lightllm_b200.csrc import ops
+from lightllm_b200.csrc import build, ops
 
 T, S, L, SLOTS, HQ, HKV, HD, PAGES, PAGE, WIDTH = 6, 2, 3, 32, 4, 2, 16, 3, 8, 4
 
@@ -89,3 +92,18 @@ def test_eviction_refuses_planes_that_overlap(written, under, moved):
     assert "must not lie over" in refusal(*evict_call(dict(at, **{written: at[under] + moved}), True))
     if written in ("k_cache", "v_cache"):
         assert "must not lie over" in refusal(*evict_call(dict(at, **{written: at[under] + moved}), False))
+
+
+@pytest.mark.parametrize("kernel", ["span_attention_tc_kernel", "span_mass_tc_kernel"])
+def test_a_block_that_gives_up_waits_for_all_its_loads(kernel):
+    """A load that is still on its way when its block ends writes to shared memory that the next block may own: the loader waits, with a limit, on
+    every barrier that its loads complete on."""
+    with open(os.path.join(build.CSRC_DIR, "span_attention_tcgen05.cu")) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    body = text[text.index(kernel + "(const __grid_constant__"):]
+    body = body[:body.index("\n}\n")]
+    loads = set(re.findall(r"tma_load_\dd\([^;]*?&(\w+)\[[^\]]*\]\)", body))
+    waited = set(re.findall(r"(?:loads_arrive\(&|ring_arrives\()(\w+)", body))
+    assert loads and waited == loads
+    for bar in re.findall(r"loads_arrive\(&(\w+)\[", body):          # (named one by one: both of them)
+        assert {int(i) for i in re.findall(r"loads_arrive\(&%s\[(\d)\]" % bar, body)} == set(range(int(re.search(r"%s\[(\d)\]" % bar, body).group(1))))
