@@ -3,6 +3,7 @@
 #include "cache_calls.h"
 #include "common.cuh"
 #include "memory_ranges.h"
+#include "shared_memory.h"
 #include "tcgen05_common.cuh"
 
 namespace {
@@ -594,7 +595,8 @@ template <typename U> int launch_evict(EvictParams p, int L, cudaStream_t stream
     p.cache_places = places < 20000 ? places : 20000;
     if (bit_words > 8192) p.cache_places = 8192;
     const size_t smem = sizeof(unsigned) * ((size_t)bit_words + p.cache_places);
-    cudaError_t e = cudaFuncSetAttribute(cache_evict_any_kernel<U>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static LlbSharedMemory room;
+    cudaError_t e = room.allow(cache_evict_any_kernel<U>, smem);
     if (e != cudaSuccess) return llb_fail("cache_evict: cannot opt in to %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
     llb_launch(cache_evict_any_kernel<U>, dim3(p.S * p.Hkv, L), dim3(EV_THREADS), smem, stream, p);
     return llb_check_launch("cache_evict");

@@ -14,21 +14,7 @@
 // 33 us instead of 18.)  Everything is worked out on the device: a captured graph serves other lengths.
 #pragma once
 #include "common.cuh"
-
-// A kernel's opt-in to more shared memory than 48 KB, once a device (the attribute belongs to the current one): the call to ask costs the host
-// 0.4 us.  A kernel is always given the same size, or (`size` changes) the largest so far.
-struct LlbSharedMemory {
-    int size[64] = {};
-    template <typename Kernel> cudaError_t allow(Kernel* kernel, size_t bytes) {
-        int device = 0;
-        cudaError_t e = cudaGetDevice(&device);
-        if (e != cudaSuccess) return e;
-        if (device >= 0 && device < 64 && size[device] >= (int)bytes) return cudaSuccess;
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e == cudaSuccess && device >= 0 && device < 64) size[device] = (int)bytes;
-        return e;
-    }
-};
+#include "shared_memory.h"
 
 constexpr int LLB_SPAN_BLOCKS = 512;          // blocks of a kernel at most
 constexpr int LLB_SPAN_TC_LEAST = 2;          // tiles a block of the tensor-core kernel has at least: one for each of its groups

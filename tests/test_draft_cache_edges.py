@@ -1,6 +1,8 @@
 """The library's own refusals of the operators of a cache that is drafted into and thinned out; no GPU needed."""
 import os
 import re
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -107,3 +109,51 @@ def test_a_block_that_gives_up_waits_for_all_its_loads(kernel):
     assert loads and waited == loads
     for bar in re.findall(r"loads_arrive\(&(\w+)\[", body):          # (named one by one: both of them)
         assert {int(i) for i in re.findall(r"loads_arrive\(&%s\[(\d)\]" % bar, body)} == set(range(int(re.search(r"%s\[(\d)\]" % bar, body).group(1))))
+
+
+TWO_THREADS = r"""
+#include "shared_memory.h"
+
+#include <chrono>
+#include <thread>
+
+// A runtime whose attribute is slow to set for the smaller size: the larger one would be set meanwhile, if it could.
+std::atomic<int> attribute{0}, setting{0};
+extern "C" cudaError_t cudaGetDevice(int* device) { *device = 0; return cudaSuccess; }
+extern "C" cudaError_t cudaFuncSetAttribute(const void*, cudaFuncAttribute, int bytes) {
+    ++setting;
+    if (bytes == 1000)
+        for (int i = 0; i < 500 && attribute < 2000; ++i) std::this_thread::sleep_for(std::chrono::milliseconds(1));
+    attribute = bytes;
+    return cudaSuccess;
+}
+
+int main() {
+    static LlbSharedMemory room;
+    static int kernel;
+    bool fits[2];
+    std::thread small([&] { fits[0] = room.allow(&kernel, 1000) == cudaSuccess && attribute >= 1000; });
+    while (setting == 0) std::this_thread::yield();
+    std::thread large([&] { fits[1] = room.allow(&kernel, 2000) == cudaSuccess && attribute >= 2000; });
+    small.join();
+    large.join();
+    // what either launches next, and a smaller size behind them
+    return fits[0] && fits[1] && attribute == 2000 && room.allow(&kernel, 1500) == cudaSuccess && attribute == 2000 ? 0 : 1;
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None or not os.path.exists("/usr/local/cuda/include/cuda_runtime.h"), reason="g++ and the CUDA headers are needed")
+def test_two_host_threads_opt_in_to_shared_memory(tmp_path):
+    """Calls of different head sizes at once: the limit that one of them is about to launch with is not lowered by the other."""
+    source, program = tmp_path / "threads.cpp", tmp_path / "threads"
+    source.write_text(TWO_THREADS)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-pthread", "-I", build.CSRC_DIR, "-I", "/usr/local/cuda/include", str(source), "-o", str(program)], check=True)
+    assert subprocess.run([str(program)], timeout=60).returncode == 0
+
+
+def test_kernels_of_the_drafted_cache_opt_in_that_way():
+    for name in ("span_attention.cu", "span_attention_tcgen05.cu", "cache_rows.cu"):
+        with open(os.path.join(build.CSRC_DIR, name)) as f:
+            text = f.read()
+        assert "cudaFuncSetAttribute" not in text and "LlbSharedMemory" in text, name
