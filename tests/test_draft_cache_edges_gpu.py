@@ -288,3 +288,145 @@ def test_a_decode_step_right_behind_a_commit(ops, heads):
             step()
         torch.cuda.synchronize()
         assert torch.equal(out, want), i
+
+
+def shifted(t, by):
+    """The same numbers in memory that begins ``by`` numbers behind a boundary of 16 bytes."""
+    room = torch.empty(t.numel() + 16, dtype=t.dtype, device=dev())
+    assert room.data_ptr() % 16 == 0
+    return room[by:by + t.numel()].view(t.shape).copy_(t)
+
+
+ODD = [(3, 1, 5), (4, 2, 18), (6, 2, 67), (12, 4, 130), (2, 1, 255), (7, 7, 1)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", ODD, ids=str)
+def test_odd_heads(ops, dtype, heads):
+    """Heads of no whole groups of four numbers: trees, portions and single tokens, uncut jobs and cut ones."""
+    rng = random.Random(11)
+    held, rows = [0, 1, 63, 200, 17, 1500], [5, 1, 37, 90, 0, 3]
+    r = Requests(held, rows, heads, dtype, 16, 301)
+    mask = spread_mask(ops, r, trees(rng, rows))
+    check_rows(r, run_tree(ops, r, mask), tree_sees(r, mask))
+    mass_in = torch.rand((r.hkv, r.num_slots), generator=torch.Generator().manual_seed(302))
+    for n in (rows, [1] * 6, [2, 1, 2, 0, 1, 2]):
+        r = Requests(held, n, heads, dtype, 16, 303)
+        mass_in = torch.rand((r.hkv, r.num_slots), generator=torch.Generator().manual_seed(304))
+        got, mass = run_mass(ops, r, mass_in)
+        G.check_mass(r, got, mass, mass_in, torch.full_like(mass_in, -5.0))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (12, 2, 128), (6, 2, 67), (5, 1, 20)], ids=str)
+@pytest.mark.parametrize("by", [1, 2, 4, 5])
+@pytest.mark.parametrize("which", ["q", "k", "v", "out", "all"])
+def test_addresses_behind_a_boundary(ops, dtype, heads, by, which):
+    """Operands that begin 2, 4, 8 or more bytes behind 16: each of them alone, and all, with little and much to do."""
+    for held, rows in (([0, 90, 1100], [6, 40, 3]), ([33, 2, 700], [1, 1, 1])):
+        r = Requests(held, rows, heads, dtype, 16, 305)
+        at = lambda name, t: shifted(t, by) if which in (name, "all") else t.to(dev())  # noqa: E731
+        q, k, v = at("q", r.q.reshape(r.T, -1)), at("k", r.k), at("v", r.v)
+        mask = spread_mask(ops, r, trees(random.Random(2), rows))
+        out = at("out", torch.full((r.T, r.hq * r.hd), 7.0, dtype=dtype))
+        ops.tree_attention(q, k, v, out, mask.to(dev()), *r.args())
+        check_rows(r, out.cpu().reshape(r.T, r.hq, r.hd), tree_sees(r, mask))
+        mass_in = torch.rand((r.hkv, r.num_slots), generator=torch.Generator().manual_seed(306))
+        mass, out = shifted(torch.full_like(mass_in, -5.0), 1), at("out", torch.full((r.T, r.hq * r.hd), 7.0, dtype=dtype))
+        ops.paged_attention_mass(q, k, v, out, mass, *r.args(), max(rows), mass_in=shifted(mass_in, 3))
+        G.check_mass(r, out.cpu().reshape(r.T, r.hq, r.hd), mass.cpu(), mass_in, torch.full_like(mass_in, -5.0))
+    ops.check_async_errors(dev())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (12, 2, 128), (5, 1, 20)], ids=str)
+def test_scales_below_zero(ops, dtype, heads):
+    """Scores of the queries turned round, and of a scale of nothing: every key that a row sees weighs the same."""
+    for held, rows in (([0, 90, 1100], [6, 40, 3]), ([33, 2, 700], [1, 1, 1])):
+        r = Requests(held, rows, heads, dtype, 16, 307)
+        q, scale = r.q, r.scale
+        mask = spread_mask(ops, r, trees(random.Random(3), rows))
+        r.q, r.scale = -q, -scale
+        tree, (got, mass) = run_tree(ops, r, mask), run_mass(ops, r, None)
+        r.q, r.scale = q, scale
+        check_rows(r, tree, tree_sees(r, mask))
+        G.check_mass(r, got, mass, None, torch.full_like(mass, -5.0))
+        r.scale = 0.0
+        check_rows(r, run_tree(ops, r, mask), tree_sees(r, mask))
+        got, mass = run_mass(ops, r, None)
+        G.check_mass(r, got, mass, None, torch.full_like(mass, -5.0))
+
+
+@pytest.mark.parametrize("heads", [(3, 1, 4), (4, 2, 2), (2, 1, 20), (5, 5, 12), (2, 1, 33)], ids=str)
+@pytest.mark.parametrize("layers", [0, 3])
+def test_rows_of_other_widths_move(ops, heads, layers):
+    """Rows of 8 bytes and of eights, fours and twos of them."""
+    G.test_commit(ops, torch.bfloat16, heads, layers)
+    for held, budget in (([33, 5, 200, 0], 32), ([129, 128], 128), ([3000, 77], 1000)):
+        for apart in (False, True):
+            G.test_evict(ops, torch.bfloat16, heads, held, budget, 3, 8, apart, False)
+
+
+@pytest.mark.parametrize("by", [1, 2, 4])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("held", [600, 5000])
+def test_planes_behind_a_boundary_move(ops, by, dtype, held):
+    """Rows of a whole number of 16 bytes in planes that begin between them (K alone, V alone, both): what aligned planes have afterwards."""
+    S, L, budget = 3, 2, 500
+    r, k, v, mass, pos, ends = G.evict_case([held] * S, (8, 4, 16), dtype, 16, L, 308)
+    planes = lambda a, b: (shifted(k, by) if a else k.to(dev()), shifted(v, by) if b else v.to(dev()), shifted(mass, 1), shifted(pos, 3))  # noqa: E731
+    spans, args = r.spans(), (i32([held] * S), i32(ends), r.spans()[3], 16, budget, 4, 100)
+    want = (k.to(dev()), v.to(dev()), mass.to(dev()), pos.to(dev()))
+    ops.cache_evict(*want, *args)
+    parents = [-1] + [max(0, i - 2) for i in range(1, 40)]
+    tokens = [i % 2 for i in range(40)]
+    trees_of = [i32(x * S) for x in (tokens, parents, [0] * 40)]
+    row, length, at = i32([0, 40, 80]), i32([40] * S), i32([held - 40] * S)
+    for planes_at in ((1, 0), (0, 1), (1, 1)):
+        got = planes(*planes_at)
+        ops.cache_evict(*got, *args)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    commit = lambda a, b: ops.tree_commit(*trees_of, a, b, row, length, at, spans[3], 16, i32([[0] * 30] * S), i32([0] * S), i32([0] * S))  # noqa: E731
+    want = (k.to(dev()), v.to(dev()))
+    commit(*want)
+    assert not torch.equal(want[0].cpu(), k)
+    for planes_at in ((1, 0), (0, 1), (1, 1)):
+        got = planes(*planes_at)[:2]
+        commit(*got)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_captured_eviction_into_other_planes(ops):
+    """A replay's weights and positions, in planes of their own, against the plain form, for other lengths, tables and weights of the same sizes."""
+    heads, page, budget = (4, 2, 16), 16, 64
+    graph, args, planes = torch.cuda.CUDAGraph(), None, None
+    for i, held in enumerate(([100, 64, 200, 65], [300, 20, 64, 90], [63, 70, 80, 299])):
+        r, k, v, mass, pos, ends = G.evict_case(held, heads, torch.bfloat16, page, 2, 310 + i)
+        slots, width = 80 * page, 24
+        fill = lambda t, axis: torch.cat([t, t.new_zeros([n if d != axis else slots - t.shape[axis] for d, n in enumerate(t.shape)])], axis).to(dev())  # noqa: E731
+        new = (fill(k, 1), fill(v, 1), fill(mass, 2), fill(pos, 2))
+        table = i32([row + [-1] * (width - len(row)) for row in r.table])
+        if planes is None:
+            planes, args = [x.clone() for x in new], (i32(held), i32(ends), table)
+            mo, po = torch.empty_like(planes[2]), torch.empty_like(planes[3])
+            with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+                ops.cache_evict(*planes, *args, page, budget, 4, 20, mass_out=mo, positions_out=po)
+        for a, b in zip((*planes, *args), (*new, i32(held), i32(ends), table)):
+            a.copy_(b)
+        mo.fill_(-3.0), po.fill_(-3)
+        graph.replay()
+        torch.cuda.synchronize()
+        want_m, want_p = torch.full_like(mass, -3.0), torch.full_like(pos, -3)
+        for l in range(2):
+            for h in range(r.hkv):
+                for s, n in enumerate(held):
+                    at = r.slots[s]
+                    stay = at[:min(n, budget)]
+                    want_m[l, h, stay], want_p[l, h, stay] = mass[l, h, stay], pos[l, h, stay]
+                    for a, b in P.evict(mass[l, h, at].tolist(), pos[l, h, at].tolist(), ends[s], budget, 4, 20):
+                        want_m[l, h, at[a]], want_p[l, h, at[a]] = mass[l, h, at[b]], pos[l, h, at[b]]
+                        k[l, at[a], h], v[l, at[a], h] = k[l, at[b], h].clone(), v[l, at[b], h].clone()
+        n = r.num_slots
+        assert torch.equal(mo[:, :, :n].cpu(), want_m) and torch.equal(po[:, :, :n].cpu(), want_p)
+        assert torch.equal(planes[0][:, :n].cpu(), k) and torch.equal(planes[1][:, :n].cpu(), v)
+        assert bool((mo[:, :, n:] == -3.0).all()) and bool((po[:, :, n:] == -3).all())
