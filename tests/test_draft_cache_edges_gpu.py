@@ -430,3 +430,199 @@ def test_a_captured_eviction_into_other_planes(ops):
         assert torch.equal(mo[:, :, :n].cpu(), want_m) and torch.equal(po[:, :, :n].cpu(), want_p)
         assert torch.equal(planes[0][:, :n].cpu(), k) and torch.equal(planes[1][:, :n].cpu(), v)
         assert bool((mo[:, :, n:] == -3.0).all()) and bool((po[:, :, n:] == -3).all())
+
+
+class Served:
+    """One layer's cache of three requests as a served model steps over it, with lengths on the device: portions and single tokens whose keys'
+    weights are counted, thinning, drafted trees and what of them is confirmed, decode steps.  ``look`` is called behind every step."""
+    BUDGET, PAGE, WIDTH, LENS, TREES = 96, 16, 16, [140, 40, 97], [9, 5, 12]
+
+    def __init__(self, ops, heads, dtype, look):
+        self.ops, self.heads, self.look = ops, heads, look
+        hq, hkv, hd = heads
+        g, rng = torch.Generator().manual_seed(401), random.Random(401)
+        S = len(self.LENS)
+        order = torch.randperm(S * self.WIDTH + 2, generator=g).tolist()
+        self.table = i32([order[s * self.WIDTH:(s + 1) * self.WIDTH] for s in range(S)])
+        slots = len(order) * self.PAGE
+        self.k, self.v = (torch.full((slots, hkv, hd), math.nan, dtype=dtype, device=dev()) for _ in range(2))
+        self.mass, self.pos = torch.full((hkv, slots), math.nan, device=dev()), torch.zeros((hkv, slots), dtype=torch.int32, device=dev())
+        self.held, self.ends = i32([0] * S), i32([0] * S)
+        self.inv = (10000.0 ** (-torch.arange(0, hd, 2, dtype=torch.float64) / hd)).float().to(dev())
+        self.rounds = []
+        for n in (self.LENS, [1] * S, [1] * S):
+            parents = trees(rng, self.TREES)
+            tokens = [[rng.randrange(3) for _ in t] for t in parents]
+            targets = [[rng.randrange(3) for _ in t] for t in parents]
+            depth = []
+            for t in parents:
+                d = []
+                for p in t:
+                    d.append(d[p] + 1 if p >= 0 else 0)
+                depth += d
+            qkv = [torch.randn((sum(rows), (hq + 2 * hkv) * hd), generator=g).to(dtype).to(dev()) for rows in (n, self.TREES, [1] * S)]
+            flat = [i32([x for t in lists for x in t]) for lists in (tokens, parents, targets)]
+            self.rounds.append((n, parents, tokens, targets, i32(depth), qkv, flat, ops.tree_mask(parents).to(dev())))
+        self.first = {str(n): i32([sum(n[:s]) for s in range(S)]) for n in (self.LENS, self.TREES, [1] * S)}
+        self.row = {str(n): (torch.tensor([s for s in range(S) for _ in range(n[s])], device=dev()), torch.tensor([i for s in range(S) for i in range(n[s])], device=dev()))
+                    for n in (self.LENS, self.TREES, [1] * S)}
+        self.lengths = {str(n): i32(n) for n in (self.LENS, self.TREES, [1] * S)}
+        self.outs = [torch.zeros((sum(n), hq * hd), dtype=dtype, device=dev()) for r in self.rounds for n in (r[0], self.TREES, [1] * S)]
+        self.paths = [(i32([[0] * 12] * S), i32([0] * S), i32([0] * S)) for _ in self.rounds]
+
+    def places(self, req, at):
+        return (self.table[req, at // self.PAGE] * self.PAGE + at % self.PAGE).long()
+
+    def bring(self, n, qkv, depth=None):
+        """The rows' keys and values, rotated by their positions, behind what the requests hold; the rotated queries."""
+        hq, hkv, hd = self.heads
+        req, i = self.row[str(n)]
+        slot = self.places(req, self.held[req] + i)
+        position = (self.ends[req] + (i if depth is None else depth)).int()
+        q = torch.empty((qkv.shape[0], hq * hd), dtype=qkv.dtype, device=dev())
+        self.ops.rope_kv_write(qkv, position, slot.int(), self.inv, hd, False, q, self.k, self.v, hq, hkv, hd)
+        return q, slot, position
+
+    def run(self):
+        ops, (hq, hkv, hd), S = self.ops, self.heads, len(self.LENS)
+        outs = iter(self.outs)
+        for (n, parents, tokens, targets, depth, qkv, flat, mask), (path, count, nxt) in zip(self.rounds, self.paths):
+            args = (self.table, self.PAGE, hq, hkv, hd, hd ** -0.5)
+            # a portion of each, or a token
+            q, slot, position = self.bring(n, qkv[0])
+            self.pos[:, slot] = position
+            self.look("bring", self)
+            out = next(outs)
+            ops.paged_attention_mass(q, self.k, self.v, out, self.mass, self.first[str(n)], self.lengths[str(n)], self.held, *args, max(n), mass_in=self.mass)
+            self.look("mass", self, n, q, out)
+            self.held += self.lengths[str(n)]
+            self.ends += self.lengths[str(n)]
+            ops.cache_evict(self.k, self.v, self.mass, self.pos, self.held, self.ends, self.table, self.PAGE, self.BUDGET, 4, 16)
+            self.look("evict", self)
+            self.held.clamp_(max=self.BUDGET)
+            # drafted trees
+            n = self.TREES
+            q, _, _ = self.bring(n, qkv[1], depth)
+            out, spans = next(outs), (self.first[str(n)], self.lengths[str(n)], self.held)
+            ops.tree_attention(q, self.k, self.v, out, mask, *spans, *args)
+            self.look("tree", self, n, q, out, parents)
+            ops.tree_commit(*flat, self.k, self.v, *spans, self.table, self.PAGE, path, count, nxt)
+            self.look("commit", self, tokens, parents, targets, path, count, nxt)
+            d = torch.arange(12, device=dev())
+            req = torch.arange(S, device=dev())[:, None].expand(S, 12)
+            slot = torch.where(d < count[:, None], self.places(req, self.held[:, None] + d), self.places(req[:, :1], self.held[:, None]))
+            self.mass.index_fill_(1, slot.reshape(-1), 0.0)
+            self.pos[:, slot] = torch.where(d < count[:, None], self.ends[:, None] + d, self.ends[:, None]).int()
+            self.held += count
+            self.ends += count
+            # a token each
+            n = [1] * S
+            q, slot, position = self.bring(n, qkv[2])
+            self.mass.index_fill_(1, slot.reshape(-1), 0.0)
+            self.pos[:, slot] = position
+            q, slot, position = self.bring(n, qkv[2])          # (again, so that no other launch lies between the write and the decode)
+            out = next(outs)
+            iota, zeros = self.first[str(n)], self.first[str(n)] * 0
+            ops.paged_decode_mma(q, self.k, self.v, out, iota, zeros, S, iota, self.held, self.table, self.WIDTH, self.PAGE, hq, hkv, hd, 0, hd ** -0.5, 2, None,
+                                 fresh=1)
+            self.look("decode", self, n, q, out)
+            self.held += 1
+            self.ends += 1
+
+    def state(self):
+        return [self.k, self.v, self.mass, self.pos, self.held, self.ends, *self.outs, *(x for p in self.paths for x in p)]
+
+
+class Looker:
+    """The plain forms beside every step, from what the caches held before it."""
+
+    def __init__(self):
+        self.calls = 0
+
+    def of(self, a, s, more):
+        at = torch.arange(self.held[s] + more)
+        return (a.table.cpu()[s, at // a.PAGE] * a.PAGE + at % a.PAGE).long()
+
+    def attend(self, a, n, q, out, sees):
+        r = Requests([0], [1], a.heads, q.dtype, 16, 0)
+        for s, rows in enumerate(n):
+            first = sum(n[:s])
+            slots = self.of(a, s, rows)
+            mine = q.cpu().view(-1, a.heads[0], a.heads[2])[first:first + rows], a.k.cpu()[slots], a.v.cpu()[slots]
+            want, w = P.attention(*mine, sees(s, rows), a.heads[2] ** -0.5)
+            r.of, r.slots = lambda _: mine, [slots.tolist()]
+            got = out.cpu().double().view(-1, a.heads[0], a.heads[2])[first:first + rows]
+            assert bool(((got - want).abs() <= r.tolerance(0, want)).all()), (self.calls, s)
+            yield s, slots, mine, w
+
+    def causal(self, s, rows):
+        return torch.cat([torch.ones((rows, self.held[s]), dtype=torch.bool), torch.ones((rows, rows), dtype=torch.bool).tril()], 1)
+
+    def __call__(self, what, a, *more):
+        self.calls += 1
+        torch.cuda.synchronize()
+        self.held = a.held.tolist()          # (as the step was given it)
+        if what == "mass":
+            n, q, out = more
+            for s, slots, (mq, mk, _), w in self.attend(a, n, q, out, self.causal):
+                sums = w.reshape(a.heads[1], -1, w.shape[-1]).sum(1)
+                before = torch.zeros_like(sums)
+                before[:, :self.held[s]] = self.mass[:, slots[:self.held[s]]].double()
+                rel = 2 * P.score_error(mq, mk, a.heads[2] ** -0.5) + (n[s] * a.heads[0] // a.heads[1] + len(slots) + 16) * 2.0 ** -24 + 2.0 ** -20
+                assert bool(((a.mass.cpu()[:, slots].double() - before - sums).abs() <= rel * sums + 2.0 ** -23 * before).all())
+        elif what == "tree":
+            n, q, out, parents = more
+            list(self.attend(a, n, q, out, lambda s, rows: torch.cat([torch.ones((rows, self.held[s]), dtype=torch.bool), P.ancestors(parents[s])], 1)))
+        elif what == "decode":
+            n, q, out = more
+            list(self.attend(a, n, q, out, self.causal))
+        elif what == "evict":
+            for s in range(3):
+                at, ends = self.of(a, s, 0), a.ends.tolist()
+                for h in range(a.heads[1]):
+                    for hole, filler in P.evict(self.new_mass[h, at].tolist(), self.new_pos[h, at].tolist(), ends[s], a.BUDGET, 4, 16):
+                        for t in (self.k, self.v):
+                            t[at[hole], h] = t[at[filler], h].clone()
+                        for t in (self.new_mass, self.new_pos):
+                            t[h, at[hole]] = t[h, at[filler]].clone()
+            for got, want in ((a.k, self.k), (a.v, self.v), (a.mass, self.new_mass), (a.pos, self.new_pos)):
+                assert torch.equal(got.cpu().nan_to_num(9.0), want.nan_to_num(9.0))
+        elif what == "commit":
+            tokens, parents, targets, path, count, nxt = more
+            for s in range(3):
+                took, last = P.commit(tokens[s], parents[s], targets[s], 12)
+                assert path[s].tolist() == took + [-1] * (12 - len(took)) and int(count[s]) == len(took) and int(nxt[s]) == last
+                slots = self.of(a, s, 12)[self.held[s]:]
+                for t in (self.k, self.v):
+                    t[slots[:len(took)]] = t[slots[took]].clone()
+            assert torch.equal(a.k.cpu().nan_to_num(9.0), self.k.nan_to_num(9.0)) and torch.equal(a.v.cpu().nan_to_num(9.0), self.v.nan_to_num(9.0))
+        # what the next step finds
+        self.k, self.v, self.new_mass, self.new_pos = a.k.cpu(), a.v.cpu(), a.mass.cpu(), a.pos.cpu()
+        self.mass = self.new_mass
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (12, 2, 128)], ids=str)
+def test_served_steps_in_bf16(ops, heads):
+    """Cache writes, counted attention, thinning, drafted trees, their commit and decode steps behind one another: every step against the plain
+    forms, then all of them without a look between, eager and as one graph, with equal bits."""
+    look = Looker()
+    a = Served(ops, heads, torch.bfloat16, look)
+    a.run()
+    ops.check_async_errors(dev())
+    assert look.calls == 18 and a.held.tolist() != a.ends.tolist()
+    want = [x.clone() for x in a.state()]
+    b = Served(ops, heads, torch.bfloat16, lambda *_: None)
+    start = [x.clone() for x in b.state()]
+    b.run()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0)) for x, y in zip(b.state(), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        b.run()
+    for _ in range(3):
+        for x, y in zip(b.state(), start):
+            x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0)) for x, y in zip(b.state(), want))
+    ops.check_async_errors(dev())
