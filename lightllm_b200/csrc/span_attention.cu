@@ -105,6 +105,10 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
             own[i] = r >= rows ? -1 : bits ? job.z.pos : job.z.pos + node + 1;
             mask_at[i] = (size_t)(job.z.row + node) * a.words;
         }
+        auto sees = [&](int i, int key) {
+            if (key < own[i]) return true;
+            return bits && own[i] > -1 && key < job.keys && ((bits[mask_at[i] + ((key - job.z.pos) >> 6)] >> ((key - job.z.pos) & 63)) & 1ull);
+        };
         for (int kt = k0; kt < k1; ++kt) {
             const int key0 = kt * KT;
             __syncthreads();                           // the tile before has been read
@@ -145,8 +149,7 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
 #pragma unroll
                 for (int j = 0; j < KPT; ++j) {
                     const int key = key0 + tx + CT * j;
-                    bool on = key < own[i];
-                    if (!inner && bits && own[i] > -1 && !on && key < job.keys) on = (bits[mask_at[i] + ((key - job.z.pos) >> 6)] >> ((key - job.z.pos) & 63)) & 1ull;
+                    const bool on = inner ? own[i] > -1 : sees(i, key);
                     float lo, hi;
                     llb_unpack2(x[i][j], lo, hi);
                     s_s[(ty * 4 + i) * SP + tx + CT * j] = on ? (lo + hi) * a.scale_log2e : -INFINITY;
@@ -209,9 +212,11 @@ __global__ void __launch_bounds__(THREADS) span_attention_kernel(const SimtParam
                     }
                     if (odd) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                        for (int i = 0; i < 4; ++i) {
+                            if (!sees(i, key0 + j + e)) continue;          // (a weight of a key that the row sees may be 0 as well)
 #pragma unroll
-                            for (int d = 0; d < DPT; ++d) o[i][d] = pr[i][e] == 0.0f ? o[i][d] : fmaf(pr[i][e], vv[d], o[i][d]);
+                            for (int d = 0; d < DPT; ++d) o[i][d] = fmaf(pr[i][e], vv[d], o[i][d]);
+                        }
                     } else if (DPT % 2 == 0) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {

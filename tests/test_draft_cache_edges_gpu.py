@@ -626,3 +626,26 @@ def test_served_steps_in_bf16(ops, heads):
         torch.cuda.synchronize()
         assert all(torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0)) for x, y in zip(b.state(), want))
     ops.check_async_errors(dev())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (12, 2, 128), (5, 1, 20)], ids=str)
+@pytest.mark.parametrize("held", [0, 40, 700])
+def test_infinite_values_of_keys_that_weigh_next_to_nothing(ops, dtype, heads, held):
+    """A weight of less than 32 bits show times infinity is infinity (or, with a weight of 0, NaN): it shows in the rows that see the key, and in no
+    others."""
+    r = Requests([held, 9], [30, 6], heads, dtype, 16, 209)
+    r.q[:, :, 0] = r.q[:, :, 0].abs() + 1.0
+    at = held + 11
+    r.k[r.slots[0][at], :, 0] = -300.0 / r.scale          # scores of -300 and less
+    r.v[r.slots[0][at], :, 2] = math.inf
+    mask = spread_mask(ops, r, trees(random.Random(8), r.rows))
+    sees = tree_sees(r, mask)
+    assert bool(sees[0][:, at].any()) and not bool(sees[0][:, at].all())
+    got = run_tree(ops, r, mask)[r.first[0]:r.first[0] + 30]
+    assert torch.equal(~got.isfinite()[:, :, 2], sees[0][:, at, None].expand(30, r.hq)) and bool(got[:, :, :2].isfinite().all())
+    got, mass = run_mass(ops, r, None)
+    got = got[r.first[0]:r.first[0] + 30]
+    assert torch.equal(~got.isfinite()[:, :, 2], causal(r)[0][:, at, None].expand(30, r.hq)) and bool(got[:, :, :2].isfinite().all())
+    # (a row that sees no key but this one gives it everything: there is none here)
+    assert bool((mass[:, r.slots[0][at]] == 0).all())
