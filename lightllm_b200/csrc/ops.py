@@ -1539,7 +1539,9 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, targets: torch.Tens
 
     (count 0 and next_token -1 where a request brings no rows; a path ends at its width).  The row of node ``path[s, d]`` moves from place
     ``span_pos[s] + path[s, d]`` to ``span_pos[s] + d`` in every layer: the request then holds ``span_pos[s] + count[s]`` keys, what lies
-    behind them is left over.  :func:`paged_decode_mma` may be the next launch, with ``fresh``: moved keys are there.
+    behind them is left over.  :func:`paged_decode_mma` may be the next launch, with ``fresh``: moved keys are there.  Keys and values are
+    all that moves: weights and positions of the confirmed places (:func:`cache_evict` goes by them) are the caller's to set, or an
+    earlier owner's stay there.
 
     tokens, parents, targets int32 [T]; caches [slots, kv heads, head_dim] or [layers, ...]; path int32 [requests, width], width up
     to 1,024; count, next_token int32 [requests].  Results lie over nothing else of the call."""

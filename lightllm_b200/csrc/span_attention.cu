@@ -616,7 +616,8 @@ namespace {
 
 // (row, head) pairs a job of the CUDA-core kernel holds: 16 where requests bring that many or fewer on average.  (float32, 14/2 heads of 64, 5
 // requests of 77 to 1,103 keys, us with 16 | 64: a row each 15 | 20, two 15.4 | 20.5, four 18.5 | 21.5, eight 25 | 22, 64 rows 103 | 48;
-// 27 requests: two 26 | 31, four 37 | 33.)
+// 27 requests: two 26 | 31, four 37 | 33.  Four rows, 28 pairs, go to 64: few requests lose 3 us by that, many gain 4.  Where it changes depends on
+// how many blocks have work, which the rule does not ask.)
 int simt_rows(int T, int S, int group) { return group <= 16 && (long long)T * group <= 16ll * S ? 16 : 64; }
 int simt_blocks() { return min(2 * llb_device_sms(), LLB_SPAN_BLOCKS); }
 int tc_blocks() { return min(llb_device_sms(), LLB_SPAN_BLOCKS); }
