@@ -13,7 +13,7 @@ struct LlbRange {
     long long bytes;
     bool over(const LlbRange& b) const {
         const uintptr_t x = (uintptr_t)at, y = (uintptr_t)b.at;
-        return at && b.at && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)bytes;
+        return at && b.at && bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)bytes;
     }
 };
 

@@ -157,3 +157,12 @@ def test_kernels_of_the_drafted_cache_opt_in_that_way():
         with open(os.path.join(build.CSRC_DIR, name)) as f:
             text = f.read()
         assert "cudaFuncSetAttribute" not in text and "LlbSharedMemory" in text, name
+
+
+def test_empty_ranges_lie_over_nothing():
+    """A commit's drafted tokens may be none: what their address is says nothing.  (Refused all the same here, for its path.)"""
+    at = memory()
+    order = ("tokens", "parents", "targets", "k_cache", "v_cache", "span_row", "span_len", "span_pos", "block_table", "path", "count", "next_token")
+    there = dict(at, tokens=at["k_cache"] + 64, parents=at["path"] + 4, path=at["count"])
+    said = refusal(ops.lib().llb_tree_commit, ops._TREE_COMMIT, *(there[x] for x in order), S, 0, 1, PAGES, PAGE, SLOTS, HKV * HD * 4, WIDTH)
+    assert said.endswith("path must not lie over count")
