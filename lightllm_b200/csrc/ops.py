@@ -1576,7 +1576,8 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor
 
     Caches [slots, kv heads, head_dim] or [layers, ...]; mass float32 and positions int32 [kv heads, slots] or [layers, ...];
     lengths, ends int32 [requests].  ``mass_out`` and ``positions_out`` (both or neither): planes that receive the mass and position
-    of every place that is held afterwards, in the place of the planes that are read; nothing else in them is written."""
+    of every place that is held afterwards, in the place of the planes that are read; nothing else in them is written.  They are the
+    planes that are read or lie over nothing else of the call, and so do the caches."""
     L, slots, heads, hd = _check_planes("cache_evict", k_cache, v_cache)
     each = lengths.shape
     S = each[0]
